@@ -7,9 +7,9 @@ The directory name is not a Python identifier, so load it with
 """
 from .abi import (DGM_ERR_ARG, DGM_ERR_BITS, DGM_ERR_HIP, DGM_ERR_NOT_BEGUN,
                   DGM_ERR_SHAPE, DGM_ERR_UNSUPPORTED, DGM_MATH_BF16,
-                  DGM_MATH_FP32, DGM_NOALLOC_SCRATCH_BYTES, DGM_OK, HEADER, LIB_PATH, PROTOTYPES,
+                  DGM_MATH_FP32, DGM_NOALLOC_SCRATCH_BYTES, DGM_OK, DGM_TYPE_BF16, DGM_TYPE_F32, HEADER, LIB_PATH, PROTOTYPES,
                   DIT_LINEARS, DIT_NORMS, DgmError, DiTCfg, DiTLinear,
-                  DiTWeights, GemmP, QuantP, AdamP, EmbP, EmbBwdP, PosP, BiasP,
+                  DiTWeights, AttnCfg, CacheCfg, GemmP, QuantP, AdamP, EmbP, EmbBwdP, PosP, BiasP,
                   ReduceP, ScaleP, UnaryP, DiTGrads, load_library)
 from .gpu import GPU, Buf, RawBuf
 from .dit import DiTBlock, DiTConfig, rope_tables
@@ -24,5 +24,5 @@ __all__ = [
     "DiTWeights", "DIT_LINEARS", "DIT_NORMS", "rope_tables", "AdamP", "EmbP", "EmbBwdP",
     "PosP", "BiasP", "ReduceP", "ScaleP", "UnaryP", "Param", "bias_corrections", "grad_norm",
     "optimizer_step", "zero_grads", "DiTGrads", "load_dit_block", "load_gpt", "read_tdit", "read_tgmt",
-    "save_tdit", "save_tgmt",
+    "save_tdit", "save_tgmt", "AttnCfg", "CacheCfg", "DGM_TYPE_F32", "DGM_TYPE_BF16",
 ]

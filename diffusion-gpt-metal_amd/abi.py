@@ -21,6 +21,9 @@ DGM_ERR_HIP = 4
 DGM_ERR_BITS = 5
 DGM_ERR_UNSUPPORTED = 6
 
+DGM_TYPE_F32 = 0
+DGM_TYPE_BF16 = 1
+
 DGM_MATH_FP32 = 0
 DGM_MATH_BF16 = 1
 DGM_NOALLOC_SCRATCH_BYTES = 8 << 20   # static scratch of dgm_gemmNT_noalloc (include/dgm_quant.h)
@@ -64,6 +67,21 @@ class DiTGrads(ctypes.Structure):
     """dgm_dit_grads: fp32 gradients (+=) of the seven linears and five norms."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("wq", "wk", "wv", "wo", "wgate", "wup", "wdown")] + \
                [(n, ctypes.c_void_p) for n in ("n1", "n1b", "n2", "n2b", "nf")]
+
+
+class AttnCfg(ctypes.Structure):
+    """dgm_attn_cfg: packed sequences (row strides of 0: rows back to back)."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("type", "H", "KVH", "D", "causal")] + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int64) for n in ("rows", "nseq", "ldq", "ldk", "ldv", "ldo")])
+
+
+class CacheCfg(ctypes.Structure):
+    """dgm_cache_cfg: a paged key-value cache, [numPages, KVH, pageSize, D] each."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("type", "KVH", "D", "pageSize")]
+                + [(n, ctypes.c_int64) for n in ("numPages", "maxPages")])
+
+
+assert ctypes.sizeof(AttnCfg) == 72 and ctypes.sizeof(CacheCfg) == 32
 
 
 class TgmtHeader(ctypes.Structure):
@@ -203,6 +221,12 @@ PROTOTYPES = {
     "dgm_dit_forward_train": (_I, [_P, ctypes.POINTER(DiTCfg), ctypes.POINTER(DiTWeights), _P, _P, _P, _P, _I64]),
     "dgm_dit_backward": (_I, [_P, ctypes.POINTER(DiTCfg), ctypes.POINTER(DiTWeights), ctypes.POINTER(DiTGrads),
                               _P, _P, _P, _I64, _P, _P, _I64]),
+    "dgm_attnPackedFwd": (_I, [_P, ctypes.POINTER(AttnCfg)] + [_P] * 6),
+    "dgm_attnPackedBwd_ws_bytes": (_I64, [ctypes.POINTER(AttnCfg)]),
+    "dgm_attnPackedBwd": (_I, [_P, ctypes.POINTER(AttnCfg)] + [_P] * 11 + [_I64]),
+    "dgm_cacheWrite": (_I, [_P, ctypes.POINTER(CacheCfg), _I64] + [_P] * 7 + [_I64] * 4),
+    "dgm_attnPagedDecode_ws_bytes": (_I64, [ctypes.POINTER(CacheCfg), _I64, _I64]),
+    "dgm_attnPagedDecode": (_I, [_P, ctypes.POINTER(CacheCfg), _I64] + [_P] * 7 + [_I64] * 5 + [_F]),
     "dgm_adamw": (_I, [_P, _P, _P, _P, _P, ctypes.POINTER(AdamP)]),
     "dgm_adam": (_I, [_P, _P, _P, _P, _P, _I64] + [_F] * 7),
     "dgm_adam_quantize": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64] + [_F] * 7),

@@ -1,0 +1,655 @@
+// A paged cache of keys and values, and the attention of one new token per
+// sequence over it (gfx950). HBM-bound: a cached element is used once per query head of its group.
+//
+// Decode design:
+//  * Work is cut over the sequences' lengths as the device finds them: all
+//    tiles (128 keys of a bf16 cache, 64 of an fp32 one) of all sequences lie in a row, and
+//    each of W workgroups per key head takes an equal run of them, so that 48
+//    ragged sequences keep the chip as busy as one long one. A run ends in at most a few sequences;
+//    worker w's part of sequence s is slot w + s of the partial results (w and s only
+//    grow along the row of tiles, so slots never collide). A sequence inside one
+//    run is written out by its worker; the others are joined by a second kernel.
+//  * No LDS on the way from HBM to the matrix unit. S^T = K Q^T takes K as it
+//    lies in the cache (16 keys x 8 columns of 16 bytes a lane), with the heads of
+//    the group as columns; P^T then is in the layout of the B operand of
+//    O^T = V^T P^T, whose A operand a lane builds from 8 keys' rows by byte
+//    permutes among its own registers. A wave takes 32 keys (16 of an fp32
+//    cache) at a time and loads those of the next round before it computes.
+//  * A bf16 cache meets fp32 queries as three bf16 pieces (8 bits each: all 24),
+//    and so do the probabilities, with fp32 sums: nothing of fp32 is lost. bf16
+//    queries take one piece each, P rounded to bf16. An fp32 cache runs on fp32 MFMA.
+//  * Slots behind a sequence's end, and of pages that are not the cache's, are
+//    not read: they count as zero keys with a weight of zero.
+#include <climits>
+#include <cmath>
+
+#include "attn.hpp"
+
+namespace {
+
+using namespace dgm_attn;
+
+struct Cache {
+    const int32_t* pages;
+    uint32_t* flag;
+    int64_t numPages, maxPages;
+    int KVH, D, capacity;   // positions that a sequence's row of the table holds
+    Div page;
+    // As cache_row; pos below capacity.
+    __device__ __forceinline__ int row(int64_t s, uint32_t pos, int h) const {
+        return cache_row(pages, page, numPages, maxPages, KVH, s, pos, h);
+    }
+};
+
+// ---- write ---------------------------------------------------------------------
+
+struct WriteArgs {
+    Cache c;
+    const void *k, *v;
+    void *kc, *vc;
+    const int32_t *starts, *lens;
+    int64_t rows, nseq, ldk, ldv;
+};
+
+template <typename IN, typename CT>
+__device__ __forceinline__ void convert8(const IN* from, CT* to) {
+    if constexpr (sizeof(IN) == 2 && sizeof(CT) == 2) {
+        *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(from);
+    } else if constexpr (sizeof(IN) == 4 && sizeof(CT) == 4) {
+        const u32x4 a = reinterpret_cast<const u32x4*>(from)[0], b = reinterpret_cast<const u32x4*>(from)[1];
+        reinterpret_cast<u32x4*>(to)[0] = a;
+        reinterpret_cast<u32x4*>(to)[1] = b;
+    } else if constexpr (sizeof(IN) == 4) {
+        const f32x4 a = reinterpret_cast<const f32x4*>(from)[0], b = reinterpret_cast<const f32x4*>(from)[1];
+        bf16x8 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[i] = __bf16(a[i]);
+            o[4 + i] = __bf16(b[i]);
+        }
+        *reinterpret_cast<bf16x8*>(to) = o;
+    } else {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(from);
+        u32x4 lo, hi;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            lo[2 * i] = a[i] << 16;
+            lo[2 * i + 1] = a[i] & 0xffff0000u;
+            hi[2 * i] = a[2 + i] << 16;
+            hi[2 * i + 1] = a[2 + i] & 0xffff0000u;
+        }
+        reinterpret_cast<u32x4*>(to)[0] = lo;
+        reinterpret_cast<u32x4*>(to)[1] = hi;
+    }
+}
+
+// A thread moves 8 elements of k and of v of one (row, head).
+template <typename IN, typename CT>
+__global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
+    if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.nseq, a.rows, a.c.flag);
+    const int per_head = a.c.D / 8, per_row = a.c.KVH * per_head;
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, row = i / per_row;
+    if (row >= a.rows) return;
+    const int e = int(i % per_row), head = e / per_head, d = e % per_head * 8;
+    int64_t s = row, first = row;
+    if (a.starts) {   // the last sequence that starts at or before the row
+        if (a.starts[0] > row) return;
+        int64_t lo = 0, hi = a.nseq;
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (a.starts[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        if (a.starts[lo + 1] <= row) return;
+        s = lo;
+        first = a.starts[lo];
+    }
+    const int64_t pos = (a.lens ? int64_t(a.lens[s]) : 0) + (row - first);
+    const int at = pos >= 0 && pos < a.c.capacity ? a.c.row(s, uint32_t(pos), head) : -1;
+    if (at < 0) {
+        if (e == 0) atomicOr(a.c.flag, kBadPages);
+        return;
+    }
+    const int64_t to = int64_t(at) * a.c.D + d;
+    convert8(static_cast<const IN*>(a.k) + row * a.ldk + int64_t(head) * a.c.D + d, static_cast<CT*>(a.kc) + to);
+    convert8(static_cast<const IN*>(a.v) + row * a.ldv + int64_t(head) * a.c.D + d, static_cast<CT*>(a.vc) + to);
+}
+
+// ---- decode --------------------------------------------------------------------
+
+constexpr int kHeads = 16;      // query heads of a workgroup: the columns of an MFMA tile
+constexpr int kWorkers = 512;   // workgroups that share the tiles, over all key heads
+
+template <typename CT>
+constexpr int kWaveKeys = sizeof(CT) == 2 ? 32 : 16;
+template <typename CT>
+constexpr int kTileKeys = 4 * kWaveKeys<CT>;   // four waves
+
+struct DecodeArgs {
+    Cache c;
+    const void *q, *kc, *vc;
+    void* out;
+    float* part;   // [units][workers + nseq][heads][D]; behind them m and l, [..][heads][2]
+    float* stat;
+    const int32_t* lens;
+    int64_t nseq, ldq, ldo;
+    int H, G, heads, parts, workers, units;   // heads of a unit; units of a key head
+    float scale2;                             // scale * log2 e
+};
+
+__device__ __forceinline__ int length_of(const DecodeArgs& a, int64_t s) {
+    const int n = a.lens[s];
+    return n < 0 ? 0 : n > a.c.capacity ? a.c.capacity : n;
+}
+
+// Tiles of sequences 0 .. s-1 (s <= nseq), by a whole wave.
+template <int KEYS>
+__device__ inline int64_t tiles_before(const DecodeArgs& a, int64_t s) {
+    int64_t sum = 0;
+    for (int64_t i = threadIdx.x & 63; i < s; i += 64) sum += (length_of(a, i) + KEYS - 1) / KEYS;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, 64);
+    return sum;
+}
+
+// Three bf16 pieces of 8 bits each that add up to x exactly (high to low); a
+// non-finite x is its first piece.
+__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    const uint32_t u = __float_as_uint(x);
+    const bool fin = (u & 0x7f800000u) != 0x7f800000u;
+    hi = (u & 0x007fffffu) && !fin ? 0x7fc00000u : u & 0xffff0000u;
+    const float r = fin ? x - __uint_as_float(hi) : 0.0f;
+    mid = __float_as_uint(r) & 0xffff0000u;
+    lo = __float_as_uint(r - __uint_as_float(mid)) & 0xffff0000u;
+}
+
+template <int PIECES>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&o)[PIECES]) {
+    if constexpr (PIECES == 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[0][j] = __bf16(x[j]);
+    } else {
+        u32x4 w[3];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            uint32_t a[3], b[3];
+            split3(x[j], a[0], a[1], a[2]);
+            split3(x[j + 1], b[0], b[1], b[2]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) w[p][j / 2] = (a[p] >> 16) | b[p];
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) o[p] = __builtin_bit_cast(bf16x8, w[p]);
+    }
+}
+
+template <typename IN>
+__device__ __forceinline__ void load8(const IN* p, float (&x)[8]) {
+    if constexpr (sizeof(IN) == 4) {
+        const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+    } else {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = float(a[i]);
+    }
+}
+
+// VW consecutive elements of a value row in registers.
+template <int BYTES>
+struct Piece {
+    uint32_t w[BYTES / 4];
+};
+template <int BYTES>
+__device__ __forceinline__ Piece<BYTES> load_piece(const void* p, int64_t bytes) {   // those up to `bytes`
+    Piece<BYTES> o{};
+    if (bytes > 0) {
+        if constexpr (BYTES >= 16) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) {
+                if (i * 16 >= bytes) continue;
+                const u32x4 v = static_cast<const u32x4*>(p)[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o.w[4 * i + j] = v[j];
+            }
+        } else if constexpr (BYTES == 8) {
+            const u32x2 v = *static_cast<const u32x2*>(p);
+            o.w[0] = v[0];
+            o.w[1] = v[1];
+        } else {
+            o.w[0] = *static_cast<const uint32_t*>(p);
+        }
+    }
+    return o;
+}
+
+// One wave's 32 (16) keys on their way: rows of the cache, then the data.
+template <typename CT, int DP>
+struct Round {
+    static constexpr int EB = sizeof(CT), NB = kWaveKeys<CT> / 16;   // blocks of 16 keys
+    static constexpr int KC = DP * EB / 64;                          // 16-byte chunks of a key to a lane
+    static constexpr int VW = DP / 16, VB = VW * EB;                 // elements and bytes of a value row to a lane
+    u32x4 k[NB][KC];
+    Piece<VB> v[4 * NB];
+    int row;               // of key lane % (16 NB)
+    int vrow[4 * NB];      // of key 16 b + 4 g + i
+
+    // The rows of keys key0 .. of sequence s, those below len.
+    __device__ __forceinline__ void find(const Cache& c, int64_t s, int kvh, int key0, int len) {
+        const int key = key0 + (int(threadIdx.x) & (16 * NB - 1));
+        row = key < len ? c.row(s, uint32_t(key), kvh) : -1;
+        if (key < len && row < 0) atomicOr(c.flag, kBadPages);
+    }
+    __device__ __forceinline__ void load(const Cache& c, const uint8_t* kc, const uint8_t* vc) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const int64_t rb = int64_t(c.D) * EB;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int at = __shfl(row, 16 * b + r, 64);
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk) {
+                const int off = kk * 64 + g * 16;
+                k[b][kk] = u32x4{0, 0, 0, 0};
+                if (at >= 0 && off < rb) k[b][kk] = *reinterpret_cast<const u32x4*>(kc + at * rb + off);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4 * NB; ++j) {
+            vrow[j] = __shfl(row, 16 * (j / 4) + 4 * g + j % 4, 64);
+            v[j] = load_piece<VB>(vc + vrow[j] * rb + r * VB, vrow[j] >= 0 ? rb - r * VB : 0);
+        }
+    }
+};
+
+// The queries of a unit as B operand, columns = heads.
+template <typename IN, typename CT, int DP>
+struct Queries {
+    static constexpr int PIECES = sizeof(IN) == 4 && sizeof(CT) == 2 ? 3 : 1;
+    static constexpr int KC = DP * int(sizeof(CT)) / 64;
+    u32x4 f[PIECES][KC];
+    __device__ __forceinline__ void load(const IN* q, int D, bool in) {   // q: of the lane's head
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int kk = 0; kk < KC; ++kk) {
+            if constexpr (sizeof(CT) == 2) {
+                const int d = 32 * kk + 8 * g;
+                float x[8] = {};
+                if (in && d < D) load8(q + d, x);
+                bf16x8 o[PIECES];
+                split8<PIECES>(x, o);
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) f[p][kk] = __builtin_bit_cast(u32x4, o[p]);
+            } else {
+                const int d = 16 * kk + 4 * g;
+                f32x4 x = {};
+                if (in && d < D) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = float(q[d + i]);
+                }
+                f[0][kk] = __builtin_bit_cast(u32x4, x);
+            }
+        }
+    }
+};
+
+template <typename IN, typename CT, int DP>
+__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attn_paged_decode_kernel(DecodeArgs a) {
+    using R = Round<CT, DP>;
+    using Q = Queries<IN, CT, DP>;
+    constexpr int KEYS = kTileKeys<CT>, WK = kWaveKeys<CT>, NB = R::NB, VW = R::VW;
+    __shared__ float part[4][kHeads][DP];
+    __shared__ float stat[4][kHeads][2];
+    const int unit = blockIdx.x % a.units, worker = blockIdx.x / a.units;
+    const int kvh = unit / a.parts, h0 = kvh * a.G + unit % a.parts * kHeads;   // first query head
+    const int heads = min(kHeads, a.G - unit % a.parts * kHeads);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    if (blockIdx.x == 0)
+        for (int64_t i = threadIdx.x; i < a.nseq; i += 256)
+            if (a.lens[i] > a.c.capacity) atomicOr(a.c.flag, kBadPages);
+    const int64_t total = tiles_before<KEYS>(a, a.nseq), per = (total + a.workers - 1) / a.workers;
+    int64_t at = worker * per;
+    const int64_t end = at + per < total ? at + per : total;
+    const uint8_t* kc = static_cast<const uint8_t*>(a.kc);
+    const uint8_t* vc = static_cast<const uint8_t*>(a.vc);
+    // Sequences without keys have no tile: their rows are zeros.
+    if (worker == 0)
+        for (int64_t s0 = 0; s0 < a.nseq; s0 += 64) {
+            unsigned long long none = __ballot(s0 + lane < a.nseq && length_of(a, s0 + lane) == 0);
+            for (; none; none &= none - 1)
+                for (int e = threadIdx.x; e < heads * a.c.D; e += 256)
+                    static_cast<IN*>(a.out)[(s0 + __ffsll(none) - 1) * a.ldo + int64_t(h0) * a.c.D + e] = IN(0.0f);
+        }
+    if (at >= end) return;
+    // The sequence of the first tile, and that sequence's first tile.
+    int64_t s = 0, base = 0;
+    for (int64_t s0 = 0;; s0 += 64) {
+        const int64_t i = s0 + lane;
+        const int64_t own = i < a.nseq ? (length_of(a, i) + KEYS - 1) / KEYS : 0;
+        int64_t sum = own;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            const int64_t y = __shfl_up(sum, x, 64);
+            if (lane >= x) sum += y;
+        }
+        const unsigned long long past = __ballot(base + sum > at);
+        if (past) {
+            const int first = __ffsll(past) - 1;
+            s = s0 + first;
+            base += __shfl(sum - own, first, 64);
+            break;
+        }
+        base += __shfl(sum, 63, 64);
+    }
+    while (true) {
+        const int len = length_of(a, s);
+        const int64_t tiles = (len + KEYS - 1) / KEYS;
+        const int t0 = int(at - base), t1 = int(base + tiles < end ? tiles : end - base);
+
+        Q q;
+        q.load(static_cast<const IN*>(a.q) + s * a.ldq + int64_t(h0 + col) * a.c.D, a.c.D, col < heads);
+        f32x4 o[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) o[i] = f32x4{0, 0, 0, 0};
+        float m = kNegInf, l = 0.0f;
+        R now, next;
+        now.find(a.c, s, kvh, t0 * KEYS + wave * WK, len);
+        now.load(a.c, kc, vc);
+        next.find(a.c, s, kvh, (t0 + 1) * KEYS + wave * WK, t0 + 1 < t1 ? len : 0);
+        for (int t = t0; t < t1; ++t) {
+            if (t + 1 < t1) next.load(a.c, kc, vc);
+            next.find(a.c, s, kvh, (t + 2) * KEYS + wave * WK, t + 2 < t1 ? len : 0);
+            f32x4 sc[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                sc[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int kk = 0; kk < Q::KC; ++kk) {
+                    if constexpr (sizeof(CT) == 2) {
+#pragma unroll
+                        for (int p = Q::PIECES - 1; p >= 0; --p)
+                            sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, now.k[b][kk]),
+                                                                            __builtin_bit_cast(bf16x8, q.f[p][kk]),
+                                                                            sc[b], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][kk][i]),
+                                                                         __uint_as_float(q.f[0][kk][i]), sc[b], 0, 0, 0);
+                    }
+                }
+            }
+            float mx = kNegInf;
+#pragma unroll
+            for (int j = 0; j < 4 * NB; ++j) {
+                sc[j / 4][j % 4] = now.vrow[j] >= 0 ? sc[j / 4][j % 4] : kNegInf;
+                mx = fmaxf(mx, sc[j / 4][j % 4]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any((mx - m) * a.scale2 > 8.0f)) {
+                const float to = fmaxf(m, mx), f = m == kNegInf ? 0.0f : exp2_hw((m - to) * a.scale2);
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[i] *= f;
+                m = to;
+            }
+            const float mc = m == kNegInf ? 0.0f : m * a.scale2;
+            float p[4 * NB];
+#pragma unroll
+            for (int j = 0; j < 4 * NB; ++j) {
+                p[j] = exp2_hw(__builtin_fmaf(sc[j / 4][j % 4], a.scale2, -mc));
+                l += p[j];
+            }
+            if constexpr (sizeof(CT) == 2) {
+                bf16x8 w[Q::PIECES];
+                split8<Q::PIECES>(p, w);
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+                    u32x4 x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        x[j] = __builtin_amdgcn_perm(now.v[2 * j + 1].w[i / 2], now.v[2 * j].w[i / 2], sel);
+#pragma unroll
+                    for (int n = Q::PIECES - 1; n >= 0; --n)
+                        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), w[n], o[i], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < VW; ++i)
+                        o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.v[j].w[i]), p[j], o[i], 0, 0, 0);
+            }
+            now = next;
+        }
+        // The four waves' parts, joined: o[i][r] is column (4 g + r) VW + i of head `col`.
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0) {
+            stat[wave][col][0] = m;
+            stat[wave][col][1] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < VW; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) part[wave][col][(4 * g + r) * VW + i] = o[i][r];
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == tiles;
+        const int64_t slot = unit * (a.workers + a.nseq) + worker + s;
+        for (int e = threadIdx.x; e < heads * DP; e += 256) {
+            const int hd = e / DP, d = e % DP;
+            float M = kNegInf;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, stat[w][hd][0]);
+            float sum = 0.0f, x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {   // a wave without keys has m = -inf, l = 0 and zeros
+                const float f = stat[w][hd][0] == M ? 1.0f : exp2_hw((stat[w][hd][0] - M) * a.scale2);
+                sum = __builtin_fmaf(stat[w][hd][1], f, sum);
+                x = __builtin_fmaf(part[w][hd][d], f, x);
+            }
+            if (d >= a.c.D) continue;
+            if (whole) {
+                static_cast<IN*>(a.out)[s * a.ldo + int64_t(h0 + hd) * a.c.D + d] = IN(sum == 0.0f ? 0.0f : x / sum);
+            } else {
+                a.part[(slot * a.heads + hd) * a.c.D + d] = x;
+                if (d == 0) {
+                    a.stat[(slot * a.heads + hd) * 2] = M;
+                    a.stat[(slot * a.heads + hd) * 2 + 1] = sum;
+                }
+            }
+        }
+        at = base + t1;
+        if (at >= end) break;
+        __syncthreads();
+        base += tiles;
+        do ++s;
+        while (length_of(a, s) == 0);
+    }
+}
+
+// Joins the parts of the sequences that several workers share: one workgroup a (sequence, query head).
+template <typename IN, int KEYS>
+__global__ void __launch_bounds__(256) attn_paged_join_kernel(DecodeArgs a) {
+    const int64_t s = blockIdx.x / a.H;
+    const int head = blockIdx.x % a.H, kvh = head / a.G, of = head % a.G;
+    const int unit = kvh * a.parts + of / kHeads, hd = of % kHeads;
+    const int64_t tiles = (length_of(a, s) + KEYS - 1) / KEYS;
+    if (tiles == 0) return;
+    const int64_t total = tiles_before<KEYS>(a, a.nseq), per = (total + a.workers - 1) / a.workers;
+    const int64_t base = tiles_before<KEYS>(a, s), w0 = base / per, w1 = (base + tiles - 1) / per;
+    if (w0 == w1) return;
+    const int64_t slot0 = unit * (a.workers + a.nseq) + s;
+    float M = kNegInf;
+    for (int64_t w = w0 + (threadIdx.x & 63); w <= w1; w += 64) M = fmaxf(M, a.stat[((slot0 + w) * a.heads + hd) * 2]);
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+    for (int d = threadIdx.x; d < a.c.D; d += 256) {
+        float sum = 0.0f, x = 0.0f;
+        for (int64_t w = w0; w <= w1; ++w) {
+            const int64_t at = (slot0 + w) * a.heads + hd;
+            const float m = a.stat[at * 2], f = m == M ? 1.0f : exp2_hw((m - M) * a.scale2);
+            sum = __builtin_fmaf(a.stat[at * 2 + 1], f, sum);
+            x = __builtin_fmaf(a.part[at * a.c.D + d], f, x);
+        }
+        static_cast<IN*>(a.out)[s * a.ldo + int64_t(head) * a.c.D + d] = IN(sum == 0.0f ? 0.0f : x / sum);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------
+
+int check_cache(dgm_gpu* g, const char* name, const dgm_cache_cfg* c, int64_t type, int64_t nseq) {
+    if (!c) return dgm::fail(g, DGM_ERR_ARG, "%s: null configuration", name);
+    if (!type_bytes(c->type) || !type_bytes(type))
+        return dgm::fail(g, DGM_ERR_ARG, "%s: unknown type %d or %lld", name, c->type, (long long)type);
+    if (nseq < 0 || c->KVH < 1 || c->D < 1 || c->pageSize < 1 || c->numPages < 0 || c->maxPages < 0)
+        return dgm::fail(g, DGM_ERR_ARG, "%s: bad sizes", name);
+    if (c->D % 8 != 0 || c->D > 256)
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: head dim %d is not a multiple of 8 up to 256", name, c->D);
+    if (c->numPages > INT_MAX || c->maxPages > INT_MAX || nseq > 65536 ||
+        c->numPages > INT_MAX / (int64_t(c->KVH) * c->pageSize))
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: more than 2^31 cache rows, or too many sequences", name);
+    return DGM_OK;
+}
+
+Cache cache_of(dgm_gpu* g, const dgm_cache_cfg* c, const int32_t* pages) {
+    const int64_t most = INT_MAX - 1024;   // tiles past the end keep within 32 bits
+    const int64_t cap = c->maxPages * c->pageSize;
+    return Cache{pages, g->seq_flag, c->numPages, c->maxPages, c->KVH, c->D, int(cap < most ? cap : most),
+                 Div(uint32_t(c->pageSize))};
+}
+
+// Workgroups of a key head's unit that share the tiles, and units of a key head.
+struct Split {
+    int parts, units, workers, heads;
+};
+Split split_of(const dgm_cache_cfg* c, int64_t H) {
+    const int G = int(H / c->KVH), parts = (G + kHeads - 1) / kHeads, units = c->KVH * parts;
+    return {parts, units, units < kWorkers ? kWorkers / units : 1, G < kHeads ? G : kHeads};
+}
+int64_t part_floats(const dgm_cache_cfg* c, int64_t nseq, int64_t H) {
+    const Split s = split_of(c, H);
+    return int64_t(s.units) * (s.workers + nseq) * s.heads;
+}
+int64_t decode_ws_bytes(const dgm_cache_cfg* c, int64_t nseq, int64_t H) {
+    return part_floats(c, nseq, H) * (c->D + 2) * int64_t(sizeof(float));
+}
+
+template <typename IN, typename CT>
+int run_decode(dgm_gpu* g, const DecodeArgs& a) {
+    const dim3 grid(unsigned(a.units) * unsigned(a.workers)), block(256);
+    if (a.c.D <= 32) attn_paged_decode_kernel<IN, CT, 32><<<grid, block, 0, g->stream>>>(a);
+    else if (a.c.D <= 64) attn_paged_decode_kernel<IN, CT, 64><<<grid, block, 0, g->stream>>>(a);
+    else if (a.c.D <= 128) attn_paged_decode_kernel<IN, CT, 128><<<grid, block, 0, g->stream>>>(a);
+    else attn_paged_decode_kernel<IN, CT, 256><<<grid, block, 0, g->stream>>>(a);
+    DGM_LAUNCH_CHECK(g, "attn_paged_decode");
+    attn_paged_join_kernel<IN, kTileKeys<CT>><<<dim3(unsigned(a.nseq * a.H)), block, 0, g->stream>>>(a);
+    DGM_LAUNCH_CHECK(g, "attn_paged_join");
+    return DGM_OK;
+}
+
+template <typename IN, typename CT>
+int run_write(dgm_gpu* g, const WriteArgs& a) {
+    const int64_t blocks = (a.rows * (a.c.KVH * a.c.D / 8) + 255) / 256;
+    if (blocks * 256 > int64_t(UINT32_MAX))
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "cacheWrite: %lld rows exceed one launch", (long long)a.rows);
+    cache_write_kernel<IN, CT><<<dim3(unsigned(blocks)), dim3(256), 0, g->stream>>>(a);
+    DGM_LAUNCH_CHECK(g, "cache_write");
+    return DGM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dgm_cacheWrite(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, const void* k, const void* v,
+                   const int32_t* starts, const int32_t* lens, const int32_t* pages, void* kcache, void* vcache,
+                   int64_t rows, int64_t nseq, int64_t ldk, int64_t ldv) {
+    int rc = dgm::enter(g, "cache_write");
+    if (rc) return rc;
+    rc = check_cache(g, "cacheWrite", cfg, type, nseq);
+    if (rc) return rc;
+    if (rows < 0) return dgm::fail(g, DGM_ERR_ARG, "cacheWrite: rows=%lld", (long long)rows);
+    if (!starts && rows != nseq)
+        return dgm::fail(g, DGM_ERR_SHAPE, "cacheWrite: %lld rows of %lld sequences without starts", (long long)rows,
+                         (long long)nseq);
+    const int64_t width = int64_t(cfg->KVH) * cfg->D;
+    if (!ldk) ldk = width;
+    if (!ldv) ldv = width;
+    if (ldk < width || ldv < width)
+        return dgm::fail(g, DGM_ERR_SHAPE, "cacheWrite: a row stride is shorter than the row's heads");
+    if ((ldk | ldv) % 8 != 0 || ldk > (int64_t(1) << 31) || ldv > (int64_t(1) << 31) || rows > (int64_t(1) << 30) ||
+        width > (int64_t(1) << 24))
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "cacheWrite: strides must be multiples of 8 elements up to 2^31, "
+                                                 "rows up to 2^30");
+    if (rows == 0 || nseq == 0) return DGM_OK;
+    if (!k || !v || !pages || !kcache || !vcache) return dgm::fail(g, DGM_ERR_ARG, "cacheWrite: null buffer");
+    if (!dgm::aligned(k, 16) || !dgm::aligned(v, 16) || !dgm::aligned(kcache, 16) || !dgm::aligned(vcache, 16) ||
+        !dgm::aligned(pages, 4) || !dgm::aligned(lens, 4) || !dgm::aligned(starts, 4))
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "cacheWrite: a buffer is not 16-byte (starts, lens, pages: 4-byte) aligned");
+    OnDevice on(g->device);
+    if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "cacheWrite: %s", hipGetErrorString(on.err));
+    const WriteArgs a{cache_of(g, cfg, pages), k, v, kcache, vcache, starts, lens, rows, nseq, ldk, ldv};
+    g->seq_checks = true;
+    if (type == DGM_TYPE_F32)
+        return cfg->type == DGM_TYPE_F32 ? run_write<float, float>(g, a) : run_write<float, __bf16>(g, a);
+    return cfg->type == DGM_TYPE_F32 ? run_write<__bf16, float>(g, a) : run_write<__bf16, __bf16>(g, a);
+}
+
+int64_t dgm_attnPagedDecode_ws_bytes(const dgm_cache_cfg* cfg, int64_t nseq, int64_t H) {
+    if (!cfg || cfg->KVH < 1 || cfg->D < 1 || cfg->D > 256 || H < 1 || H > 65536 || nseq < 0 || nseq > 65536 ||
+        H % cfg->KVH != 0)
+        return -1;
+    return decode_ws_bytes(cfg, nseq, H);
+}
+
+int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, const void* q, const void* kcache,
+                        const void* vcache, const int32_t* pages, const int32_t* lens, void* out, void* ws,
+                        int64_t ws_bytes, int64_t nseq, int64_t H, int64_t ldq, int64_t ldo, float scale) {
+    int rc = dgm::enter(g, "attn_paged_decode");
+    if (rc) return rc;
+    rc = check_cache(g, "attnPagedDecode", cfg, type, nseq);
+    if (rc) return rc;
+    if (H < 1) return dgm::fail(g, DGM_ERR_ARG, "attnPagedDecode: H=%lld", (long long)H);
+    if (!(scale > 0.0f) || !std::isfinite(scale * kLog2e))
+        return dgm::fail(g, DGM_ERR_ARG, "attnPagedDecode: scale must be positive and finite");
+    if (H % cfg->KVH != 0)
+        return dgm::fail(g, DGM_ERR_SHAPE, "attnPagedDecode: %lld query heads over %d key heads", (long long)H, cfg->KVH);
+    const int64_t width = H * cfg->D;
+    if (!ldq) ldq = width;
+    if (!ldo) ldo = width;
+    if (ldq < width || ldo < width)
+        return dgm::fail(g, DGM_ERR_SHAPE, "attnPagedDecode: a row stride is shorter than the row's heads");
+    if (H > 65536 || (ldq | ldo) % 8 != 0 || ldq > (int64_t(1) << 31) || ldo > (int64_t(1) << 31) ||
+        nseq * H > int64_t(UINT32_MAX) / 256)
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "attnPagedDecode: strides must be multiples of 8 elements up to 2^31, "
+                                                 "sequences x heads below 2^24");
+    if (nseq == 0) return DGM_OK;
+    if (!q || !kcache || !vcache || !pages || !lens || !out || !ws)
+        return dgm::fail(g, DGM_ERR_ARG, "attnPagedDecode: null buffer");
+    if (ws_bytes < decode_ws_bytes(cfg, nseq, H))
+        return dgm::fail(g, DGM_ERR_ARG, "attnPagedDecode: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
+                         (long long)decode_ws_bytes(cfg, nseq, H));
+    for (const void* p : {q, kcache, vcache, static_cast<const void*>(out), static_cast<const void*>(ws)})
+        if (!dgm::aligned(p, 16)) return dgm::fail(g, DGM_ERR_UNSUPPORTED, "attnPagedDecode: a buffer is not 16-byte aligned");
+    if (!dgm::aligned(pages, 4) || !dgm::aligned(lens, 4))
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "attnPagedDecode: pages or lens is not 4-byte aligned");
+    OnDevice on(g->device);
+    if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "attnPagedDecode: %s", hipGetErrorString(on.err));
+    const Split sp = split_of(cfg, H);
+    float* part = static_cast<float*>(ws);
+    const DecodeArgs a{cache_of(g, cfg, pages), q, kcache, vcache, out, part, part + part_floats(cfg, nseq, H) * cfg->D,
+                       lens, nseq, ldq, ldo, int(H), int(H / cfg->KVH), sp.heads, sp.parts, sp.workers, sp.units,
+                       scale * kLog2e};
+    g->seq_checks = true;
+    if (type == DGM_TYPE_F32)
+        return cfg->type == DGM_TYPE_F32 ? run_decode<float, float>(g, a) : run_decode<float, __bf16>(g, a);
+    return cfg->type == DGM_TYPE_F32 ? run_decode<__bf16, float>(g, a) : run_decode<__bf16, __bf16>(g, a);
+}
+
+}  // extern "C"

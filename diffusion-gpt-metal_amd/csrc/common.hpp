@@ -62,6 +62,10 @@ struct dgm_gpu {
     bool lending = false;
     uint8_t* lent = nullptr;
     size_t lent_bytes = 0;
+    // The device's flag of bad sequence starts and pages (set by the attention and
+    // cache kernels), and whether such a kernel ran since the last dgm_end.
+    uint32_t* seq_flag = nullptr;
+    bool seq_checks = false;
 };
 
 namespace dgm {

@@ -5,6 +5,7 @@
 #include <mutex>
 #include <new>
 
+#include "attn.hpp"
 #include "common.hpp"
 
 namespace {
@@ -13,6 +14,10 @@ namespace {
 // device holds its own copy from library load to process end. Host code uses
 // only the per-device address from hipGetSymbolAddress, never this name.
 __device__ __align__(256) uint8_t scratch[dgm::kScratchBytes];
+
+// What the attention and cache kernels found wrong in sequence starts, lengths and
+// page tables (which only the device reads): bits of attn.hpp. One per device, read and cleared by dgm_end.
+__device__ uint32_t sequence_flag;
 
 constexpr int kMaxDevices = 64;
 std::mutex scratch_mu;
@@ -189,6 +194,29 @@ uint8_t* planes_buffer(dgm_gpu* g, size_t bytes) {
     return static_cast<uint8_t*>(g->planes);
 }
 
+// After a synchronize: records an error if such a kernel set the flag, and clears it.
+void sequence_check(dgm_gpu* g) {
+    g->seq_checks = false;
+    dgm_attn::OnDevice on(g->device);
+    uint32_t flag = 0;
+    const uint32_t zero = 0;
+    hipError_t e = on.err;
+    // On the context's stream: the null stream would disturb a capture elsewhere.
+    if (e == hipSuccess) e = hipMemcpyAsync(&flag, g->seq_flag, sizeof(flag), hipMemcpyDeviceToHost, g->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(g->stream);
+    if (e == hipSuccess && flag) {
+        e = hipMemcpyAsync(g->seq_flag, &zero, sizeof(zero), hipMemcpyHostToDevice, g->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(g->stream);
+    }
+    if (e != hipSuccess)
+        fail(g, DGM_ERR_HIP, "the sequence flag could not be read: %s", hipGetErrorString(e));
+    else if (flag & dgm_attn::kBadStarts)
+        fail(g, DGM_ERR_SHAPE, "sequence starts are out of order or beyond the rows: results are not valid");
+    else if (flag)
+        fail(g, DGM_ERR_SHAPE, "a sequence is longer than its page table, or names a page that the cache does not have: "
+                               "those rows were left out");
+}
+
 int ws_error(dgm_gpu* g) { return g->first_err != DGM_OK ? g->first_err : DGM_ERR_HIP; }
 
 }  // namespace dgm
@@ -208,6 +236,11 @@ int dgm_gpu_create(dgm_gpu** out) {
     // per device; a failure surfaces only when that entry point is called).
     hipError_t se;
     g->scratch = scratch_for(g->device, &se);
+    if (hipGetSymbolAddress(reinterpret_cast<void**>(&g->seq_flag), HIP_SYMBOL(sequence_flag)) != hipSuccess) {
+        (void)hipGetLastError();
+        delete g;
+        return DGM_ERR_HIP;
+    }
     // A blocking stream: it orders itself after work on the null stream, where
     // callers that allocate with torch or hipMemset may still be filling the
     // buffers they hand over.
@@ -280,8 +313,10 @@ int dgm_end(dgm_gpu* g) {
     if (e == hipSuccess) e = hipGetLastError();
     if (e != hipSuccess)
         dgm::fail(g, DGM_ERR_HIP, "HIP error after %s: %s", g->last_kernel, hipGetErrorString(e));
-    else if (g->spin_waits)
-        dgm::decode_wait_check(g);
+    else {
+        if (g->spin_waits) dgm::decode_wait_check(g);
+        if (g->seq_checks) dgm::sequence_check(g);
+    }
     return g->first_err;
 }
 

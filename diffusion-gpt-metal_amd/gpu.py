@@ -14,7 +14,7 @@ from __future__ import annotations
 import ctypes
 from typing import Any, Optional
 
-from .abi import (DGM_MATH_BF16, DGM_MATH_FP32, AdamP, BiasP, DgmError, DiTCfg,
+from .abi import (DGM_MATH_BF16, DGM_MATH_FP32, AdamP, AttnCfg, BiasP, CacheCfg, DgmError, DiTCfg,
                   DiTGrads, DiTWeights, EmbBwdP, EmbP, GemmP, PosP, QuantP, ReduceP, ScaleP,
                   UnaryP, load_library)
 
@@ -235,6 +235,40 @@ class GPU:
     def dit_forward(self, cfg: DiTCfg, w: DiTWeights, cos, sin, x, ws, ws_floats: int) -> None:
         self._check(self.lib.dgm_dit_forward(self.h, ctypes.byref(cfg), ctypes.byref(w), _ptr(cos), _ptr(sin),
                                              _ptr(x), _ptr(ws), ws_floats))
+
+    # -- attention over packed sequences and over a paged cache ---------------
+    def attnPackedFwd(self, cfg: AttnCfg, q, k, v, starts, out, lse=None) -> None:
+        """Attention of sequences back to back, starts int32 [nseq + 1] on the
+        device; lse [H, rows] for a backward."""
+        self._check(self.lib.dgm_attnPackedFwd(self.h, ctypes.byref(cfg), _ptr(q), _ptr(k), _ptr(v), _ptr(starts),
+                                               _ptr(out), _ptr(lse)))
+
+    def attnPackedBwd_ws_bytes(self, cfg: AttnCfg) -> int:
+        return int(self.lib.dgm_attnPackedBwd_ws_bytes(ctypes.byref(cfg)))
+
+    def attnPackedBwd(self, cfg: AttnCfg, q, k, v, starts, out, lse, dout, dq, dk, dv, ws, ws_bytes: int) -> None:
+        """The gradients of attnPackedFwd from its out and lse (overwritten)."""
+        self._check(self.lib.dgm_attnPackedBwd(self.h, ctypes.byref(cfg), _ptr(q), _ptr(k), _ptr(v), _ptr(starts),
+                                               _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv),
+                                               _ptr(ws), ws_bytes))
+
+    def cacheWrite(self, cfg: CacheCfg, type: int, k, v, starts, lens, pages, kcache, vcache, rows: int, nseq: int,
+                   ldk: int = 0, ldv: int = 0) -> None:
+        """Rows of k and v into the pages of a cache: row r of sequence s
+        becomes position lens[s] + r - starts[s]."""
+        self._check(self.lib.dgm_cacheWrite(self.h, ctypes.byref(cfg), type, _ptr(k), _ptr(v), _ptr(starts),
+                                            _ptr(lens), _ptr(pages), _ptr(kcache), _ptr(vcache), rows, nseq, ldk, ldv))
+
+    def attnPagedDecode_ws_bytes(self, cfg: CacheCfg, nseq: int, H: int) -> int:
+        return int(self.lib.dgm_attnPagedDecode_ws_bytes(ctypes.byref(cfg), nseq, H))
+
+    def attnPagedDecode(self, cfg: CacheCfg, type: int, q, kcache, vcache, pages, lens, out, ws, ws_bytes: int,
+                        nseq: int, H: int, ldq: int = 0, ldo: int = 0, scale: Optional[float] = None) -> None:
+        """Attention of one new token per sequence over lens[s] cached positions;
+        scale defaults to 1 / sqrt(D)."""
+        self._check(self.lib.dgm_attnPagedDecode(self.h, ctypes.byref(cfg), type, _ptr(q), _ptr(kcache), _ptr(vcache),
+                                                 _ptr(pages), _ptr(lens), _ptr(out), _ptr(ws), ws_bytes, nseq, H, ldq,
+                                                 ldo, cfg.D ** -0.5 if scale is None else scale))
 
     # -- training step (src/GPU.swift:200-210, 274-277, 324-350, 420-429) -----
     def adam(self, w, g, m, v, n: int, lr: float, b1: float, b2: float, eps: float, wd: float,

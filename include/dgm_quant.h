@@ -471,6 +471,92 @@ int dgm_bias_grad(dgm_gpu* g, const float* dY, float* db, const dgm_BiasP* p);
 /* GPU.biasGrad (src/GPU.swift:274-277). */
 int dgm_biasGrad(dgm_gpu* g, const float* dy, float* db, int64_t M, int64_t N);
 
+/* ---- attention over packed sequences, and over a paged cache ----------------
+ * No counterpart in the reference, whose attention (dgm_attnFwd, dgm_attnBwd)
+ * takes equal lengths and heads and writes out [B,H,T,T] scores. Here
+ * sequences of any lengths lie back to back, H query heads share KVH key and value
+ * heads (query head h reads key head h / (H / KVH)), no score reaches memory, and
+ * keys and values of past tokens can be kept in pages.
+ *
+ * Types: DGM_TYPE_F32 or DGM_TYPE_BF16. Scores, softmax statistics and sums
+ * are fp32 for both; for bf16 the probabilities (and in the backward their
+ * gradients) are rounded to bf16 between the two products. dgm_set_math does not
+ * change these calls.
+ *
+ * Sequence starts, lengths and page tables are read on the device only, so that
+ * captured graphs can be replayed with other ones. Where they are wrong (starts out of
+ * order or beyond the rows, a page that the cache does not have, a length beyond
+ * the page table) nothing outside the buffers is touched, and the next
+ * dgm_end of a context on the device returns DGM_ERR_SHAPE.
+ *
+ * Buffers 16-byte aligned (starts, lengths, pages, lse: 4), row strides
+ * multiples of 8 elements and at least the row's heads, 0 for rows back to back;
+ * D a multiple of 8 up to 256 (DGM_ERR_UNSUPPORTED otherwise). Outputs must
+ * not overlap inputs or one another, except that strided rows may interleave
+ * (q, k, v of one fused projection, dq, dk, dv of its gradient). Nothing is allocated, and
+ * every call can be captured. Results are the same bits every time. */
+#define DGM_TYPE_F32  0
+#define DGM_TYPE_BF16 1
+
+typedef struct dgm_attn_cfg {
+    int32_t type;                  /* DGM_TYPE_* of q, k, v, out and gradients  */
+    int32_t H, KVH, D;             /* H % KVH == 0                              */
+    int32_t causal;                /* query i of a sequence sees keys 0 .. i    */
+    float scale;                   /* of the scores, > 0 (1 / sqrt(D))          */
+    int64_t rows, nseq;
+    int64_t ldq, ldk, ldv, ldo;    /* row strides in elements; dq, dk, dv have
+                                      those of q, k, v, and dout that of out    */
+} dgm_attn_cfg;
+
+/* out[r, h, :] = softmax(scale * q[r, h] . k[j, h']) v[j, h'] over the keys j of
+ * row r's sequence (up to r when causal). starts: int32 [nseq + 1], sequence s
+ * is rows starts[s] .. starts[s + 1] - 1 (none when they are equal); rows before the first
+ * and behind the last sequence are left as they were. lse (may be NULL; the
+ * backward reads it): float [H, rows], the base-2 logarithm of the row's sum
+ * of 2^(score * log2 e). A masked position takes no part whatever its
+ * values; an infinity or NaN elsewhere makes what it enters infinite or NaN. */
+int dgm_attnPackedFwd(dgm_gpu* g, const dgm_attn_cfg* cfg, const void* q, const void* k, const void* v,
+                      const int32_t* starts, void* out, float* lse);
+/* The gradients of dgm_attnPackedFwd from its out and lse and from dout = dL/dout:
+ * dq [rows, H, D], dk and dv [rows, KVH, D] (summed over the query heads of a key
+ * head), overwritten where a sequence has rows. D up to 128. ws: device memory
+ * of at least dgm_attnPackedBwd_ws_bytes(cfg) bytes (-1 for sizes that are
+ * refused), 16-byte aligned; calls that overlap in time need one each. */
+int64_t dgm_attnPackedBwd_ws_bytes(const dgm_attn_cfg* cfg);
+int dgm_attnPackedBwd(dgm_gpu* g, const dgm_attn_cfg* cfg, const void* q, const void* k, const void* v,
+                      const int32_t* starts, const void* out, const float* lse, const void* dout, void* dq,
+                      void* dk, void* dv, void* ws, int64_t ws_bytes);
+
+/* A cache of keys and one of values, each [numPages, KVH, pageSize, D]. Sequence
+ * s keeps position p at slot p % pageSize of page pages[s * maxPages + p / pageSize]
+ * (int32; entries that no position needs are not read). */
+typedef struct dgm_cache_cfg {
+    int32_t type;                  /* DGM_TYPE_* of the caches                  */
+    int32_t KVH, D, pageSize;
+    int64_t numPages, maxPages;    /* pages of the cache; columns of the table  */
+} dgm_cache_cfg;
+
+/* Writes rows of k and v [rows, KVH, D] of type `type` into the caches (rounded
+ * to the nearest, ties to even, where those are bf16): row r of sequence s
+ * becomes position lens[s] + r - starts[s]. lens (int32 [nseq], tokens that s
+ * had before) may be NULL for all 0; starts as above, or NULL for one row per
+ * sequence (rows == nseq). Rows whose position the table does not hold are left
+ * out (and reported by dgm_end). Two rows of one slot: either may stay. */
+int dgm_cacheWrite(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, const void* k, const void* v,
+                   const int32_t* starts, const int32_t* lens, const int32_t* pages, void* kcache, void* vcache,
+                   int64_t rows, int64_t nseq, int64_t ldk, int64_t ldv);
+/* One new token per sequence over its cache: out[s, h, :] = softmax(scale *
+ * q[s, h] . k_j) v_j over positions j < lens[s] (the new token's own, already
+ * written, among them); zeros where none is left. q, out [nseq, H, D] of type
+ * `type`. Positions that the table does not hold are left out (and
+ * reported by dgm_end). ws: device memory of at least
+ * dgm_attnPagedDecode_ws_bytes bytes (-1 for sizes that are refused), 16-byte
+ * aligned; calls that overlap in time need one each. */
+int64_t dgm_attnPagedDecode_ws_bytes(const dgm_cache_cfg* cfg, int64_t nseq, int64_t H);
+int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, const void* q, const void* kcache,
+                        const void* vcache, const int32_t* pages, const int32_t* lens, void* out, void* ws,
+                        int64_t ws_bytes, int64_t nseq, int64_t H, int64_t ldq, int64_t ldo, float scale);
+
 /* ---- checkpoints (host code, no context) ----------------------------------
  * The reference's checkpoint files: a little-endian header, then every
  * parameter's fp32 master in the model's creation order. These validate a
