@@ -15,11 +15,11 @@
 //    2^-9 of each weight, and the roundings of a row's weights are independent, so a
 //    row's error stays below that of rounding the row's output once); fp32 runs on
 //    v_mfma_f32_32x32x2_f32. Scores, statistics and accumulators are fp32.
-//  * Tiles of 64 keys are read once per workgroup, 16 bytes a lane, into
-//    registers while the previous tile is computed on, and stored to one of two LDS
-//    buffers: row-major (A operand of S^T) and for bf16 also transposed (A operand
-//    of the second product; 4 x 8 blocks are transposed in registers). 16-byte
-//    chunks are XOR-swizzled so that both reads are free of bank conflicts.
+//  * Tiles of 64 keys go from memory straight into one of two LDS buffers while
+//    the other is computed on (one barrier a tile, no registers on the way).
+//    They stay row-major: the A operand of the second product is read transposed
+//    (ds_read_b64_tr_b16; for fp32, whose A operand is one element a lane, plainly).
+//    16-byte chunks are XOR-swizzled so that both reads are free of bank conflicts.
 //  * Rows are found on the device: sequence s owns the tile slots from
 //    starts[s] / rows-per-tile + s on, which never overlap, so the grid needs no host
 //    copy of the lengths, and a captured graph may be replayed with other lengths.
@@ -28,16 +28,19 @@
 //    times in a row instead of at every tile.
 //  * A masked position takes no part even if its v (or in the backward its k, q
 //    or dout) is infinite or NaN, where 0 * inf would spread it over a whole
-//    tile: tiles that hold both masked positions and such values take a slower
-//    product that counts them apart.
+//    tile: tiles that hold both masked positions and such values are cleaned of them
+//    first, and the sums that they belong to spoilt afterwards.
 //
-// The backward recomputes P from lse. One kernel owns 32 queries per wave and
+// The backward recomputes P from lse; for bf16, dS enters its products as two
+// bf16 pieces (rounded once, as P is, dq and dk were 1.5 times as far off as one
+// rounding of the result). One kernel owns 32 queries per wave and
 // accumulates dq; another owns 32 keys per wave and accumulates dk and dv over all
 // query heads of the key head's group, so no gradient is added to by two
 // workgroups: no atomics, the same bits every time.
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "attn.hpp"
 
@@ -47,91 +50,87 @@ using namespace dgm_attn;
 
 constexpr int kTile = 64;   // rows of a staged tile
 
-// ---- LDS layouts ---------------------------------------------------------------
+// ---- tiles in LDS ----------------------------------------------------------------
 
+// 64 rows of D elements, row-major, padded to DP columns. The 16-byte chunk c of
+// row r sits at slot c ^ swizzle(r): 16 rows' chunk c (the A operand of mm_rows) and 8
+// rows' four chunks (its transposed reads in mm_cols) then lie in different banks.
 template <typename T, int DP>
 struct Lds {
     static constexpr int EB = sizeof(T), EPC = 16 / EB;       // bytes of an element, elements of a chunk
     static constexpr int RB = DP * EB, CPR = RB / 16;         // bytes and chunks of a row
     static constexpr int RPB = RB >= 256 ? 1 : 256 / RB;      // rows that span all banks
-    static constexpr int SW = CPR < 16 ? CPR : 16;
-    static constexpr int ROWS = kTile * RB;                   // bytes of a row-major tile
-    static constexpr bool TR = EB == 2;                       // a transposed copy is kept
-    static constexpr int COLS = TR ? DP * kTile * EB : 0;     // its bytes
-    static __device__ __forceinline__ int row_off(int row, int chunk) {
-        return row * RB + ((chunk ^ ((row / RPB) & (SW - 1))) << 4);
-    }
-    // Transposed: row d holds 64 keys in 8 chunks, in the order of mm_cols.
-    static __device__ __forceinline__ int col_off(int d, int chunk) {
-        return d * (kTile * EB) + ((chunk ^ (((d >> 1) ^ (d >> 3)) & 7)) << 4);
-    }
+    static constexpr int BYTES = kTile * RB;
+    static __device__ __forceinline__ int swizzle(int row) { return (row & 3) / RPB << 2 | (row >> 2 & 3); }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
 };
 
-// ---- staging -------------------------------------------------------------------
+__device__ __forceinline__ bool nonfinite(u32x4 v, bool half) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (half) bad |= ((v[w] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        else bad |= ((v[w] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+    }
+    return bad != 0;
+}
 
-// A thread's part of a tile: blocks of 4 rows x one chunk.
+// A workgroup's copies of tiles from memory straight into LDS: a wave's
+// instruction fills 1 KB in lane order, so that each lane fetches the chunk that belongs in
+// its slot. The copies are waited for by tile_ready.
 template <typename T, int DP, int NT>
-struct Stage {
+struct Copy {
     using L = Lds<T, DP>;
-    static constexpr int BLOCKS = kTile / 4 * L::CPR, NB = (BLOCKS + NT - 1) / NT;
-    u32x4 r[NB][4];
+    static constexpr int N = L::BYTES / 16 / NT, STEP = NT / L::CPR;   // chunks of a thread, rows between them
+    static_assert(L::BYTES % (16 * NT) == 0 && NT % L::CPR == 0, "every thread copies whole chunks of one slot");
+    int64_t ldb;        // bytes from row to row
+    int row, slot, wave;
 
-    // Rows row0 .. row0+63 of `base` (element pointer of row 0's head) that are
-    // below `limit`; the rest, and columns from D on, are zero.
-    __device__ __forceinline__ void load(const T* base, int64_t ld, int row0, int limit, int D) {
+    __device__ __forceinline__ explicit Copy(int64_t ld)
+        : ldb(ld * L::EB), row(int(threadIdx.x) / L::CPR), slot(int(threadIdx.x) % L::CPR),
+          wave(__builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6)) {}
+
+    // `rows` rows from `from` on (the first `D` columns); the rest of the tile is zero.
+    __device__ __forceinline__ void start(uint8_t* lds, const T* from, int rows, int D) const {
+        const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>(lds)) + uint32_t(wave) * 1024u;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(from);
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+        if (rows >= kTile && D == DP) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int b = int(threadIdx.x) + n * NT, c = b % L::CPR, rg = b / L::CPR;
-            const bool in = (BLOCKS % NT == 0 || b < BLOCKS) && c * L::EPC < D;
+            for (int i = 0; i < N; ++i) {
+                const uint32_t off = uint32_t(row) * uint32_t(ldb) + uint32_t((slot ^ L::swizzle(row + i * STEP)) << 4);
+                asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(base + i * NT * 16), "v"(off),
+                             "s"(src + i * STEP * ldb)
+                             : "memory", "m0");
+            }
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = row0 + 4 * rg + i;
-                r[n][i] = u32x4{0, 0, 0, 0};
-                if (in && row < limit) r[n][i] = *reinterpret_cast<const u32x4*>(base + int64_t(row) * ld + c * L::EPC);
+            for (int i = 0; i < N; ++i) {
+                const int r = row + i * STEP, c = slot ^ L::swizzle(r);
+                if (r < rows && c * L::EPC < D)
+                    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base + i * NT * 16),
+                                 "v"(src + r * ldb + c * 16)
+                                 : "memory", "m0");
+                else
+                    *reinterpret_cast<u32x4*>(lds + (i * NT + int(threadIdx.x)) * 16) = u32x4{0, 0, 0, 0};
             }
         }
+#pragma clang diagnostic pop
     }
-    // Whether any element is an infinity or a NaN.
-    __device__ __forceinline__ bool nonfinite() const {
-        uint32_t bad = 0;
+    // Whether this thread's chunks of a tile hold infinities or NaN.
+    __device__ __forceinline__ bool bad(const uint8_t* lds) const {
+        bool b = false;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if constexpr (L::EB == 2) bad |= ((r[n][i][w] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                    else bad |= ((r[n][i][w] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
-                }
-        return bad != 0;
-    }
-    __device__ __forceinline__ void store_rows(uint8_t* lds) const {
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int b = int(threadIdx.x) + n * NT, c = b % L::CPR, rg = b / L::CPR;
-            if (BLOCKS % NT != 0 && b >= BLOCKS) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(lds + L::row_off(4 * rg + i, c)) = r[n][i];
-        }
-    }
-    // bf16 only. Rows 4rg .. 4rg+3 are half (rg >> 1) & 1 of the chunk that lanes of half rg & 1 read.
-    __device__ __forceinline__ void store_cols(uint8_t* lds) const {
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int b = int(threadIdx.x) + n * NT, c = b % L::CPR, rg = b / L::CPR;
-            if (BLOCKS % NT != 0 && b >= BLOCKS) continue;
-            const int chunk = 2 * (rg >> 2) + (rg & 1), half = ((rg >> 1) & 1) * 8;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const uint32_t a0 = r[n][0][w], a1 = r[n][1][w], a2 = r[n][2][w], a3 = r[n][3][w];
-                *reinterpret_cast<u32x2*>(lds + L::col_off(8 * c + 2 * w, chunk) + half) =
-                    u32x2{__builtin_amdgcn_perm(a1, a0, 0x05040100u), __builtin_amdgcn_perm(a3, a2, 0x05040100u)};
-                *reinterpret_cast<u32x2*>(lds + L::col_off(8 * c + 2 * w + 1, chunk) + half) =
-                    u32x2{__builtin_amdgcn_perm(a1, a0, 0x07060302u), __builtin_amdgcn_perm(a3, a2, 0x07060302u)};
-            }
-        }
+        for (int i = 0; i < N; ++i)
+            b = b || nonfinite(*reinterpret_cast<const u32x4*>(lds + (i * NT + int(threadIdx.x)) * 16), L::EB == 2);
+        return b;
     }
 };
+
+// Every copy that the workgroup has started is in LDS, and every wave's reads of what the
+// next copies overwrite are done.
+__device__ __forceinline__ void tile_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ---- products ------------------------------------------------------------------
 
@@ -174,7 +173,7 @@ __device__ __forceinline__ void mm_rows(f32x16 (&out)[2], const uint8_t* rows, c
     for (int kk = 0; kk < Frags<T, DP>::NK; ++kk)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
-            mfma_chunk<T>(out[kb], *reinterpret_cast<const u32x4*>(rows + L::row_off(32 * kb + r, 2 * kk + h)), b.f[kk]);
+            mfma_chunk<T>(out[kb], *reinterpret_cast<const u32x4*>(rows + L::at(32 * kb + r, 2 * kk + h)), b.f[kk]);
 }
 
 __device__ __forceinline__ bf16x8 pack8(const f32x16& p, int at) {
@@ -184,22 +183,45 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& p, int at) {
     return o;
 }
 
-// acc[dt] (32 columns d x the wave's 32 columns) += tile^T times p, p as mm_rows leaves it.
-template <typename T, int DP>
+// A operand of mm_cols for bf16: element j of a lane is column d = 32 dt + lane %
+// 32 of row 32 kb + 16 st + 8 (j / 4) + 4h + j % 4, the order in which mm_rows leaves
+// a lane's results. The transposed read takes, for each 16 lanes, 4 rows of 16
+// columns (4 lanes a row) and gives each lane one column of them.
+template <int DP>
+__device__ __forceinline__ bf16x8 read_cols(const uint8_t* tile, int kb, int st, int dt, int lane) {
+    using L = Lds<__bf16, DP>;
+    const int row = 32 * kb + 16 * st + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int chunk = 4 * dt + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), in = (lane & 1) * 8;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* At;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)(tile + L::at(row, chunk) + in));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((At)(tile + L::at(row + 8, chunk) + in));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// acc[dt] (32 columns d x the wave's 32 columns) += tile^T times p, p as mm_rows
+// leaves it; for bf16 in PIECES pieces of 8 bits.
+template <typename T, int DP, int PIECES = 1>
 __device__ __forceinline__ void mm_cols(f32x16 (&acc)[DP / 32], const uint8_t* tile, const f32x16 (&p)[2], int lane) {
     using L = Lds<T, DP>;
     const int h = lane >> 5, r = lane & 31;
-    if constexpr (L::TR) {
+    if constexpr (L::EB == 2) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const bf16x8 b = pack8(p[kb], 8 * st);
+                bf16x8 rest;
+                if constexpr (PIECES == 2) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) rest[j] = __bf16(p[kb][8 * st + j] - float(b[j]));
+                }
 #pragma unroll
                 for (int dt = 0; dt < DP / 32; ++dt) {
-                    const bf16x8 a =
-                        *reinterpret_cast<const bf16x8*>(tile + L::col_off(32 * dt + r, 4 * kb + 2 * st + h));
+                    const bf16x8 a = read_cols<DP>(tile, kb, st, dt, lane);
                     acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[dt], 0, 0, 0);
+                    if constexpr (PIECES == 2)
+                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, rest, acc[dt], 0, 0, 0);
                 }
             }
     } else {
@@ -211,62 +233,60 @@ __device__ __forceinline__ void mm_cols(f32x16 (&acc)[DP / 32], const uint8_t* t
 #pragma unroll
                 for (int dt = 0; dt < DP / 32; ++dt) {
                     const int d = 32 * dt + r;
-                    const float a = *reinterpret_cast<const float*>(tile + L::row_off(row, d >> 2) + (d & 3) * 4);
+                    const float a = *reinterpret_cast<const float*>(tile + L::at(row, d >> 2) + (d & 3) * 4);
                     acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[kb][e], acc[dt], 0, 0, 0);
                 }
             }
     }
 }
 
-// The same where the tile holds infinities or NaN and positions are masked (p
-// is 0 there): the finite elements as above, and beside them counts of the
-// +inf, -inf and NaN elements at positions that are not masked. `shown(kb, e)`:
-// whether the lane's element e of block kb is not masked. With kSigned the
-// weights are positive, so that infinities keep their sign; else every such element gives NaN.
-template <typename T, int DP, bool kSigned, typename Shown>
-__device__ __forceinline__ void mm_cols_apart(f32x16 (&acc)[DP / 32], const uint8_t* tile, const f32x16 (&p)[2],
-                                           const Shown& shown, int lane) {
+// What a tile's infinities and NaN do to sums that masked positions take no part in:
+// the tile is cleaned (they become 0, as the weights of masked positions are) and
+// for each column d the first (kLast: last) row that holds such a value is
+// kept; a query (key) that sees that row has its sum spoilt. Rare, so it may cost barriers.
+template <int DP, int KINDS>
+struct Marks {
+    int row[KINDS][DP];   // kinds: NaN, +inf, -inf; or all of them as one
+};
+
+template <typename T, int DP, int NT, int KINDS, bool kLast>
+__device__ __forceinline__ void clean_tile(const Copy<T, DP, NT>& c, uint8_t* lds, Marks<DP, KINDS>& marks) {
     using L = Lds<T, DP>;
-    const int h = lane >> 5, r = lane & 31;
+    for (int i = threadIdx.x; i < KINDS * DP; i += NT) marks.row[i / DP][i % DP] = kLast ? -1 : INT_MAX;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < Copy<T, DP, NT>::N; ++i) {
+        const int r = c.row + i * Copy<T, DP, NT>::STEP, d0 = (c.slot ^ L::swizzle(r)) * L::EPC;
+        T* at = reinterpret_cast<T*>(lds + (i * NT + int(threadIdx.x)) * 16);
+#pragma unroll 1
+        for (int j = 0; j < L::EPC; ++j) {
+            const float x = float(at[j]);
+            if (fabsf(x) < __builtin_huge_valf()) continue;
+            int* m = &marks.row[KINDS == 1 || x != x ? 0 : x > 0.0f ? 1 : 2][d0 + j];
+            if (kLast) atomicMax(m, r);
+            else atomicMin(m, r);
+            at[j] = T(0.0f);
+        }
+    }
+    __syncthreads();
+}
+
+// acc after mm_cols on a clean tile. `sees(row)`: whether the lane's column sees a row marked so.
+template <int DP, int KINDS, typename Sees>
+__device__ __forceinline__ void spoil(f32x16 (&acc)[DP / 32], const Marks<DP, KINDS>& marks, const Sees& sees, int lane) {
     const float inf = __builtin_huge_valf();
+    asm volatile("" : "+v"(lane));   // no addresses of this rare path kept through the loop
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {   // the finite elements; the +inf, -inf and NaN ones
-            f32x16 x = n == 0 ? acc[dt] : f32x16{};
-            const auto part = [n, inf](float v) {
-                const bool one = n == 1 ? v == inf : n == 2 ? v == -inf : v != v;
-                return n == 0 ? (fabsf(v) < inf ? v : 0.0f) : one ? 1.0f : 0.0f;
-            };
-            const auto weight = [&](int kb, int e) { return n == 0 ? p[kb][e] : shown(kb, e) ? 1.0f : 0.0f; };
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    if constexpr (L::TR) {
-                        const bf16x8 t =
-                            *reinterpret_cast<const bf16x8*>(tile + L::col_off(32 * dt + r, 4 * kb + 2 * st + h));
-                        bf16x8 a, b;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            a[j] = __bf16(part(float(t[j])));
-                            b[j] = __bf16(weight(kb, 8 * st + j));
-                        }
-                        x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, x, 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int e = 8 * st + j, row = 32 * kb + 8 * (e / 4) + 4 * h + e % 4, d = 32 * dt + r;
-                            const float t = *reinterpret_cast<const float*>(tile + L::row_off(row, d >> 2) + (d & 3) * 4);
-                            x = __builtin_amdgcn_mfma_f32_32x32x2f32(part(t), weight(kb, e), x, 0, 0, 0);
-                        }
-                    }
-                }
-            if (n == 0) acc[dt] = x;
-            else
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (x[e] > 0.0f) acc[dt][e] = kSigned && n < 3 ? acc[dt][e] + (n == 1 ? inf : -inf) : __builtin_nanf("");
+        for (int e = 0; e < 16; ++e) {
+            const int d = 32 * dt + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+            float x = acc[dt][e];
+            if constexpr (KINDS == 3) {
+                x += sees(marks.row[1][d]) ? inf : 0.0f;
+                x += sees(marks.row[2][d]) ? -inf : 0.0f;
+            }
+            acc[dt][e] = sees(marks.row[0][d]) ? __builtin_nanf("") : x;
         }
 }
 
@@ -311,11 +331,12 @@ struct FwdArgs {
 __device__ __forceinline__ int head_of(int i, int H, int KVH) { return (i % KVH) * (H / KVH) + i / KVH; }
 
 template <typename T, int DP, int QB, int NW, int NBUF>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 128 ? 2 : 1) attn_packed_fwd_kernel(FwdArgs a) {
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 128 && QB == 1 ? 2 : 1)
+    attn_packed_fwd_kernel(FwdArgs a) {
     using L = Lds<T, DP>;
     constexpr int NT = 64 * NW, BQ = 32 * QB * NW, DT = DP / 32;
-    constexpr int BUF = L::ROWS + (L::TR ? L::COLS : L::ROWS);
-    __shared__ __align__(16) uint8_t lds[NBUF][BUF];
+    __shared__ __align__(16) uint8_t lds[NBUF][2][L::BYTES];   // k and v
+    __shared__ Marks<DP, 3> marks;
     if (blockIdx.x == 0) check_starts(a.starts, a.nseq, a.rows, a.flag);
     Rows rw;
     // The last tiles of a causal sequence are the longest: they start first.
@@ -326,6 +347,13 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 128 ? 2 : 1) 
     const T* q = static_cast<const T*>(a.q) + int64_t(rw.first) * a.ldq + int64_t(head) * a.D;
     const T* k = static_cast<const T*>(a.k) + int64_t(rw.first) * a.ldk + int64_t(kvh) * a.D;
     const T* v = static_cast<const T*>(a.v) + int64_t(rw.first) * a.ldv + int64_t(kvh) * a.D;
+    const Copy<T, DP, NT> ck(a.ldk), cv(a.ldv);
+    const auto start = [&](int t) __attribute__((always_inline)) {
+        const int key0 = t * kTile;
+        ck.start(lds[t % NBUF][0], k + key0 * a.ldk, rw.len - key0, a.D);
+        cv.start(lds[t % NBUF][1], v + key0 * a.ldv, rw.len - key0, a.D);
+    };
+    start(0);
 
     Frags<T, DP> qf[QB];
     f32x16 o[QB][DT];
@@ -347,68 +375,64 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 128 ? 2 : 1) 
     const int masked_from = a.causal ? rw.tile * BQ / kTile : rw.len / kTile;
     const int wave_keys = a.causal ? min(keys, q0 + 32 * QB) : keys;
 
-    Stage<T, DP, NT> sk, sv;
-    sk.load(k, a.ldk, 0, rw.len, a.D);
-    sv.load(v, a.ldv, 0, rw.len, a.D);
-    for (int t = 0; t < tiles; ++t) {
-        uint8_t* buf = lds[t % NBUF];
-        if (NBUF == 1 && t > 0) __syncthreads();
-        sk.store_rows(buf);
-        if constexpr (L::TR) sv.store_cols(buf + L::ROWS);
-        else sv.store_rows(buf + L::ROWS);
-        const bool masked = t >= masked_from;
-        int apart = 0;
-        if (masked && a.causal) apart = __syncthreads_or(sv.nonfinite());
-        else __syncthreads();
-        if (t + 1 < tiles) {
-            sk.load(k, a.ldk, (t + 1) * kTile, rw.len, a.D);
-            sv.load(v, a.ldv, (t + 1) * kTile, rw.len, a.D);
-        }
+    const auto step = [&](int t, auto masked) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked)::value;
+        const uint8_t* kt = lds[t % NBUF][0];
+        uint8_t* vt = lds[t % NBUF][1];
+        tile_ready();
+        if (NBUF > 1 && t + 1 < tiles) start(t + 1);
+        bool dirty = false;
+        if (kMasked && a.causal) dirty = __syncthreads_or(cv.bad(vt));
+        if (dirty) clean_tile<T, DP, NT, 3, false>(cv, vt, marks);
         const int key0 = t * kTile;
-        if (key0 >= wave_keys || q0 >= rw.len) continue;
+        if (key0 < wave_keys && q0 < rw.len) {
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            f32x16 s[2];
-            mm_rows<T, DP>(s, buf, qf[b], lane);
-            const int lim = last[b] - key0 - 4 * h;   // element e of block kb is seen up to here
-            if (masked) {
+            for (int b = 0; b < QB; ++b) {
+                f32x16 s[2];
+                mm_rows<T, DP>(s, kt, qf[b], lane);
+                const int lim = last[b] - key0 - 4 * h;   // element e of block kb is seen up to here
+                if constexpr (kMasked) {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            s[kb][e] = 32 * kb + 8 * (e / 4) + e % 4 <= lim ? s[kb][e] : kNegInf;
+                }
+                float mx = s[0][0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[0][e]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[1][e]);
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                if (__any((mx - m[b]) * a.c > 8.0f)) {   // also from -inf; inf - inf is NaN: no move
+                    const float to = fmaxf(m[b], mx), f = m[b] == kNegInf ? 0.0f : exp2_hw((m[b] - to) * a.c);
+                    l[b] *= f;
+#pragma unroll
+                    for (int n = 0; n < DT; ++n) o[b][n] *= f;
+                    m[b] = to;
+                }
+                const float mc = m[b] == kNegInf ? 0.0f : m[b] * a.c;
+                float sum = 0.0f;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        s[kb][e] = 32 * kb + 8 * (e / 4) + e % 4 <= lim ? s[kb][e] : kNegInf;
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[0][e]);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[1][e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            if (__any((mx - m[b]) * a.c > 8.0f)) {   // also from -inf; inf - inf is NaN: no move
-                const float to = fmaxf(m[b], mx), f = m[b] == kNegInf ? 0.0f : exp2_hw((m[b] - to) * a.c);
-                l[b] *= f;
-#pragma unroll
-                for (int n = 0; n < DT; ++n) o[b][n] *= f;
-                m[b] = to;
-            }
-            const float mc = m[b] == kNegInf ? 0.0f : m[b] * a.c;
-            float sum = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[kb][e] = exp2_hw(__builtin_fmaf(s[kb][e], a.c, -mc));
-                    sum += s[kb][e];
-                }
-            l[b] += sum;
-            if (apart) {
-                const auto shown = [lim](int kb, int e) { return 32 * kb + 8 * (e / 4) + e % 4 <= lim; };
-                mm_cols_apart<T, DP, true>(o[b], buf + L::ROWS, s, shown, lane);
-            } else {
-                mm_cols<T, DP>(o[b], buf + L::ROWS, s, lane);
+                    for (int e = 0; e < 16; ++e) {
+                        s[kb][e] = exp2_hw(__builtin_fmaf(s[kb][e], a.c, -mc));
+                        sum += s[kb][e];
+                    }
+                l[b] += sum;
+                mm_cols<T, DP>(o[b], vt, s, lane);
+                if (dirty) spoil<DP>(o[b], marks, [&](int row) { return row <= last[b] - key0; }, lane);
             }
         }
-    }
+        if (NBUF == 1 && t + 1 < tiles) {
+            __syncthreads();
+            start(t + 1);
+        }
+    };
+    int t = 0;
+    for (; t < min(masked_from, tiles); ++t) step(t, std::false_type{});
+    for (; t < tiles; ++t) step(t, std::true_type{});
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
         const int row = q0 + 32 * b + (lane & 31);
@@ -424,7 +448,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 128 ? 2 : 1) 
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * n + 8 * g + 4 * h;
                 if (d >= a.D) continue;
-                if constexpr (L::TR) {
+                if constexpr (L::EB == 2) {
                     typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
                     bf16x4 w;
 #pragma unroll
@@ -504,8 +528,8 @@ template <typename T, int DP, int NW, int NBUF>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_dq_kernel(BwdArgs a) {
     using L = Lds<T, DP>;
     constexpr int NT = 64 * NW, BQ = 32 * NW, DT = DP / 32;
-    constexpr int BUF = 2 * L::ROWS + L::COLS;   // k, v row-major; k transposed
-    __shared__ __align__(16) uint8_t lds[NBUF][BUF];
+    __shared__ __align__(16) uint8_t lds[NBUF][2][L::BYTES];   // k and v
+    __shared__ Marks<DP, 1> marks;
     if (blockIdx.x == 0) check_starts(a.starts, a.nseq, a.rows, a.flag);
     Rows rw;
     if (!find_rows(a.starts, a.nseq, a.rows, BQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
@@ -516,6 +540,13 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
     const int64_t at = int64_t(rw.first) + row;
     const T* k = static_cast<const T*>(a.k) + int64_t(rw.first) * a.ldk + int64_t(kvh) * a.D;
     const T* v = static_cast<const T*>(a.v) + int64_t(rw.first) * a.ldv + int64_t(kvh) * a.D;
+    const Copy<T, DP, NT> ck(a.ldk), cv(a.ldv);
+    const auto start = [&](int t) __attribute__((always_inline)) {
+        const int key0 = t * kTile;
+        ck.start(lds[t % NBUF][0], k + key0 * a.ldk, rw.len - key0, a.D);
+        cv.start(lds[t % NBUF][1], v + key0 * a.ldv, rw.len - key0, a.D);
+    };
+    start(0);
     Frags<T, DP> qf, gf;
     qf.load(static_cast<const T*>(a.q) + at * a.ldq + int64_t(head) * a.D, in, a.D, h);
     gf.load(static_cast<const T*>(a.dout) + at * a.ldo + int64_t(head) * a.D, in, a.D, h);
@@ -529,41 +560,45 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
     const int keys = a.causal ? min(rw.len, (rw.tile + 1) * BQ) : rw.len, tiles = (keys + kTile - 1) / kTile;
     const int masked_from = a.causal ? rw.tile * BQ / kTile : rw.len / kTile;
     const int wave_keys = a.causal ? min(keys, q0 + 32) : keys;
-    Stage<T, DP, NT> sk, sv;
-    sk.load(k, a.ldk, 0, rw.len, a.D);
-    sv.load(v, a.ldv, 0, rw.len, a.D);
-    for (int t = 0; t < tiles; ++t) {
-        uint8_t* buf = lds[t % NBUF];
-        if (NBUF == 1 && t > 0) __syncthreads();
-        sk.store_rows(buf);
-        sv.store_rows(buf + L::ROWS);
-        if constexpr (L::TR) sk.store_cols(buf + 2 * L::ROWS);
-        const bool masked = t >= masked_from;
-        int apart = 0;
-        if (masked && a.causal) apart = __syncthreads_or(sk.nonfinite());
-        else __syncthreads();
-        if (t + 1 < tiles) {
-            sk.load(k, a.ldk, (t + 1) * kTile, rw.len, a.D);
-            sv.load(v, a.ldv, (t + 1) * kTile, rw.len, a.D);
-        }
+    const auto step = [&](int t, auto masked) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked)::value;
+        uint8_t* kt = lds[t % NBUF][0];
+        const uint8_t* vt = lds[t % NBUF][1];
+        tile_ready();
+        if (NBUF > 1 && t + 1 < tiles) start(t + 1);
+        bool dirty = false;
+        if (kMasked && a.causal) dirty = __syncthreads_or(ck.bad(kt));
         const int key0 = t * kTile;
-        if (key0 >= wave_keys || q0 >= rw.len) continue;
+        const bool active = key0 < wave_keys && q0 < rw.len;
         f32x16 s[2], dp[2];
-        mm_rows<T, DP>(s, buf, qf, lane);
-        mm_rows<T, DP>(dp, buf + L::ROWS, gf, lane);
-        const int lim = last - key0 - 4 * h;
-        const auto shown = [lim](int kb, int e) { return 32 * kb + 8 * (e / 4) + e % 4 <= lim; };
+        if (active) {
+            mm_rows<T, DP>(s, kt, qf, lane);
+            mm_rows<T, DP>(dp, vt, gf, lane);
+            const int lim = last - key0 - 4 * h;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p = exp2_hw(__builtin_fmaf(s[kb][e], a.c, -lse));
-                s[kb][e] = !masked || shown(kb, e) ? p * (dp[kb][e] - delta) : 0.0f;
-            }
-        const uint8_t* cols = L::TR ? buf + 2 * L::ROWS : buf;
-        if (apart) mm_cols_apart<T, DP, false>(acc, cols, s, shown, lane);
-        else mm_cols<T, DP>(acc, cols, s, lane);
-    }
+                for (int e = 0; e < 16; ++e) {
+                    const float p = exp2_hw(__builtin_fmaf(s[kb][e], a.c, -lse));
+                    s[kb][e] = !kMasked || 32 * kb + 8 * (e / 4) + e % 4 <= lim ? p * (dp[kb][e] - delta) : 0.0f;
+                }
+        }
+        if (dirty) {
+            __syncthreads();   // the tile has been read as it is
+            clean_tile<T, DP, NT, 1, false>(ck, kt, marks);
+        }
+        if (active) {
+            mm_cols<T, DP, 2>(acc, kt, s, lane);
+            if (dirty) spoil<DP>(acc, marks, [&](int row) { return row <= last - key0; }, lane);
+        }
+        if (NBUF == 1 && t + 1 < tiles) {
+            __syncthreads();
+            start(t + 1);
+        }
+    };
+    int t = 0;
+    for (; t < min(masked_from, tiles); ++t) step(t, std::false_type{});
+    for (; t < tiles; ++t) step(t, std::true_type{});
     if (in) store_grad<T, DT>(static_cast<T*>(a.dq) + at * a.ldq + int64_t(head) * a.D, acc, a.scale, a.D, h);
 }
 
@@ -573,9 +608,9 @@ template <typename T, int DP, int NW, int NBUF>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) attn_packed_dkv_kernel(BwdArgs a) {
     using L = Lds<T, DP>;
     constexpr int NT = 64 * NW, BK = 32 * NW, DT = DP / 32;
-    constexpr int BUF = 2 * L::ROWS + 2 * L::COLS;   // q, dout row-major; both transposed
-    __shared__ __align__(16) uint8_t lds[NBUF][BUF];
-    __shared__ __align__(16) float stat[NBUF][2][kTile];
+    __shared__ __align__(16) uint8_t lds[NBUF][2][L::BYTES];   // q and dout
+    __shared__ __align__(16) float stat[NBUF][2][kTile];       // lse and delta
+    __shared__ Marks<DP, 1> marks[2];
     Rows rw;
     if (!find_rows(a.starts, a.nseq, a.rows, BK, blockIdx.x / a.KVH, rw)) return;
     const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH;
@@ -583,6 +618,27 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) a
     const int k0 = rw.tile * BK + wave * 32, row = k0 + (lane & 31);
     const bool in = row < rw.len;
     const int64_t at = int64_t(rw.first) + row;
+    const int first = a.causal ? rw.tile * BK / kTile : 0, per_head = (rw.len + kTile - 1) / kTile - first;
+    const int steps = per_head * G;
+    const Copy<T, DP, NT> cq(a.ldq), cg(a.ldo);
+    static_assert(NT >= 2 * kTile, "a thread stages one statistic");
+    int head = kvh * G, tile = first;   // of the next copy
+    const auto start = [&](int buf) __attribute__((always_inline)) {
+        const int row0 = tile * kTile;
+        const int64_t r0 = int64_t(rw.first) + row0;
+        cq.start(lds[buf][0], static_cast<const T*>(a.q) + r0 * a.ldq + int64_t(head) * a.D, rw.len - row0, a.D);
+        cg.start(lds[buf][1], static_cast<const T*>(a.dout) + r0 * a.ldo + int64_t(head) * a.D, rw.len - row0, a.D);
+        if (threadIdx.x < 2 * kTile) {
+            const int r = threadIdx.x & (kTile - 1);
+            const float* from = threadIdx.x < kTile ? a.lse : a.delta;
+            stat[buf][threadIdx.x / kTile][r] = row0 + r < rw.len ? from[int64_t(head) * a.rows + r0 + r] : 0.0f;
+        }
+        if (++tile - first == per_head) {
+            tile = first;
+            ++head;
+        }
+    };
+    start(0);
     Frags<T, DP> kf, vf;
     kf.load(static_cast<const T*>(a.k) + at * a.ldk + int64_t(kvh) * a.D, in, a.D, h);
     vf.load(static_cast<const T*>(a.v) + at * a.ldv + int64_t(kvh) * a.D, in, a.D, h);
@@ -590,76 +646,69 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) a
 #pragma unroll
     for (int n = 0; n < DT; ++n) dk[n] = dv[n] = f32x16{};
 
-    const int first = a.causal ? rw.tile * BK / kTile : 0, per_head = (rw.len + kTile - 1) / kTile - first;
-    const int steps = per_head * G;
-    Stage<T, DP, NT> sq, sg;
-    float stat_reg = 0.0f;
-    const auto load = [&](int t) {
-        const int head = kvh * G + t / per_head, row0 = (first + t % per_head) * kTile;
-        sq.load(static_cast<const T*>(a.q) + int64_t(rw.first) * a.ldq + int64_t(head) * a.D, a.ldq, row0, rw.len, a.D);
-        sg.load(static_cast<const T*>(a.dout) + int64_t(rw.first) * a.ldo + int64_t(head) * a.D, a.ldo, row0, rw.len,
-                a.D);
-        if (threadIdx.x < 2 * kTile) {
-            const int r = row0 + (threadIdx.x & (kTile - 1));
-            const float* from = threadIdx.x < kTile ? a.lse : a.delta;
-            stat_reg = r < rw.len ? from[int64_t(head) * a.rows + rw.first + r] : 0.0f;
-        }
-    };
-    static_assert(NT >= 2 * kTile, "a thread stages one statistic");
-    load(0);
-    for (int t = 0; t < steps; ++t) {
-        uint8_t* buf = lds[t % NBUF];
-        if (NBUF == 1 && t > 0) __syncthreads();
-        sq.store_rows(buf);
-        sg.store_rows(buf + L::ROWS);
-        if constexpr (L::TR) {
-            sq.store_cols(buf + 2 * L::ROWS);
-            sg.store_cols(buf + 2 * L::ROWS + L::COLS);
-        }
-        if (threadIdx.x < 2 * kTile) stat[t % NBUF][threadIdx.x / kTile][threadIdx.x & (kTile - 1)] = stat_reg;
-        const int row0 = (first + t % per_head) * kTile;
-        // Positions not seen: queries before the workgroup's last key, or behind the sequence.
-        const bool hidden = a.causal && row0 < (rw.tile + 1) * BK, masked = hidden || row0 + kTile > rw.len;
-        int apart = 0;
-        if (hidden) apart = __syncthreads_or(sq.nonfinite() || sg.nonfinite());
-        else __syncthreads();
-        const float* lse = stat[t % NBUF][0];
-        const float* delta = stat[t % NBUF][1];
-        if (t + 1 < steps) load(t + 1);
-        if (k0 >= rw.len || (a.causal && row0 + kTile <= k0)) continue;
+    int now = first;   // the tile that is computed on
+    const auto step = [&](int t, auto masked, bool hidden) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked)::value;
+        const int buf = t % NBUF, row0 = now * kTile;
+        uint8_t* qt = lds[buf][0];
+        uint8_t* gt = lds[buf][1];
+        const float* lse = stat[buf][0];
+        const float* delta = stat[buf][1];
+        tile_ready();
+        if (NBUF > 1 && t + 1 < steps) start((t + 1) % NBUF);
+        bool dirty = false;
+        if (kMasked && hidden) dirty = __syncthreads_or(cq.bad(qt) || cg.bad(gt));
+        const bool active = k0 < rw.len && !(a.causal && row0 + kTile <= k0);
+        const int from = (a.causal ? row : 0) - row0;   // the tile's rows that the key sees
         f32x16 p[2], ds[2];
-        mm_rows<T, DP>(p, buf, kf, lane);
-        mm_rows<T, DP>(ds, buf + L::ROWS, vf, lane);
-        // Element e of block kb is query row0 + 32kb + 8(e/4) + e%4 + 4h: seen from the key's row on.
-        const int lo = (a.causal ? row : 0) - row0 - 4 * h, hi = rw.len - row0 - 4 * h;
-        const auto shown = [lo, hi](int kb, int e) {
-            const int i = 32 * kb + 8 * (e / 4) + e % 4;
-            return i >= lo && i < hi;
-        };
+        if (active) {
+            mm_rows<T, DP>(p, qt, kf, lane);
+            mm_rows<T, DP>(ds, gt, vf, lane);
+            // Element e of block kb is row 32kb + 8(e/4) + e%4 + 4h.
+            const int lo = from - 4 * h, hi = rw.len - row0 - 4 * h;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int i0 = 32 * kb + 8 * g + 4 * h;
-                const f32x4 ls = *reinterpret_cast<const f32x4*>(lse + i0), de = *reinterpret_cast<const f32x4*>(delta + i0);
+                for (int g = 0; g < 4; ++g) {
+                    const int i0 = 32 * kb + 8 * g;
+                    const f32x4 ls = *reinterpret_cast<const f32x4*>(lse + i0 + 4 * h);
+                    const f32x4 de = *reinterpret_cast<const f32x4*>(delta + i0 + 4 * h);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = 4 * g + i;
-                    const bool see = !masked || shown(kb, e);
-                    const float w = see ? exp2_hw(__builtin_fmaf(p[kb][e], a.c, -ls[i])) : 0.0f;
-                    ds[kb][e] = see ? w * (ds[kb][e] - de[i]) : 0.0f;
-                    p[kb][e] = w;
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * g + i;
+                        const bool see = !kMasked || (i0 + i >= lo && i0 + i < hi);
+                        const float w = see ? exp2_hw(__builtin_fmaf(p[kb][e], a.c, -ls[i])) : 0.0f;
+                        ds[kb][e] = see ? w * (ds[kb][e] - de[i]) : 0.0f;
+                        p[kb][e] = w;
+                    }
                 }
-            }
-        const uint8_t* qc = L::TR ? buf + 2 * L::ROWS : buf;
-        const uint8_t* gc = L::TR ? buf + 2 * L::ROWS + L::COLS : buf + L::ROWS;
-        if (apart) {
-            mm_cols_apart<T, DP, false>(dv, gc, p, shown, lane);
-            mm_cols_apart<T, DP, false>(dk, qc, ds, shown, lane);
-        } else {
-            mm_cols<T, DP>(dv, gc, p, lane);
-            mm_cols<T, DP>(dk, qc, ds, lane);
         }
+        if (dirty) {
+            __syncthreads();   // the tiles have been read as they are
+            clean_tile<T, DP, NT, 1, true>(cq, qt, marks[0]);
+            clean_tile<T, DP, NT, 1, true>(cg, gt, marks[1]);
+        }
+        if (active) {
+            mm_cols<T, DP>(dv, gt, p, lane);
+            mm_cols<T, DP, 2>(dk, qt, ds, lane);
+            if (dirty) {
+                const auto sees = [&](int row) { return row >= 0 && row >= from; };
+                spoil<DP>(dk, marks[0], sees, lane);
+                spoil<DP>(dv, marks[1], sees, lane);
+            }
+        }
+        if (NBUF == 1 && t + 1 < steps) {
+            __syncthreads();
+            start(0);
+        }
+        if (++now - first == per_head) now = first;
+    };
+    for (int t = 0; t < steps; ++t) {
+        // Positions not seen: queries before the workgroup's last key, or behind the sequence.
+        const int row0 = now * kTile;
+        const bool hidden = a.causal && row0 < (rw.tile + 1) * BK;
+        if (hidden || row0 + kTile > rw.len) step(t, std::true_type{}, hidden);
+        else step(t, std::false_type{}, false);
     }
     if (in) {
         store_grad<T, DT>(static_cast<T*>(a.dk) + at * a.ldk + int64_t(kvh) * a.D, dk, a.scale, a.D, h);
@@ -668,6 +717,8 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 && DP <= 64 ? 2 : 1) a
 }
 
 // ---- host ----------------------------------------------------------------------
+
+constexpr int64_t kMaxStride = int64_t(1) << 23;   // a tile's 64 rows within the copies' 32-bit offsets
 
 // Strides of 0 mean rows back to back.
 struct Strides {
@@ -698,8 +749,8 @@ int check_cfg(dgm_gpu* g, const char* name, const dgm_attn_cfg* c, int max_d) {
         return dgm::fail(g, DGM_ERR_SHAPE, "%s: a row stride is shorter than the row's heads", name);
     if ((s.q | s.k | s.v | s.o) % 8 != 0)
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: row strides must be multiples of 8 elements", name);
-    if (std::max(std::max(s.q, s.o), std::max(s.k, s.v)) > (int64_t(1) << 31))
-        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: a row stride beyond 2^31 elements", name);
+    if (std::max(std::max(s.q, s.o), std::max(s.k, s.v)) > kMaxStride)
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: a row stride beyond %lld elements", name, (long long)kMaxStride);
     return DGM_OK;
 }
 
