@@ -41,6 +41,57 @@ struct OnDevice {
     OnDevice& operator=(const OnDevice&) = delete;
 };
 
+// Three bf16 pieces of 8 bits each that add up to x exactly, the high one first
+// (x's low 16 bits cut off, not rounded, so that none overflows). An infinity or
+// NaN is the last piece, which meets the other operand's first one alone.
+__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    const float fin = fabsf(x) < __builtin_huge_valf() ? x : 0.0f;
+    hi = __float_as_uint(fin) & 0xffff0000u;
+    const float r = fin - __uint_as_float(hi);
+    mid = __float_as_uint(r) & 0xffff0000u;
+    lo = __float_as_uint(r - __uint_as_float(mid) + (x - fin)) & 0xffff0000u;
+}
+
+// 8 values as PIECES bf16 pieces: the value rounded, that and what rounding left, or split3's.
+template <int PIECES>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&o)[PIECES]) {
+    if constexpr (PIECES < 3) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            o[0][j] = __bf16(x[j]);
+            if constexpr (PIECES == 2) o[1][j] = __bf16(x[j] - float(o[0][j]));
+        }
+    } else {
+        u32x4 w[3];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            uint32_t a[3], b[3];
+            split3(x[j], a[0], a[1], a[2]);
+            split3(x[j + 1], b[0], b[1], b[2]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) w[p][j / 2] = __builtin_amdgcn_perm(b[p], a[p], 0x07060302u);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) o[p] = __builtin_bit_cast(bf16x8, w[p]);
+    }
+}
+
+template <typename IN>
+__device__ __forceinline__ void load8(const IN* p, float (&x)[8]) {
+    if constexpr (sizeof(IN) == 4) {
+        const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+    } else {
+        const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = float(a[i]);
+    }
+}
+
 inline int type_bytes(int64_t type) { return type == DGM_TYPE_F32 ? 4 : type == DGM_TYPE_BF16 ? 2 : 0; }
 
 // starts[0 .. nseq] is in order and within [0, rows]; else the flag is set. Run by one workgroup.

@@ -152,53 +152,6 @@ __device__ inline int64_t tiles_before(const DecodeArgs& a, int64_t s) {
     return sum;
 }
 
-// Three bf16 pieces of 8 bits each that add up to x exactly (high to low); a
-// non-finite x is its first piece.
-__device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-    const uint32_t u = __float_as_uint(x);
-    const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-    hi = (u & 0x007fffffu) && !fin ? 0x7fc00000u : u & 0xffff0000u;
-    const float r = fin ? x - __uint_as_float(hi) : 0.0f;
-    mid = __float_as_uint(r) & 0xffff0000u;
-    lo = __float_as_uint(r - __uint_as_float(mid)) & 0xffff0000u;
-}
-
-template <int PIECES>
-__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&o)[PIECES]) {
-    if constexpr (PIECES == 1) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[0][j] = __bf16(x[j]);
-    } else {
-        u32x4 w[3];
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            uint32_t a[3], b[3];
-            split3(x[j], a[0], a[1], a[2]);
-            split3(x[j + 1], b[0], b[1], b[2]);
-#pragma unroll
-            for (int p = 0; p < 3; ++p) w[p][j / 2] = (a[p] >> 16) | b[p];
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p) o[p] = __builtin_bit_cast(bf16x8, w[p]);
-    }
-}
-
-template <typename IN>
-__device__ __forceinline__ void load8(const IN* p, float (&x)[8]) {
-    if constexpr (sizeof(IN) == 4) {
-        const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = a[i];
-            x[4 + i] = b[i];
-        }
-    } else {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = float(a[i]);
-    }
-}
-
 // VW consecutive elements of a value row in registers.
 template <int BYTES>
 struct Piece {
