@@ -58,9 +58,13 @@ constexpr int kPieces = sizeof(T) == 2 ? 1 : 3;
 // piece. The 16-byte chunk c (8 columns) of row r sits at slot c ^ swizzle(r): 16
 // rows' chunk c (the A operand of mm_rows) and 8 rows' four chunks (its transposed reads in
 // mm_cols) then lie in different banks.
+// Rows of a tile: fp32 has three planes, and the registers of three pieces.
 template <typename T, int DP>
+constexpr int kTileRows = sizeof(T) == 4 && DP > 64 ? 32 : 64;
+
+template <typename T, int DP, int ROWS = kTileRows<T, DP>>
 struct Lds {
-    static constexpr int kRows = sizeof(T) == 4 && DP > 64 ? 32 : 64;   // fp32: three planes and the registers of three pieces
+    static constexpr int kRows = ROWS;
     static constexpr int KB = kRows / 32;                     // blocks of 32 rows
     static constexpr int RB = DP * 2, CPR = RB / 16;          // bytes and chunks of a row
     static constexpr int RPB = RB >= 256 ? 1 : 256 / RB;      // rows that span all banks
@@ -78,9 +82,9 @@ struct Lds {
 // each lane fetches the chunk that belongs in its slot) while the other
 // buffer is computed on. fp32: loads into registers while the one buffer is
 // computed on, split into pieces and stored between two barriers.
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, int ROWS = kTileRows<T, DP>>
 struct Feed {
-    using L = Lds<T, DP>;
+    using L = Lds<T, DP, ROWS>;
     static constexpr int N = L::PLANE / 16 / NT, STEP = NT / L::CPR;   // STEP: rows between a thread's chunks
     static_assert(L::PLANE % (16 * NT) == 0 && NT % L::CPR == 0, "every thread has whole chunks of one slot");
     int64_t ldb;        // bytes from row to row
@@ -170,9 +174,9 @@ __device__ __forceinline__ void copies_ready() {
 }
 
 // Waits for the pair of tiles that was started last, in buffer `now`, and starts the next with `next()`.
-template <typename T, int DP, int NT, typename Next>
-__device__ __forceinline__ void turn(Feed<T, DP, NT>& a, Feed<T, DP, NT>& b, uint8_t (*now)[Lds<T, DP>::BYTES],
-                                     const Next& next) {
+template <typename T, int DP, int NT, int ROWS, typename Next>
+__device__ __forceinline__ void turn(Feed<T, DP, NT, ROWS>& a, Feed<T, DP, NT, ROWS>& b,
+                                     uint8_t (*now)[Lds<T, DP, ROWS>::BYTES], const Next& next) {
     if constexpr (sizeof(T) == 2) {
         copies_ready();
     } else {
@@ -226,8 +230,26 @@ __device__ __forceinline__ void mfma_pieces(f32x16& acc, const bf16x8 (&a)[PA], 
 template <typename T, int DP>
 using Blocks = f32x16[Lds<T, DP>::KB];
 
-// out[kb] (32 rows x the wave's 32 columns) = tile rows 32kb .. 32kb+31 times the columns' vectors.
+// out (32 rows x the wave's 32 columns) = tile rows 32kb .. 32kb+31 times the columns' vectors.
 // Element r of a lane: row 32kb + 8(r/4) + 4h + r%4, column lane % 32.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void mm_block(f32x16& out, const uint8_t* tile, int kb, const Frags<T, DP>& b, int lane) {
+    using L = Lds<T, DP, ROWS>;
+    constexpr int P = kPieces<T>;
+    const int h = lane >> 5, r = lane & 31;
+    out = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < Frags<T, DP>::NK; ++kk) {
+        bf16x8 x[P], y[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            x[p] = *reinterpret_cast<const bf16x8*>(tile + p * L::PLANE + L::at(32 * kb + r, 2 * kk + h));
+            y[p] = b.f[p][kk];
+        }
+        mfma_pieces(out, x, y);
+    }
+}
+// out[kb] for all blocks of a tile.
 template <typename T, int DP>
 __device__ __forceinline__ void mm_rows(Blocks<T, DP>& out, const uint8_t* tile, const Frags<T, DP>& b, int lane) {
     using L = Lds<T, DP>;
@@ -305,12 +327,14 @@ struct Marks {
 };
 
 // The tile's first row is row0 of the sequence.
-template <typename T, int DP, int NT, int KINDS, bool kLast>
-__device__ __forceinline__ void clean_tile(const Feed<T, DP, NT>& c, uint8_t* lds, int row0, Marks<DP, KINDS>& marks) {
-    using L = Lds<T, DP>;
+template <typename T, int DP, int NT, int KINDS, bool kLast, int ROWS>
+__device__ __forceinline__ void clean_tile(const Feed<T, DP, NT, ROWS>& c, uint8_t* lds, int row0,
+                                           Marks<DP, KINDS>& marks) {
+    using F = Feed<T, DP, NT, ROWS>;
+    using L = typename F::L;
 #pragma unroll 1
-    for (int i = 0; i < Feed<T, DP, NT>::N; ++i) {
-        const int r = c.row + i * Feed<T, DP, NT>::STEP, d0 = (c.slot ^ L::swizzle(r)) * 8;
+    for (int i = 0; i < F::N; ++i) {
+        const int r = c.row + i * F::STEP, d0 = (c.slot ^ L::swizzle(r)) * 8;
         __bf16* at = reinterpret_cast<__bf16*>(lds + L::BYTES - L::PLANE + (i * NT + int(threadIdx.x)) * 16);
 #pragma unroll 1
         for (int j = 0; j < 8; ++j) {
@@ -326,14 +350,15 @@ __device__ __forceinline__ void clean_tile(const Feed<T, DP, NT>& c, uint8_t* ld
 }
 
 // `sees(row)`: whether the lane's column sees a row marked so.
-template <int DP, int KINDS, typename Sees>
-__device__ __forceinline__ void spoil(f32x16 (&acc)[DP / 32], const Marks<DP, KINDS>& marks, const Sees& sees, int lane) {
+template <int DP, int DT, int KINDS, typename Sees>
+__device__ __forceinline__ void spoil(f32x16 (&acc)[DT], const Marks<DP, KINDS>& marks, int d0, const Sees& sees,
+                                      int lane) {
     const float inf = __builtin_huge_valf();
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int d = 32 * dt + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+            const int d = d0 + 32 * dt + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
             float x = acc[dt][e];
             if constexpr (KINDS == 3) {
                 x += sees(marks.row[1][d]) ? inf : 0.0f;
@@ -383,14 +408,14 @@ struct FwdArgs {
 // different XCDs, so the heads of one group, which read the same k and v, are KVH apart.
 __device__ __forceinline__ int head_of(int i, int H, int KVH) { return (i % KVH) * (H / KVH) + i / KVH; }
 
-// Rows 32n + 8g + 4h .. +3 of a lane's column, times f, to its row of the output.
+// Rows 32n + 8g + 4h .. +3 of a lane's column, times f, to columns d0 + .. of its row of the output.
 template <typename T, int DT>
-__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DT], float f, int D, int h) {
+__device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DT], float f, int d0, int D, int h) {
 #pragma unroll
     for (int n = 0; n < DT; ++n)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int d = 32 * n + 8 * g + 4 * h;
+            const int d = d0 + 32 * n + 8 * g + 4 * h;
             if (d >= D) continue;
             if constexpr (sizeof(T) == 2) {
                 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -494,12 +519,12 @@ __global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2
         l += sum;
         mm_cols<T, DP, kPieces<T>>(o, vt, s, lane);
     }
-    if (spoilt) spoil<DP>(o, marks, [&](int r) { return r <= last; }, lane);
+    if (spoilt) spoil<DP>(o, marks, 0, [&](int r) { return r <= last; }, lane);
 
     const float sum = l + __shfl_xor(l, 32, 64);
     if (!in) return;
     if (a.lse && h == 0) a.lse[int64_t(head) * a.rows + at] = (m == kNegInf ? 0.0f : m * a.c) + log2_hw(sum);
-    store_row<T, DT>(static_cast<T*>(a.out) + at * a.ldo + int64_t(head) * a.D, o, 1.0f / sum, a.D, h);
+    store_row<T, DT>(static_cast<T*>(a.out) + at * a.ldo + int64_t(head) * a.D, o, 1.0f / sum, 0, a.D, h);
 }
 
 // ---- backward ------------------------------------------------------------------
@@ -514,10 +539,11 @@ struct BwdArgs {
     void *dq, *dk, *dv;
     const float* lse;
     float* delta;   // [H, rows]
+    float* sums;    // [parts][dk, dv][rows, KVH, D], with several parts
     const int32_t* starts;
     uint32_t* flag;
     int64_t rows, nseq, ldq, ldk, ldv, ldo, slots;
-    int H, KVH, D, causal;
+    int H, KVH, D, causal, parts;
     float c, scale;
 };
 
@@ -608,33 +634,56 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
         }
         if (active) mm_cols<T, DP, kSlopePieces<T>>(acc, kt, s, lane);
     }
-    if (spoilt) spoil<DP>(acc, marks, [&](int r) { return r <= last; }, lane);
-    if (in) store_row<T, DT>(static_cast<T*>(a.dq) + at * a.ldq + int64_t(head) * a.D, acc, a.scale, a.D, h);
+    if (spoilt) spoil<DP>(acc, marks, 0, [&](int r) { return r <= last; }, lane);
+    if (in) store_row<T, DT>(static_cast<T*>(a.dq) + at * a.ldq + int64_t(head) * a.D, acc, a.scale, 0, a.D, h);
 }
 
-// dk, dv: a wave's 32 keys as columns against tiles of 64 queries, over the query heads of
-// the group one after the other. S = Q K^T, dP = dout V^T; dv^T += dout^T P, dk^T += Q^T dS.
-template <typename T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 64 : 32) ? 2 : 1) attn_packed_dkv_kernel(BwdArgs a) {
-    using L = Lds<T, DP>;
-    constexpr int NT = 64 * NW, BK = 32 * NW, DT = DP / 32, KB = L::KB, TILE = L::kRows;
-    __shared__ __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];   // q and dout
-    __shared__ __align__(16) float stat[2][2][TILE];              // lse and delta, of two tiles
+// dk, dv: a pair of waves' 32 keys as columns against tiles of 64 queries, over the query heads
+// of the group one after the other. S = Q K^T, dP = dout V^T; dv^T += dout^T P, dk^T += Q^T dS.
+//
+// dk and dv of 32 keys are 128 registers at D = 128, and a wave with them, k, v and the
+// scores has room for one on a SIMD, where nothing runs beside its waits and its
+// exponentials. So a pair shares the keys: each wave computes P and dS for half of the tile's
+// rows, hands them to the other through LDS as the B operands that they are, and
+// accumulates half of the columns of dk and dv. Four blocks of 2048 (16 heads on 8
+// of 128, bf16): 428 us with whole waves, 336 so.
+//
+// Where that gives too few workgroups (few key heads, short batches), `parts` of
+// them share a key tile's steps and leave fp32 sums in the workspace, which a
+// second kernel adds up in order.
+template <typename T, int DP>
+struct DkvShape {
+    // Waves: as many as leave room for the tiles and the handed-over operands (2 KB a piece and wave).
+    static constexpr int NW = sizeof(T) == 2 ? (DP == 128 ? 8 : 4) : (DP == 64 ? 8 : 4);
+    static constexpr int BK = 16 * NW;   // keys
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 && DP == 128 ? 1 : 2))
+    attn_packed_dkv_kernel(BwdArgs a) {
+    using L = Lds<T, DP, 64>;
+    constexpr int NW = DkvShape<T, DP>::NW, NT = 64 * NW, BK = DkvShape<T, DP>::BK, TILE = 64;
+    constexpr int PP = kPieces<T>, PS = kSlopePieces<T>;
+    constexpr bool kSplitD = DP > 32;              // else the pair's waves take dv and dk, one each
+    constexpr int DT = kSplitD ? DP / 64 : 1;      // blocks of 32 columns of a wave
+    __shared__ __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];    // q and dout
+    __shared__ bf16x8 hand[NW][PP + PS][2][64];                    // P and dS, by wave, piece, 16 rows
+    __shared__ __align__(16) float stat[2][2][TILE];               // lse and delta, of two tiles
     __shared__ Marks<DP, 1> marks[2];
     marks[0].init(-1);
     marks[1].init(-1);
     Rows rw;
-    if (!find_rows(a.starts, a.nseq, a.rows, BK, blockIdx.x / a.KVH, rw)) return;
-    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int k0 = rw.tile * BK + wave * 32, row = k0 + (lane & 31);
+    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, part = int(blockIdx.x / a.KVH % a.parts);
+    if (!find_rows(a.starts, a.nseq, a.rows, BK, blockIdx.x / a.KVH / a.parts, rw)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, half = wave & 1;
+    const int k0 = rw.tile * BK + wave / 2 * 32, row = k0 + (lane & 31);
     const bool in = row < rw.len;
     const int64_t at = int64_t(rw.first) + row;
     const int first = a.causal ? rw.tile * BK / TILE : 0, per_head = (rw.len + TILE - 1) / TILE - first;
-    const int steps = per_head * G;
-    Feed<T, DP, NT> cq(a.ldq), cg(a.ldo);
+    const int t0 = int(int64_t(per_head) * G * part / a.parts), t1 = int(int64_t(per_head) * G * (part + 1) / a.parts);
+    Feed<T, DP, NT, 64> cq(a.ldq), cg(a.ldo);
     static_assert(NT >= 2 * TILE, "a thread stages one statistic");
-    int head = kvh * G, tile = first;   // of the next copy
+    int head = kvh * G + t0 / per_head, tile = first + t0 % per_head, now = tile;   // of the next copy; computed on
     const auto start = [&](int t) __attribute__((always_inline)) {
         const int row0 = tile * TILE;
         const int64_t r0 = int64_t(rw.first) + row0;
@@ -651,7 +700,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 64 : 32) ? 2 
             ++head;
         }
     };
-    start(0);
+    if (t0 < t1) start(t0);
     Frags<T, DP> kf, vf;
     kf.load(static_cast<const T*>(a.k) + at * a.ldk + int64_t(kvh) * a.D, in, a.D, h);
     vf.load(static_cast<const T*>(a.v) + at * a.ldv + int64_t(kvh) * a.D, in, a.D, h);
@@ -659,72 +708,136 @@ __global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 64 : 32) ? 2 
 #pragma unroll
     for (int n = 0; n < DT; ++n) dk[n] = dv[n] = f32x16{};
 
-    int now = first;   // the tile that is computed on
     bool spoilt = false;
-    for (int t = 0; t < steps; ++t) {
+    for (int t = t0; t < t1; ++t) {
         const int row0 = now * TILE;
         uint8_t* qt = lds[t % L::NBUF][0];
         uint8_t* gt = lds[t % L::NBUF][1];
-        const float* lse = stat[t % 2][0];
-        const float* delta = stat[t % 2][1];
+        const float* lse = stat[t % 2][0] + 32 * half + 4 * h;
+        const float* delta = stat[t % 2][1] + 32 * half + 4 * h;
         turn(cq, cg, lds[t % L::NBUF], [&]() __attribute__((always_inline)) {
-            if (t + 1 < steps) start(t + 1);
+            if (t + 1 < t1) start(t + 1);
         });
         // Positions not seen: queries before the workgroup's last key, or behind the sequence.
         const bool hidden = a.causal && row0 < (rw.tile + 1) * BK;
         const bool active = k0 < rw.len && !(a.causal && row0 + TILE <= k0);
         const bool dirty = hidden && __syncthreads_or(cq.bad(qt) || cg.bad(gt));
-        f32x16 p[KB], ds[KB];
         if (active) {
-            mm_rows<T, DP>(p, qt, kf, lane);
-            mm_rows<T, DP>(ds, gt, vf, lane);
-            // Element e of block kb is row 32kb + 8(e/4) + e%4 + 4h.
+            f32x16 p, ds;
+            mm_block<T, DP, 64>(p, qt, half, kf, lane);
+            mm_block<T, DP, 64>(ds, gt, half, vf, lane);
+            // Element e is row 32 half + 8(e/4) + e%4 + 4h.
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 ls = *reinterpret_cast<const f32x4*>(lse + 8 * g);
+                const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 8 * g);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 ls = *reinterpret_cast<const f32x4*>(lse + 32 * kb + 8 * g + 4 * h);
-                    const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 32 * kb + 8 * g + 4 * h);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int e = 4 * g + i;
-                        p[kb][e] = exp2_hw(__builtin_fmaf(p[kb][e], a.c, -ls[i]));
-                        ds[kb][e] = p[kb][e] * (ds[kb][e] - de[i]);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * g + i;
+                    p[e] = exp2_hw(__builtin_fmaf(p[e], a.c, -ls[i]));
+                    ds[e] = p[e] * (ds[e] - de[i]);
                 }
+            }
             if (hidden || row0 + TILE > rw.len) {
-                const int lo = (a.causal ? row : 0) - row0 - 4 * h, hi = rw.len - row0 - 4 * h;
+                const int r0 = row0 + 32 * half + 4 * h, lo = (a.causal ? row : 0) - r0, hi = rw.len - r0;
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+                for (int e = 0; e < 16; ++e) {
+                    const int i = 8 * (e / 4) + e % 4;
+                    const bool see = i >= lo && i < hi;
+                    p[e] = see ? p[e] : 0.0f;
+                    ds[e] = see ? ds[e] : 0.0f;
+                }
+            }
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int i = 32 * kb + 8 * (e / 4) + e % 4;
-                        const bool see = i >= lo && i < hi;
-                        p[kb][e] = see ? p[kb][e] : 0.0f;
-                        ds[kb][e] = see ? ds[kb][e] : 0.0f;
-                    }
+            for (int st = 0; st < 2; ++st) {
+                float x[8], y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[j] = p[8 * st + j];
+                    y[j] = ds[8 * st + j];
+                }
+                bf16x8 px[PP], sx[PS];
+                split8<PP>(x, px);
+                split8<PS>(y, sx);
+#pragma unroll
+                for (int n = 0; n < PP; ++n) hand[wave][n][st][lane] = px[n];
+#pragma unroll
+                for (int n = 0; n < PS; ++n) hand[wave][PP + n][st][lane] = sx[n];
             }
         }
-        if (dirty) {
-            __syncthreads();   // the tiles have been read as they are
+        __syncthreads();
+        if (dirty) {   // the tiles have been read as they are
             clean_tile<T, DP, NT, 1, true>(cq, qt, row0, marks[0]);
             clean_tile<T, DP, NT, 1, true>(cg, gt, row0, marks[1]);
             spoilt = true;
         }
         if (active) {
-            mm_cols<T, DP, kPieces<T>>(dv, gt, p, lane);
-            mm_cols<T, DP, kSlopePieces<T>>(dk, qt, ds, lane);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const auto& from = hand[(wave & ~1) + kb];
+                    bf16x8 px[PP], sx[PS];
+#pragma unroll
+                    for (int n = 0; n < PP; ++n) px[n] = from[n][st][lane];
+#pragma unroll
+                    for (int n = 0; n < PS; ++n) sx[n] = from[PP + n][st][lane];
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const int d = kSplitD ? half * DT + dt : 0;
+                        bf16x8 x[PP], y[PP];
+#pragma unroll
+                        for (int n = 0; n < PP; ++n) {
+                            x[n] = read_cols<T, DP>(gt + n * L::PLANE, kb, st, d, lane);
+                            y[n] = read_cols<T, DP>(qt + n * L::PLANE, kb, st, d, lane);
+                        }
+                        if (kSplitD || half == 0) mfma_pieces(dv[dt], x, px);
+                        if (kSplitD || half == 1) mfma_pieces(dk[dt], y, sx);
+                    }
+                }
         }
         if (++now - first == per_head) now = first;
     }
+    const int d0 = kSplitD ? half * 32 * DT : 0;
     if (spoilt) {
         const auto sees = [&](int r) { return r >= 0 && r >= row; };
-        spoil<DP>(dk, marks[0], sees, lane);
-        spoil<DP>(dv, marks[1], sees, lane);
+        spoil<DP>(dk, marks[0], d0, sees, lane);
+        spoil<DP>(dv, marks[1], d0, sees, lane);
     }
-    if (in) {
-        store_row<T, DT>(static_cast<T*>(a.dk) + at * a.ldk + int64_t(kvh) * a.D, dk, a.scale, a.D, h);
-        store_row<T, DT>(static_cast<T*>(a.dv) + at * a.ldv + int64_t(kvh) * a.D, dv, 1.0f, a.D, h);
+    if (!in) return;
+    const bool mine_v = kSplitD || half == 0, mine_k = kSplitD || half == 1;
+    if (a.parts > 1) {
+        const int64_t r = at * a.KVH + kvh, all = a.rows * a.KVH;
+        float* sums = a.sums + (int64_t(part) * 2 * all + r) * a.D;
+        if (mine_k) store_row<float, DT>(sums, dk, 1.0f, d0, a.D, h);
+        if (mine_v) store_row<float, DT>(sums + all * a.D, dv, 1.0f, d0, a.D, h);
+        return;
+    }
+    if (mine_k) store_row<T, DT>(static_cast<T*>(a.dk) + at * a.ldk + int64_t(kvh) * a.D, dk, a.scale, d0, a.D, h);
+    if (mine_v) store_row<T, DT>(static_cast<T*>(a.dv) + at * a.ldv + int64_t(kvh) * a.D, dv, 1.0f, d0, a.D, h);
+}
+
+// The parts' sums of dk and dv, added in order: a workgroup takes 32 rows of one
+// sequence and head, 4 columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_packed_sum_kernel(BwdArgs a) {
+    Rows rw;
+    const int kvh = blockIdx.x % a.KVH;
+    if (!find_rows(a.starts, a.nseq, a.rows, 32, blockIdx.x / a.KVH, rw)) return;
+    const int64_t all = a.rows * a.KVH;
+    const int quads = a.D / 4;
+    for (int i = threadIdx.x; i < 64 * quads; i += 256) {
+        const int which = i / (32 * quads), r = i / quads % 32, d = i % quads * 4;
+        if (rw.tile * 32 + r >= rw.len) continue;
+        const int64_t at = int64_t(rw.first) + rw.tile * 32 + r;
+        const float* from = a.sums + (which * all + at * a.KVH + kvh) * a.D + d;
+        f32x4 sum = *reinterpret_cast<const f32x4*>(from);
+        for (int p = 1; p < a.parts; ++p) sum += *reinterpret_cast<const f32x4*>(from + p * 2 * all * a.D);
+        T* to = which ? static_cast<T*>(a.dv) + at * a.ldv + int64_t(kvh) * a.D
+                      : static_cast<T*>(a.dk) + at * a.ldk + int64_t(kvh) * a.D;
+        const float f = which ? 1.0f : a.scale;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[d + j] = T(sum[j] * f);
     }
 }
 
@@ -791,29 +904,58 @@ int run_fwd(dgm_gpu* g, const dgm_attn_cfg* c, const FwdArgs& a) {
     return launch_fwd<T, 256, 4>(g, c, a);
 }
 
-template <typename T, int DP, int NW>
+// Keys of a workgroup of the dk, dv kernel.
+int dkv_keys(const dgm_attn_cfg* c) {
+    if (c->type == DGM_TYPE_BF16)
+        return c->D <= 32 ? DkvShape<__bf16, 32>::BK : c->D <= 64 ? DkvShape<__bf16, 64>::BK : DkvShape<__bf16, 128>::BK;
+    return c->D <= 32 ? DkvShape<float, 32>::BK : c->D <= 64 ? DkvShape<float, 64>::BK : DkvShape<float, 128>::BK;
+}
+
+// Workgroups that share a key tile's steps: enough for three to a CU, each with two
+// steps or more at the sequences' average length (four blocks of 2048, 544 causal tiles: 336 us
+// whole; two parts 279 and 28 for the sums).
+int64_t dkv_parts(const dgm_attn_cfg* c) {
+    const int64_t tiles = slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH;
+    const int64_t steps = (c->rows / std::max<int64_t>(c->nseq, 1) + 63) / 64 * (c->H / c->KVH);
+    return std::max<int64_t>(1, std::min<int64_t>({16, (3 * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps / 2}));
+}
+
+template <typename T, int DP>
 int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs a) {
+    constexpr int NW = 4, NK = DkvShape<T, DP>::NW;
     BwdArgs kv = a;
     int rc = slots_of(g, "attnPackedBwd", c, 32 * NW, c->H, 64 * NW, a.slots);
-    if (!rc) rc = slots_of(g, "attnPackedBwd", c, 32 * NW, c->KVH, 64 * NW, kv.slots);
+    if (!rc) rc = slots_of(g, "attnPackedBwd", c, DkvShape<T, DP>::BK, c->KVH * a.parts, 64 * NK, kv.slots);
     if (rc) return rc;
     attn_packed_dq_kernel<T, DP, NW><<<dim3(unsigned(a.slots * c->H)), dim3(64 * NW), 0, g->stream>>>(a);
     DGM_LAUNCH_CHECK(g, "attn_packed_dq");
-    attn_packed_dkv_kernel<T, DP, NW><<<dim3(unsigned(kv.slots * c->KVH)), dim3(64 * NW), 0, g->stream>>>(kv);
+    attn_packed_dkv_kernel<T, DP>
+        <<<dim3(unsigned(kv.slots * c->KVH * a.parts)), dim3(64 * NK), 0, g->stream>>>(kv);
     DGM_LAUNCH_CHECK(g, "attn_packed_dkv");
+    if (a.parts > 1) {
+        rc = slots_of(g, "attnPackedBwd", c, 32, c->KVH, 256, kv.slots);
+        if (rc) return rc;
+        attn_packed_sum_kernel<T><<<dim3(unsigned(kv.slots * c->KVH)), dim3(256), 0, g->stream>>>(kv);
+        DGM_LAUNCH_CHECK(g, "attn_packed_sum");
+    }
     return DGM_OK;
 }
 
 template <typename T>
 int run_bwd(dgm_gpu* g, const dgm_attn_cfg* c, const BwdArgs& a) {
-    if (c->D <= 32) return launch_bwd<T, 32, 4>(g, c, a);
-    if (c->D <= 64) return launch_bwd<T, 64, 4>(g, c, a);
-    return launch_bwd<T, 128, 4>(g, c, a);
+    if (c->D <= 32) return launch_bwd<T, 32>(g, c, a);
+    if (c->D <= 64) return launch_bwd<T, 64>(g, c, a);
+    return launch_bwd<T, 128>(g, c, a);
 }
 
 constexpr int kMaxD = 256, kMaxDBwd = 128;
 
-int64_t bwd_ws_bytes(const dgm_attn_cfg* c) { return c->rows * c->H * int64_t(sizeof(float)); }
+// delta, and the parts' sums.
+int64_t delta_floats(const dgm_attn_cfg* c) { return (c->rows * c->H + 3) / 4 * 4; }
+int64_t bwd_ws_bytes(const dgm_attn_cfg* c) {
+    const int64_t parts = dkv_parts(c);
+    return (delta_floats(c) + (parts > 1 ? parts * 2 * c->rows * c->KVH * c->D : 0)) * int64_t(sizeof(float));
+}
 
 }  // namespace
 
@@ -841,7 +983,7 @@ int dgm_attnPackedFwd(dgm_gpu* g, const dgm_attn_cfg* cfg, const void* q, const 
 }
 
 int64_t dgm_attnPackedBwd_ws_bytes(const dgm_attn_cfg* cfg) {
-    if (!cfg || cfg->rows < 0 || cfg->H < 1 || cfg->rows > (int64_t(1) << 30) || cfg->H > 65536) return -1;
+    if (!cfg || check_cfg(nullptr, "", cfg, kMaxDBwd) != DGM_OK) return -1;
     return bwd_ws_bytes(cfg);
 }
 
@@ -866,9 +1008,10 @@ int dgm_attnPackedBwd(dgm_gpu* g, const dgm_attn_cfg* cfg, const void* q, const 
     OnDevice on(g->device);
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "attnPackedBwd: %s", hipGetErrorString(on.err));
     const Strides s = strides(cfg);
-    const BwdArgs a{q, k, v, out, dout, dq, dk, dv, lse, static_cast<float*>(ws), starts, g->seq_flag, cfg->rows,
-                    cfg->nseq, s.q, s.k, s.v, s.o, 0, cfg->H, cfg->KVH, cfg->D, cfg->causal != 0, cfg->scale * kLog2e,
-                    cfg->scale};
+    float* delta = static_cast<float*>(ws);
+    const BwdArgs a{q, k, v, out, dout, dq, dk, dv, lse, delta, delta + delta_floats(cfg), starts, g->seq_flag,
+                    cfg->rows, cfg->nseq, s.q, s.k, s.v, s.o, 0, cfg->H, cfg->KVH, cfg->D, cfg->causal != 0,
+                    int(dkv_parts(cfg)), cfg->scale * kLog2e, cfg->scale};
     g->seq_checks = true;
     return cfg->type == DGM_TYPE_F32 ? run_bwd<float>(g, cfg, a) : run_bwd<__bf16>(g, cfg, a);
 }
