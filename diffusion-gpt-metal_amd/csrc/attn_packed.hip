@@ -213,6 +213,13 @@ struct Frags {
             }
         }
     }
+    // Waits for the loads here: in a loop the wait would also be one for the copies that the loop starts.
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int p = 0; p < kPieces<T>; ++p)
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) asm volatile("" : "+v"(f[p][kk]));
+    }
 };
 
 // acc += A B over their pieces: for fp32 the six products that reach 2^-24 of the largest.
@@ -224,6 +231,24 @@ __device__ __forceinline__ void mfma_pieces(f32x16& acc, const bf16x8 (&a)[PA], 
         for (int i = 0; i < PA; ++i)
             if (s < 3 && s - i >= 0 && s - i < PB)
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[s - i], acc, 0, 0, 0);
+}
+
+// The order of N operand reads (P pieces each) and their products: some reads ahead of
+// the product that takes them. Left alone, the compiler reads into the registers
+// that the product before has just taken, and every product waits for its own read
+// (a prompt of 8192: 528 us so, 515 with six ahead).
+template <int P, int N>
+__device__ __forceinline__ void reads_ahead() {
+    constexpr int kRead = 0x100, kMfma = 0x8, M = P == 1 ? 1 : 6, AHEAD = P == 1 ? 6 : 2;
+    if constexpr (N > AHEAD) {
+        __builtin_amdgcn_sched_group_barrier(kRead, P * AHEAD, 0);
+#pragma unroll
+        for (int i = 0; i < N - AHEAD; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, M, 0);
+            __builtin_amdgcn_sched_group_barrier(kRead, P, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, M * AHEAD, 0);
+    }
 }
 
 // Results for the rows of a tile and a wave's 32 columns.
@@ -248,6 +273,7 @@ __device__ __forceinline__ void mm_block(f32x16& out, const uint8_t* tile, int k
         }
         mfma_pieces(out, x, y);
     }
+    reads_ahead<P, Frags<T, DP>::NK>();
 }
 // out[kb] for all blocks of a tile.
 template <typename T, int DP>
@@ -271,6 +297,7 @@ __device__ __forceinline__ void mm_rows(Blocks<T, DP>& out, const uint8_t* tile,
             mfma_pieces(out[kb], x, y);
         }
     }
+    reads_ahead<P, Frags<T, DP>::NK * L::KB>();
 }
 
 // A operand of mm_cols: element j of a lane is column d = 32 dt + lane % 32 of
@@ -470,6 +497,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2
     const int masked_from = a.causal ? rw.tile * BQ / TILE : rw.len / TILE;
     const int wave_keys = a.causal ? min(keys, q0 + 32) : keys;
 
+    qf.settle();
     bool spoilt = false;
     for (int t = 0; t < tiles; ++t) {
         const uint8_t* kt = lds[t % L::NBUF][0];
@@ -590,7 +618,8 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
         }
     delta += __shfl_xor(delta, 32, 64);
     if (in && h == 0) a.delta[int64_t(head) * a.rows + at] = delta;
-    const float lse = in ? a.lse[int64_t(head) * a.rows + at] : 0.0f;
+    float lse = in ? a.lse[int64_t(head) * a.rows + at] : 0.0f;
+    asm volatile("" : "+v"(lse), "+v"(delta));
     const int last = a.causal && in ? row : rw.len - 1;
     f32x16 acc[DT];
 #pragma unroll
@@ -599,6 +628,8 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
     const int keys = a.causal ? min(rw.len, (rw.tile + 1) * BQ) : rw.len, tiles = (keys + TILE - 1) / TILE;
     const int masked_from = a.causal ? rw.tile * BQ / TILE : rw.len / TILE;
     const int wave_keys = a.causal ? min(keys, q0 + 32) : keys;
+    qf.settle();
+    gf.settle();
     bool spoilt = false;
     for (int t = 0; t < tiles; ++t) {
         uint8_t* kt = lds[t % L::NBUF][0];
@@ -708,6 +739,8 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
 #pragma unroll
     for (int n = 0; n < DT; ++n) dk[n] = dv[n] = f32x16{};
 
+    kf.settle();
+    vf.settle();
     bool spoilt = false;
     for (int t = t0; t < t1; ++t) {
         const int row0 = now * TILE;

@@ -142,14 +142,44 @@ __device__ __forceinline__ int length_of(const DecodeArgs& a, int64_t s) {
     return n < 0 ? 0 : n > a.c.capacity ? a.c.capacity : n;
 }
 
-// Tiles of sequences 0 .. s-1 (s <= nseq), by a whole wave.
-template <int KEYS>
-__device__ inline int64_t tiles_before(const DecodeArgs& a, int64_t s) {
-    int64_t sum = 0;
-    for (int64_t i = threadIdx.x & 63; i < s; i += 64) sum += (length_of(a, i) + KEYS - 1) / KEYS;
+// All tiles of all sequences in a row, and how many a worker takes.
+struct Plan {
+    int64_t total, per;
+};
+
+// Inclusive sum over a wave's lanes.
+__device__ __forceinline__ int64_t scan(int64_t x) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, 64);
-    return sum;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up(x, d, 64);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// Sequences in runs of 64, one a lane: calls visit(first sequence, length, tiles, tiles up
+// to and with this one) run by run until it returns true.
+template <int KEYS, typename Visit>
+__device__ __forceinline__ void each_run(const DecodeArgs& a, const Visit& visit) {
+    const int lane = threadIdx.x & 63;
+    int64_t before = 0;
+    for (int64_t s0 = 0; s0 < a.nseq; s0 += 64) {
+        const int len = s0 + lane < a.nseq ? length_of(a, s0 + lane) : 0;
+        const int64_t tiles = (len + KEYS - 1) / KEYS, upto = before + scan(tiles);
+        if (visit(s0, len, tiles, upto)) return;
+        before = __shfl(upto, 63, 64);
+    }
+}
+
+template <int KEYS>
+__device__ __forceinline__ Plan plan_of(const DecodeArgs& a) {
+    int64_t total = 0;
+    each_run<KEYS>(a, [&](int64_t, int, int64_t, int64_t upto) {
+        total = __shfl(upto, 63, 64);
+        return false;
+    });
+    return {total, (total + a.workers - 1) / a.workers};
 }
 
 // VW consecutive elements of a value row in registers.
@@ -260,45 +290,37 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attn_paged_decode_kern
     const int kvh = unit / a.parts, h0 = kvh * a.G + unit % a.parts * kHeads;   // first query head
     const int heads = min(kHeads, a.G - unit % a.parts * kHeads);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-    if (blockIdx.x == 0)
+    if (blockIdx.x == gridDim.x - 1)
         for (int64_t i = threadIdx.x; i < a.nseq; i += 256)
             if (a.lens[i] > a.c.capacity) atomicOr(a.c.flag, kBadPages);
-    const int64_t total = tiles_before<KEYS>(a, a.nseq), per = (total + a.workers - 1) / a.workers;
-    int64_t at = worker * per;
-    const int64_t end = at + per < total ? at + per : total;
+    const Plan plan = plan_of<KEYS>(a);
+    int64_t at = worker * plan.per;
+    const int64_t end = at + plan.per < plan.total ? at + plan.per : plan.total;
     const uint8_t* kc = static_cast<const uint8_t*>(a.kc);
     const uint8_t* vc = static_cast<const uint8_t*>(a.vc);
     // Sequences without keys have no tile: their rows are zeros.
-    if (worker == 0)
-        for (int64_t s0 = 0; s0 < a.nseq; s0 += 64) {
-            unsigned long long none = __ballot(s0 + lane < a.nseq && length_of(a, s0 + lane) == 0);
+    if (worker == a.workers - 1)
+        each_run<KEYS>(a, [&](int64_t s0, int, int64_t tiles, int64_t) {
+            unsigned long long none = __ballot(s0 + lane < a.nseq && tiles == 0);
             for (; none; none &= none - 1)
                 for (int e = threadIdx.x; e < heads * a.c.D; e += 256)
                     static_cast<IN*>(a.out)[(s0 + __ffsll(none) - 1) * a.ldo + int64_t(h0) * a.c.D + e] = IN(0.0f);
-        }
+            return false;
+        });
     if (at >= end) return;
-    // The sequence of the first tile, and that sequence's first tile.
+    // The sequence of the first tile, its length and its own first tile.
     int64_t s = 0, base = 0;
-    for (int64_t s0 = 0;; s0 += 64) {
-        const int64_t i = s0 + lane;
-        const int64_t own = i < a.nseq ? (length_of(a, i) + KEYS - 1) / KEYS : 0;
-        int64_t sum = own;
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) {
-            const int64_t y = __shfl_up(sum, x, 64);
-            if (lane >= x) sum += y;
-        }
-        const unsigned long long past = __ballot(base + sum > at);
-        if (past) {
-            const int first = __ffsll(past) - 1;
-            s = s0 + first;
-            base += __shfl(sum - own, first, 64);
-            break;
-        }
-        base += __shfl(sum, 63, 64);
-    }
+    int len = 0;
+    each_run<KEYS>(a, [&](int64_t s0, int n, int64_t tiles, int64_t upto) {
+        const unsigned long long past = __ballot(upto > at);
+        if (!past) return false;
+        const int first = __ffsll(past) - 1;
+        s = s0 + first;
+        len = __shfl(n, first, 64);
+        base = __shfl(upto - tiles, first, 64);
+        return true;
+    });
     while (true) {
-        const int len = length_of(a, s);
         const int64_t tiles = (len + KEYS - 1) / KEYS;
         const int t0 = int(at - base), t1 = int(base + tiles < end ? tiles : end - base);
 
@@ -421,37 +443,62 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attn_paged_decode_kern
         if (at >= end) break;
         __syncthreads();
         base += tiles;
-        do ++s;
-        while (length_of(a, s) == 0);
+        do len = length_of(a, ++s);
+        while (len == 0);
     }
 }
 
 // Joins the parts of the sequences that several workers share: one workgroup a (sequence, query head).
 template <typename IN, int KEYS>
 __global__ void __launch_bounds__(256) attn_paged_join_kernel(DecodeArgs a) {
+    __shared__ float factor[kWorkers], sums[256];
     const int64_t s = blockIdx.x / a.H;
     const int head = blockIdx.x % a.H, kvh = head / a.G, of = head % a.G;
     const int unit = kvh * a.parts + of / kHeads, hd = of % kHeads;
-    const int64_t tiles = (length_of(a, s) + KEYS - 1) / KEYS;
+    int64_t base = 0, tiles = 0, total = 0;
+    each_run<KEYS>(a, [&](int64_t s0, int, int64_t n, int64_t upto) {
+        if (s >= s0 && s < s0 + 64) {
+            tiles = __shfl(n, int(s - s0), 64);
+            base = __shfl(upto, int(s - s0), 64) - tiles;
+        }
+        total = __shfl(upto, 63, 64);
+        return false;
+    });
     if (tiles == 0) return;
-    const int64_t total = tiles_before<KEYS>(a, a.nseq), per = (total + a.workers - 1) / a.workers;
-    const int64_t base = tiles_before<KEYS>(a, s), w0 = base / per, w1 = (base + tiles - 1) / per;
-    if (w0 == w1) return;
-    const int64_t slot0 = unit * (a.workers + a.nseq) + s;
+    const int64_t per = (total + a.workers - 1) / a.workers, w0 = base / per;
+    const int parts = int((base + tiles - 1) / per - w0) + 1;   // at most kWorkers
+    if (parts == 1) return;
+    const int64_t row0 = (unit * (a.workers + a.nseq) + w0 + s) * a.heads + hd;   // of the first part; heads apart
+    // Every wave: the largest maximum, the parts' factors and their sum.
     float M = kNegInf;
-    for (int64_t w = w0 + (threadIdx.x & 63); w <= w1; w += 64) M = fmaxf(M, a.stat[((slot0 + w) * a.heads + hd) * 2]);
+    for (int w = threadIdx.x & 63; w < parts; w += 64) M = fmaxf(M, a.stat[(row0 + int64_t(w) * a.heads) * 2]);
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-    for (int d = threadIdx.x; d < a.c.D; d += 256) {
-        float sum = 0.0f, x = 0.0f;
-        for (int64_t w = w0; w <= w1; ++w) {
-            const int64_t at = (slot0 + w) * a.heads + hd;
-            const float m = a.stat[at * 2], f = m == M ? 1.0f : exp2_hw((m - M) * a.scale2);
-            sum = __builtin_fmaf(a.stat[at * 2 + 1], f, sum);
-            x = __builtin_fmaf(a.part[at * a.c.D + d], f, x);
-        }
-        static_cast<IN*>(a.out)[s * a.ldo + int64_t(head) * a.c.D + d] = IN(sum == 0.0f ? 0.0f : x / sum);
+    float sum = 0.0f;
+    for (int w = threadIdx.x & 63; w < parts; w += 64) {
+        const float* st = a.stat + (row0 + int64_t(w) * a.heads) * 2;
+        const float f = st[0] == M ? 1.0f : exp2_hw((st[0] - M) * a.scale2);
+        if (threadIdx.x < 64) factor[w] = f;
+        sum = __builtin_fmaf(st[1], f, sum);
     }
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, 64);
+    __syncthreads();
+    // Columns over the threads, parts over the groups of threads that are left.
+    const int cols = a.c.D <= 32 ? 32 : a.c.D <= 64 ? 64 : a.c.D <= 128 ? 128 : 256, groups = 256 / cols;
+    const int d = threadIdx.x % cols, group = threadIdx.x / cols;
+    float x = 0.0f;
+    if (d < a.c.D) {
+        const float* part = a.part + row0 * a.c.D + d;
+        const int64_t step = int64_t(a.heads) * a.c.D;
+#pragma unroll 8
+        for (int w = group; w < parts; w += groups) x = __builtin_fmaf(part[w * step], factor[w], x);
+    }
+    sums[threadIdx.x] = x;
+    __syncthreads();
+    if (group > 0 || d >= a.c.D) return;
+    for (int i = 1; i < groups; ++i) x += sums[i * cols + d];
+    static_cast<IN*>(a.out)[s * a.ldo + int64_t(head) * a.c.D + d] = IN(sum == 0.0f ? 0.0f : x / sum);
 }
 
 // ---- host ----------------------------------------------------------------------
