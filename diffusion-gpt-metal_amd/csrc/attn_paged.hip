@@ -14,12 +14,16 @@
 //    the group as columns; P^T then is in the layout of the B operand of
 //    O^T = V^T P^T, whose A operand a lane builds from 8 keys' rows by byte
 //    permutes among its own registers. A wave takes 32 keys (16 of an fp32
-//    cache) at a time and loads those of the next round before it computes.
+//    cache) at a time, and asks for those of the next round as soon as the product
+//    that took this round's registers is issued: two waves to a SIMD then keep up to 128 KB
+//    a CU under way. 48 sequences, 708 MB: 133 us, 5.3 TB/s (with two sets of
+//    registers, which spill, 182; with three waves, which spill more, 235).
 //  * A bf16 cache meets fp32 queries as three bf16 pieces (8 bits each: all 24),
 //    and so do the probabilities, with fp32 sums: nothing of fp32 is lost. bf16
 //    queries take one piece each, P rounded to bf16. An fp32 cache runs on fp32 MFMA.
 //  * Slots behind a sequence's end, and of pages that are not the cache's, are
 //    not read: they count as zero keys with a weight of zero.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -135,6 +139,7 @@ struct DecodeArgs {
     int64_t nseq, ldq, ldo;
     int H, G, heads, parts, workers, units;   // heads of a unit; units of a key head
     float scale2;                             // scale * log2 e
+    Div share;                                // by workers
 };
 
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int64_t s) {
@@ -142,44 +147,43 @@ __device__ __forceinline__ int length_of(const DecodeArgs& a, int64_t s) {
     return n < 0 ? 0 : n > a.c.capacity ? a.c.capacity : n;
 }
 
-// All tiles of all sequences in a row, and how many a worker takes.
-struct Plan {
-    int64_t total, per;
-};
-
-// Inclusive sum over a wave's lanes.
-__device__ __forceinline__ int64_t scan(int64_t x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
+// Inclusive sum over a wave's lanes, by DPP: rows of 16, then across them.
+__device__ __forceinline__ int scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
     return x;
 }
 
-// Sequences in runs of 64, one a lane: calls visit(first sequence, length, tiles, tiles up
-// to and with this one) run by run until it returns true.
-template <int KEYS, typename Visit>
-__device__ __forceinline__ void each_run(const DecodeArgs& a, const Visit& visit) {
-    const int lane = threadIdx.x & 63;
-    int64_t before = 0;
-    for (int64_t s0 = 0; s0 < a.nseq; s0 += 64) {
-        const int len = s0 + lane < a.nseq ? length_of(a, s0 + lane) : 0;
-        const int64_t tiles = (len + KEYS - 1) / KEYS, upto = before + scan(tiles);
-        if (visit(s0, len, tiles, upto)) return;
-        before = __shfl(upto, 63, 64);
-    }
-}
-
+// A wave's view of a run of 64 sequences, one a lane: length, tiles, and tiles up to and with this one.
 template <int KEYS>
-__device__ __forceinline__ Plan plan_of(const DecodeArgs& a) {
-    int64_t total = 0;
-    each_run<KEYS>(a, [&](int64_t, int, int64_t, int64_t upto) {
-        total = __shfl(upto, 63, 64);
-        return false;
-    });
-    return {total, (total + a.workers - 1) / a.workers};
+struct Run {
+    int64_t first;
+    int len, tiles, upto;
+    __device__ __forceinline__ void load(const DecodeArgs& a, int64_t s0, int before) {
+        const int64_t s = s0 + (threadIdx.x & 63);
+        first = s0;
+        len = s < a.nseq ? length_of(a, s) : 0;
+        tiles = (len + KEYS - 1) / KEYS;
+        upto = before + scan(tiles);
+    }
+    __device__ __forceinline__ int last() const { return __builtin_amdgcn_readlane(upto, 63); }
+};
+
+// All tiles of all sequences; `run` is left on the first 64.
+template <int KEYS>
+__device__ __forceinline__ int total_tiles(const DecodeArgs& a, Run<KEYS>& run) {
+    run.load(a, 0, 0);
+    int total = run.last();
+    for (int64_t s0 = 64; s0 < a.nseq; s0 += 64) {
+        Run<KEYS> r;
+        r.load(a, s0, total);
+        total = r.last();
+    }
+    return total;
 }
 
 // VW consecutive elements of a value row in registers.
@@ -188,7 +192,7 @@ struct Piece {
     uint32_t w[BYTES / 4];
 };
 template <int BYTES>
-__device__ __forceinline__ Piece<BYTES> load_piece(const void* p, int64_t bytes) {   // those up to `bytes`
+__device__ __forceinline__ Piece<BYTES> load_piece(const void* p, int bytes) {   // those up to `bytes`
     Piece<BYTES> o{};
     if (bytes > 0) {
         if constexpr (BYTES >= 16) {
@@ -210,54 +214,51 @@ __device__ __forceinline__ Piece<BYTES> load_piece(const void* p, int64_t bytes)
     return o;
 }
 
-// One wave's 32 (16) keys on their way: rows of the cache, then the data.
+// One wave's 32 (16) keys on their way.
 template <typename CT, int DP>
 struct Round {
-    static constexpr int EB = sizeof(CT), NB = kWaveKeys<CT> / 16;   // blocks of 16 keys
+    static constexpr int EB = sizeof(CT), KEYS = kWaveKeys<CT>, NB = KEYS / 16;   // blocks of 16 keys
     static constexpr int KC = DP * EB / 64;                          // 16-byte chunks of a key to a lane
     static constexpr int VW = DP / 16, VB = VW * EB;                 // elements and bytes of a value row to a lane
     u32x4 k[NB][KC];
     Piece<VB> v[4 * NB];
-    int row;               // of key lane % (16 NB)
-    int vrow[4 * NB];      // of key 16 b + 4 g + i
 
-    // The rows of keys key0 .. of sequence s, those below len.
-    __device__ __forceinline__ void find(const Cache& c, int64_t s, int kvh, int key0, int len) {
-        const int key = key0 + (int(threadIdx.x) & (16 * NB - 1));
-        row = key < len ? c.row(s, uint32_t(key), kvh) : -1;
-        if (key < len && row < 0) atomicOr(c.flag, kBadPages);
-    }
-    __device__ __forceinline__ void load(const Cache& c, const uint8_t* kc, const uint8_t* vc) {
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        const int64_t rb = int64_t(c.D) * EB;
+    // Rows of key lane % KEYS (-1: none) for the lane's part of the keys, and of the values.
+    __device__ __forceinline__ void load_k(const Cache& c, const uint8_t* kc, int row) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const int rb = c.D * EB;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const int at = __shfl(row, 16 * b + r, 64);
+            const int at = __shfl(row, 16 * b + (lane & 15), 64);
+            const uint8_t* p = kc + int64_t(at) * rb + g * 16;
 #pragma unroll
             for (int kk = 0; kk < KC; ++kk) {
-                const int off = kk * 64 + g * 16;
                 k[b][kk] = u32x4{0, 0, 0, 0};
-                if (at >= 0 && off < rb) k[b][kk] = *reinterpret_cast<const u32x4*>(kc + at * rb + off);
+                if (at >= 0 && kk * 64 + g * 16 < rb) k[b][kk] = *reinterpret_cast<const u32x4*>(p + kk * 64);
             }
         }
+    }
+    __device__ __forceinline__ void load_v(const Cache& c, const uint8_t* vc, int row) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        const int rb = c.D * EB;
 #pragma unroll
-        for (int j = 0; j < 4 * NB; ++j) {
-            vrow[j] = __shfl(row, 16 * (j / 4) + 4 * g + j % 4, 64);
-            v[j] = load_piece<VB>(vc + vrow[j] * rb + r * VB, vrow[j] >= 0 ? rb - r * VB : 0);
+        for (int j = 0; j < 4 * NB; ++j) {   // key 16 (j / 4) + 4 g + j % 4
+            const int at = __shfl(row, 16 * (j / 4) + 4 * g + j % 4, 64);
+            v[j] = load_piece<VB>(vc + int64_t(at) * rb + r * VB, at >= 0 ? rb - r * VB : 0);
         }
     }
 };
 
-// The queries of a unit as B operand, columns = heads.
+// The queries of a unit as B operand, columns = heads, in LDS: 16 bytes a lane, chunk and piece.
 template <typename IN, typename CT, int DP>
 struct Queries {
     static constexpr int PIECES = sizeof(IN) == 4 && sizeof(CT) == 2 ? 3 : 1;
     static constexpr int KC = DP * int(sizeof(CT)) / 64;
-    u32x4 f[PIECES][KC];
-    __device__ __forceinline__ void load(const IN* q, int D, bool in) {   // q: of the lane's head
-        const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-        for (int kk = 0; kk < KC; ++kk) {
+    u32x4 f[PIECES][KC][64];
+    // Chunk kk by the wave kk % 4; q: of the lane's head.
+    __device__ __forceinline__ void load(const IN* q, int D, bool in) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6;
+        for (int kk = wave; kk < KC; kk += 4) {
             if constexpr (sizeof(CT) == 2) {
                 const int d = 32 * kk + 8 * g;
                 float x[8] = {};
@@ -265,7 +266,7 @@ struct Queries {
                 bf16x8 o[PIECES];
                 split8<PIECES>(x, o);
 #pragma unroll
-                for (int p = 0; p < PIECES; ++p) f[p][kk] = __builtin_bit_cast(u32x4, o[p]);
+                for (int p = 0; p < PIECES; ++p) f[p][kk][lane] = __builtin_bit_cast(u32x4, o[p]);
             } else {
                 const int d = 16 * kk + 4 * g;
                 f32x4 x = {};
@@ -273,96 +274,119 @@ struct Queries {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = float(q[d + i]);
                 }
-                f[0][kk] = __builtin_bit_cast(u32x4, x);
+                f[0][kk][lane] = __builtin_bit_cast(u32x4, x);
             }
         }
     }
 };
 
 template <typename IN, typename CT, int DP>
-__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attn_paged_decode_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_paged_decode_kernel(DecodeArgs a) {
     using R = Round<CT, DP>;
     using Q = Queries<IN, CT, DP>;
     constexpr int KEYS = kTileKeys<CT>, WK = kWaveKeys<CT>, NB = R::NB, VW = R::VW;
+    __shared__ Q q;
     __shared__ float part[4][kHeads][DP];
     __shared__ float stat[4][kHeads][2];
     const int unit = blockIdx.x % a.units, worker = blockIdx.x / a.units;
     const int kvh = unit / a.parts, h0 = kvh * a.G + unit % a.parts * kHeads;   // first query head
     const int heads = min(kHeads, a.G - unit % a.parts * kHeads);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-    if (blockIdx.x == gridDim.x - 1)
-        for (int64_t i = threadIdx.x; i < a.nseq; i += 256)
-            if (a.lens[i] > a.c.capacity) atomicOr(a.c.flag, kBadPages);
-    const Plan plan = plan_of<KEYS>(a);
-    int64_t at = worker * plan.per;
-    const int64_t end = at + plan.per < plan.total ? at + plan.per : plan.total;
-    const uint8_t* kc = static_cast<const uint8_t*>(a.kc);
-    const uint8_t* vc = static_cast<const uint8_t*>(a.vc);
-    // Sequences without keys have no tile: their rows are zeros.
+    Run<KEYS> run;
+    const int total = total_tiles(a, run), per = int(a.share(uint32_t(total + a.workers - 1)));
+    int at = worker * per;
+    const int end = min(at + per, total);
     if (worker == a.workers - 1)
-        each_run<KEYS>(a, [&](int64_t s0, int, int64_t tiles, int64_t) {
-            unsigned long long none = __ballot(s0 + lane < a.nseq && tiles == 0);
+        // Sequences without keys have no tile: their rows are zeros. Lengths beyond the table are reported.
+        for (int64_t s0 = 0; s0 < a.nseq; s0 += 64) {
+            const bool there = s0 + lane < a.nseq;
+            if (there && a.lens[s0 + lane] > a.c.capacity) atomicOr(a.c.flag, kBadPages);
+            unsigned long long none = __ballot(there && length_of(a, s0 + lane) == 0);
             for (; none; none &= none - 1)
                 for (int e = threadIdx.x; e < heads * a.c.D; e += 256)
                     static_cast<IN*>(a.out)[(s0 + __ffsll(none) - 1) * a.ldo + int64_t(h0) * a.c.D + e] = IN(0.0f);
-            return false;
-        });
+        }
     if (at >= end) return;
     // The sequence of the first tile, its length and its own first tile.
-    int64_t s = 0, base = 0;
-    int len = 0;
-    each_run<KEYS>(a, [&](int64_t s0, int n, int64_t tiles, int64_t upto) {
-        const unsigned long long past = __ballot(upto > at);
-        if (!past) return false;
-        const int first = __ffsll(past) - 1;
-        s = s0 + first;
-        len = __shfl(n, first, 64);
-        base = __shfl(upto - tiles, first, 64);
-        return true;
-    });
+    unsigned long long past = __ballot(run.upto > at);
+    while (!past) {
+        run.load(a, run.first + 64, run.last());
+        past = __ballot(run.upto > at);
+    }
+    const int first = __ffsll(past) - 1;
+    int64_t s = run.first + first;
+    int len = __builtin_amdgcn_readlane(run.len, first);
+    int base = __builtin_amdgcn_readlane(run.upto - run.tiles, first);
+    const uint8_t* kc = static_cast<const uint8_t*>(a.kc);
+    const uint8_t* vc = static_cast<const uint8_t*>(a.vc);
     while (true) {
-        const int64_t tiles = (len + KEYS - 1) / KEYS;
-        const int t0 = int(at - base), t1 = int(base + tiles < end ? tiles : end - base);
-
-        Q q;
+        const int tiles = (len + KEYS - 1) / KEYS;
+        const int t0 = at - base, t1 = min(tiles, end - base);
+        // The page of this lane's key (lane % WK) in tile t, read ahead; its row, -1 for none.
+        const int64_t table = s * a.c.maxPages;
+        const auto page_of = [&](int t) {
+            const int key = t * KEYS + wave * WK + (lane & (WK - 1));
+            return t < t1 && key < len ? a.c.pages[table + a.c.page(uint32_t(key))] : -1;
+        };
+        const auto row_of = [&](int t, int id) {
+            const int key = t * KEYS + wave * WK + (lane & (WK - 1));
+            if (t >= t1 || key >= len) return -1;
+            if (id < 0 || id >= a.c.numPages) {
+                atomicOr(a.c.flag, kBadPages);
+                return -1;
+            }
+            const int page = int(a.c.page.d);
+            return (id * a.c.KVH + kvh) * page + key - int(a.c.page(uint32_t(key))) * page;
+        };
+        int id1 = page_of(t0), id2 = page_of(t0 + 1);
         q.load(static_cast<const IN*>(a.q) + s * a.ldq + int64_t(h0 + col) * a.c.D, a.c.D, col < heads);
         f32x4 o[VW];
 #pragma unroll
         for (int i = 0; i < VW; ++i) o[i] = f32x4{0, 0, 0, 0};
         float m = kNegInf, l = 0.0f;
-        R now, next;
-        now.find(a.c, s, kvh, t0 * KEYS + wave * WK, len);
-        now.load(a.c, kc, vc);
-        next.find(a.c, s, kvh, (t0 + 1) * KEYS + wave * WK, t0 + 1 < t1 ? len : 0);
+        R now;
+        int row = row_of(t0, id1);
+        now.load_k(a.c, kc, row);
+        now.load_v(a.c, vc, row);
+        __syncthreads();   // the queries are there
         for (int t = t0; t < t1; ++t) {
-            if (t + 1 < t1) next.load(a.c, kc, vc);
-            next.find(a.c, s, kvh, (t + 2) * KEYS + wave * WK, t + 2 < t1 ? len : 0);
+            id1 = id2;
+            id2 = page_of(t + 2);
+            // Bit i: key i of the wave's is there.
+            const uint32_t there = uint32_t(__ballot(row >= 0)) & uint32_t((uint64_t(1) << WK) - 1);
             f32x4 sc[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                sc[b] = f32x4{0, 0, 0, 0};
+            for (int b = 0; b < NB; ++b) sc[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int kk = 0; kk < Q::KC; ++kk) {
-                    if constexpr (sizeof(CT) == 2) {
+            for (int kk = 0; kk < Q::KC; ++kk)
 #pragma unroll
-                        for (int p = Q::PIECES - 1; p >= 0; --p)
+                for (int p = Q::PIECES - 1; p >= 0; --p) {
+                    const u32x4 y = q.f[p][kk][lane];
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        if constexpr (sizeof(CT) == 2) {
                             sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, now.k[b][kk]),
-                                                                            __builtin_bit_cast(bf16x8, q.f[p][kk]),
-                                                                            sc[b], 0, 0, 0);
-                    } else {
+                                                                            __builtin_bit_cast(bf16x8, y), sc[b], 0, 0, 0);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            sc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][kk][i]),
-                                                                         __uint_as_float(q.f[0][kk][i]), sc[b], 0, 0, 0);
+                            for (int i = 0; i < 4; ++i)
+                                sc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][kk][i]),
+                                                                             __uint_as_float(y[i]), sc[b], 0, 0, 0);
+                        }
                     }
                 }
+            // The keys' registers are free for those of the next round.
+            row = row_of(t + 1, id1);
+            if (t + 1 < t1) now.load_k(a.c, kc, row);
+            if (there != uint32_t((uint64_t(1) << WK) - 1)) {
+                const uint32_t mine = there >> (4 * g);
+#pragma unroll
+                for (int j = 0; j < 4 * NB; ++j)
+                    sc[j / 4][j % 4] = mine >> (16 * (j / 4) + j % 4) & 1 ? sc[j / 4][j % 4] : kNegInf;
             }
             float mx = kNegInf;
 #pragma unroll
-            for (int j = 0; j < 4 * NB; ++j) {
-                sc[j / 4][j % 4] = now.vrow[j] >= 0 ? sc[j / 4][j % 4] : kNegInf;
-                mx = fmaxf(mx, sc[j / 4][j % 4]);
-            }
+            for (int j = 0; j < 4 * NB; ++j) mx = fmaxf(mx, sc[j / 4][j % 4]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             if (__any((mx - m) * a.scale2 > 8.0f)) {
@@ -400,7 +424,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attn_paged_decode_kern
                     for (int i = 0; i < VW; ++i)
                         o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.v[j].w[i]), p[j], o[i], 0, 0, 0);
             }
-            now = next;
+            if (t + 1 < t1) now.load_v(a.c, vc, row);
         }
         // The four waves' parts, joined: o[i][r] is column (4 g + r) VW + i of head `col`.
         l += __shfl_xor(l, 16, 64);
@@ -415,7 +439,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attn_paged_decode_kern
             for (int r = 0; r < 4; ++r) part[wave][col][(4 * g + r) * VW + i] = o[i][r];
         __syncthreads();
         const bool whole = t0 == 0 && t1 == tiles;
-        const int64_t slot = unit * (a.workers + a.nseq) + worker + s;
+        const int64_t slot = int64_t(unit) * (a.workers + a.nseq) + worker + s;
         for (int e = threadIdx.x; e < heads * DP; e += 256) {
             const int hd = e / DP, d = e % DP;
             float M = kNegInf;
@@ -455,20 +479,15 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(DecodeArgs a) {
     const int64_t s = blockIdx.x / a.H;
     const int head = blockIdx.x % a.H, kvh = head / a.G, of = head % a.G;
     const int unit = kvh * a.parts + of / kHeads, hd = of % kHeads;
-    int64_t base = 0, tiles = 0, total = 0;
-    each_run<KEYS>(a, [&](int64_t s0, int, int64_t n, int64_t upto) {
-        if (s >= s0 && s < s0 + 64) {
-            tiles = __shfl(n, int(s - s0), 64);
-            base = __shfl(upto, int(s - s0), 64) - tiles;
-        }
-        total = __shfl(upto, 63, 64);
-        return false;
-    });
+    Run<KEYS> run;
+    const int total = total_tiles(a, run), per = int(a.share(uint32_t(total + a.workers - 1)));
+    while (s >= run.first + 64) run.load(a, run.first + 64, run.last());
+    const int tiles = __builtin_amdgcn_readlane(run.tiles, int(s - run.first));
+    const int base = __builtin_amdgcn_readlane(run.upto, int(s - run.first)) - tiles;
     if (tiles == 0) return;
-    const int64_t per = (total + a.workers - 1) / a.workers, w0 = base / per;
-    const int parts = int((base + tiles - 1) / per - w0) + 1;   // at most kWorkers
+    const int w0 = base / per, parts = (base + tiles - 1) / per - w0 + 1;   // at most kWorkers
     if (parts == 1) return;
-    const int64_t row0 = (unit * (a.workers + a.nseq) + w0 + s) * a.heads + hd;   // of the first part; heads apart
+    const int64_t row0 = (int64_t(unit) * (a.workers + a.nseq) + w0 + s) * a.heads + hd;   // of the first part; heads apart
     // Every wave: the largest maximum, the parts' factors and their sum.
     float M = kNegInf;
     for (int w = threadIdx.x & 63; w < parts; w += 64) M = fmaxf(M, a.stat[(row0 + int64_t(w) * a.heads) * 2]);
@@ -503,6 +522,11 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(DecodeArgs a) {
 
 // ---- host ----------------------------------------------------------------------
 
+// Positions that a sequence's row of the table holds; tiles past the end keep within 32 bits.
+int64_t capacity_of(const dgm_cache_cfg* c) {
+    return std::min<int64_t>(c->maxPages * c->pageSize, INT_MAX - 1024);
+}
+
 int check_cache(dgm_gpu* g, const char* name, const dgm_cache_cfg* c, int64_t type, int64_t nseq) {
     if (!c) return dgm::fail(g, DGM_ERR_ARG, "%s: null configuration", name);
     if (!type_bytes(c->type) || !type_bytes(type))
@@ -512,15 +536,15 @@ int check_cache(dgm_gpu* g, const char* name, const dgm_cache_cfg* c, int64_t ty
     if (c->D % 8 != 0 || c->D > 256)
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: head dim %d is not a multiple of 8 up to 256", name, c->D);
     if (c->numPages > INT_MAX || c->maxPages > INT_MAX || nseq > 65536 ||
-        c->numPages > INT_MAX / (int64_t(c->KVH) * c->pageSize))
-        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: more than 2^31 cache rows, or too many sequences", name);
+        c->numPages > INT_MAX / (int64_t(c->KVH) * c->pageSize) ||
+        nseq * ((capacity_of(c) + 63) / 64) > INT_MAX - kWorkers)
+        return dgm::fail(g, DGM_ERR_UNSUPPORTED, "%s: more than 2^31 cache rows or table positions, or too many sequences",
+                         name);
     return DGM_OK;
 }
 
 Cache cache_of(dgm_gpu* g, const dgm_cache_cfg* c, const int32_t* pages) {
-    const int64_t most = INT_MAX - 1024;   // tiles past the end keep within 32 bits
-    const int64_t cap = c->maxPages * c->pageSize;
-    return Cache{pages, g->seq_flag, c->numPages, c->maxPages, c->KVH, c->D, int(cap < most ? cap : most),
+    return Cache{pages, g->seq_flag, c->numPages, c->maxPages, c->KVH, c->D, int(capacity_of(c)),
                  Div(uint32_t(c->pageSize))};
 }
 
@@ -645,7 +669,7 @@ int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, cons
     float* part = static_cast<float*>(ws);
     const DecodeArgs a{cache_of(g, cfg, pages), q, kcache, vcache, out, part, part + part_floats(cfg, nseq, H) * cfg->D,
                        lens, nseq, ldq, ldo, int(H), int(H / cfg->KVH), sp.heads, sp.parts, sp.workers, sp.units,
-                       scale * kLog2e};
+                       scale * kLog2e, Div(uint32_t(sp.workers))};
     g->seq_checks = true;
     if (type == DGM_TYPE_F32)
         return cfg->type == DGM_TYPE_F32 ? run_decode<float, float>(g, a) : run_decode<float, __bf16>(g, a);
