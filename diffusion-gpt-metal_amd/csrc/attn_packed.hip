@@ -401,21 +401,26 @@ __device__ __forceinline__ void spoil(f32x16 (&acc)[DT], const Marks<DP, KINDS>&
 struct Rows {
     int first, len, tile;   // the sequence's first row and length; the tile's number in it
 };
-__device__ inline bool find_rows(const int32_t* starts, int64_t nseq, int64_t rows, int per, int64_t slot, Rows& out) {
+__device__ __forceinline__ bool find_rows(const int32_t* starts, int64_t nseq, int64_t rows, int per, int64_t slot,
+                                          Rows& out) {
     const int lane = threadIdx.x & 63;
     int64_t lo = 0, n = nseq;
-    while (true) {   // 64 candidates a round
+    while (n > 64) {   // 64 candidates a round
         const int64_t step = (n + 63) / 64, at = lo + lane * step;
         const bool below = lane * step < n && slot_base(clamped(starts, at, rows), at, per) <= slot;
         const int c = __popcll(__ballot(below));
         if (c == 0) return false;
         lo += (c - 1) * step;
-        if (step == 1) break;
         n = n - (c - 1) * step < step ? n - (c - 1) * step : step;
     }
-    out.first = clamped(starts, lo, rows);
-    out.len = clamped(starts, lo + 1, rows) - out.first;
-    const int64_t tile = slot - slot_base(out.first, lo, per);
+    // The last round reads the sequences' ends beside their starts: one wait, not two.
+    const bool there = lane < n;
+    const int first = there ? clamped(starts, lo + lane, rows) : 0, end = there ? clamped(starts, lo + lane + 1, rows) : 0;
+    const int c = __popcll(__ballot(there && slot_base(first, lo + lane, per) <= slot));
+    if (c == 0) return false;
+    out.first = __builtin_amdgcn_readlane(first, c - 1);
+    out.len = __builtin_amdgcn_readlane(end, c - 1) - out.first;
+    const int64_t tile = slot - slot_base(out.first, lo + c - 1, per);
     out.tile = int(tile);
     return tile >= 0 && tile * per < out.len;
 }
@@ -466,7 +471,7 @@ __global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2
     __shared__ __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];   // k and v
     __shared__ Marks<DP, 3> marks;
     marks.init(INT_MAX);
-    if (blockIdx.x == 0) check_starts(a.starts, a.nseq, a.rows, a.flag);
+    if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
     Rows rw;
     // The last tiles of a causal sequence are the longest: they start first.
     if (!find_rows(a.starts, a.nseq, a.rows, BQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
@@ -584,7 +589,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
     __shared__ __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];   // k and v
     __shared__ Marks<DP, 1> marks;
     marks.init(INT_MAX);
-    if (blockIdx.x == 0) check_starts(a.starts, a.nseq, a.rows, a.flag);
+    if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
     Rows rw;
     if (!find_rows(a.starts, a.nseq, a.rows, BQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
     const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);

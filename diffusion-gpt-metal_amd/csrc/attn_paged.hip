@@ -53,6 +53,7 @@ struct WriteArgs {
     void *kc, *vc;
     const int32_t *starts, *lens;
     int64_t rows, nseq, ldk, ldv;
+    Div per_row;   // threads of a row
 };
 
 template <typename IN, typename CT>
@@ -87,27 +88,43 @@ __device__ __forceinline__ void convert8(const IN* from, CT* to) {
     }
 }
 
-// A thread moves 8 elements of k and of v of one (row, head).
+// A thread moves 8 elements of k and of v of one (row, head). The sequence of the
+// workgroup's first row is looked up by whole waves, 64 candidates a round; a thread's own row
+// lies in that or a later one. A write of few rows is a chain of waits: starts,
+// lengths, pages, rows.
 template <typename IN, typename CT>
 __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
-    if (blockIdx.x == 0 && a.starts) check_starts(a.starts, a.nseq, a.rows, a.c.flag);
     const int per_head = a.c.D / 8, per_row = a.c.KVH * per_head;
-    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, row = i / per_row;
-    if (row >= a.rows) return;
-    const int e = int(i % per_row), head = e / per_head, d = e % per_head * 8;
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    // 32 bits where they hold all of it: a 64-bit division is a call's worth of instructions.
+    const int64_t row = a.rows <= INT_MAX / per_row ? int64_t(a.per_row(uint32_t(i))) : i / per_row;
+    const int64_t row0 = a.rows <= INT_MAX / per_row ? int64_t(a.per_row(blockIdx.x * 256u)) : int64_t(blockIdx.x) * 256 / per_row;
     int64_t s = row, first = row;
     if (a.starts) {   // the last sequence that starts at or before the row
-        if (a.starts[0] > row) return;
-        int64_t lo = 0, hi = a.nseq;
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) / 2;
-            if (a.starts[mid] <= row) lo = mid;
-            else hi = mid;
+        const int lane = threadIdx.x & 63;
+        int64_t lo = 0, n = a.nseq;
+        while (n > 1) {
+            const int64_t step = (n + 63) / 64;
+            const int c = __popcll(__ballot(lane * step < n && a.starts[lo + lane * step] <= row0));
+            const int64_t skip = (c > 0 ? c - 1 : 0) * step;
+            lo += skip;
+            n = n - skip < step ? n - skip : step;
         }
-        if (a.starts[lo + 1] <= row) return;
-        s = lo;
+        if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.c.flag);
+        if (row >= a.rows) return;
         first = a.starts[lo];
+        int64_t next = a.starts[lo + 1];
+        while (next <= row) {
+            if (++lo == a.nseq) return;
+            first = next;
+            next = a.starts[lo + 1];
+        }
+        if (first > row) return;
+        s = lo;
+    } else if (row >= a.rows) {
+        return;
     }
+    const int e = int(i - row * per_row), head = e / per_head, d = e % per_head * 8;
     const int64_t pos = (a.lens ? int64_t(a.lens[s]) : 0) + (row - first);
     const int at = pos >= 0 && pos < a.c.capacity ? a.c.row(s, uint32_t(pos), head) : -1;
     if (at < 0) {
@@ -472,13 +489,17 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
     }
 }
 
-// Joins the parts of the sequences that several workers share: one workgroup a (sequence, query head).
+// Joins the parts of the sequences that several workers share: one workgroup a
+// (sequence, query head), columns over its threads, parts over the groups of threads that are
+// left. A thread asks for its first parts before it knows their factors: the
+// kernel is a chain of waits (lengths, maxima and sums, parts) and little else.
 template <typename IN, int KEYS>
-__global__ void __launch_bounds__(256) attn_paged_join_kernel(DecodeArgs a) {
-    __shared__ float factor[kWorkers], sums[256];
+__global__ void __launch_bounds__(1024) attn_paged_join_kernel(DecodeArgs a) {
+    constexpr int AHEAD = 8;
+    __shared__ float factor[kWorkers], sums[1024];
     const int64_t s = blockIdx.x / a.H;
     const int head = blockIdx.x % a.H, kvh = head / a.G, of = head % a.G;
-    const int unit = kvh * a.parts + of / kHeads, hd = of % kHeads;
+    const int unit = kvh * a.parts + of / kHeads, hd = of % kHeads, lane = threadIdx.x & 63;
     Run<KEYS> run;
     const int total = total_tiles(a, run), per = int(a.share(uint32_t(total + a.workers - 1)));
     while (s >= run.first + 64) run.load(a, run.first + 64, run.last());
@@ -488,31 +509,42 @@ __global__ void __launch_bounds__(256) attn_paged_join_kernel(DecodeArgs a) {
     const int w0 = base / per, parts = (base + tiles - 1) / per - w0 + 1;   // at most kWorkers
     if (parts == 1) return;
     const int64_t row0 = (int64_t(unit) * (a.workers + a.nseq) + w0 + s) * a.heads + hd;   // of the first part; heads apart
+    const int cols = a.c.D <= 32 ? 32 : a.c.D <= 64 ? 64 : a.c.D <= 128 ? 128 : 256, groups = int(blockDim.x) / cols;
+    const int d = threadIdx.x % cols, group = threadIdx.x / cols;
+    const float* part = a.part + row0 * a.c.D + d;
+    const int64_t step = int64_t(a.heads) * a.c.D;
+    float held[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        const int w = group + i * groups;
+        held[i] = w < parts && d < a.c.D ? part[w * step] : 0.0f;
+    }
     // Every wave: the largest maximum, the parts' factors and their sum.
-    float M = kNegInf;
-    for (int w = threadIdx.x & 63; w < parts; w += 64) M = fmaxf(M, a.stat[(row0 + int64_t(w) * a.heads) * 2]);
+    const float2* st = reinterpret_cast<const float2*>(a.stat) + row0;
+    const float2 mine = lane < parts ? st[int64_t(lane) * a.heads] : float2{kNegInf, 0.0f};
+    float M = mine.x;
+    for (int w = lane + 64; w < parts; w += 64) M = fmaxf(M, st[int64_t(w) * a.heads].x);
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
     float sum = 0.0f;
-    for (int w = threadIdx.x & 63; w < parts; w += 64) {
-        const float* st = a.stat + (row0 + int64_t(w) * a.heads) * 2;
-        const float f = st[0] == M ? 1.0f : exp2_hw((st[0] - M) * a.scale2);
+    for (int w = lane; w < parts; w += 64) {
+        const float2 v = w < 64 ? mine : st[int64_t(w) * a.heads];
+        const float f = v.x == M ? 1.0f : exp2_hw((v.x - M) * a.scale2);
         if (threadIdx.x < 64) factor[w] = f;
-        sum = __builtin_fmaf(st[1], f, sum);
+        sum = __builtin_fmaf(v.y, f, sum);
     }
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, 64);
     __syncthreads();
-    // Columns over the threads, parts over the groups of threads that are left.
-    const int cols = a.c.D <= 32 ? 32 : a.c.D <= 64 ? 64 : a.c.D <= 128 ? 128 : 256, groups = 256 / cols;
-    const int d = threadIdx.x % cols, group = threadIdx.x / cols;
     float x = 0.0f;
-    if (d < a.c.D) {
-        const float* part = a.part + row0 * a.c.D + d;
-        const int64_t step = int64_t(a.heads) * a.c.D;
-#pragma unroll 8
-        for (int w = group; w < parts; w += groups) x = __builtin_fmaf(part[w * step], factor[w], x);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        const int w = group + i * groups;
+        if (w < parts) x = __builtin_fmaf(held[i], factor[w], x);
     }
+    if (d < a.c.D)
+#pragma unroll 8
+        for (int w = group + AHEAD * groups; w < parts; w += groups) x = __builtin_fmaf(part[w * step], factor[w], x);
     sums[threadIdx.x] = x;
     __syncthreads();
     if (group > 0 || d >= a.c.D) return;
@@ -572,7 +604,9 @@ int run_decode(dgm_gpu* g, const DecodeArgs& a) {
     else if (a.c.D <= 128) attn_paged_decode_kernel<IN, CT, 128><<<grid, block, 0, g->stream>>>(a);
     else attn_paged_decode_kernel<IN, CT, 256><<<grid, block, 0, g->stream>>>(a);
     DGM_LAUNCH_CHECK(g, "attn_paged_decode");
-    attn_paged_join_kernel<IN, kTileKeys<CT>><<<dim3(unsigned(a.nseq * a.H)), block, 0, g->stream>>>(a);
+    // Few sequences have many parts each: 1024 threads ask for more of them at once.
+    const dim3 join(a.workers / a.nseq >= 32 ? 1024 : 256);
+    attn_paged_join_kernel<IN, kTileKeys<CT>><<<dim3(unsigned(a.nseq * a.H)), join, 0, g->stream>>>(a);
     DGM_LAUNCH_CHECK(g, "attn_paged_join");
     return DGM_OK;
 }
@@ -618,7 +652,8 @@ int dgm_cacheWrite(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, const voi
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "cacheWrite: a buffer is not 16-byte (starts, lens, pages: 4-byte) aligned");
     OnDevice on(g->device);
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "cacheWrite: %s", hipGetErrorString(on.err));
-    const WriteArgs a{cache_of(g, cfg, pages), k, v, kcache, vcache, starts, lens, rows, nseq, ldk, ldv};
+    const WriteArgs a{cache_of(g, cfg, pages), k, v, kcache, vcache, starts, lens, rows, nseq, ldk, ldv,
+                      Div(uint32_t(width / 8))};
     g->seq_checks = true;
     if (type == DGM_TYPE_F32)
         return cfg->type == DGM_TYPE_F32 ? run_write<float, float>(g, a) : run_write<float, __bf16>(g, a);
@@ -650,9 +685,9 @@ int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, cons
     if (ldq < width || ldo < width)
         return dgm::fail(g, DGM_ERR_SHAPE, "attnPagedDecode: a row stride is shorter than the row's heads");
     if (H > 65536 || (ldq | ldo) % 8 != 0 || ldq > (int64_t(1) << 31) || ldo > (int64_t(1) << 31) ||
-        nseq * H > int64_t(UINT32_MAX) / 256)
+        nseq * H > int64_t(UINT32_MAX) / 1024)
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "attnPagedDecode: strides must be multiples of 8 elements up to 2^31, "
-                                                 "sequences x heads below 2^24");
+                                                 "sequences x heads below 2^22");
     if (nseq == 0) return DGM_OK;
     if (!q || !kcache || !vcache || !pages || !lens || !out || !ws)
         return dgm::fail(g, DGM_ERR_ARG, "attnPagedDecode: null buffer");

@@ -22,10 +22,12 @@ from .abi import (DGM_MATH_BF16, DGM_MATH_FP32, AdamP, AttnCfg, BiasP, CacheCfg,
 def _ptr(t: Any) -> Optional[int]:
     if t is None:
         return None
+    if getattr(t, "is_cuda", False):   # a device tensor, what most calls pass
+        return t.data_ptr()
     if isinstance(t, int):
         return t
     if hasattr(t, "data_ptr"):
-        if hasattr(t, "is_cuda") and not t.is_cuda:
+        if hasattr(t, "is_cuda"):
             raise ValueError("buffers must live in device memory")
         return t.data_ptr()
     raise TypeError(f"cannot take a device address of {type(t).__name__}")
