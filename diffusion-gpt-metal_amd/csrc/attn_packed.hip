@@ -275,8 +275,8 @@ __device__ __forceinline__ void mm_block(f32x16& out, const uint8_t* tile, int k
     }
     reads_ahead<P, Frags<T, DP>::NK>();
 }
-// out[kb] for all blocks of a tile.
-template <typename T, int DP>
+// out[kb] for all blocks of a tile, which is part of one of ROWS rows.
+template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void mm_rows(Blocks<T, DP>& out, const uint8_t* tile, const Frags<T, DP>& b, int lane) {
     using L = Lds<T, DP>;
     constexpr int P = kPieces<T>;
@@ -293,7 +293,7 @@ __device__ __forceinline__ void mm_rows(Blocks<T, DP>& out, const uint8_t* tile,
             bf16x8 x[P];
 #pragma unroll
             for (int p = 0; p < P; ++p)
-                x[p] = *reinterpret_cast<const bf16x8*>(tile + p * L::PLANE + L::at(32 * kb + r, 2 * kk + h));
+                x[p] = *reinterpret_cast<const bf16x8*>(tile + p * Lds<T, DP, ROWS>::PLANE + L::at(32 * kb + r, 2 * kk + h));
             mfma_pieces(out[kb], x, y);
         }
     }
@@ -318,7 +318,7 @@ __device__ __forceinline__ bf16x8 read_cols(const uint8_t* plane, int kb, int st
 
 // acc[dt] (32 columns d x the wave's 32 columns) += tile^T times p, p as mm_rows
 // leaves it, taken in PB pieces.
-template <typename T, int DP, int PB>
+template <typename T, int DP, int PB, int ROWS>
 __device__ __forceinline__ void mm_cols(f32x16 (&acc)[DP / 32], const uint8_t* tile, const Blocks<T, DP>& p, int lane) {
     using L = Lds<T, DP>;
     constexpr int PA = kPieces<T>;
@@ -335,7 +335,8 @@ __device__ __forceinline__ void mm_cols(f32x16 (&acc)[DP / 32], const uint8_t* t
             for (int dt = 0; dt < DP / 32; ++dt) {
                 bf16x8 a[PA];
 #pragma unroll
-                for (int n = 0; n < PA; ++n) a[n] = read_cols<T, DP>(tile + n * L::PLANE, kb, st, dt, lane);
+                for (int n = 0; n < PA; ++n)
+                    a[n] = read_cols<T, DP>(tile + n * Lds<T, DP, ROWS>::PLANE, kb, st, dt, lane);
                 mfma_pieces(acc[dt], a, b);
             }
         }
@@ -464,27 +465,34 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DT], float
         }
 }
 
-template <typename T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) attn_packed_fwd_kernel(FwdArgs a) {
-    using L = Lds<T, DP>;
-    constexpr int NT = 64 * NW, BQ = 32 * NW, DT = DP / 32, KB = L::KB, TILE = L::kRows;
-    __shared__ __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];   // k and v
+// Waves of a workgroup: 4 blocks of 32 queries, each by KS waves that take every KS-th
+// tile of keys and are joined in the end (two_waves says when there are two).
+constexpr int kBQ = 128;
+
+template <typename T, int DP, int KS>
+__global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) attn_packed_fwd_kernel(FwdArgs a) {
+    constexpr int TILE = kTileRows<T, DP>, ROWS = KS * TILE;
+    using L = Lds<T, DP, ROWS>;
+    constexpr int NT = 256 * KS, DT = DP / 32, KB = TILE / 32;
+    constexpr int kTiles = L::NBUF * 2 * L::BYTES, kJoin = KS == 1 ? 0 : 4 * (DT * 16 + 2) * 256;
+    __shared__ __align__(16) uint8_t room[kTiles > kJoin ? kTiles : kJoin];
+    uint8_t(*lds)[2][L::BYTES] = reinterpret_cast<uint8_t(*)[2][L::BYTES]>(room);   // k and v
     __shared__ Marks<DP, 3> marks;
     marks.init(INT_MAX);
     if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
     Rows rw;
     // The last tiles of a causal sequence are the longest: they start first.
-    if (!find_rows(a.starts, a.nseq, a.rows, BQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
+    if (!find_rows(a.starts, a.nseq, a.rows, kBQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
     const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int q0 = rw.tile * BQ + wave * 32, row = q0 + (lane & 31);   // in the sequence
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave >> 2;
+    const int q0 = rw.tile * kBQ + (wave & 3) * 32, row = q0 + (lane & 31);   // in the sequence
     const bool in = row < rw.len;
     const int64_t at = int64_t(rw.first) + row;
     const T* k = static_cast<const T*>(a.k) + int64_t(rw.first) * a.ldk + int64_t(kvh) * a.D;
     const T* v = static_cast<const T*>(a.v) + int64_t(rw.first) * a.ldv + int64_t(kvh) * a.D;
-    Feed<T, DP, NT> ck(a.ldk), cv(a.ldv);
+    Feed<T, DP, NT, ROWS> ck(a.ldk), cv(a.ldv);
     const auto start = [&](int t) __attribute__((always_inline)) {
-        const int key0 = t * TILE;
+        const int key0 = t * ROWS;
         ck.start(lds[t % L::NBUF][0], k + key0 * a.ldk, rw.len - key0, a.D);
         cv.start(lds[t % L::NBUF][1], v + key0 * a.ldv, rw.len - key0, a.D);
     };
@@ -497,28 +505,28 @@ __global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2
     for (int n = 0; n < DT; ++n) o[n] = f32x16{};
     float m = kNegInf, l = 0.0f;
     const int last = a.causal && in ? row : rw.len - 1;   // the last key that the lane's query sees
-    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * BQ) : rw.len, tiles = (keys + TILE - 1) / TILE;
-    // Tiles from here on hold positions that some query of the workgroup does not see.
-    const int masked_from = a.causal ? rw.tile * BQ / TILE : rw.len / TILE;
+    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * kBQ) : rw.len, steps = (keys + ROWS - 1) / ROWS;
+    // Steps from here on hold positions that some query of the workgroup does not see.
+    const int masked_from = a.causal ? rw.tile * kBQ / ROWS : rw.len / ROWS;
     const int wave_keys = a.causal ? min(keys, q0 + 32) : keys;
 
     qf.settle();
     bool spoilt = false;
-    for (int t = 0; t < tiles; ++t) {
-        const uint8_t* kt = lds[t % L::NBUF][0];
-        uint8_t* vt = lds[t % L::NBUF][1];
+    for (int t = 0; t < steps; ++t) {
         turn(ck, cv, lds[t % L::NBUF], [&]() __attribute__((always_inline)) {
-            if (t + 1 < tiles) start(t + 1);
+            if (t + 1 < steps) start(t + 1);
         });
-        const int key0 = t * TILE;
         const bool masked = t >= masked_from;
-        if (masked && a.causal && __syncthreads_or(cv.bad(vt))) {
-            clean_tile<T, DP, NT, 3, false>(cv, vt, key0, marks);
+        if (masked && a.causal && __syncthreads_or(cv.bad(lds[t % L::NBUF][1]))) {
+            clean_tile<T, DP, NT, 3, false>(cv, lds[t % L::NBUF][1], t * ROWS, marks);
             spoilt = true;
         }
+        const int key0 = t * ROWS + kg * TILE;
         if (key0 >= wave_keys || q0 >= rw.len) continue;
+        const uint8_t* kt = lds[t % L::NBUF][0] + kg * TILE * L::RB;
+        const uint8_t* vt = lds[t % L::NBUF][1] + kg * TILE * L::RB;
         f32x16 s[KB];
-        mm_rows<T, DP>(s, kt, qf, lane);
+        mm_rows<T, DP, ROWS>(s, kt, qf, lane);
         if (masked) {
             const int lim = last - key0 - 4 * h;   // element e of block kb is seen up to here
 #pragma unroll
@@ -550,7 +558,29 @@ __global__ void __launch_bounds__(64 * NW, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2
                 sum += s[kb][e];
             }
         l += sum;
-        mm_cols<T, DP, kPieces<T>>(o, vt, s, lane);
+        mm_cols<T, DP, kPieces<T>, ROWS>(o, vt, s, lane);
+    }
+    if constexpr (KS == 2) {   // the second wave's part of a block, through LDS
+        float* part = reinterpret_cast<float*>(room) + (wave & 3) * (DT * 16 + 2) * 64 + lane;
+        __syncthreads();
+        if (kg == 1) {
+            part[0] = m;
+            part[64] = l;
+#pragma unroll
+            for (int n = 0; n < DT; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) part[(2 + n * 16 + e) * 64] = o[n][e];
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m1 = part[0], to = fmaxf(m, m1);
+        const float f0 = m == to ? 1.0f : exp2_hw((m - to) * a.c), f1 = m1 == to ? 1.0f : exp2_hw((m1 - to) * a.c);
+        m = to;
+        l = l * f0 + part[64] * f1;
+#pragma unroll
+        for (int n = 0; n < DT; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[n][e] = o[n][e] * f0 + part[(2 + n * 16 + e) * 64] * f1;
     }
     if (spoilt) spoil<DP>(o, marks, 0, [&](int r) { return r <= last; }, lane);
 
@@ -582,26 +612,29 @@ struct BwdArgs {
 
 // dq: a wave's 32 queries against tiles of 64 keys. dS^T = P^T (dP^T - delta)
 // with dP^T = V dout^T; dq^T += K^T dS^T. delta = dout . out on the way, kept for the next kernel.
-template <typename T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_dq_kernel(BwdArgs a) {
-    using L = Lds<T, DP>;
-    constexpr int NT = 64 * NW, BQ = 32 * NW, DT = DP / 32, KB = L::KB, TILE = L::kRows;
-    __shared__ __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];   // k and v
+template <typename T, int DP, int KS>
+__global__ void __launch_bounds__(256 * KS, sizeof(T) == 2 || KS == 2 ? 2 : 1) attn_packed_dq_kernel(BwdArgs a) {
+    constexpr int TILE = kTileRows<T, DP>, ROWS = KS * TILE;
+    using L = Lds<T, DP, ROWS>;
+    constexpr int NT = 256 * KS, DT = DP / 32, KB = TILE / 32;
+    constexpr int kTiles = L::NBUF * 2 * L::BYTES, kJoin = KS == 1 ? 0 : 4 * DT * 16 * 256;
+    __shared__ __align__(16) uint8_t room[kTiles > kJoin ? kTiles : kJoin];
+    uint8_t(*lds)[2][L::BYTES] = reinterpret_cast<uint8_t(*)[2][L::BYTES]>(room);   // k and v
     __shared__ Marks<DP, 1> marks;
     marks.init(INT_MAX);
     if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
     Rows rw;
-    if (!find_rows(a.starts, a.nseq, a.rows, BQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
+    if (!find_rows(a.starts, a.nseq, a.rows, kBQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
     const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int q0 = rw.tile * BQ + wave * 32, row = q0 + (lane & 31);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave >> 2;
+    const int q0 = rw.tile * kBQ + (wave & 3) * 32, row = q0 + (lane & 31);
     const bool in = row < rw.len;
     const int64_t at = int64_t(rw.first) + row;
     const T* k = static_cast<const T*>(a.k) + int64_t(rw.first) * a.ldk + int64_t(kvh) * a.D;
     const T* v = static_cast<const T*>(a.v) + int64_t(rw.first) * a.ldv + int64_t(kvh) * a.D;
-    Feed<T, DP, NT> ck(a.ldk), cv(a.ldv);
+    Feed<T, DP, NT, ROWS> ck(a.ldk), cv(a.ldv);
     const auto start = [&](int t) __attribute__((always_inline)) {
-        const int key0 = t * TILE;
+        const int key0 = t * ROWS;
         ck.start(lds[t % L::NBUF][0], k + key0 * a.ldk, rw.len - key0, a.D);
         cv.start(lds[t % L::NBUF][1], v + key0 * a.ldv, rw.len - key0, a.D);
     };
@@ -622,7 +655,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
             for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(x[j], y[j], delta);
         }
     delta += __shfl_xor(delta, 32, 64);
-    if (in && h == 0) a.delta[int64_t(head) * a.rows + at] = delta;
+    if (in && h == 0 && kg == 0) a.delta[int64_t(head) * a.rows + at] = delta;
     float lse = in ? a.lse[int64_t(head) * a.rows + at] : 0.0f;
     asm volatile("" : "+v"(lse), "+v"(delta));
     const int last = a.causal && in ? row : rw.len - 1;
@@ -630,25 +663,25 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
 #pragma unroll
     for (int n = 0; n < DT; ++n) acc[n] = f32x16{};
 
-    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * BQ) : rw.len, tiles = (keys + TILE - 1) / TILE;
-    const int masked_from = a.causal ? rw.tile * BQ / TILE : rw.len / TILE;
+    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * kBQ) : rw.len, steps = (keys + ROWS - 1) / ROWS;
+    const int masked_from = a.causal ? rw.tile * kBQ / ROWS : rw.len / ROWS;
     const int wave_keys = a.causal ? min(keys, q0 + 32) : keys;
     qf.settle();
     gf.settle();
     bool spoilt = false;
-    for (int t = 0; t < tiles; ++t) {
-        uint8_t* kt = lds[t % L::NBUF][0];
-        const uint8_t* vt = lds[t % L::NBUF][1];
+    for (int t = 0; t < steps; ++t) {
         turn(ck, cv, lds[t % L::NBUF], [&]() __attribute__((always_inline)) {
-            if (t + 1 < tiles) start(t + 1);
+            if (t + 1 < steps) start(t + 1);
         });
-        const int key0 = t * TILE;
+        const int key0 = t * ROWS + kg * TILE;
+        const uint8_t* kt = lds[t % L::NBUF][0] + kg * TILE * L::RB;
+        const uint8_t* vt = lds[t % L::NBUF][1] + kg * TILE * L::RB;
         const bool masked = t >= masked_from, active = key0 < wave_keys && q0 < rw.len;
-        const bool dirty = masked && a.causal && __syncthreads_or(ck.bad(kt));
+        const bool dirty = masked && a.causal && __syncthreads_or(ck.bad(lds[t % L::NBUF][0]));
         f32x16 s[KB], dp[KB];
         if (active) {
-            mm_rows<T, DP>(s, kt, qf, lane);
-            mm_rows<T, DP>(dp, vt, gf, lane);
+            mm_rows<T, DP, ROWS>(s, kt, qf, lane);
+            mm_rows<T, DP, ROWS>(dp, vt, gf, lane);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -665,10 +698,25 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) attn_packed_d
         }
         if (dirty) {
             __syncthreads();   // the tile has been read as it is
-            clean_tile<T, DP, NT, 1, false>(ck, kt, key0, marks);
+            clean_tile<T, DP, NT, 1, false>(ck, lds[t % L::NBUF][0], t * ROWS, marks);
             spoilt = true;
         }
-        if (active) mm_cols<T, DP, kSlopePieces<T>>(acc, kt, s, lane);
+        if (active) mm_cols<T, DP, kSlopePieces<T>, ROWS>(acc, kt, s, lane);
+    }
+    if constexpr (KS == 2) {
+        float* part = reinterpret_cast<float*>(room) + (wave & 3) * DT * 16 * 64 + lane;
+        __syncthreads();
+        if (kg == 1)
+#pragma unroll
+            for (int n = 0; n < DT; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) part[(n * 16 + e) * 64] = acc[n][e];
+        __syncthreads();
+        if (kg == 1) return;
+#pragma unroll
+        for (int n = 0; n < DT; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[n][e] += part[(n * 16 + e) * 64];
     }
     if (spoilt) spoil<DP>(acc, marks, 0, [&](int r) { return r <= last; }, lane);
     if (in) store_row<T, DT>(static_cast<T*>(a.dq) + at * a.ldq + int64_t(head) * a.D, acc, a.scale, 0, a.D, h);
@@ -925,21 +973,42 @@ int slots_of(dgm_gpu* g, const char* name, const dgm_attn_cfg* c, int per, int h
     return DGM_OK;
 }
 
-template <typename T, int DP, int NW>
+// Two waves for a block of queries halve the longest workgroup, which a launch of few
+// workgroups waits for, but all eight waves of a CU then wait for one another. bf16 gains where
+// the grid is no more than two to a CU (8 heads of 128, 2048 causal: 44 us, 36 with two; 16
+// heads, six of 1024: 49, 54). fp32, where two workgroups of four waves
+// leave less overlap, gains on any grid (16 heads of 64, 2048 and shorter: 149, 128) but not in
+// its backward, short of registers (four of 1024: 370, 376). Short sequences have nothing to share (16 of 64: 6.6, 7.5).
+template <typename T>
+bool two_waves(const dgm_attn_cfg* c, bool forward) {
+    const int64_t groups = slot_count(c->rows, c->nseq, kBQ) * c->H;
+    return c->rows / c->nseq > 128 && ((sizeof(T) == 4 && forward) || groups <= 2 * dgm::kCus);
+}
+template <typename T, int DP>
+constexpr bool kTwoWaves = DP <= (sizeof(T) == 2 ? 128 : 64);
+
+template <typename T, int DP, int KS>
 int launch_fwd(dgm_gpu* g, const dgm_attn_cfg* c, FwdArgs a) {
-    const int rc = slots_of(g, "attnPackedFwd", c, 32 * NW, c->H, 64 * NW, a.slots);
+    const int rc = slots_of(g, "attnPackedFwd", c, kBQ, c->H, 256 * KS, a.slots);
     if (rc) return rc;
-    attn_packed_fwd_kernel<T, DP, NW><<<dim3(unsigned(a.slots * c->H)), dim3(64 * NW), 0, g->stream>>>(a);
+    attn_packed_fwd_kernel<T, DP, KS><<<dim3(unsigned(a.slots * c->H)), dim3(256 * KS), 0, g->stream>>>(a);
     DGM_LAUNCH_CHECK(g, "attn_packed_fwd");
     return DGM_OK;
 }
 
+template <typename T, int DP>
+int choose_fwd(dgm_gpu* g, const dgm_attn_cfg* c, const FwdArgs& a) {
+    if constexpr (kTwoWaves<T, DP>)
+        if (two_waves<T>(c, true)) return launch_fwd<T, DP, 2>(g, c, a);
+    return launch_fwd<T, DP, 1>(g, c, a);
+}
+
 template <typename T>
 int run_fwd(dgm_gpu* g, const dgm_attn_cfg* c, const FwdArgs& a) {
-    if (c->D <= 32) return launch_fwd<T, 32, 4>(g, c, a);
-    if (c->D <= 64) return launch_fwd<T, 64, 4>(g, c, a);
-    if (c->D <= 128) return launch_fwd<T, 128, 4>(g, c, a);
-    return launch_fwd<T, 256, 4>(g, c, a);
+    if (c->D <= 32) return choose_fwd<T, 32>(g, c, a);
+    if (c->D <= 64) return choose_fwd<T, 64>(g, c, a);
+    if (c->D <= 128) return choose_fwd<T, 128>(g, c, a);
+    return choose_fwd<T, 256>(g, c, a);
 }
 
 // Keys of a workgroup of the dk, dv kernel.
@@ -958,19 +1027,31 @@ int64_t dkv_parts(const dgm_attn_cfg* c) {
     return std::max<int64_t>(1, std::min<int64_t>({16, (3 * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps / 2}));
 }
 
-template <typename T, int DP>
-int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs a) {
-    constexpr int NW = 4, NK = DkvShape<T, DP>::NW;
-    BwdArgs kv = a;
-    int rc = slots_of(g, "attnPackedBwd", c, 32 * NW, c->H, 64 * NW, a.slots);
-    if (!rc) rc = slots_of(g, "attnPackedBwd", c, DkvShape<T, DP>::BK, c->KVH * a.parts, 64 * NK, kv.slots);
+template <typename T, int DP, int KS>
+int launch_dq(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs a) {
+    const int rc = slots_of(g, "attnPackedBwd", c, kBQ, c->H, 256 * KS, a.slots);
     if (rc) return rc;
-    attn_packed_dq_kernel<T, DP, NW><<<dim3(unsigned(a.slots * c->H)), dim3(64 * NW), 0, g->stream>>>(a);
+    attn_packed_dq_kernel<T, DP, KS><<<dim3(unsigned(a.slots * c->H)), dim3(256 * KS), 0, g->stream>>>(a);
     DGM_LAUNCH_CHECK(g, "attn_packed_dq");
+    return DGM_OK;
+}
+template <typename T, int DP>
+int choose_dq(dgm_gpu* g, const dgm_attn_cfg* c, const BwdArgs& a) {
+    if constexpr (kTwoWaves<T, DP>)
+        if (two_waves<T>(c, false)) return launch_dq<T, DP, 2>(g, c, a);
+    return launch_dq<T, DP, 1>(g, c, a);
+}
+
+template <typename T, int DP>
+int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs kv) {
+    constexpr int NK = DkvShape<T, DP>::NW;
+    int rc = slots_of(g, "attnPackedBwd", c, DkvShape<T, DP>::BK, c->KVH * kv.parts, 64 * NK, kv.slots);
+    if (!rc) rc = choose_dq<T, DP>(g, c, kv);
+    if (rc) return rc;
     attn_packed_dkv_kernel<T, DP>
-        <<<dim3(unsigned(kv.slots * c->KVH * a.parts)), dim3(64 * NK), 0, g->stream>>>(kv);
+        <<<dim3(unsigned(kv.slots * c->KVH * kv.parts)), dim3(64 * NK), 0, g->stream>>>(kv);
     DGM_LAUNCH_CHECK(g, "attn_packed_dkv");
-    if (a.parts > 1) {
+    if (kv.parts > 1) {
         rc = slots_of(g, "attnPackedBwd", c, 32, c->KVH, 256, kv.slots);
         if (rc) return rc;
         attn_packed_sum_kernel<T><<<dim3(unsigned(kv.slots * c->KVH)), dim3(256), 0, g->stream>>>(kv);

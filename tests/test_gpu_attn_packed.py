@@ -74,6 +74,12 @@ FORWARD = [
     ("bf16", 3, 1, 96, [255, 256, 257], False, False, 0, 0),
     ("bf16", 12, 1, 24, [513], True, False, 0, 0),
     ("f32", 2, 2, 128, [1000], True, False, 0, 0),
+    ("bf16", 4, 2, 64, [700, 150, 65, 449], True, True, 2, 3),
+    ("f32", 4, 2, 64, [700, 150, 65, 449], True, True, 2, 3),
+    ("f32", 2, 1, 32, [385, 129, 1], False, False, 0, 4),
+    ("bf16", 2, 1, 128, [385, 129, 1], False, False, 0, 4),
+    ("bf16", 72, 8, 64, [300, 1, 640], True, False, 0, 0),      # over two workgroups to a CU
+    ("f32", 72, 8, 64, [300, 1, 640], True, False, 0, 0),
 ]
 
 
@@ -133,10 +139,11 @@ def test_sharp_scores(gpu, dgm):
 
 @pytest.mark.parametrize("type_", ["f32", "bf16"])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
-def test_masked_values_take_no_part(gpu, dgm, type_, bad):
+@pytest.mark.parametrize("mid", [131, 331])     # one wave for a block of queries, and two
+def test_masked_values_take_no_part(gpu, dgm, type_, bad, mid):
     """Infinite and NaN k, v of a token leave earlier tokens and other sequences as they are; a bad q or dout leaves later keys."""
-    lens = [50, 131, 40]
-    for what, at in (("v", 90), ("k", 90), ("v", 180), ("q", 90), ("dout", 90)):
+    lens, end = [50, mid, 40], 50 + mid
+    for what, at in (("v", 90), ("k", 90), ("v", end - 1), ("q", 90), ("dout", 90), ("v", 50 + mid // 2)):
         c = Case(dgm, type_, 4, 2, 64, lens, True)
         clean = Case(dgm, type_, 4, 2, 64, lens, True)
         getattr(c, what)[at] = bad
@@ -146,10 +153,10 @@ def test_masked_values_take_no_part(gpu, dgm, type_, bad):
             x.backward(gpu)
         gpu.end()
         others = torch.ones(c.rows, dtype=torch.bool, device="cuda")
-        others[50:181] = False
+        others[50:end] = False
         early, late = others.clone(), others.clone()
         early[50:at] = True                  # rows before the token
-        late[at + 1:181] = True              # and behind it
+        late[at + 1:end] = True              # and behind it
         rest = torch.ones_like(others)
         rest[at] = False
         clean_rows = {"v": {"out": early, "dq": early, "dk": others, "dv": others},
@@ -159,7 +166,7 @@ def test_masked_values_take_no_part(gpu, dgm, type_, bad):
         for name, rows in clean_rows.items():
             assert torch.equal(getattr(c, name)[rows], getattr(clean, name)[rows]), (what, at, name)
         if what == "v":                      # seen by the token itself and what follows it
-            o = c.out[at:181].float()
+            o = c.out[at:end].float()
             assert (o.isnan() if math.isnan(bad) else o == bad).all()
             assert not c.dq[at].float().isfinite().any()
         if what == "k":
