@@ -233,13 +233,15 @@ __device__ __forceinline__ void mfma_pieces(f32x16& acc, const bf16x8 (&a)[PA], 
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[s - i], acc, 0, 0, 0);
 }
 
+constexpr int kRead = 0x100, kMfma = 0x8;   // instruction classes of __builtin_amdgcn_sched_group_barrier
+
 // The order of N operand reads (P pieces each) and their products: some reads ahead of
 // the product that takes them. Left alone, the compiler reads into the registers
 // that the product before has just taken, and every product waits for its own read
 // (a prompt of 8192: 528 us so, 515 with six ahead).
 template <int P, int N>
 __device__ __forceinline__ void reads_ahead() {
-    constexpr int kRead = 0x100, kMfma = 0x8, M = P == 1 ? 1 : 6, AHEAD = P == 1 ? 6 : 2;
+    constexpr int M = P == 1 ? 1 : 6, AHEAD = P == 1 ? 6 : 2;
     if constexpr (N > AHEAD) {
         __builtin_amdgcn_sched_group_barrier(kRead, P * AHEAD, 0);
 #pragma unroll
@@ -255,49 +257,64 @@ __device__ __forceinline__ void reads_ahead() {
 template <typename T, int DP>
 using Blocks = f32x16[Lds<T, DP>::KB];
 
-// out (32 rows x the wave's 32 columns) = tile rows 32kb .. 32kb+31 times the columns' vectors.
-// Element r of a lane: row 32kb + 8(r/4) + 4h + r%4, column lane % 32.
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void mm_block(f32x16& out, const uint8_t* tile, int kb, const Frags<T, DP>& b, int lane) {
-    using L = Lds<T, DP, ROWS>;
-    constexpr int P = kPieces<T>;
-    const int h = lane >> 5, r = lane & 31;
-    out = f32x16{};
-#pragma unroll
-    for (int kk = 0; kk < Frags<T, DP>::NK; ++kk) {
-        bf16x8 x[P], y[P];
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            x[p] = *reinterpret_cast<const bf16x8*>(tile + p * L::PLANE + L::at(32 * kb + r, 2 * kk + h));
-            y[p] = b.f[p][kk];
-        }
-        mfma_pieces(out, x, y);
-    }
-    reads_ahead<P, Frags<T, DP>::NK>();
-}
-// out[kb] for all blocks of a tile, which is part of one of ROWS rows.
+// out[kb] (32 rows x the wave's 32 columns) = the tile's rows 32kb .. 32kb+31 times the
+// columns' vectors. Element r of a lane: row 32kb + 8(r/4) + 4h + r%4, column lane %
+// 32. The tile is part of one of ROWS rows.
 template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void mm_rows(Blocks<T, DP>& out, const uint8_t* tile, const Frags<T, DP>& b, int lane) {
-    using L = Lds<T, DP>;
-    constexpr int P = kPieces<T>;
+    using L = Lds<T, DP, ROWS>;
+    constexpr int P = kPieces<T>, KB = kTileRows<T, DP> / 32;
     const int h = lane >> 5, r = lane & 31;
 #pragma unroll
-    for (int kb = 0; kb < L::KB; ++kb) out[kb] = f32x16{};
+    for (int kb = 0; kb < KB; ++kb) out[kb] = f32x16{};
 #pragma unroll
     for (int kk = 0; kk < Frags<T, DP>::NK; ++kk) {
         bf16x8 y[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) y[p] = b.f[p][kk];
 #pragma unroll
-        for (int kb = 0; kb < L::KB; ++kb) {
+        for (int kb = 0; kb < KB; ++kb) {
             bf16x8 x[P];
 #pragma unroll
             for (int p = 0; p < P; ++p)
-                x[p] = *reinterpret_cast<const bf16x8*>(tile + p * Lds<T, DP, ROWS>::PLANE + L::at(32 * kb + r, 2 * kk + h));
+                x[p] = *reinterpret_cast<const bf16x8*>(tile + p * L::PLANE + L::at(32 * kb + r, 2 * kk + h));
             mfma_pieces(out[kb], x, y);
         }
     }
-    reads_ahead<P, Frags<T, DP>::NK * L::KB>();
+    reads_ahead<P, Frags<T, DP>::NK * KB>();
+}
+
+// The same of two tiles and two sets of vectors, for KB blocks from kb0 on.
+template <typename T, int DP, int ROWS, int KB>
+__device__ __forceinline__ void mm_rows2(f32x16 (&out)[KB], f32x16 (&out2)[KB], const uint8_t* tile, const uint8_t* tile2,
+                                         int kb0, const Frags<T, DP>& b, const Frags<T, DP>& b2, int lane) {
+    using L = Lds<T, DP, ROWS>;
+    constexpr int P = kPieces<T>;
+    const int h = lane >> 5, r = lane & 31;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) out[kb] = out2[kb] = f32x16{};
+#pragma unroll
+    for (int kk = 0; kk < Frags<T, DP>::NK; ++kk) {
+        bf16x8 y[P], y2[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            y[p] = b.f[p][kk];
+            y2[p] = b2.f[p][kk];
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const int at = L::at(32 * (kb0 + kb) + r, 2 * kk + h);
+            bf16x8 x[P], x2[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                x[p] = *reinterpret_cast<const bf16x8*>(tile + p * L::PLANE + at);
+                x2[p] = *reinterpret_cast<const bf16x8*>(tile2 + p * L::PLANE + at);
+            }
+            mfma_pieces(out[kb], x, y);
+            mfma_pieces(out2[kb], x2, y2);
+        }
+    }
+    reads_ahead<P, 2 * Frags<T, DP>::NK * KB>();
 }
 
 // A operand of mm_cols: element j of a lane is column d = 32 dt + lane % 32 of
@@ -680,8 +697,12 @@ __global__ void __launch_bounds__(256 * KS, sizeof(T) == 2 || KS == 2 ? 2 : 1) a
         const bool dirty = masked && a.causal && __syncthreads_or(ck.bad(lds[t % L::NBUF][0]));
         f32x16 s[KB], dp[KB];
         if (active) {
-            mm_rows<T, DP, ROWS>(s, kt, qf, lane);
-            mm_rows<T, DP, ROWS>(dp, vt, gf, lane);
+            if constexpr (sizeof(T) == 2) {
+                mm_rows2<T, DP, ROWS>(s, dp, kt, vt, 0, qf, gf, lane);
+            } else {   // one after the other: there are no registers for reads of both
+                mm_rows<T, DP, ROWS>(s, kt, qf, lane);
+                mm_rows<T, DP, ROWS>(dp, vt, gf, lane);
+            }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -809,9 +830,9 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
         const bool active = k0 < rw.len && !(a.causal && row0 + TILE <= k0);
         const bool dirty = hidden && __syncthreads_or(cq.bad(qt) || cg.bad(gt));
         if (active) {
-            f32x16 p, ds;
-            mm_block<T, DP, 64>(p, qt, half, kf, lane);
-            mm_block<T, DP, 64>(ds, gt, half, vf, lane);
+            f32x16 p1[1], ds1[1];
+            mm_rows2<T, DP, 64>(p1, ds1, qt, gt, half, kf, vf, lane);
+            f32x16 &p = p1[0], &ds = ds1[0];
             // Element e is row 32 half + 8(e/4) + e%4 + 4h.
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -881,6 +902,14 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
                         if (kSplitD || half == 1) mfma_pieces(dk[dt], y, sx);
                     }
                 }
+            if constexpr (sizeof(T) == 2 && kSplitD) {   // as reads_ahead, two reads to a product
+                __builtin_amdgcn_sched_group_barrier(kRead, 14, 0);
+#pragma unroll
+                for (int i = 0; i < 4 * DT * 3; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+                }
+            }
         }
         if (++now - first == per_head) now = first;
     }
