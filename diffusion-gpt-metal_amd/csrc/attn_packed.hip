@@ -415,12 +415,55 @@ __device__ __forceinline__ void spoil(f32x16 (&acc)[DT], const Marks<DP, KINDS>&
 
 // ---- rows ----------------------------------------------------------------------
 
-// The sequence and its tile behind slot `slot` of tiles of `per` rows. False where the slot has no rows.
+// The tile of `per` rows that the n-th workgroup of a head takes. False where it has no rows.
 struct Rows {
     int first, len, tile;   // the sequence's first row and length; the tile's number in it
 };
-__device__ __forceinline__ bool find_rows(const int32_t* starts, int64_t nseq, int64_t rows, int per, int64_t slot,
-                                          Rows& out) {
+
+// Sum over a wave of values >= 0, by DPP.
+__device__ __forceinline__ int wave_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Up to 64 sequences: the n-th tile in the order of falling tile numbers (kFromEnd: as
+// counted from the sequence's end), over all sequences. With a causal mask
+// that is the order of falling work, so that the longest workgroups start first.
+// sum_s max(0, tiles_s - i) tiles have number i or more; a search by bits finds the n-th's.
+template <bool kFromEnd>
+__device__ __forceinline__ bool rank_rows(const int32_t* starts, int nseq, int64_t rows, int per, int n, Rows& out) {
+    const int lane = threadIdx.x & 63;
+    const bool there = lane < nseq;
+    const int first = there ? clamped(starts, lane, rows) : 0;
+    const int len = there ? max(clamped(starts, lane + 1, rows) - first, 0) : 0;
+    const int tiles = (len + per - 1) / per;
+    if (wave_sum(tiles) <= n) return false;
+    int number = 0, bit = 1;
+    while (__ballot(tiles > bit)) bit <<= 1;
+    for (; bit; bit >>= 1)
+        if (wave_sum(max(tiles - number - bit, 0)) > n) number += bit;
+    const int before = wave_sum(max(tiles - number - 1, 0));
+    const unsigned long long with = __ballot(tiles > number);
+    const int rank = __builtin_amdgcn_mbcnt_hi(uint32_t(with >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(with), 0));
+    const unsigned long long mine = __ballot(tiles > number && rank == n - before);
+    const int s = __ffsll(mine) - 1;
+    out.first = __builtin_amdgcn_readlane(first, s);
+    out.len = __builtin_amdgcn_readlane(len, s);
+    out.tile = kFromEnd ? __builtin_amdgcn_readlane(tiles, s) - 1 - number : number;
+    return true;
+}
+
+// More: in the order of the tile slots (kFromEnd) or against it.
+template <bool kFromEnd>
+__device__ __forceinline__ bool find_rows(const int32_t* starts, int64_t nseq, int64_t rows, int per, int64_t slots,
+                                          int64_t index, Rows& out) {
+    if (nseq <= 64) return rank_rows<kFromEnd>(starts, int(nseq), rows, per, int(index), out);
+    const int64_t slot = kFromEnd ? index : slots - 1 - index;
     const int lane = threadIdx.x & 63;
     int64_t lo = 0, n = nseq;
     while (n > 64) {   // 64 candidates a round
@@ -498,8 +541,7 @@ __global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 
     marks.init(INT_MAX);
     if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
     Rows rw;
-    // The last tiles of a causal sequence are the longest: they start first.
-    if (!find_rows(a.starts, a.nseq, a.rows, kBQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
+    if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, blockIdx.x / a.H, rw)) return;
     const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave >> 2;
     const int q0 = rw.tile * kBQ + (wave & 3) * 32, row = q0 + (lane & 31);   // in the sequence
@@ -641,7 +683,7 @@ __global__ void __launch_bounds__(256 * KS, sizeof(T) == 2 || KS == 2 ? 2 : 1) a
     marks.init(INT_MAX);
     if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
     Rows rw;
-    if (!find_rows(a.starts, a.nseq, a.rows, kBQ, a.slots - 1 - blockIdx.x / a.H, rw)) return;
+    if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, blockIdx.x / a.H, rw)) return;
     const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave >> 2;
     const int q0 = rw.tile * kBQ + (wave & 3) * 32, row = q0 + (lane & 31);
@@ -779,7 +821,7 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
     marks[1].init(-1);
     Rows rw;
     const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, part = int(blockIdx.x / a.KVH % a.parts);
-    if (!find_rows(a.starts, a.nseq, a.rows, BK, blockIdx.x / a.KVH / a.parts, rw)) return;
+    if (!find_rows<true>(a.starts, a.nseq, a.rows, BK, a.slots, blockIdx.x / a.KVH / a.parts, rw)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, half = wave & 1;
     const int k0 = rw.tile * BK + wave / 2 * 32, row = k0 + (lane & 31);
     const bool in = row < rw.len;
@@ -938,7 +980,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) attn_packed_sum_kernel(BwdArgs a) {
     Rows rw;
     const int kvh = blockIdx.x % a.KVH;
-    if (!find_rows(a.starts, a.nseq, a.rows, 32, blockIdx.x / a.KVH, rw)) return;
+    if (!find_rows<true>(a.starts, a.nseq, a.rows, 32, a.slots, blockIdx.x / a.KVH, rw)) return;
     const int64_t all = a.rows * a.KVH;
     const int quads = a.D / 4;
     for (int i = threadIdx.x; i < 64 * quads; i += 256) {
