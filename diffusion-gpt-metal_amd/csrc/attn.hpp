@@ -41,19 +41,23 @@ struct OnDevice {
     OnDevice& operator=(const OnDevice&) = delete;
 };
 
-// Three bf16 pieces of 8 bits each that add up to x exactly, the high one first
-// (x's low 16 bits cut off, not rounded, so that none overflows). An infinity or
-// NaN is the last piece, which meets the other operand's first one alone.
+// Three bf16 pieces of 8 bits each (the high halves of the words) that add up to a
+// finite x exactly, the high one first: x's low 16 bits cut off, not rounded, so that none overflows.
 __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-    const float fin = fabsf(x) < __builtin_huge_valf() ? x : 0.0f;
-    hi = __float_as_uint(fin) & 0xffff0000u;
-    const float r = fin - __uint_as_float(hi);
-    mid = __float_as_uint(r) & 0xffff0000u;
-    lo = __float_as_uint(r - __uint_as_float(mid) + (x - fin)) & 0xffff0000u;
+    hi = __float_as_uint(x);
+    const float r = x - __uint_as_float(hi & 0xffff0000u);
+    mid = __float_as_uint(r);
+    lo = __float_as_uint(r - __uint_as_float(mid & 0xffff0000u));
 }
 
+// What split8 makes of an infinity or NaN among values that it takes in three pieces:
+// kSpoils: NaN in the later ones. The other two leave it the last piece alone, which
+// meets the other operand's first one only: kRare by a branch (fewer
+// instructions), kSelect without one (fewer registers).
+enum NonFinite { kSpoils, kRare, kSelect };
+
 // 8 values as PIECES bf16 pieces: the value rounded, that and what rounding left, or split3's.
-template <int PIECES>
+template <int PIECES, NonFinite kAny>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&o)[PIECES]) {
     if constexpr (PIECES < 3) {
 #pragma unroll
@@ -66,10 +70,36 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&o)[PIECES])
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             uint32_t a[3], b[3];
-            split3(x[j], a[0], a[1], a[2]);
-            split3(x[j + 1], b[0], b[1], b[2]);
+            if constexpr (kAny == kSelect) {
+                const float y0 = fabsf(x[j]) < __builtin_huge_valf() ? x[j] : 0.0f;
+                const float y1 = fabsf(x[j + 1]) < __builtin_huge_valf() ? x[j + 1] : 0.0f;
+                split3(y0, a[0], a[1], a[2]);
+                split3(y1, b[0], b[1], b[2]);
+                a[2] = __float_as_uint(__uint_as_float(a[2]) + (x[j] - y0));
+                b[2] = __float_as_uint(__uint_as_float(b[2]) + (x[j + 1] - y1));
+            } else {
+                split3(x[j], a[0], a[1], a[2]);
+                split3(x[j + 1], b[0], b[1], b[2]);
+            }
 #pragma unroll
             for (int p = 0; p < 3; ++p) w[p][j / 2] = __builtin_amdgcn_perm(b[p], a[p], 0x07060302u);
+        }
+        if constexpr (kAny == kRare) {
+            float t = 0.0f;   // NaN if any value is not finite
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t = __builtin_fmaf(x[j], 0.0f, t);
+            if (t != t) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = x[j];
+                    if (fabsf(y) < __builtin_huge_valf()) continue;
+                    const uint32_t keep = j % 2 ? 0x0000ffffu : 0xffff0000u;
+                    const uint32_t as = y != y ? 0x7fc07fc0u : y > 0.0f ? 0x7f807f80u : 0xff80ff80u;
+                    w[0][j / 2] &= keep;
+                    w[1][j / 2] &= keep;
+                    w[2][j / 2] = (w[2][j / 2] & keep) | (as & ~keep);
+                }
+            }
         }
 #pragma unroll
         for (int p = 0; p < 3; ++p) o[p] = __builtin_bit_cast(bf16x8, w[p]);

@@ -146,7 +146,7 @@ struct Feed {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(held[i][j / 4][j % 4]);
                 bf16x8 o[3];
-                split8<3>(x, o);
+                split8<3, kRare>(x, o);
 #pragma unroll
                 for (int p = 0; p < 3; ++p)
                     *reinterpret_cast<bf16x8*>(lds + p * L::PLANE + (i * NT + int(threadIdx.x)) * 16) = o[p];
@@ -207,7 +207,7 @@ struct Frags {
                 float x[8] = {};
                 if (in && d < D) load8(row + d, x);
                 bf16x8 o[3];
-                split8<3>(x, o);
+                split8<3, kSelect>(x, o);
 #pragma unroll
                 for (int p = 0; p < 3; ++p) f[p][kk] = o[p];
             }
@@ -347,7 +347,7 @@ __device__ __forceinline__ void mm_cols(f32x16 (&acc)[DP / 32], const uint8_t* t
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = p[kb][8 * st + j];
             bf16x8 b[PB];
-            split8<PB>(x, b);
+            split8<PB, kSpoils>(x, b);
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt) {
                 bf16x8 a[PA];
@@ -906,8 +906,8 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
                     y[j] = ds[8 * st + j];
                 }
                 bf16x8 px[PP], sx[PS];
-                split8<PP>(x, px);
-                split8<PS>(y, sx);
+                split8<PP, kSpoils>(x, px);
+                split8<PS, kSpoils>(y, sx);
 #pragma unroll
                 for (int n = 0; n < PP; ++n) hand[wave][n][st][lane] = px[n];
 #pragma unroll

@@ -281,7 +281,7 @@ struct Queries {
                 float x[8] = {};
                 if (in && d < D) load8(q + d, x);
                 bf16x8 o[PIECES];
-                split8<PIECES>(x, o);
+                split8<PIECES, kSelect>(x, o);
 #pragma unroll
                 for (int p = 0; p < PIECES; ++p) f[p][kk][lane] = __builtin_bit_cast(u32x4, o[p]);
             } else {
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
             }
             if constexpr (sizeof(CT) == 2) {
                 bf16x8 w[Q::PIECES];
-                split8<Q::PIECES>(p, w);
+                split8<Q::PIECES, kSpoils>(p, w);
 #pragma unroll
                 for (int i = 0; i < VW; ++i) {
                     const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
