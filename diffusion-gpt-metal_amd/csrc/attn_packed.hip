@@ -75,6 +75,9 @@ struct Lds {
     static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
 };
 
+// The value of the first lane, for one that all share: the copies' instructions want it in scalar registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
+
 // A workgroup's way of bringing tiles to LDS. Each thread has N chunks of 8 columns, at
 // 16 bytes x its number from the tile's (a plane's) start.
 //
@@ -110,7 +113,10 @@ struct Feed {
                 }
             }
         } else {
-            const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>(lds)) + uint32_t(wave) * 1024u;
+            const uint32_t base = uniform(uint32_t(reinterpret_cast<uintptr_t>(lds)) + uint32_t(wave) * 1024u);
+            const uint64_t at = reinterpret_cast<uintptr_t>(from);
+            const uint8_t* const first = reinterpret_cast<const uint8_t*>(
+                uint64_t(uniform(uint32_t(at >> 32))) << 32 | uniform(uint32_t(at)));
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
             if (rows >= L::kRows && D == DP) {
@@ -119,7 +125,7 @@ struct Feed {
                     const uint32_t off =
                         uint32_t(row) * uint32_t(ldb) + uint32_t((slot ^ L::swizzle(row + i * STEP)) << 4);
                     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(base + i * NT * 16),
-                                 "v"(off), "s"(src + i * STEP * ldb)
+                                 "v"(off), "s"(first + i * STEP * ldb)
                                  : "memory", "m0");
                 }
             } else {
@@ -672,19 +678,26 @@ struct BwdArgs {
 // dq: a wave's 32 queries against tiles of 64 keys. dS^T = P^T (dP^T - delta)
 // with dP^T = V dout^T; dq^T += K^T dS^T. delta = dout . out on the way, kept for the next kernel.
 template <typename T, int DP, int KS>
-__global__ void __launch_bounds__(256 * KS, sizeof(T) == 2 || KS == 2 ? 2 : 1) attn_packed_dq_kernel(BwdArgs a) {
+struct DqRoom {
+    using L = Lds<T, DP, KS * kTileRows<T, DP>>;
+    static constexpr int kTiles = L::NBUF * 2 * L::BYTES, kJoin = KS == 1 ? 0 : 4 * (DP / 32) * 16 * 256;
+    __align__(16) uint8_t room[kTiles > kJoin ? kTiles : kJoin];
+    Marks<DP, 1> marks;
+};
+
+template <typename T, int DP, int KS>
+__device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<T, DP, KS>& sh, uint32_t index, bool last_block) {
     constexpr int TILE = kTileRows<T, DP>, ROWS = KS * TILE;
     using L = Lds<T, DP, ROWS>;
     constexpr int NT = 256 * KS, DT = DP / 32, KB = TILE / 32;
-    constexpr int kTiles = L::NBUF * 2 * L::BYTES, kJoin = KS == 1 ? 0 : 4 * DT * 16 * 256;
-    __shared__ __align__(16) uint8_t room[kTiles > kJoin ? kTiles : kJoin];
+    uint8_t* const room = sh.room;
     uint8_t(*lds)[2][L::BYTES] = reinterpret_cast<uint8_t(*)[2][L::BYTES]>(room);   // k and v
-    __shared__ Marks<DP, 1> marks;
+    Marks<DP, 1>& marks = sh.marks;
     marks.init(INT_MAX);
-    if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
+    if (last_block) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
     Rows rw;
-    if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, blockIdx.x / a.H, rw)) return;
-    const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
+    if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, index / a.H, rw)) return;
+    const int head = head_of(index % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave >> 2;
     const int q0 = rw.tile * kBQ + (wave & 3) * 32, row = q0 + (lane & 31);
     const bool in = row < rw.len;
@@ -785,6 +798,12 @@ __global__ void __launch_bounds__(256 * KS, sizeof(T) == 2 || KS == 2 ? 2 : 1) a
     if (in) store_row<T, DT>(static_cast<T*>(a.dq) + at * a.ldq + int64_t(head) * a.D, acc, a.scale, 0, a.D, h);
 }
 
+template <typename T, int DP, int KS>
+__global__ void __launch_bounds__(256 * KS, sizeof(T) == 2 || KS == 2 ? 2 : 1) attn_packed_dq_kernel(BwdArgs a) {
+    __shared__ DqRoom<T, DP, KS> room;
+    dq_body<T, DP, KS>(a, room, blockIdx.x, blockIdx.x == gridDim.x - 1);
+}
+
 // dk, dv: a pair of waves' 32 keys as columns against tiles of 64 queries, over the query heads
 // of the group one after the other. S = Q K^T, dP = dout V^T; dv^T += dout^T P, dk^T += Q^T dS.
 //
@@ -806,22 +825,31 @@ struct DkvShape {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 && DP == 128 ? 1 : 2))
-    attn_packed_dkv_kernel(BwdArgs a) {
+struct DkvRoom {
+    using L = Lds<T, DP, 64>;
+    __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];                                  // q and dout
+    bf16x8 hand[DkvShape<T, DP>::NW][kPieces<T> + kSlopePieces<T>][2][64];            // P and dS, by wave, piece, 16 rows
+    __align__(16) float stat[2][2][64];                                               // lse and delta, of two tiles
+    Marks<DP, 1> marks[2];
+};
+
+// kOwnDelta: delta from out and dout here, not from the dq kernel.
+template <typename T, int DP, bool kOwnDelta>
+__device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, uint32_t index) {
     using L = Lds<T, DP, 64>;
     constexpr int NW = DkvShape<T, DP>::NW, NT = 64 * NW, BK = DkvShape<T, DP>::BK, TILE = 64;
     constexpr int PP = kPieces<T>, PS = kSlopePieces<T>;
     constexpr bool kSplitD = DP > 32;              // else the pair's waves take dv and dk, one each
     constexpr int DT = kSplitD ? DP / 64 : 1;      // blocks of 32 columns of a wave
-    __shared__ __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];    // q and dout
-    __shared__ bf16x8 hand[NW][PP + PS][2][64];                    // P and dS, by wave, piece, 16 rows
-    __shared__ __align__(16) float stat[2][2][TILE];               // lse and delta, of two tiles
-    __shared__ Marks<DP, 1> marks[2];
+    auto& lds = sh.lds;
+    auto& hand = sh.hand;
+    auto& stat = sh.stat;
+    auto& marks = sh.marks;
     marks[0].init(-1);
     marks[1].init(-1);
     Rows rw;
-    const int kvh = blockIdx.x % a.KVH, G = a.H / a.KVH, part = int(blockIdx.x / a.KVH % a.parts);
-    if (!find_rows<true>(a.starts, a.nseq, a.rows, BK, a.slots, blockIdx.x / a.KVH / a.parts, rw)) return;
+    const int kvh = index % a.KVH, G = a.H / a.KVH, part = int(index / a.KVH % a.parts);
+    if (!find_rows<true>(a.starts, a.nseq, a.rows, BK, a.slots, index / a.KVH / a.parts, rw)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, half = wave & 1;
     const int k0 = rw.tile * BK + wave / 2 * 32, row = k0 + (lane & 31);
     const bool in = row < rw.len;
@@ -831,17 +859,54 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
     Feed<T, DP, NT, 64> cq(a.ldq), cg(a.ldo);
     static_assert(NT >= 2 * TILE, "a thread stages one statistic");
     int head = kvh * G + t0 / per_head, tile = first + t0 % per_head, now = tile;   // of the next copy; computed on
+    struct Raw8 {
+        u32x4 w[sizeof(T) / 2];
+    };
+    float stat_held = 0.0f;
+    Raw8 grad_held[kOwnDelta ? DP / 32 : 1], out_held[kOwnDelta ? DP / 32 : 1];
+    const auto store_stat = [&](int t) __attribute__((always_inline)) {
+        if (threadIdx.x < (kOwnDelta ? TILE : 2 * TILE)) stat[t % 2][threadIdx.x / TILE][threadIdx.x & (TILE - 1)] = stat_held;
+        if constexpr (kOwnDelta) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                float x[8], y[8];
+                load8(reinterpret_cast<const T*>(&grad_held[i]), x);
+                load8(reinterpret_cast<const T*>(&out_held[i]), y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(x[j], y[j], sum);
+            }
+            sum += __shfl_xor(sum, 1, 64);
+            sum += __shfl_xor(sum, 2, 64);
+            if ((threadIdx.x & 3) == 0) stat[t % 2][1][threadIdx.x / 4] = sum;
+        }
+    };
     const auto start = [&](int t) __attribute__((always_inline)) {
         const int row0 = tile * TILE;
         const int64_t r0 = int64_t(rw.first) + row0;
+        // First, and kept in registers until the tile's turn: a wait for these is one for all that was asked for before.
+        if (threadIdx.x < (kOwnDelta ? TILE : 2 * TILE)) {
+            const int r = threadIdx.x & (TILE - 1);
+            const float* from = threadIdx.x < TILE ? a.lse : a.delta;
+            stat_held = row0 + r < rw.len ? from[int64_t(head) * a.rows + r0 + r] : 0.0f;
+        }
+        if constexpr (kOwnDelta) {   // 4 lanes a row
+            static_assert(NT == 4 * TILE, "every thread has a quarter of a row");
+            const int r = threadIdx.x / 4;
+            const int64_t from = (r0 + r) * a.ldo + int64_t(head) * a.D;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                const int d = 32 * i + 8 * (threadIdx.x & 3);
+                grad_held[i] = out_held[i] = {};
+                if (row0 + r < rw.len && d < a.D) {
+                    grad_held[i] = *reinterpret_cast<const Raw8*>(static_cast<const T*>(a.dout) + from + d);
+                    out_held[i] = *reinterpret_cast<const Raw8*>(static_cast<const T*>(a.out) + from + d);
+                }
+            }
+        }
         cq.start(lds[t % L::NBUF][0], static_cast<const T*>(a.q) + r0 * a.ldq + int64_t(head) * a.D, rw.len - row0, a.D);
         cg.start(lds[t % L::NBUF][1], static_cast<const T*>(a.dout) + r0 * a.ldo + int64_t(head) * a.D, rw.len - row0,
                  a.D);
-        if (threadIdx.x < 2 * TILE) {
-            const int r = threadIdx.x & (TILE - 1);
-            const float* from = threadIdx.x < TILE ? a.lse : a.delta;
-            stat[t % 2][threadIdx.x / TILE][r] = row0 + r < rw.len ? from[int64_t(head) * a.rows + r0 + r] : 0.0f;
-        }
         if (++tile - first == per_head) {
             tile = first;
             ++head;
@@ -864,6 +929,7 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
         uint8_t* gt = lds[t % L::NBUF][1];
         const float* lse = stat[t % 2][0] + 32 * half + 4 * h;
         const float* delta = stat[t % 2][1] + 32 * half + 4 * h;
+        store_stat(t);
         turn(cq, cg, lds[t % L::NBUF], [&]() __attribute__((always_inline)) {
             if (t + 1 < t1) start(t + 1);
         });
@@ -972,6 +1038,30 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
     }
     if (mine_k) store_row<T, DT>(static_cast<T*>(a.dk) + at * a.ldk + int64_t(kvh) * a.D, dk, a.scale, d0, a.D, h);
     if (mine_v) store_row<T, DT>(static_cast<T*>(a.dv) + at * a.ldv + int64_t(kvh) * a.D, dv, 1.0f, d0, a.D, h);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 && DP == 128 ? 1 : 2))
+    attn_packed_dkv_kernel(BwdArgs a) {
+    __shared__ DkvRoom<T, DP> room;
+    dkv_body<T, DP, false>(a, room, blockIdx.x);
+}
+
+// Both in one launch, a workgroup one or the other, for grids that the chip holds at once:
+// forward and backward of 16 sequences of 64 (4 heads of 32, fp32) take 15 us so, 22 in three launches.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, 2) attn_packed_grads_kernel(BwdArgs a, uint32_t first, int64_t dkv_slots) {
+    __shared__ union Room {
+        DqRoom<T, DP, 1> dq;
+        DkvRoom<T, DP> dkv;
+        __device__ Room() {}
+    } room;
+    if (blockIdx.x < first) {
+        dq_body<T, DP, 1>(a, room.dq, blockIdx.x, blockIdx.x == first - 1);
+    } else {
+        a.slots = dkv_slots;
+        dkv_body<T, DP, true>(a, room.dkv, blockIdx.x - first);
+    }
 }
 
 // The parts' sums of dk and dv, added in order: a workgroup takes 32 rows of one
@@ -1089,12 +1179,26 @@ int dkv_keys(const dgm_attn_cfg* c) {
     return c->D <= 32 ? DkvShape<float, 32>::BK : c->D <= 64 ? DkvShape<float, 64>::BK : DkvShape<float, 128>::BK;
 }
 
+// dq and dk, dv can go in one launch: with as many threads to a workgroup, and no more
+// workgroups than two to a CU.
+template <typename T, int DP>
+constexpr bool kOneLaunch = DkvShape<T, DP>::NW == 4 && DP <= 64;
+bool one_launch(const dgm_attn_cfg* c) {
+    const bool fits = c->D <= 32 || (c->D <= 64 && c->type == DGM_TYPE_BF16);
+    return fits && slot_count(c->rows, c->nseq, kBQ) * c->H + slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH <=
+                       2 * dgm::kCus;
+}
+
 // Workgroups that share a key tile's steps: enough for three to a CU, each with two
 // steps or more at the sequences' average length (four blocks of 2048, 544 causal tiles: 336 us
-// whole; two parts 279 and 28 for the sums).
+// whole; two parts 279 and 28 for the sums). One launch for dq, dk and dv is worth more than
+// parts of a few steps: dq then runs beside them. fp32, 4 heads of 32 over four times 256, 41 us in
+// parts, 28 whole; bf16, 4 heads of 64 over 1024, 62 and 47; but 8 query heads
+// on 2 over 900 rows 40 and 50.
 int64_t dkv_parts(const dgm_attn_cfg* c) {
     const int64_t tiles = slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH;
     const int64_t steps = (c->rows / std::max<int64_t>(c->nseq, 1) + 63) / 64 * (c->H / c->KVH);
+    if (steps <= (c->H == c->KVH ? 16 : 4) && one_launch(c)) return 1;
     return std::max<int64_t>(1, std::min<int64_t>({16, (3 * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps / 2}));
 }
 
@@ -1117,7 +1221,19 @@ template <typename T, int DP>
 int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs kv) {
     constexpr int NK = DkvShape<T, DP>::NW;
     int rc = slots_of(g, "attnPackedBwd", c, DkvShape<T, DP>::BK, c->KVH * kv.parts, 64 * NK, kv.slots);
-    if (!rc) rc = choose_dq<T, DP>(g, c, kv);
+    if (rc) return rc;
+    if constexpr (kOneLaunch<T, DP>) {
+        if (kv.parts == 1 && one_launch(c)) {
+            BwdArgs q = kv;
+            q.slots = slot_count(c->rows, c->nseq, kBQ);
+            const int64_t first = q.slots * c->H, all = first + kv.slots * c->KVH;
+            attn_packed_grads_kernel<T, DP>
+                <<<dim3(unsigned(all)), dim3(256), 0, g->stream>>>(q, uint32_t(first), kv.slots);
+            DGM_LAUNCH_CHECK(g, "attn_packed_grads");
+            return DGM_OK;
+        }
+    }
+    rc = choose_dq<T, DP>(g, c, kv);
     if (rc) return rc;
     attn_packed_dkv_kernel<T, DP>
         <<<dim3(unsigned(kv.slots * c->KVH * kv.parts)), dim3(64 * NK), 0, g->stream>>>(kv);
