@@ -1,6 +1,6 @@
 // Shared by the attention kernels over packed sequences and over a paged cache
-// (attn_packed.hip, attn_paged.hip): element types, 16-byte loads, the status
-// flag that dgm_end reads.
+// (attn_packed.hip, attn_paged.hip): element types, 16-byte loads, what
+// dgm_end is told.
 #pragma once
 #include "attn_index.hpp"
 #include "common.hpp"
@@ -16,8 +16,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// Bits of the device's sequence flag (dgm_gpu::seq_flag).
-constexpr uint32_t kBadStarts = 1, kBadPages = 2;
+// Words of the context's report (dgm_gpu::seq_report), which dgm_end reads.
+constexpr int kBadStarts = 0, kBadPages = 1;
+
+__device__ __forceinline__ void report(uint32_t* words, int which) {
+    __hip_atomic_store(words + which, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }   // 2^x to about an ulp
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }
@@ -124,14 +128,14 @@ __device__ __forceinline__ void load8(const IN* p, float (&x)[8]) {
 
 inline int type_bytes(int64_t type) { return type == DGM_TYPE_F32 ? 4 : type == DGM_TYPE_BF16 ? 2 : 0; }
 
-// starts[0 .. nseq] is in order and within [0, rows]; else the flag is set. Run by one workgroup.
-__device__ inline void check_starts(const int32_t* starts, int64_t nseq, int64_t rows, uint32_t* flag) {
+// starts[0 .. nseq] is in order and within [0, rows]; else it is reported. Run by one workgroup.
+__device__ inline void check_starts(const int32_t* starts, int64_t nseq, int64_t rows, uint32_t* words) {
     bool bad = false;
     for (int64_t i = threadIdx.x; i <= nseq; i += blockDim.x) {
         const int32_t s = starts[i];
         bad = bad || s < 0 || s > rows || (i > 0 && s < starts[i - 1]);
     }
-    if (bad) atomicOr(flag, kBadStarts);
+    if (bad) report(words, kBadStarts);
 }
 
 }  // namespace dgm_attn

@@ -457,6 +457,7 @@ __device__ __forceinline__ bool rank_rows(const int32_t* starts, int nseq, int64
     const unsigned long long with = __ballot(tiles > number);
     const int rank = __builtin_amdgcn_mbcnt_hi(uint32_t(with >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(with), 0));
     const unsigned long long mine = __ballot(tiles > number && rank == n - before);
+    if (!mine) return false;   // starts out of order, whose tiles add up to more than 32 bits
     const int s = __ffsll(mine) - 1;
     out.first = __builtin_amdgcn_readlane(first, s);
     out.len = __builtin_amdgcn_readlane(len, s);
@@ -497,7 +498,7 @@ struct FwdArgs {
     void* out;
     float* lse;
     const int32_t* starts;
-    uint32_t* flag;
+    uint32_t* report;
     int64_t rows, nseq, ldq, ldk, ldv, ldo, slots;
     int H, KVH, D, causal;
     float c;   // scale * log2 e
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 
     uint8_t(*lds)[2][L::BYTES] = reinterpret_cast<uint8_t(*)[2][L::BYTES]>(room);   // k and v
     __shared__ Marks<DP, 3> marks;
     marks.init(INT_MAX);
-    if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
+    if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.report);   // one with little to do
     Rows rw;
     if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, blockIdx.x / a.H, rw)) return;
     const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
@@ -669,7 +670,7 @@ struct BwdArgs {
     float* delta;   // [H, rows]
     float* sums;    // [parts][dk, dv][rows, KVH, D], with several parts
     const int32_t* starts;
-    uint32_t* flag;
+    uint32_t* report;
     int64_t rows, nseq, ldq, ldk, ldv, ldo, slots;
     int H, KVH, D, causal, parts;
     float c, scale;
@@ -694,7 +695,7 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<T, DP, KS>& sh,
     uint8_t(*lds)[2][L::BYTES] = reinterpret_cast<uint8_t(*)[2][L::BYTES]>(room);   // k and v
     Marks<DP, 1>& marks = sh.marks;
     marks.init(INT_MAX);
-    if (last_block) check_starts(a.starts, a.nseq, a.rows, a.flag);   // one with little to do
+    if (last_block) check_starts(a.starts, a.nseq, a.rows, a.report);   // one with little to do
     Rows rw;
     if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, index / a.H, rw)) return;
     const int head = head_of(index % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
@@ -1282,9 +1283,8 @@ int dgm_attnPackedFwd(dgm_gpu* g, const dgm_attn_cfg* cfg, const void* q, const 
     OnDevice on(g->device);
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "attnPackedFwd: %s", hipGetErrorString(on.err));
     const Strides s = strides(cfg);
-    FwdArgs a{q, k, v, out, lse, starts, g->seq_flag, cfg->rows, cfg->nseq, s.q, s.k, s.v, s.o, 0, cfg->H, cfg->KVH,
+    FwdArgs a{q, k, v, out, lse, starts, g->seq_report, cfg->rows, cfg->nseq, s.q, s.k, s.v, s.o, 0, cfg->H, cfg->KVH,
               cfg->D, cfg->causal != 0, cfg->scale * kLog2e};
-    g->seq_checks = true;
     return cfg->type == DGM_TYPE_F32 ? run_fwd<float>(g, cfg, a) : run_fwd<__bf16>(g, cfg, a);
 }
 
@@ -1315,10 +1315,9 @@ int dgm_attnPackedBwd(dgm_gpu* g, const dgm_attn_cfg* cfg, const void* q, const 
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "attnPackedBwd: %s", hipGetErrorString(on.err));
     const Strides s = strides(cfg);
     float* delta = static_cast<float*>(ws);
-    const BwdArgs a{q, k, v, out, dout, dq, dk, dv, lse, delta, delta + delta_floats(cfg), starts, g->seq_flag,
+    const BwdArgs a{q, k, v, out, dout, dq, dk, dv, lse, delta, delta + delta_floats(cfg), starts, g->seq_report,
                     cfg->rows, cfg->nseq, s.q, s.k, s.v, s.o, 0, cfg->H, cfg->KVH, cfg->D, cfg->causal != 0,
                     int(dkv_parts(cfg)), cfg->scale * kLog2e, cfg->scale};
-    g->seq_checks = true;
     return cfg->type == DGM_TYPE_F32 ? run_bwd<float>(g, cfg, a) : run_bwd<__bf16>(g, cfg, a);
 }
 

@@ -35,7 +35,7 @@ using namespace dgm_attn;
 
 struct Cache {
     const int32_t* pages;
-    uint32_t* flag;
+    uint32_t* words;   // the report
     int64_t numPages, maxPages;
     int KVH, D, capacity;   // positions that a sequence's row of the table holds
     Div page;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
             lo += skip;
             n = n - skip < step ? n - skip : step;
         }
-        if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.c.flag);
+        if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.c.words);
         if (row >= a.rows) return;
         first = a.starts[lo];
         int64_t next = a.starts[lo + 1];
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
     const int64_t pos = (a.lens ? int64_t(a.lens[s]) : 0) + (row - first);
     const int at = pos >= 0 && pos < a.c.capacity ? a.c.row(s, uint32_t(pos), head) : -1;
     if (at < 0) {
-        if (e == 0) atomicOr(a.c.flag, kBadPages);
+        if (e == 0) report(a.c.words, kBadPages);
         return;
     }
     const int64_t to = int64_t(at) * a.c.D + d;
@@ -173,6 +173,11 @@ __device__ __forceinline__ int scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
     return x;
+}
+
+// What a head's sums come to, its largest score M.
+__device__ __forceinline__ float quotient(float x, float sum, float M) {
+    return sum == 0.0f ? 0.0f : M == kNegInf ? __builtin_nanf("") : x / sum;
 }
 
 // A wave's view of a run of 64 sequences, one a lane: length, tiles, and tiles up to and with this one.
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
         // Sequences without keys have no tile: their rows are zeros. Lengths beyond the table are reported.
         for (int64_t s0 = 0; s0 < a.nseq; s0 += 64) {
             const bool there = s0 + lane < a.nseq;
-            if (there && a.lens[s0 + lane] > a.c.capacity) atomicOr(a.c.flag, kBadPages);
+            if (there && a.lens[s0 + lane] > a.c.capacity) report(a.c.words, kBadPages);
             unsigned long long none = __ballot(there && length_of(a, s0 + lane) == 0);
             for (; none; none &= none - 1)
                 for (int e = threadIdx.x; e < heads * a.c.D; e += 256)
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
             const int key = t * KEYS + wave * WK + (lane & (WK - 1));
             if (t >= t1 || key >= len) return -1;
             if (id < 0 || id >= a.c.numPages) {
-                atomicOr(a.c.flag, kBadPages);
+                report(a.c.words, kBadPages);
                 return -1;
             }
             const int page = int(a.c.page.d);
@@ -361,6 +366,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
 #pragma unroll
         for (int i = 0; i < VW; ++i) o[i] = f32x4{0, 0, 0, 0};
         float m = kNegInf, l = 0.0f;
+        bool seen = false;   // a key
         R now;
         int row = row_of(t0, id1);
         now.load_k(a.c, kc, row);
@@ -371,6 +377,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
             id2 = page_of(t + 2);
             // Bit i: key i of the wave's is there.
             const uint32_t there = uint32_t(__ballot(row >= 0)) & uint32_t((uint64_t(1) << WK) - 1);
+            seen = seen || there;
             f32x4 sc[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) sc[b] = f32x4{0, 0, 0, 0};
@@ -446,6 +453,9 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
         // The four waves' parts, joined: o[i][r] is column (4 g + r) VW + i of head `col`.
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
+        // Keys whose scores are all -inf: no softmax, and not the zeros of no keys. Beside
+        // any other score the factor of this sum is 0.
+        if (seen && m == kNegInf && l == 0.0f) l = 1.0f;
         if (g == 0) {
             stat[wave][col][0] = m;
             stat[wave][col][1] = l;
@@ -471,7 +481,7 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
             }
             if (d >= a.c.D) continue;
             if (whole) {
-                static_cast<IN*>(a.out)[s * a.ldo + int64_t(h0 + hd) * a.c.D + d] = IN(sum == 0.0f ? 0.0f : x / sum);
+                static_cast<IN*>(a.out)[s * a.ldo + int64_t(h0 + hd) * a.c.D + d] = IN(quotient(x, sum, M));
             } else {
                 a.part[(slot * a.heads + hd) * a.c.D + d] = x;
                 if (d == 0) {
@@ -549,7 +559,7 @@ __global__ void __launch_bounds__(1024) attn_paged_join_kernel(DecodeArgs a) {
     __syncthreads();
     if (group > 0 || d >= a.c.D) return;
     for (int i = 1; i < groups; ++i) x += sums[i * cols + d];
-    static_cast<IN*>(a.out)[s * a.ldo + int64_t(head) * a.c.D + d] = IN(sum == 0.0f ? 0.0f : x / sum);
+    static_cast<IN*>(a.out)[s * a.ldo + int64_t(head) * a.c.D + d] = IN(quotient(x, sum, M));
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -575,8 +585,11 @@ int check_cache(dgm_gpu* g, const char* name, const dgm_cache_cfg* c, int64_t ty
     return DGM_OK;
 }
 
+// A workgroup of up to 1024 threads for each, in hipLaunchKernel's bound on a grid's threads.
+bool heads_fit(int64_t nseq, int64_t H) { return H <= 65536 && nseq * H <= int64_t(UINT32_MAX) / 1024; }
+
 Cache cache_of(dgm_gpu* g, const dgm_cache_cfg* c, const int32_t* pages) {
-    return Cache{pages, g->seq_flag, c->numPages, c->maxPages, c->KVH, c->D, int(capacity_of(c)),
+    return Cache{pages, g->seq_report, c->numPages, c->maxPages, c->KVH, c->D, int(capacity_of(c)),
                  Div(uint32_t(c->pageSize))};
 }
 
@@ -654,14 +667,13 @@ int dgm_cacheWrite(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, const voi
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "cacheWrite: %s", hipGetErrorString(on.err));
     const WriteArgs a{cache_of(g, cfg, pages), k, v, kcache, vcache, starts, lens, rows, nseq, ldk, ldv,
                       Div(uint32_t(width / 8))};
-    g->seq_checks = true;
     if (type == DGM_TYPE_F32)
         return cfg->type == DGM_TYPE_F32 ? run_write<float, float>(g, a) : run_write<float, __bf16>(g, a);
     return cfg->type == DGM_TYPE_F32 ? run_write<__bf16, float>(g, a) : run_write<__bf16, __bf16>(g, a);
 }
 
 int64_t dgm_attnPagedDecode_ws_bytes(const dgm_cache_cfg* cfg, int64_t nseq, int64_t H) {
-    if (!cfg || cfg->KVH < 1 || cfg->D < 1 || cfg->D > 256 || H < 1 || H > 65536 || nseq < 0 || nseq > 65536 ||
+    if (!cfg || check_cache(nullptr, "", cfg, cfg->type, nseq) != DGM_OK || H < 1 || !heads_fit(nseq, H) ||
         H % cfg->KVH != 0)
         return -1;
     return decode_ws_bytes(cfg, nseq, H);
@@ -684,8 +696,7 @@ int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, cons
     if (!ldo) ldo = width;
     if (ldq < width || ldo < width)
         return dgm::fail(g, DGM_ERR_SHAPE, "attnPagedDecode: a row stride is shorter than the row's heads");
-    if (H > 65536 || (ldq | ldo) % 8 != 0 || ldq > (int64_t(1) << 31) || ldo > (int64_t(1) << 31) ||
-        nseq * H > int64_t(UINT32_MAX) / 1024)
+    if (!heads_fit(nseq, H) || (ldq | ldo) % 8 != 0 || ldq > (int64_t(1) << 31) || ldo > (int64_t(1) << 31))
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "attnPagedDecode: strides must be multiples of 8 elements up to 2^31, "
                                                  "sequences x heads below 2^22");
     if (nseq == 0) return DGM_OK;
@@ -705,7 +716,6 @@ int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, cons
     const DecodeArgs a{cache_of(g, cfg, pages), q, kcache, vcache, out, part, part + part_floats(cfg, nseq, H) * cfg->D,
                        lens, nseq, ldq, ldo, int(H), int(H / cfg->KVH), sp.heads, sp.parts, sp.workers, sp.units,
                        scale * kLog2e, Div(uint32_t(sp.workers))};
-    g->seq_checks = true;
     if (type == DGM_TYPE_F32)
         return cfg->type == DGM_TYPE_F32 ? run_decode<float, float>(g, a) : run_decode<float, __bf16>(g, a);
     return cfg->type == DGM_TYPE_F32 ? run_decode<__bf16, float>(g, a) : run_decode<__bf16, __bf16>(g, a);

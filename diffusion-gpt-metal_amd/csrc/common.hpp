@@ -62,10 +62,9 @@ struct dgm_gpu {
     bool lending = false;
     uint8_t* lent = nullptr;
     size_t lent_bytes = 0;
-    // The device's flag of bad sequence starts and pages (set by the attention and
-    // cache kernels), and whether such a kernel ran since the last dgm_end.
-    uint32_t* seq_flag = nullptr;
-    bool seq_checks = false;
+    // Two words of host memory that the attention and cache kernels set where they find
+    // bad sequence starts and pages; read and cleared by dgm_end.
+    uint32_t* seq_report = nullptr;
 };
 
 namespace dgm {

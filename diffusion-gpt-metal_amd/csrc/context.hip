@@ -15,9 +15,35 @@ namespace {
 // only the per-device address from hipGetSymbolAddress, never this name.
 __device__ __align__(256) uint8_t scratch[dgm::kScratchBytes];
 
-// What the attention and cache kernels found wrong in sequence starts, lengths and
-// page tables (which only the device reads): bits of attn.hpp. One per device, read and cleared by dgm_end.
-__device__ uint32_t sequence_flag;
+// What the attention and cache kernels find wrong in sequence starts, lengths and page
+// tables, which only the device reads: two words a context, in host memory, so that
+// dgm_end looks at them without a copy. Never freed: a captured graph may outlive its
+// context. Contexts beyond kReports at once share the last.
+constexpr int kReports = 512;
+std::mutex reports_mu;
+uint32_t* reports = nullptr;
+bool report_used[kReports] = {};
+
+uint32_t* take_report() {
+    std::lock_guard<std::mutex> lock(reports_mu);
+    if (!reports) {
+        void* p = nullptr;
+        if (hipHostMalloc(&p, kReports * 2 * sizeof(uint32_t), hipHostMallocPortable | hipHostMallocMapped) != hipSuccess) {
+            (void)hipGetLastError();
+            return nullptr;
+        }
+        reports = static_cast<uint32_t*>(p);
+    }
+    int i = 0;
+    while (i < kReports - 1 && report_used[i]) ++i;
+    report_used[i] = true;
+    reports[2 * i] = reports[2 * i + 1] = 0;
+    return reports + 2 * i;
+}
+void return_report(uint32_t* words) {
+    std::lock_guard<std::mutex> lock(reports_mu);
+    if (words) report_used[(words - reports) / 2] = false;
+}
 
 constexpr int kMaxDevices = 64;
 std::mutex scratch_mu;
@@ -194,25 +220,13 @@ uint8_t* planes_buffer(dgm_gpu* g, size_t bytes) {
     return static_cast<uint8_t*>(g->planes);
 }
 
-// After a synchronize: records an error if such a kernel set the flag, and clears it.
+// After a synchronize: records an error if such a kernel reported one.
 void sequence_check(dgm_gpu* g) {
-    g->seq_checks = false;
-    dgm_attn::OnDevice on(g->device);
-    uint32_t flag = 0;
-    const uint32_t zero = 0;
-    hipError_t e = on.err;
-    // On the context's stream: the null stream would disturb a capture elsewhere.
-    if (e == hipSuccess) e = hipMemcpyAsync(&flag, g->seq_flag, sizeof(flag), hipMemcpyDeviceToHost, g->stream);
-    if (e == hipSuccess) e = hipStreamSynchronize(g->stream);
-    if (e == hipSuccess && flag) {
-        e = hipMemcpyAsync(g->seq_flag, &zero, sizeof(zero), hipMemcpyHostToDevice, g->stream);
-        if (e == hipSuccess) e = hipStreamSynchronize(g->stream);
-    }
-    if (e != hipSuccess)
-        fail(g, DGM_ERR_HIP, "the sequence flag could not be read: %s", hipGetErrorString(e));
-    else if (flag & dgm_attn::kBadStarts)
+    const bool starts = __atomic_exchange_n(g->seq_report + dgm_attn::kBadStarts, 0u, __ATOMIC_ACQUIRE);
+    const bool pages = __atomic_exchange_n(g->seq_report + dgm_attn::kBadPages, 0u, __ATOMIC_ACQUIRE);
+    if (starts)
         fail(g, DGM_ERR_SHAPE, "sequence starts are out of order or beyond the rows: results are not valid");
-    else if (flag)
+    else if (pages)
         fail(g, DGM_ERR_SHAPE, "a sequence is longer than its page table, or names a page that the cache does not have: "
                                "those rows were left out");
 }
@@ -236,11 +250,6 @@ int dgm_gpu_create(dgm_gpu** out) {
     // per device; a failure surfaces only when that entry point is called).
     hipError_t se;
     g->scratch = scratch_for(g->device, &se);
-    if (hipGetSymbolAddress(reinterpret_cast<void**>(&g->seq_flag), HIP_SYMBOL(sequence_flag)) != hipSuccess) {
-        (void)hipGetLastError();
-        delete g;
-        return DGM_ERR_HIP;
-    }
     // A blocking stream: it orders itself after work on the null stream, where
     // callers that allocate with torch or hipMemset may still be filling the
     // buffers they hand over.
@@ -249,6 +258,12 @@ int dgm_gpu_create(dgm_gpu** out) {
         return DGM_ERR_HIP;
     }
     g->stream = g->own_stream;
+    g->seq_report = take_report();
+    if (!g->seq_report) {
+        (void)hipStreamDestroy(g->own_stream);
+        delete g;
+        return DGM_ERR_HIP;
+    }
     *out = g;
     return DGM_OK;
 }
@@ -269,6 +284,7 @@ void dgm_gpu_destroy(dgm_gpu* g) {
     for (int i = 0; i < g->n_planes_retired; ++i) (void)hipFree(g->planes_retired[i]);
     if (g->planes_event) (void)hipEventDestroy(g->planes_event);
     if (g->own_stream) (void)hipStreamDestroy(g->own_stream);
+    return_report(g->seq_report);
     delete g;
 }
 
@@ -315,7 +331,7 @@ int dgm_end(dgm_gpu* g) {
         dgm::fail(g, DGM_ERR_HIP, "HIP error after %s: %s", g->last_kernel, hipGetErrorString(e));
     else {
         if (g->spin_waits) dgm::decode_wait_check(g);
-        if (g->seq_checks) dgm::sequence_check(g);
+        dgm::sequence_check(g);
     }
     return g->first_err;
 }

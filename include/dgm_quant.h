@@ -486,12 +486,15 @@ int dgm_biasGrad(dgm_gpu* g, const float* dy, float* db, int64_t M, int64_t N);
  * Sequence starts, lengths and page tables are read on the device only, so that
  * captured graphs can be replayed with other ones. Where they are wrong (starts out of
  * order or beyond the rows, a page that the cache does not have, a length beyond
- * the page table) nothing outside the buffers is touched, and the next
- * dgm_end of a context on the device returns DGM_ERR_SHAPE.
+ * the page table) nothing outside the buffers is touched, and the context's next
+ * dgm_end (after a replay of a graph captured with the context, too) returns DGM_ERR_SHAPE.
  *
  * Buffers 16-byte aligned (starts, lengths, pages, lse: 4), row strides
  * multiples of 8 elements and at least the row's heads, 0 for rows back to back;
- * D a multiple of 8 up to 256 (DGM_ERR_UNSUPPORTED otherwise). Outputs must
+ * D a multiple of 8 up to 256 (DGM_ERR_UNSUPPORTED otherwise). DGM_ERR_UNSUPPORTED
+ * too beyond 2^30 rows, for packed rows beyond 2^23 elements apart, other rows beyond 2^31, for
+ * caches of 2^31 rows (page x key head x slot) or more, beyond 65536 sequences in a cache or
+ * 2^22 of its sequences x query heads, and where one launch cannot hold the work. Outputs must
  * not overlap inputs or one another, except that strided rows may interleave
  * (q, k, v of one fused projection, dq, dk, dv of its gradient). Nothing is allocated, and
  * every call can be captured. Results are the same bits every time. */

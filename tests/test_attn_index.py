@@ -103,4 +103,8 @@ def test_workspace_sizes_are_host_arithmetic(dgm):
     size = lib.dgm_attnPagedDecode_ws_bytes
     assert size(ctypes.byref(c), 4, 32) > size(ctypes.byref(c), 1, 32) > 0
     assert size(ctypes.byref(c), -1, 32) == size(ctypes.byref(c), 1, 9) == size(None, 1, 8) == -1
-    assert size(ctypes.byref(c), 65537, 32) == -1
+    assert size(ctypes.byref(c), 65537, 32) == size(ctypes.byref(c), 65536, 128) == -1
+    for name, value in (("D", 100), ("D", 264), ("type", 7), ("pageSize", 0), ("numPages", 1 << 30)):
+        broken = dgm.CacheCfg.from_buffer_copy(c)
+        setattr(broken, name, value)
+        assert size(ctypes.byref(broken), 4, 32) == -1

@@ -140,6 +140,29 @@ def test_bad_pages_and_lengths_are_left_out(gpu, dgm, cache):
     attn_ref.assert_within(out, want, bound)
 
 
+@pytest.mark.parametrize("io,cache", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_scores_of_minus_infinity(gpu, dgm, io, cache):
+    """Keys that all score -inf leave no softmax (NaN), not the zeros of a sequence
+    without keys; among others, where no operand is taken in pieces, they weigh nothing."""
+    lens = [300, 300, 0, 9000]
+    cfg, q, kc, vc, pages, n = cache_case(dgm, io, cache, 4, 2, 64, 16, lens)
+    q.abs_().add_(0.1)
+    for s, upto in ((0, 304), (1, 208), (3, 8000)):
+        kc[pages[s, :upto // 16].long()] = -math.inf
+    gpu.begin()
+    out = decode(gpu, dgm, cfg, io, q, kc, vc, pages, n)
+    gpu.end()
+    assert out[0].isnan().all() and (out[2] == 0).all()
+    if io == "bf16" or cache == "f32":
+        for s, upto in ((1, 208), (3, 8000)):
+            pos = torch.arange(upto, lens[s], device="cuda")
+            ids, seen = pages[s].long()[pos // 16], torch.ones(1, len(pos), dtype=torch.bool, device="cuda")
+            for h in range(4):
+                k, v = (c[ids, h // 2, pos % 16].double() for c in (kc, vc))
+                want, bound = attn_ref.forward(q[s, h:h + 1].double(), k, v, 0.125, seen, q.dtype, cache == "bf16")
+                attn_ref.assert_within(out[s, h:h + 1], want, bound)
+
+
 def write_ref(k, v, starts, lens, pages, kc, vc, page):
     kc, vc = kc.clone(), vc.clone()
     for s in range(len(starts) - 1):
@@ -315,6 +338,48 @@ def test_graph_replays_with_growing_lengths(dgm, torch_cuda):
                 step(kc2, vc2, eager)
                 stream.synchronize()
                 assert torch.equal(out, eager) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+            g.end()
+    finally:
+        g.close()
+
+
+def test_reports_belong_to_their_context(gpu, dgm, torch_cuda):
+    """A region's end reports what its own context found, in a replayed graph as well."""
+    stream = torch.cuda.Stream()
+    g = dgm.GPU(stream=stream)
+    try:
+        cfg, q, kc, vc, pages, n = cache_case(dgm, "f32", "f32", 4, 2, 32, 16, [40, 9])
+        size = g.attnPagedDecode_ws_bytes(cfg, 2, 4)
+        outs, spaces = torch.zeros(2, *q.shape, device="cuda"), torch.empty(2, size, dtype=torch.uint8, device="cuda")
+        broken = pages.clone()
+        torch.cuda.synchronize()
+
+        def step(x, i, table):
+            x.attnPagedDecode(cfg, dgm.DGM_TYPE_F32, q, kc, vc, table, n, outs[i], spaces[i], size, 2, 4)
+
+        g.begin()
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step(g, 0, broken)
+            graph.replay()
+        g.end()
+        good = outs[0].clone()
+        broken[0, 1] = -1
+        torch.cuda.synchronize()
+        for _ in range(2):
+            g.begin()
+            gpu.begin()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            stream.synchronize()
+            step(gpu, 1, pages)
+            gpu.end()
+            assert torch.equal(outs[1], good)
+            with pytest.raises(dgm.DgmError) as e:
+                g.end()
+            assert e.value.code == dgm.DGM_ERR_SHAPE
+            g.begin()
             g.end()
     finally:
         g.close()
