@@ -544,7 +544,8 @@ typedef struct dgm_cache_cfg {
  * becomes position lens[s] + r - starts[s]. lens (int32 [nseq], tokens that s
  * had before) may be NULL for all 0; starts as above, or NULL for one row per
  * sequence (rows == nseq). Rows whose position the table does not hold are left
- * out (and reported by dgm_end). Two rows of one slot: either may stay. */
+ * out (and reported by dgm_end). No two rows of a call may meet in one slot (a page
+ * named twice): its elements could be of either. */
 int dgm_cacheWrite(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, const void* k, const void* v,
                    const int32_t* starts, const int32_t* lens, const int32_t* pages, void* kcache, void* vcache,
                    int64_t rows, int64_t nseq, int64_t ldk, int64_t ldv);

@@ -308,3 +308,123 @@ def test_refusals(gpu, dgm):
     for rows, nseq in ((0, 1), (40, 0)):        # nothing to do
         assert fwd(rows=rows, nseq=nseq) == dgm.DGM_OK
     assert torch.equal(c.out, before)
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("nseq", [63, 64, 65, 129])
+def test_sequence_counts_about_a_wave(gpu, dgm, type_, nseq):
+    """Up to 64 sequences are ranked by a wave's lanes, more are searched in rounds."""
+    lens = [(i * 53) % 200 * (i % 7 != 3) for i in range(nseq)]
+    c = Case(dgm, type_, 2, 1, 32, lens, True, False, 1, 1)
+    gpu.begin()
+    c.forward(gpu)
+    c.backward(gpu)
+    gpu.end()
+    c.check(True)
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("nseq", [4, 64, 100])
+def test_backward_with_bad_starts(gpu, dgm, type_, nseq):
+    """Wild starts write to the buffers' rows only, and are reported."""
+    c = Case(dgm, type_, 4, 2, 64, [12] * nseq)
+    wild = [0, 2 ** 31 - 1, -2 ** 31, 12 * nseq, 0, 5, 12 * nseq + 1, -1] * 16
+    c.starts.copy_(torch.tensor(wild[:nseq + 1], dtype=torch.int32))
+    behind = {}
+    for name in ("out", "dq", "dk", "dv"):
+        t = getattr(c, name)
+        behind[name] = torch.full((2 * t.shape[0], *t.shape[1:]), 7.0, device="cuda").to(t.dtype)
+        setattr(c, name, behind[name][c.rows // 2:c.rows // 2 + c.rows])
+    gpu.begin()
+    c.forward(gpu)
+    c.backward(gpu)
+    with pytest.raises(dgm.DgmError) as e:
+        gpu.end()
+    assert e.value.code == dgm.DGM_ERR_SHAPE
+    for t in behind.values():
+        assert (t[:c.rows // 2] == 7).all() and (t[c.rows // 2 + c.rows:] == 7).all()
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_masked_huge_values_take_no_part(gpu, dgm, type_):
+    """Values near the type's largest and lowest, whose products overflow, at masked positions."""
+    lens, at = [50, 300, 40], 200
+    for what in ("k", "v", "q", "dout"):
+        c, clean = (Case(dgm, type_, 4, 2, 64, lens, True) for _ in range(2))
+        getattr(c, what)[at, :, ::2] = torch.finfo(TYPES[type_]).max
+        getattr(c, what)[at, :, 1::2] = torch.finfo(TYPES[type_]).min
+        gpu.begin()
+        for x in (c, clean):
+            x.forward(gpu)
+            x.backward(gpu)
+        gpu.end()
+        for name in ("out", "dq") if what in "kv" else ("dk", "dv"):
+            rows = torch.ones(c.rows, dtype=torch.bool, device="cuda")
+            if what in "kv":
+                rows[at:350] = False         # what sees the token
+            else:
+                rows[50:at + 1] = False      # what the token sees
+            assert torch.equal(getattr(c, name)[rows], getattr(clean, name)[rows]), (what, name)
+
+
+def test_rows_beyond_32_bits(gpu, dgm):
+    """Sequences at the end of buffers of over 2^31 elements."""
+    H, KVH, D, rows, lens = 4, 2, 128, (1 << 21) + 300, [200, 100]
+    wide, grad = (torch.empty(rows, H + 2 * KVH, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    out, dout = (torch.empty(rows, H, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    lse = torch.empty(H, rows, device="cuda")
+    small = Case(dgm, "bf16", H, KVH, D, lens, True, True)
+    last = slice(rows - 300, rows)
+    wide[last, :H], wide[last, H:H + KVH], wide[last, H + KVH:], dout[last] = small.q, small.k, small.v, small.dout
+    starts = torch.tensor([rows - 300, rows - 100, rows], dtype=torch.int32, device="cuda")
+    cfg = dgm.AttnCfg.from_buffer_copy(small.cfg)
+    cfg.rows, ld = rows, (H + 2 * KVH) * D
+    cfg.ldq = cfg.ldk = cfg.ldv = ld
+    assert (rows - 300) * ld >= 1 << 31
+    n = gpu.attnPackedBwd_ws_bytes(cfg)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    cut = lambda t: (t[:, :H], t[:, H:H + KVH], t[:, H + KVH:])  # noqa: E731
+    q, k, v = cut(wide)
+    dq, dk, dv = cut(grad)
+    gpu.begin()
+    gpu.attnPackedFwd(cfg, q, k, v, starts, out, lse)
+    gpu.attnPackedBwd(cfg, q, k, v, starts, out, lse, dout, dq, dk, dv, ws, n)
+    gpu.end()
+    small.out, small.lse, small.dq, small.dk, small.dv = out[last], lse[:, last], dq[last], dk[last], dv[last]
+    small.check(True)
+
+
+def test_two_contexts_at_once(dgm, torch_cuda):
+    """Two streams with a context and a workspace each give what each gives alone."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    gpus = [dgm.GPU(stream=s) for s in streams]
+    try:
+        lens = [[900, 400, 1], [128] * 12]
+        cases = [Case(dgm, t, 8, 2, 64, n) for t, n in zip(("f32", "bf16"), lens)]
+        alone = [Case(dgm, t, 8, 2, 64, n) for t, n in zip(("f32", "bf16"), lens)]
+        for x in cases + alone:
+            x.space = torch.empty(gpus[0].attnPackedBwd_ws_bytes(x.cfg), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+
+        def step(g, x):
+            g.attnPackedFwd(x.cfg, x.q, x.k, x.v, x.starts, x.out, x.lse)
+            g.attnPackedBwd(x.cfg, x.q, x.k, x.v, x.starts, x.out, x.lse, x.dout, x.dq, x.dk, x.dv, x.space,
+                            x.space.numel())
+
+        for g, x in zip(gpus, alone):
+            g.begin()
+            step(g, x)
+            g.end()
+        for g in gpus:
+            g.begin()
+        for _ in range(4):
+            for g, x in zip(gpus, cases):
+                step(g, x)
+        for g in gpus:
+            g.end()
+        for x, y in zip(cases, alone):
+            for name in ("out", "lse", "dq", "dk", "dv"):
+                assert torch.equal(getattr(x, name), getattr(y, name)), name
+    finally:
+        for g in gpus:
+            g.close()

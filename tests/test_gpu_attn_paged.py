@@ -383,3 +383,45 @@ def test_reports_belong_to_their_context(gpu, dgm, torch_cuda):
             g.end()
     finally:
         g.close()
+
+
+def test_shared_pages(gpu, dgm):
+    """Sequences with a common prompt name the same pages; one names a page twice."""
+    lens = [200, 170, 96, 200]
+    cfg, q, kc, vc, pages, n = cache_case(dgm, "bf16", "bf16", 8, 2, 128, 16, lens)
+    pages[1, :8] = pages[0, :8]
+    pages[2, :6] = pages[0, 2]
+    pages[3] = pages[0]
+    gpu.begin()
+    out = decode(gpu, dgm, cfg, "bf16", q, kc, vc, pages, n)
+    gpu.end()
+    want, bound = attn_ref.decode(q, kc, vc, pages, lens, 128 ** -0.5, True)
+    attn_ref.assert_within(out, want, bound)
+
+
+def test_cache_beyond_32_bits(gpu, dgm):
+    """Pages at the end of caches of 2^33 bytes: written, and read by the next token."""
+    KVH, D, page, total, lens = 8, 128, 16, 1 << 18, [500, 37]
+    gen = torch.Generator("cuda").manual_seed(9)
+    kc, vc = (torch.empty(total, KVH, page, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    assert kc.numel() >= 1 << 32
+    pages = torch.full((2, 40), -1, dtype=torch.int32, device="cuda")
+    order = total - 1 - torch.randperm(60, generator=gen, device="cuda").int()
+    pages[0, :32], pages[1, :3] = order[:32], order[32:35]
+    cfg = dgm.CacheCfg(type=dgm.DGM_TYPE_BF16, KVH=KVH, D=D, pageSize=page, numPages=total, maxPages=40)
+    rows = sum(lens)
+    k, v = (torch.randn(rows, KVH, D, generator=gen, device="cuda") for _ in range(2))
+    q = torch.randn(2, 16, D, generator=gen, device="cuda")
+    starts = torch.tensor([0, 500, 537], dtype=torch.int32, device="cuda")
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    gpu.begin()
+    gpu.cacheWrite(cfg, dgm.DGM_TYPE_F32, k, v, starts, None, pages, kc, vc, rows, 2)
+    out = decode(gpu, dgm, cfg, "f32", q, kc, vc, pages, n)
+    gpu.end()
+    for s in range(2):
+        pos = torch.arange(lens[s], device="cuda")
+        a, b = int(starts[s]), int(starts[s + 1])
+        assert torch.equal(kc[pages[s].long()[pos // page], :, pos % page], k[a:b].bfloat16())
+        assert torch.equal(vc[pages[s].long()[pos // page], :, pos % page], v[a:b].bfloat16())
+    want, bound = attn_ref.decode(q, kc, vc, pages, lens, D ** -0.5, False)
+    attn_ref.assert_within(out, want, bound)
