@@ -41,6 +41,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "attn.hpp"
 
@@ -58,14 +59,9 @@ constexpr int kPieces = sizeof(T) == 2 ? 1 : 3;
 // piece. The 16-byte chunk c (8 columns) of row r sits at slot c ^ swizzle(r): 16
 // rows' chunk c (the A operand of mm_rows) and 8 rows' four chunks (its transposed reads in
 // mm_cols) then lie in different banks.
-// Rows of a tile: fp32 has three planes, and the registers of three pieces.
-template <typename T, int DP>
-constexpr int kTileRows = sizeof(T) == 4 && DP > 64 ? 32 : 64;
-
-template <typename T, int DP, int ROWS = kTileRows<T, DP>>
+template <typename T, int DP, int ROWS>
 struct Lds {
     static constexpr int kRows = ROWS;
-    static constexpr int KB = kRows / 32;                     // blocks of 32 rows
     static constexpr int RB = DP * 2, CPR = RB / 16;          // bytes and chunks of a row
     static constexpr int RPB = RB >= 256 ? 1 : 256 / RB;      // rows that span all banks
     static constexpr int PLANE = kRows * RB, BYTES = kPieces<T> * PLANE;
@@ -85,7 +81,9 @@ __device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__buil
 // each lane fetches the chunk that belongs in its slot) while the other
 // buffer is computed on. fp32: loads into registers while the one buffer is
 // computed on, split into pieces and stored between two barriers.
-template <typename T, int DP, int NT, int ROWS = kTileRows<T, DP>>
+//
+// DC: the columns that the products read, D and zeros behind it.
+template <typename T, int DP, int DC, int NT, int ROWS>
 struct Feed {
     using L = Lds<T, DP, ROWS>;
     static constexpr int N = L::PLANE / 16 / NT, STEP = NT / L::CPR;   // STEP: rows between a thread's chunks
@@ -98,7 +96,7 @@ struct Feed {
         : ldb(ld * int64_t(sizeof(T))), row(int(threadIdx.x) / L::CPR), slot(int(threadIdx.x) % L::CPR),
           wave(__builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6)) {}
 
-    // `rows` rows from `from` on, their first D columns; the rest of the tile is zero.
+    // `rows` rows from `from` on, their first D columns; the rest of the tile's first DC is zero.
     __device__ __forceinline__ void start(uint8_t* lds, const T* from, int rows, int D) {
         const uint8_t* src = reinterpret_cast<const uint8_t*>(from);
         if constexpr (sizeof(T) == 4) {
@@ -119,7 +117,7 @@ struct Feed {
                 uint64_t(uniform(uint32_t(at >> 32))) << 32 | uniform(uint32_t(at)));
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-            if (rows >= L::kRows && D == DP) {
+            const auto whole = [&]() __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const uint32_t off =
@@ -128,6 +126,18 @@ struct Feed {
                                  "v"(off), "s"(first + i * STEP * ldb)
                                  : "memory", "m0");
                 }
+            };
+            constexpr bool kOneChunk = STEP % 16 == 0;   // the same one of every row that a thread has
+            if (rows >= L::kRows && D == DP) {
+                whole();
+            } else if (rows >= L::kRows && kOneChunk) {
+                const int c = slot ^ L::swizzle(row);
+                if (c * 8 < D)
+                    whole();
+                else if (c * 8 < DC)
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        *reinterpret_cast<u32x4*>(lds + (i * NT + int(threadIdx.x)) * 16) = u32x4{0, 0, 0, 0};
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -164,6 +174,7 @@ struct Feed {
         uint32_t b = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            if (DC < DP && (slot ^ L::swizzle(row + i * STEP)) * 8 >= DC) continue;
             const u32x4 v =
                 *reinterpret_cast<const u32x4*>(lds + L::BYTES - L::PLANE + (i * NT + int(threadIdx.x)) * 16);
 #pragma unroll
@@ -180,8 +191,8 @@ __device__ __forceinline__ void copies_ready() {
 }
 
 // Waits for the pair of tiles that was started last, in buffer `now`, and starts the next with `next()`.
-template <typename T, int DP, int NT, int ROWS, typename Next>
-__device__ __forceinline__ void turn(Feed<T, DP, NT, ROWS>& a, Feed<T, DP, NT, ROWS>& b,
+template <typename T, int DP, int DC, int NT, int ROWS, typename Next>
+__device__ __forceinline__ void turn(Feed<T, DP, DC, NT, ROWS>& a, Feed<T, DP, DC, NT, ROWS>& b,
                                      uint8_t (*now)[Lds<T, DP, ROWS>::BYTES], const Next& next) {
     if constexpr (sizeof(T) == 2) {
         copies_ready();
@@ -197,9 +208,9 @@ __device__ __forceinline__ void turn(Feed<T, DP, NT, ROWS>& a, Feed<T, DP, NT, R
 // ---- products ------------------------------------------------------------------
 
 // B operand of mm_rows: a wave's 32 rows of q (k, dout, v), one a lane pair.
-template <typename T, int DP>
+template <typename T, int DC>
 struct Frags {
-    static constexpr int NK = DP / 16;
+    static constexpr int NK = DC / 16;
     bf16x8 f[kPieces<T>][NK];
     __device__ __forceinline__ void load(const T* row, bool in, int D, int h) {
 #pragma unroll
@@ -259,22 +270,18 @@ __device__ __forceinline__ void reads_ahead() {
     }
 }
 
-// Results for the rows of a tile and a wave's 32 columns.
-template <typename T, int DP>
-using Blocks = f32x16[Lds<T, DP>::KB];
-
 // out[kb] (32 rows x the wave's 32 columns) = the tile's rows 32kb .. 32kb+31 times the
 // columns' vectors. Element r of a lane: row 32kb + 8(r/4) + 4h + r%4, column lane %
 // 32. The tile is part of one of ROWS rows.
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void mm_rows(Blocks<T, DP>& out, const uint8_t* tile, const Frags<T, DP>& b, int lane) {
+template <typename T, int DP, int ROWS, int KB, int DC>
+__device__ __forceinline__ void mm_rows(f32x16 (&out)[KB], const uint8_t* tile, const Frags<T, DC>& b, int lane) {
     using L = Lds<T, DP, ROWS>;
-    constexpr int P = kPieces<T>, KB = kTileRows<T, DP> / 32;
+    constexpr int P = kPieces<T>;
     const int h = lane >> 5, r = lane & 31;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) out[kb] = f32x16{};
 #pragma unroll
-    for (int kk = 0; kk < Frags<T, DP>::NK; ++kk) {
+    for (int kk = 0; kk < DC / 16; ++kk) {
         bf16x8 y[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) y[p] = b.f[p][kk];
@@ -287,20 +294,20 @@ __device__ __forceinline__ void mm_rows(Blocks<T, DP>& out, const uint8_t* tile,
             mfma_pieces(out[kb], x, y);
         }
     }
-    reads_ahead<P, Frags<T, DP>::NK * KB>();
+    reads_ahead<P, DC / 16 * KB>();
 }
 
 // The same of two tiles and two sets of vectors, for KB blocks from kb0 on.
-template <typename T, int DP, int ROWS, int KB>
+template <typename T, int DP, int ROWS, int KB, int DC>
 __device__ __forceinline__ void mm_rows2(f32x16 (&out)[KB], f32x16 (&out2)[KB], const uint8_t* tile, const uint8_t* tile2,
-                                         int kb0, const Frags<T, DP>& b, const Frags<T, DP>& b2, int lane) {
+                                         int kb0, const Frags<T, DC>& b, const Frags<T, DC>& b2, int lane) {
     using L = Lds<T, DP, ROWS>;
     constexpr int P = kPieces<T>;
     const int h = lane >> 5, r = lane & 31;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) out[kb] = out2[kb] = f32x16{};
 #pragma unroll
-    for (int kk = 0; kk < Frags<T, DP>::NK; ++kk) {
+    for (int kk = 0; kk < DC / 16; ++kk) {
         bf16x8 y[P], y2[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
@@ -320,7 +327,7 @@ __device__ __forceinline__ void mm_rows2(f32x16 (&out)[KB], f32x16 (&out2)[KB], 
             mfma_pieces(out2[kb], x2, y2);
         }
     }
-    reads_ahead<P, 2 * Frags<T, DP>::NK * KB>();
+    reads_ahead<P, 2 * (DC / 16) * KB>();
 }
 
 // A operand of mm_cols: element j of a lane is column d = 32 dt + lane % 32 of
@@ -329,7 +336,7 @@ __device__ __forceinline__ void mm_rows2(f32x16 (&out)[KB], f32x16 (&out2)[KB], 
 // columns (4 lanes a row) and gives each lane one column of them.
 template <typename T, int DP>
 __device__ __forceinline__ bf16x8 read_cols(const uint8_t* plane, int kb, int st, int dt, int lane) {
-    using L = Lds<T, DP>;
+    using L = Lds<T, DP, 32>;   // the same for any number of rows
     const int row = 32 * kb + 16 * st + 4 * (lane >> 5) + ((lane & 15) >> 2);
     const int chunk = 4 * dt + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), in = (lane & 1) * 8;
     typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -341,12 +348,11 @@ __device__ __forceinline__ bf16x8 read_cols(const uint8_t* plane, int kb, int st
 
 // acc[dt] (32 columns d x the wave's 32 columns) += tile^T times p, p as mm_rows
 // leaves it, taken in PB pieces.
-template <typename T, int DP, int PB, int ROWS>
-__device__ __forceinline__ void mm_cols(f32x16 (&acc)[DP / 32], const uint8_t* tile, const Blocks<T, DP>& p, int lane) {
-    using L = Lds<T, DP>;
+template <typename T, int DP, int PB, int ROWS, int KB, int DT>
+__device__ __forceinline__ void mm_cols(f32x16 (&acc)[DT], const uint8_t* tile, const f32x16 (&p)[KB], int lane) {
     constexpr int PA = kPieces<T>;
 #pragma unroll
-    for (int kb = 0; kb < L::KB; ++kb)
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
             float x[8];
@@ -355,7 +361,7 @@ __device__ __forceinline__ void mm_cols(f32x16 (&acc)[DP / 32], const uint8_t* t
             bf16x8 b[PB];
             split8<PB, kSpoils>(x, b);
 #pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) {
+            for (int dt = 0; dt < DT; ++dt) {
                 bf16x8 a[PA];
 #pragma unroll
                 for (int n = 0; n < PA; ++n)
@@ -378,14 +384,15 @@ struct Marks {
 };
 
 // The tile's first row is row0 of the sequence.
-template <typename T, int DP, int NT, int KINDS, bool kLast, int ROWS>
-__device__ __forceinline__ void clean_tile(const Feed<T, DP, NT, ROWS>& c, uint8_t* lds, int row0,
+template <typename T, int DP, int DC, int NT, int KINDS, bool kLast, int ROWS>
+__device__ __forceinline__ void clean_tile(const Feed<T, DP, DC, NT, ROWS>& c, uint8_t* lds, int row0,
                                            Marks<DP, KINDS>& marks) {
-    using F = Feed<T, DP, NT, ROWS>;
+    using F = Feed<T, DP, DC, NT, ROWS>;
     using L = typename F::L;
 #pragma unroll 1
     for (int i = 0; i < F::N; ++i) {
         const int r = c.row + i * F::STEP, d0 = (c.slot ^ L::swizzle(r)) * 8;
+        if (DC < DP && d0 >= DC) continue;
         __bf16* at = reinterpret_cast<__bf16*>(lds + L::BYTES - L::PLANE + (i * NT + int(threadIdx.x)) * 16);
 #pragma unroll 1
         for (int j = 0; j < 8; ++j) {
@@ -532,31 +539,62 @@ __device__ __forceinline__ void store_row(T* row, const f32x16 (&acc)[DT], float
         }
 }
 
-// Waves of a workgroup: 4 blocks of 32 queries, each by KS waves that take every KS-th
-// tile of keys and are joined in the end (two_waves says when there are two).
-constexpr int kBQ = 128;
-
-template <typename T, int DP, int KS>
-__global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 2 : 1) attn_packed_fwd_kernel(FwdArgs a) {
-    constexpr int TILE = kTileRows<T, DP>, ROWS = KS * TILE;
+// Waves of a workgroup: QW blocks of 32 queries, each by KS waves that take every KS-th tile of
+// TILE keys and are joined in the end. DP and DC: the columns of a tile, and those computed on (80 and 96 on 96 of 128: prompts of six
+// times 1024, 16 heads, fp32 201 us -> 173, bf16 44 -> 40).
+template <typename T_, int DP_, int DC_, int QW_, int KS_, int TILE_>
+struct Shape {
+    typedef T_ T;
+    static constexpr int DP = DP_, DC = DC_, QW = QW_, KS = KS_, TILE = TILE_;
+    static constexpr int BQ = 32 * QW, NT = 64 * QW * KS, ROWS = KS * TILE, KB = TILE / 32, DT = DC / 32;
     using L = Lds<T, DP, ROWS>;
-    constexpr int NT = 256 * KS, DT = DP / 32, KB = TILE / 32;
-    constexpr int kTiles = L::NBUF * 2 * L::BYTES, kJoin = KS == 1 ? 0 : 4 * (DT * 16 + 2) * 256;
-    __shared__ __align__(16) uint8_t room[kTiles > kJoin ? kTiles : kJoin];
+    using F = Feed<T, DP, DC, NT, ROWS>;
+    static constexpr int kTiles = L::NBUF * 2 * L::BYTES;
+    template <int N>   // bytes for N floats a lane of every wave but a block's first
+    static constexpr int kRoom = kTiles > QW * (KS - 1) * N * 256 ? kTiles : QW * (KS - 1) * N * 256;
+};
+
+// The three that there are; kind_of chooses.
+enum Kind { kWhole, kPairs, kNarrow };
+template <typename T, int DP, int DC>
+using Whole = Shape<T, DP, DC, 4, 1, (sizeof(T) == 4 && DP > 64 ? 32 : 64)>;
+template <typename T, int DP>
+constexpr bool kHasPairs = DP <= (sizeof(T) == 2 ? 128 : 64);
+template <typename T, int DP, int DC>
+using Pairs = Shape<T, DP, DC, (sizeof(T) == 2 ? 2 : 4), 2, (DP == 128 ? 32 : 64)>;
+template <int DP>
+constexpr bool kHasNarrow = DP <= 128;
+template <typename T, int DP, int DC>
+using Narrow = Shape<T, DP, DC, 2, (sizeof(T) == 4 && DP == 128 ? 2 : 4),
+                     (DP == 128 || (sizeof(T) == 4 && DP == 64) ? 32 : 64)>;
+
+// Waves to a SIMD that the registers are to leave room for: two, unless tiles leave room for one
+// workgroup of four waves to a CU, or the registers would spill.
+template <typename S>
+constexpr bool kAlone = S::NT == 256 && S::kTiles > 81920;
+
+template <typename S>
+__global__ void __launch_bounds__(S::NT, S::DP <= (sizeof(typename S::T) == 2 ? 128 : 64) && !kAlone<S> ? 2 : 1)
+    attn_packed_fwd_kernel(FwdArgs a) {
+    using T = typename S::T;
+    using L = typename S::L;
+    constexpr int DP = S::DP, DC = S::DC, QW = S::QW, KS = S::KS, TILE = S::TILE, ROWS = S::ROWS, NT = S::NT, DT = S::DT,
+                  KB = S::KB, BQ = S::BQ;
+    __shared__ __align__(16) uint8_t room[S::template kRoom<DT * 16 + 2>];
     uint8_t(*lds)[2][L::BYTES] = reinterpret_cast<uint8_t(*)[2][L::BYTES]>(room);   // k and v
     __shared__ Marks<DP, 3> marks;
     marks.init(INT_MAX);
     if (blockIdx.x == gridDim.x - 1) check_starts(a.starts, a.nseq, a.rows, a.report);   // one with little to do
     Rows rw;
-    if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, blockIdx.x / a.H, rw)) return;
+    if (!find_rows<false>(a.starts, a.nseq, a.rows, BQ, a.slots, blockIdx.x / a.H, rw)) return;
     const int head = head_of(blockIdx.x % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave >> 2;
-    const int q0 = rw.tile * kBQ + (wave & 3) * 32, row = q0 + (lane & 31);   // in the sequence
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave / QW;
+    const int q0 = rw.tile * BQ + wave % QW * 32, row = q0 + (lane & 31);   // in the sequence
     const bool in = row < rw.len;
     const int64_t at = int64_t(rw.first) + row;
     const T* k = static_cast<const T*>(a.k) + int64_t(rw.first) * a.ldk + int64_t(kvh) * a.D;
     const T* v = static_cast<const T*>(a.v) + int64_t(rw.first) * a.ldv + int64_t(kvh) * a.D;
-    Feed<T, DP, NT, ROWS> ck(a.ldk), cv(a.ldv);
+    typename S::F ck(a.ldk), cv(a.ldv);
     const auto start = [&](int t) __attribute__((always_inline)) {
         const int key0 = t * ROWS;
         ck.start(lds[t % L::NBUF][0], k + key0 * a.ldk, rw.len - key0, a.D);
@@ -564,16 +602,16 @@ __global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 
     };
     start(0);
 
-    Frags<T, DP> qf;
+    Frags<T, DC> qf;
     qf.load(static_cast<const T*>(a.q) + at * a.ldq + int64_t(head) * a.D, in, a.D, h);
     f32x16 o[DT];
 #pragma unroll
     for (int n = 0; n < DT; ++n) o[n] = f32x16{};
     float m = kNegInf, l = 0.0f;
     const int last = a.causal && in ? row : rw.len - 1;   // the last key that the lane's query sees
-    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * kBQ) : rw.len, steps = (keys + ROWS - 1) / ROWS;
+    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * BQ) : rw.len, steps = (keys + ROWS - 1) / ROWS;
     // Steps from here on hold positions that some query of the workgroup does not see.
-    const int masked_from = a.causal ? rw.tile * kBQ / ROWS : rw.len / ROWS;
+    const int masked_from = a.causal ? rw.tile * BQ / ROWS : rw.len / ROWS;
     const int wave_keys = a.causal ? min(keys, q0 + 32) : keys;
 
     qf.settle();
@@ -584,7 +622,7 @@ __global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 
         });
         const bool masked = t >= masked_from;
         if (masked && a.causal && __syncthreads_or(cv.bad(lds[t % L::NBUF][1]))) {
-            clean_tile<T, DP, NT, 3, false>(cv, lds[t % L::NBUF][1], t * ROWS, marks);
+            clean_tile<T, DP, DC, NT, 3, false>(cv, lds[t % L::NBUF][1], t * ROWS, marks);
             spoilt = true;
         }
         const int key0 = t * ROWS + kg * TILE;
@@ -626,10 +664,12 @@ __global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 
         l += sum;
         mm_cols<T, DP, kPieces<T>, ROWS>(o, vt, s, lane);
     }
-    if constexpr (KS == 2) {   // the second wave's part of a block, through LDS
-        float* part = reinterpret_cast<float*>(room) + (wave & 3) * (DT * 16 + 2) * 64 + lane;
+    if constexpr (KS > 1) {   // the other waves' parts of a block, through LDS
+        constexpr int N = (DT * 16 + 2) * 64;
+        float* part = reinterpret_cast<float*>(room) + wave % QW * (KS - 1) * N + lane;
         __syncthreads();
-        if (kg == 1) {
+        if (kg > 0) {
+            part += (kg - 1) * N;
             part[0] = m;
             part[64] = l;
 #pragma unroll
@@ -638,15 +678,17 @@ __global__ void __launch_bounds__(256 * KS, DP <= (sizeof(T) == 2 ? 128 : 64) ? 
                 for (int e = 0; e < 16; ++e) part[(2 + n * 16 + e) * 64] = o[n][e];
         }
         __syncthreads();
-        if (kg == 1) return;
-        const float m1 = part[0], to = fmaxf(m, m1);
-        const float f0 = m == to ? 1.0f : exp2_hw((m - to) * a.c), f1 = m1 == to ? 1.0f : exp2_hw((m1 - to) * a.c);
-        m = to;
-        l = l * f0 + part[64] * f1;
+        if (kg > 0) return;
+        for (int i = 0; i < KS - 1; ++i, part += N) {
+            const float m1 = part[0], to = fmaxf(m, m1);
+            const float f0 = m == to ? 1.0f : exp2_hw((m - to) * a.c), f1 = m1 == to ? 1.0f : exp2_hw((m1 - to) * a.c);
+            m = to;
+            l = l * f0 + part[64] * f1;
 #pragma unroll
-        for (int n = 0; n < DT; ++n)
+            for (int n = 0; n < DT; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[n][e] = o[n][e] * f0 + part[(2 + n * 16 + e) * 64] * f1;
+                for (int e = 0; e < 16; ++e) o[n][e] = o[n][e] * f0 + part[(2 + n * 16 + e) * 64] * f1;
+        }
     }
     if (spoilt) spoil<DP>(o, marks, 0, [&](int r) { return r <= last; }, lane);
 
@@ -678,34 +720,33 @@ struct BwdArgs {
 
 // dq: a wave's 32 queries against tiles of 64 keys. dS^T = P^T (dP^T - delta)
 // with dP^T = V dout^T; dq^T += K^T dS^T. delta = dout . out on the way, kept for the next kernel.
-template <typename T, int DP, int KS>
+template <typename S>
 struct DqRoom {
-    using L = Lds<T, DP, KS * kTileRows<T, DP>>;
-    static constexpr int kTiles = L::NBUF * 2 * L::BYTES, kJoin = KS == 1 ? 0 : 4 * (DP / 32) * 16 * 256;
-    __align__(16) uint8_t room[kTiles > kJoin ? kTiles : kJoin];
-    Marks<DP, 1> marks;
+    __align__(16) uint8_t room[S::template kRoom<S::DT * 16>];
+    Marks<S::DP, 1> marks;
 };
 
-template <typename T, int DP, int KS>
-__device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<T, DP, KS>& sh, uint32_t index, bool last_block) {
-    constexpr int TILE = kTileRows<T, DP>, ROWS = KS * TILE;
-    using L = Lds<T, DP, ROWS>;
-    constexpr int NT = 256 * KS, DT = DP / 32, KB = TILE / 32;
+template <typename S>
+__device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<S>& sh, uint32_t index, bool last_block) {
+    using T = typename S::T;
+    using L = typename S::L;
+    constexpr int DP = S::DP, DC = S::DC, QW = S::QW, KS = S::KS, TILE = S::TILE, ROWS = S::ROWS, NT = S::NT, DT = S::DT,
+                  KB = S::KB, BQ = S::BQ;
     uint8_t* const room = sh.room;
     uint8_t(*lds)[2][L::BYTES] = reinterpret_cast<uint8_t(*)[2][L::BYTES]>(room);   // k and v
     Marks<DP, 1>& marks = sh.marks;
     marks.init(INT_MAX);
     if (last_block) check_starts(a.starts, a.nseq, a.rows, a.report);   // one with little to do
     Rows rw;
-    if (!find_rows<false>(a.starts, a.nseq, a.rows, kBQ, a.slots, index / a.H, rw)) return;
+    if (!find_rows<false>(a.starts, a.nseq, a.rows, BQ, a.slots, index / a.H, rw)) return;
     const int head = head_of(index % a.H, a.H, a.KVH), kvh = head / (a.H / a.KVH);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave >> 2;
-    const int q0 = rw.tile * kBQ + (wave & 3) * 32, row = q0 + (lane & 31);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, kg = wave / QW;
+    const int q0 = rw.tile * BQ + wave % QW * 32, row = q0 + (lane & 31);
     const bool in = row < rw.len;
     const int64_t at = int64_t(rw.first) + row;
     const T* k = static_cast<const T*>(a.k) + int64_t(rw.first) * a.ldk + int64_t(kvh) * a.D;
     const T* v = static_cast<const T*>(a.v) + int64_t(rw.first) * a.ldv + int64_t(kvh) * a.D;
-    Feed<T, DP, NT, ROWS> ck(a.ldk), cv(a.ldv);
+    typename S::F ck(a.ldk), cv(a.ldv);
     const auto start = [&](int t) __attribute__((always_inline)) {
         const int key0 = t * ROWS;
         ck.start(lds[t % L::NBUF][0], k + key0 * a.ldk, rw.len - key0, a.D);
@@ -714,12 +755,12 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<T, DP, KS>& sh,
     start(0);
     const T* grad = static_cast<const T*>(a.dout) + at * a.ldo + int64_t(head) * a.D;
     const T* out = static_cast<const T*>(a.out) + at * a.ldo + int64_t(head) * a.D;
-    Frags<T, DP> qf, gf;
+    Frags<T, DC> qf, gf;
     qf.load(static_cast<const T*>(a.q) + at * a.ldq + int64_t(head) * a.D, in, a.D, h);
     gf.load(grad, in, a.D, h);
     float delta = 0.0f;
 #pragma unroll
-    for (int d = 8 * h; d < DP; d += 16)
+    for (int d = 8 * h; d < DC; d += 16)
         if (in && d < a.D) {
             float x[8], y[8];
             load8(grad + d, x);
@@ -736,8 +777,8 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<T, DP, KS>& sh,
 #pragma unroll
     for (int n = 0; n < DT; ++n) acc[n] = f32x16{};
 
-    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * kBQ) : rw.len, steps = (keys + ROWS - 1) / ROWS;
-    const int masked_from = a.causal ? rw.tile * kBQ / ROWS : rw.len / ROWS;
+    const int keys = a.causal ? min(rw.len, (rw.tile + 1) * BQ) : rw.len, steps = (keys + ROWS - 1) / ROWS;
+    const int masked_from = a.causal ? rw.tile * BQ / ROWS : rw.len / ROWS;
     const int wave_keys = a.causal ? min(keys, q0 + 32) : keys;
     qf.settle();
     gf.settle();
@@ -775,34 +816,37 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<T, DP, KS>& sh,
         }
         if (dirty) {
             __syncthreads();   // the tile has been read as it is
-            clean_tile<T, DP, NT, 1, false>(ck, lds[t % L::NBUF][0], t * ROWS, marks);
+            clean_tile<T, DP, DC, NT, 1, false>(ck, lds[t % L::NBUF][0], t * ROWS, marks);
             spoilt = true;
         }
         if (active) mm_cols<T, DP, kSlopePieces<T>, ROWS>(acc, kt, s, lane);
     }
-    if constexpr (KS == 2) {
-        float* part = reinterpret_cast<float*>(room) + (wave & 3) * DT * 16 * 64 + lane;
+    if constexpr (KS > 1) {
+        constexpr int N = DT * 16 * 64;
+        float* part = reinterpret_cast<float*>(room) + wave % QW * (KS - 1) * N + lane;
         __syncthreads();
-        if (kg == 1)
+        if (kg > 0)
 #pragma unroll
             for (int n = 0; n < DT; ++n)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) part[(n * 16 + e) * 64] = acc[n][e];
+                for (int e = 0; e < 16; ++e) part[(kg - 1) * N + (n * 16 + e) * 64] = acc[n][e];
         __syncthreads();
-        if (kg == 1) return;
+        if (kg > 0) return;
+        for (int i = 0; i < KS - 1; ++i, part += N)
 #pragma unroll
-        for (int n = 0; n < DT; ++n)
+            for (int n = 0; n < DT; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[n][e] += part[(n * 16 + e) * 64];
+                for (int e = 0; e < 16; ++e) acc[n][e] += part[(n * 16 + e) * 64];
     }
     if (spoilt) spoil<DP>(acc, marks, 0, [&](int r) { return r <= last; }, lane);
     if (in) store_row<T, DT>(static_cast<T*>(a.dq) + at * a.ldq + int64_t(head) * a.D, acc, a.scale, 0, a.D, h);
 }
 
-template <typename T, int DP, int KS>
-__global__ void __launch_bounds__(256 * KS, sizeof(T) == 2 || KS == 2 ? 2 : 1) attn_packed_dq_kernel(BwdArgs a) {
-    __shared__ DqRoom<T, DP, KS> room;
-    dq_body<T, DP, KS>(a, room, blockIdx.x, blockIdx.x == gridDim.x - 1);
+template <typename S>
+__global__ void __launch_bounds__(S::NT, (sizeof(typename S::T) == 2 && !kAlone<S>) || S::NT == 512 ? 2 : 1)
+    attn_packed_dq_kernel(BwdArgs a) {
+    __shared__ DqRoom<S> room;
+    dq_body<S>(a, room, blockIdx.x, blockIdx.x == gridDim.x - 1);
 }
 
 // dk, dv: a pair of waves' 32 keys as columns against tiles of 64 queries, over the query heads
@@ -835,13 +879,13 @@ struct DkvRoom {
 };
 
 // kOwnDelta: delta from out and dout here, not from the dq kernel.
-template <typename T, int DP, bool kOwnDelta>
+template <typename T, int DP, int DC, bool kOwnDelta>
 __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, uint32_t index) {
     using L = Lds<T, DP, 64>;
     constexpr int NW = DkvShape<T, DP>::NW, NT = 64 * NW, BK = DkvShape<T, DP>::BK, TILE = 64;
     constexpr int PP = kPieces<T>, PS = kSlopePieces<T>;
-    constexpr bool kSplitD = DP > 32;              // else the pair's waves take dv and dk, one each
-    constexpr int DT = kSplitD ? DP / 64 : 1;      // blocks of 32 columns of a wave
+    constexpr bool kSplitD = DC % 64 == 0;              // else the pair's waves take dv and dk, one each
+    constexpr int DT = kSplitD ? DC / 64 : DC / 32;     // blocks of 32 columns of a wave
     auto& lds = sh.lds;
     auto& hand = sh.hand;
     auto& stat = sh.stat;
@@ -857,7 +901,7 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
     const int64_t at = int64_t(rw.first) + row;
     const int first = a.causal ? rw.tile * BK / TILE : 0, per_head = (rw.len + TILE - 1) / TILE - first;
     const int t0 = int(int64_t(per_head) * G * part / a.parts), t1 = int(int64_t(per_head) * G * (part + 1) / a.parts);
-    Feed<T, DP, NT, 64> cq(a.ldq), cg(a.ldo);
+    Feed<T, DP, DC, NT, 64> cq(a.ldq), cg(a.ldo);
     static_assert(NT >= 2 * TILE, "a thread stages one statistic");
     int head = kvh * G + t0 / per_head, tile = first + t0 % per_head, now = tile;   // of the next copy; computed on
     struct Raw8 {
@@ -914,7 +958,7 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
         }
     };
     if (t0 < t1) start(t0);
-    Frags<T, DP> kf, vf;
+    Frags<T, DC> kf, vf;
     kf.load(static_cast<const T*>(a.k) + at * a.ldk + int64_t(kvh) * a.D, in, a.D, h);
     vf.load(static_cast<const T*>(a.v) + at * a.ldv + int64_t(kvh) * a.D, in, a.D, h);
     f32x16 dk[DT], dv[DT];
@@ -983,8 +1027,8 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
         }
         __syncthreads();
         if (dirty) {   // the tiles have been read as they are
-            clean_tile<T, DP, NT, 1, true>(cq, qt, row0, marks[0]);
-            clean_tile<T, DP, NT, 1, true>(cg, gt, row0, marks[1]);
+            clean_tile<T, DP, DC, NT, 1, true>(cq, qt, row0, marks[0]);
+            clean_tile<T, DP, DC, NT, 1, true>(cg, gt, row0, marks[1]);
             spoilt = true;
         }
         if (active) {
@@ -1000,7 +1044,7 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
                     for (int n = 0; n < PS; ++n) sx[n] = from[PP + n][st][lane];
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
-                        const int d = kSplitD ? half * DT + dt : 0;
+                        const int d = kSplitD ? half * DT + dt : dt;
                         bf16x8 x[PP], y[PP];
 #pragma unroll
                         for (int n = 0; n < PP; ++n) {
@@ -1041,11 +1085,11 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
     if (mine_v) store_row<T, DT>(static_cast<T*>(a.dv) + at * a.ldv + int64_t(kvh) * a.D, dv, 1.0f, d0, a.D, h);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 && DP == 128 ? 1 : 2))
     attn_packed_dkv_kernel(BwdArgs a) {
     __shared__ DkvRoom<T, DP> room;
-    dkv_body<T, DP, false>(a, room, blockIdx.x);
+    dkv_body<T, DP, DC, false>(a, room, blockIdx.x);
 }
 
 // Both in one launch, a workgroup one or the other, for grids that the chip holds at once:
@@ -1053,15 +1097,15 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, 2) attn_packed_grads_kernel(BwdArgs a, uint32_t first, int64_t dkv_slots) {
     __shared__ union Room {
-        DqRoom<T, DP, 1> dq;
+        DqRoom<Whole<T, DP, DP>> dq;
         DkvRoom<T, DP> dkv;
         __device__ Room() {}
     } room;
     if (blockIdx.x < first) {
-        dq_body<T, DP, 1>(a, room.dq, blockIdx.x, blockIdx.x == first - 1);
+        dq_body<Whole<T, DP, DP>>(a, room.dq, blockIdx.x, blockIdx.x == first - 1);
     } else {
         a.slots = dkv_slots;
-        dkv_body<T, DP, true>(a, room.dkv, blockIdx.x - first);
+        dkv_body<T, DP, DP, true>(a, room.dkv, blockIdx.x - first);
     }
 }
 
@@ -1135,42 +1179,55 @@ int slots_of(dgm_gpu* g, const char* name, const dgm_attn_cfg* c, int per, int h
     return DGM_OK;
 }
 
-// Two waves for a block of queries halve the longest workgroup, which a launch of few
-// workgroups waits for, but all eight waves of a CU then wait for one another. bf16 gains where
-// the grid is no more than two to a CU (8 heads of 128, 2048 causal: 44 us, 36 with two; 16
-// heads, six of 1024: 49, 54). fp32, where two workgroups of four waves
-// leave less overlap, gains on any grid (16 heads of 64, 2048 and shorter: 149, 128) but not in
-// its backward, short of registers (four of 1024: 370, 376). Short sequences have nothing to share (16 of 64: 6.6, 7.5).
+// A launch of few workgroups waits for its longest, and that is made shorter by more waves for a
+// block of queries, each with its share of the keys, and by blocks of fewer
+// queries. Both cost: a tile is staged for fewer queries, and the waves of a
+// workgroup wait for one another.
+//  * kNarrow, 64 queries by 8 waves (4 where fp32 tiles of 128 columns leave no room), while
+//    there is no more than one such workgroup to a CU, or two for long sequences:
+//    four of 70 to 1500 under 4 heads, fp32 of 64 60 us -> 44 (and the backward 162 -> 125), of 128
+//    157 -> 110, bf16 of 128 29.3 -> 24.9. But ten of 300 under 8 heads, bf16: 14.0, 21.4.
+//  * kPairs, two waves a block. bf16 (64 queries) gains while four waves' workgroups would be no
+//    more than two to a CU (seven of 1 to 1024 under 12 heads of 128: 28.5 -> 24.7; 16 heads of 96, six of
+//    1024: 39.8, 47.8); fp32 (128), where two workgroups of four waves leave
+//    less overlap, on any grid (16 heads of 64, 2048 and shorter: 129 -> 108), but
+//    not in its backward, short of registers (four of 1024: 370, 376).
+//  * Short sequences have nothing to share (16 of 64: 6.6, 7.5).
 template <typename T>
-bool two_waves(const dgm_attn_cfg* c, bool forward) {
-    const int64_t groups = slot_count(c->rows, c->nseq, kBQ) * c->H;
-    return c->rows / c->nseq > 128 && ((sizeof(T) == 4 && forward) || groups <= 2 * dgm::kCus);
+Kind kind_of(const dgm_attn_cfg* c, bool forward) {
+    const int64_t average = c->rows / c->nseq;
+    if (average <= 128) return kWhole;
+    if (slot_count(c->rows, c->nseq, 64) * c->H <= (average > 512 ? 2 : 1) * dgm::kCus && c->D <= 128) return kNarrow;
+    const bool few = slot_count(c->rows, c->nseq, 128) * c->H <= 2 * dgm::kCus;
+    return few || (sizeof(T) == 4 && forward) ? kPairs : kWhole;
 }
-template <typename T, int DP>
-constexpr bool kTwoWaves = DP <= (sizeof(T) == 2 ? 128 : 64);
 
-template <typename T, int DP, int KS>
+template <typename S>
 int launch_fwd(dgm_gpu* g, const dgm_attn_cfg* c, FwdArgs a) {
-    const int rc = slots_of(g, "attnPackedFwd", c, kBQ, c->H, 256 * KS, a.slots);
+    const int rc = slots_of(g, "attnPackedFwd", c, S::BQ, c->H, S::NT, a.slots);
     if (rc) return rc;
-    attn_packed_fwd_kernel<T, DP, KS><<<dim3(unsigned(a.slots * c->H)), dim3(256 * KS), 0, g->stream>>>(a);
+    attn_packed_fwd_kernel<S><<<dim3(unsigned(a.slots * c->H)), dim3(S::NT), 0, g->stream>>>(a);
     DGM_LAUNCH_CHECK(g, "attn_packed_fwd");
     return DGM_OK;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 int choose_fwd(dgm_gpu* g, const dgm_attn_cfg* c, const FwdArgs& a) {
-    if constexpr (kTwoWaves<T, DP>)
-        if (two_waves<T>(c, true)) return launch_fwd<T, DP, 2>(g, c, a);
-    return launch_fwd<T, DP, 1>(g, c, a);
+    const Kind kind = kind_of<T>(c, true);
+    if constexpr (kHasNarrow<DP>)
+        if (kind == kNarrow) return launch_fwd<Narrow<T, DP, DC>>(g, c, a);
+    if constexpr (kHasPairs<T, DP>)
+        if (kind == kPairs) return launch_fwd<Pairs<T, DP, DC>>(g, c, a);
+    return launch_fwd<Whole<T, DP, DC>>(g, c, a);
 }
 
 template <typename T>
 int run_fwd(dgm_gpu* g, const dgm_attn_cfg* c, const FwdArgs& a) {
-    if (c->D <= 32) return choose_fwd<T, 32>(g, c, a);
-    if (c->D <= 64) return choose_fwd<T, 64>(g, c, a);
-    if (c->D <= 128) return choose_fwd<T, 128>(g, c, a);
-    return choose_fwd<T, 256>(g, c, a);
+    if (c->D <= 32) return choose_fwd<T, 32, 32>(g, c, a);
+    if (c->D <= 64) return choose_fwd<T, 64, 64>(g, c, a);
+    if (c->D <= 96) return choose_fwd<T, 128, 96>(g, c, a);
+    if (c->D <= 128) return choose_fwd<T, 128, 128>(g, c, a);
+    return choose_fwd<T, 256, 256>(g, c, a);
 }
 
 // Keys of a workgroup of the dk, dv kernel.
@@ -1186,7 +1243,7 @@ template <typename T, int DP>
 constexpr bool kOneLaunch = DkvShape<T, DP>::NW == 4 && DP <= 64;
 bool one_launch(const dgm_attn_cfg* c) {
     const bool fits = c->D <= 32 || (c->D <= 64 && c->type == DGM_TYPE_BF16);
-    return fits && slot_count(c->rows, c->nseq, kBQ) * c->H + slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH <=
+    return fits && slot_count(c->rows, c->nseq, 128) * c->H + slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH <=
                        2 * dgm::kCus;
 }
 
@@ -1203,22 +1260,25 @@ int64_t dkv_parts(const dgm_attn_cfg* c) {
     return std::max<int64_t>(1, std::min<int64_t>({16, (3 * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps / 2}));
 }
 
-template <typename T, int DP, int KS>
+template <typename S>
 int launch_dq(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs a) {
-    const int rc = slots_of(g, "attnPackedBwd", c, kBQ, c->H, 256 * KS, a.slots);
+    const int rc = slots_of(g, "attnPackedBwd", c, S::BQ, c->H, S::NT, a.slots);
     if (rc) return rc;
-    attn_packed_dq_kernel<T, DP, KS><<<dim3(unsigned(a.slots * c->H)), dim3(256 * KS), 0, g->stream>>>(a);
+    attn_packed_dq_kernel<S><<<dim3(unsigned(a.slots * c->H)), dim3(S::NT), 0, g->stream>>>(a);
     DGM_LAUNCH_CHECK(g, "attn_packed_dq");
     return DGM_OK;
 }
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 int choose_dq(dgm_gpu* g, const dgm_attn_cfg* c, const BwdArgs& a) {
-    if constexpr (kTwoWaves<T, DP>)
-        if (two_waves<T>(c, false)) return launch_dq<T, DP, 2>(g, c, a);
-    return launch_dq<T, DP, 1>(g, c, a);
+    const Kind kind = kind_of<T>(c, false);
+    if constexpr (kHasNarrow<DP>)
+        if (kind == kNarrow) return launch_dq<Narrow<T, DP, DC>>(g, c, a);
+    if constexpr (kHasPairs<T, DP>)
+        if (kind == kPairs) return launch_dq<Pairs<T, DP, DC>>(g, c, a);
+    return launch_dq<Whole<T, DP, DC>>(g, c, a);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs kv) {
     constexpr int NK = DkvShape<T, DP>::NW;
     int rc = slots_of(g, "attnPackedBwd", c, DkvShape<T, DP>::BK, c->KVH * kv.parts, 64 * NK, kv.slots);
@@ -1226,7 +1286,7 @@ int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs kv) {
     if constexpr (kOneLaunch<T, DP>) {
         if (kv.parts == 1 && one_launch(c)) {
             BwdArgs q = kv;
-            q.slots = slot_count(c->rows, c->nseq, kBQ);
+            q.slots = slot_count(c->rows, c->nseq, Whole<T, DP, DP>::BQ);
             const int64_t first = q.slots * c->H, all = first + kv.slots * c->KVH;
             attn_packed_grads_kernel<T, DP>
                 <<<dim3(unsigned(all)), dim3(256), 0, g->stream>>>(q, uint32_t(first), kv.slots);
@@ -1234,9 +1294,9 @@ int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs kv) {
             return DGM_OK;
         }
     }
-    rc = choose_dq<T, DP>(g, c, kv);
+    rc = choose_dq<T, DP, DC>(g, c, kv);
     if (rc) return rc;
-    attn_packed_dkv_kernel<T, DP>
+    attn_packed_dkv_kernel<T, DP, DC>
         <<<dim3(unsigned(kv.slots * c->KVH * kv.parts)), dim3(64 * NK), 0, g->stream>>>(kv);
     DGM_LAUNCH_CHECK(g, "attn_packed_dkv");
     if (kv.parts > 1) {
@@ -1250,9 +1310,10 @@ int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs kv) {
 
 template <typename T>
 int run_bwd(dgm_gpu* g, const dgm_attn_cfg* c, const BwdArgs& a) {
-    if (c->D <= 32) return launch_bwd<T, 32>(g, c, a);
-    if (c->D <= 64) return launch_bwd<T, 64>(g, c, a);
-    return launch_bwd<T, 128>(g, c, a);
+    if (c->D <= 32) return launch_bwd<T, 32, 32>(g, c, a);
+    if (c->D <= 64) return launch_bwd<T, 64, 64>(g, c, a);
+    if (c->D <= 96) return launch_bwd<T, 128, 96>(g, c, a);
+    return launch_bwd<T, 128, 128>(g, c, a);
 }
 
 constexpr int kMaxD = 256, kMaxDBwd = 128;

@@ -428,3 +428,45 @@ def test_two_contexts_at_once(dgm, torch_cuda):
     finally:
         for g in gpus:
             g.close()
+
+
+# Grids for each way of laying a block of queries over waves: few workgroups, some, many, short sequences.
+LAYOUTS = [(4, 2, [300, 1, 640]), (24, 8, [300, 1, 640]), (72, 8, [300, 1, 640]), (8, 4, [100] * 9)]
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [16, 64, 72, 96, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("H,KVH,lens", LAYOUTS)
+def test_layouts(gpu, dgm, type_, D, causal, H, KVH, lens):
+    c = Case(dgm, type_, H, KVH, D, lens, causal, True, 2, 3)
+    gpu.begin()
+    c.forward(gpu)
+    c.backward(gpu)
+    gpu.end()
+    c.check(True)
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("H,KVH,lens", LAYOUTS)
+def test_masked_values_in_every_layout(gpu, dgm, type_, D, H, KVH, lens):
+    """A NaN token leaves what its mask hides it from as it is."""
+    first = sum(lens[:-1])
+    for what, at in (("k", first + 70), ("v", first + 33), ("q", first + 70), ("dout", first + 33)):
+        c, clean = (Case(dgm, type_, H, KVH, D, lens) for _ in range(2))
+        getattr(c, what)[at] = math.nan
+        gpu.begin()
+        for x in (c, clean):
+            x.forward(gpu)
+            x.backward(gpu)
+        gpu.end()
+        rows = torch.ones(c.rows, dtype=torch.bool, device="cuda")
+        if what in "kv":
+            rows[at:] = False
+        else:
+            rows[first:at + 1] = False
+        for name in ("out", "dq") if what in "kv" else ("dk", "dv"):
+            assert torch.equal(getattr(c, name)[rows], getattr(clean, name)[rows]), (what, name)
+        if what in "kv":
+            assert c.out[at:].isnan().any(2).all()
