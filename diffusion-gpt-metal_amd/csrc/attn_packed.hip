@@ -714,7 +714,7 @@ struct BwdArgs {
     const int32_t* starts;
     uint32_t* report;
     int64_t rows, nseq, ldq, ldk, ldv, ldo, slots;
-    int H, KVH, D, causal, parts;
+    int H, KVH, D, causal, parts, per;   // per: rows of a workgroup that adds parts
     float c, scale;
 };
 
@@ -1109,22 +1109,30 @@ __global__ void __launch_bounds__(256, 2) attn_packed_grads_kernel(BwdArgs a, ui
     }
 }
 
-// The parts' sums of dk and dv, added in order: a workgroup takes 32 rows of one
-// sequence and head, 4 columns a thread.
+// The parts' sums of dk and dv, added in order: a workgroup takes a.per rows of one
+// sequence and head, 4 columns a thread; 8 parts are asked for at once, then added
+// (one after the other, 8 heads of 128 on one over 400 rows wait 22 us longer).
 template <typename T>
 __global__ void __launch_bounds__(256) attn_packed_sum_kernel(BwdArgs a) {
     Rows rw;
     const int kvh = blockIdx.x % a.KVH;
-    if (!find_rows<true>(a.starts, a.nseq, a.rows, 32, a.slots, blockIdx.x / a.KVH, rw)) return;
+    if (!find_rows<true>(a.starts, a.nseq, a.rows, a.per, a.slots, blockIdx.x / a.KVH, rw)) return;
     const int64_t all = a.rows * a.KVH;
     const int quads = a.D / 4;
-    for (int i = threadIdx.x; i < 64 * quads; i += 256) {
-        const int which = i / (32 * quads), r = i / quads % 32, d = i % quads * 4;
-        if (rw.tile * 32 + r >= rw.len) continue;
-        const int64_t at = int64_t(rw.first) + rw.tile * 32 + r;
+    for (int i = threadIdx.x; i < 2 * a.per * quads; i += 256) {
+        const int which = i / (a.per * quads), r = rw.tile * a.per + i / quads % a.per, d = i % quads * 4;
+        if (r >= rw.len) continue;
+        const int64_t at = int64_t(rw.first) + r;
         const float* from = a.sums + (which * all + at * a.KVH + kvh) * a.D + d;
-        f32x4 sum = *reinterpret_cast<const f32x4*>(from);
-        for (int p = 1; p < a.parts; ++p) sum += *reinterpret_cast<const f32x4*>(from + p * 2 * all * a.D);
+        f32x4 sum{0, 0, 0, 0};
+        for (int p = 0; p < a.parts; p += 8) {
+            f32x4 x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = p + j < a.parts ? *reinterpret_cast<const f32x4*>(from + (p + j) * 2 * all * a.D) : f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += x[j];
+        }
         T* to = which ? static_cast<T*>(a.dv) + at * a.ldv + int64_t(kvh) * a.D
                       : static_cast<T*>(a.dk) + at * a.ldk + int64_t(kvh) * a.D;
         const float f = which ? 1.0f : a.scale;
@@ -1192,11 +1200,13 @@ int slots_of(dgm_gpu* g, const char* name, const dgm_attn_cfg* c, int per, int h
 //    1024: 39.8, 47.8); fp32 (128), where two workgroups of four waves leave
 //    less overlap, on any grid (16 heads of 64, 2048 and shorter: 129 -> 108), but
 //    not in its backward, short of registers (four of 1024: 370, 376).
-//  * Short sequences have nothing to share (16 of 64: 6.6, 7.5).
+//  * Sequences of one tile have nothing to share (16 of 64: 6.6, 7.5); lengths differ, and the longest
+//    sets the time, so that an average of two is enough (18 of 1 to 745, bf16 of 80, forward and
+//    backward 98 -> 88; nine of 100, 8 heads of 128: bf16 63, 66, fp32 135 -> 128).
 template <typename T>
 Kind kind_of(const dgm_attn_cfg* c, bool forward) {
     const int64_t average = c->rows / c->nseq;
-    if (average <= 128) return kWhole;
+    if (average <= 64) return kWhole;
     if (slot_count(c->rows, c->nseq, 64) * c->H <= (average > 512 ? 2 : 1) * dgm::kCus && c->D <= 128) return kNarrow;
     const bool few = slot_count(c->rows, c->nseq, 128) * c->H <= 2 * dgm::kCus;
     return few || (sizeof(T) == 4 && forward) ? kPairs : kWhole;
@@ -1247,17 +1257,18 @@ bool one_launch(const dgm_attn_cfg* c) {
                        2 * dgm::kCus;
 }
 
-// Workgroups that share a key tile's steps: enough for three to a CU, each with two
-// steps or more at the sequences' average length (four blocks of 2048, 544 causal tiles: 336 us
-// whole; two parts 279 and 28 for the sums). One launch for dq, dk and dv is worth more than
-// parts of a few steps: dq then runs beside them. fp32, 4 heads of 32 over four times 256, 41 us in
-// parts, 28 whole; bf16, 4 heads of 64 over 1024, 62 and 47; but 8 query heads
+// Workgroups that share a key tile's steps: enough for three to a CU, each with a step
+// or more at the sequences' average length (four blocks of 2048, 544 causal tiles: 336 us
+// whole; two parts 279 and 28 for the sums. 15 of 1 to 1280, one fp32 head of 128, forward and
+// backward 375 us, with two steps or more each; 301 so). One launch for dq, dk and dv is worth more
+// than parts of a few steps: dq then runs beside them. fp32, 4 heads of 32 over four times
+// 256, 41 us in parts, 28 whole; bf16, 4 heads of 64 over 1024, 62 and 47; but 8 query heads
 // on 2 over 900 rows 40 and 50.
 int64_t dkv_parts(const dgm_attn_cfg* c) {
     const int64_t tiles = slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH;
     const int64_t steps = (c->rows / std::max<int64_t>(c->nseq, 1) + 63) / 64 * (c->H / c->KVH);
     if (steps <= (c->H == c->KVH ? 16 : 4) && one_launch(c)) return 1;
-    return std::max<int64_t>(1, std::min<int64_t>({16, (3 * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps / 2}));
+    return std::max<int64_t>(1, std::min<int64_t>({16, (3 * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps}));
 }
 
 template <typename S>
@@ -1300,7 +1311,10 @@ int launch_bwd(dgm_gpu* g, const dgm_attn_cfg* c, BwdArgs kv) {
         <<<dim3(unsigned(kv.slots * c->KVH * kv.parts)), dim3(64 * NK), 0, g->stream>>>(kv);
     DGM_LAUNCH_CHECK(g, "attn_packed_dkv");
     if (kv.parts > 1) {
-        rc = slots_of(g, "attnPackedBwd", c, 32, c->KVH, 256, kv.slots);
+        // 32 rows where that gives four workgroups to a CU (four blocks of 2048: 31 us, with 8 rows 37), else 8 (12 of
+        // 200, 2 heads: 44 us in all, 43).
+        kv.per = slot_count(c->rows, c->nseq, 32) * c->KVH >= 4 * dgm::kCus ? 32 : 8;
+        rc = slots_of(g, "attnPackedBwd", c, kv.per, c->KVH, 256, kv.slots);
         if (rc) return rc;
         attn_packed_sum_kernel<T><<<dim3(unsigned(kv.slots * c->KVH)), dim3(256), 0, g->stream>>>(kv);
         DGM_LAUNCH_CHECK(g, "attn_packed_sum");
@@ -1378,7 +1392,7 @@ int dgm_attnPackedBwd(dgm_gpu* g, const dgm_attn_cfg* cfg, const void* q, const 
     float* delta = static_cast<float*>(ws);
     const BwdArgs a{q, k, v, out, dout, dq, dk, dv, lse, delta, delta + delta_floats(cfg), starts, g->seq_report,
                     cfg->rows, cfg->nseq, s.q, s.k, s.v, s.o, 0, cfg->H, cfg->KVH, cfg->D, cfg->causal != 0,
-                    int(dkv_parts(cfg)), cfg->scale * kLog2e, cfg->scale};
+                    int(dkv_parts(cfg)), 0, cfg->scale * kLog2e, cfg->scale};
     return cfg->type == DGM_TYPE_F32 ? run_bwd<float>(g, cfg, a) : run_bwd<__bf16>(g, cfg, a);
 }
 
