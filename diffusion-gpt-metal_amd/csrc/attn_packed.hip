@@ -9,8 +9,8 @@
 //    lane pair (its maximum and sum need one exchange between the halves), and
 //    P^T has just the layout that the next product, O^T = V^T P^T, takes as its B
 //    operand: the probabilities never leave the registers. The k index of
-//    that product follows the order in which a lane holds its scores; V^T is
-//    stored to LDS in the same order.
+//    that product follows the order in which a lane holds its scores; V is read
+//    from LDS in the same order.
 //  * The matrix unit runs on bf16 (v_mfma_f32_32x32x16_bf16). bf16 tensors take
 //    one product, with P rounded to bf16 (half a step is 2^-9 of a weight's binade, and
 //    the roundings of a row's weights are independent, so a row's error stays about that of
@@ -18,14 +18,15 @@
 //    bits, exactly, and take the six products of pieces that reach 2^-24 of the
 //    largest: 192 cycles for 32x32x16, which v_mfma_f32_32x32x2_f32 does in 512.
 //    Scores, statistics and accumulators are fp32.
-//  * Tiles of 64 keys stay row-major in LDS: the A operand of the second product
+//  * Tiles of 64 (32) keys stay row-major in LDS: the A operand of the second product
 //    is read transposed (ds_read_b64_tr_b16), and 16-byte chunks are XOR-swizzled so
 //    that both reads are free of bank conflicts. bf16 tiles go from memory straight into
 //    one of two buffers while the other is computed on, one barrier a tile; fp32 tiles
 //    pass through registers, where they are split.
-//  * Rows are found on the device: sequence s owns the tile slots from
-//    starts[s] / rows-per-tile + s on, which never overlap, so the grid needs no host
-//    copy of the lengths, and a captured graph may be replayed with other lengths.
+//  * Rows are found on the device, so that the grid needs no host copy of the lengths, and a
+//    captured graph may be replayed with other ones: up to 64 sequences are ranked by a wave, longest
+//    work first; of more, sequence s owns the tile slots from
+//    starts[s] / rows-per-tile + s on, which never overlap.
 //  * The running maximum moves only when a score exceeds it by more than 2^8:
 //    the factor then stays exact in fp32 and the accumulators are rescaled a few
 //    times in a row instead of at every tile.
@@ -34,10 +35,17 @@
 //    tile: tiles that hold both masked positions and such values are cleaned of them
 //    first, and the sums that they belong to spoilt afterwards.
 //
+// Long sequences are bound by the matrix unit: a prompt of 8192 (32 heads on 8 of 128,
+// bf16) takes 530 us, 1,037 TFLOP/s, where a library product reaches 1,158; four of 640 to 2048 in
+// fp32 (16 heads on 4 of 64) 108 us, 150 TFLOP/s, where a library product reaches 153. Short ones
+// are a chain of waits: starts, tiles, exponentials, rows out (16 of 64: 6 us).
+//
 // The backward recomputes P from lse. One kernel owns 32 queries per wave and
 // accumulates dq; another owns 32 keys per wave and accumulates dk and dv over all
 // query heads of the key head's group, so no gradient is added to by two
-// workgroups: no atomics, the same bits every time.
+// workgroups: no atomics, the same bits every time. Four of 2048 (16 heads on 8 of 128, bf16): dq 156 us,
+// dk and dv 239 and 32 for the sums of two parts; the matrix unit is busy in half
+// of dq's cycles and a third of the other's, whose pairs of waves wait for one another.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -857,7 +865,7 @@ __global__ void __launch_bounds__(S::NT, (sizeof(typename S::T) == 2 && !kAlone<
 // exponentials. So a pair shares the keys: each wave computes P and dS for half of the tile's
 // rows, hands them to the other through LDS as the B operands that they are, and
 // accumulates half of the columns of dk and dv. Four blocks of 2048 (16 heads on 8
-// of 128, bf16): 428 us with whole waves, 336 so.
+// of 128, bf16), before parts shared the steps: 428 us with whole waves, 336 so.
 //
 // Where that gives too few workgroups (few key heads, short batches), `parts` of
 // them share a key tile's steps and leave fp32 sums in the workspace, which a
@@ -1259,7 +1267,7 @@ bool one_launch(const dgm_attn_cfg* c) {
 
 // Workgroups that share a key tile's steps: enough for three to a CU, each with a step
 // or more at the sequences' average length (four blocks of 2048, 544 causal tiles: 336 us
-// whole; two parts 279 and 28 for the sums. 15 of 1 to 1280, one fp32 head of 128, forward and
+// whole, two parts 279 and 28 for the sums when this was taken. 15 of 1 to 1280, one fp32 head of 128, forward and
 // backward 375 us, with two steps or more each; 301 so). One launch for dq, dk and dv is worth more
 // than parts of a few steps: dq then runs beside them. fp32, 4 heads of 32 over four times
 // 256, 41 us in parts, 28 whole; bf16, 4 heads of 64 over 1024, 62 and 47; but 8 query heads

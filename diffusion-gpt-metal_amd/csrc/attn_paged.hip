@@ -91,7 +91,8 @@ __device__ __forceinline__ void convert8(const IN* from, CT* to) {
 // A thread moves 8 elements of k and of v of one (row, head). The sequence of the
 // workgroup's first row is looked up by whole waves, 64 candidates a round; a thread's own row
 // lies in that or a later one. A write of few rows is a chain of waits: starts,
-// lengths, pages, rows.
+// lengths, pages, rows (48 rows: 3.5 us); of many, HBM-bound (8 heads of 128, 8162 rows, fp32 to a bf16
+// cache, 100 MB: 19 us, 5.3 TB/s).
 template <typename IN, typename CT>
 __global__ void __launch_bounds__(256) cache_write_kernel(WriteArgs a) {
     const int per_head = a.c.D / 8, per_row = a.c.KVH * per_head;
