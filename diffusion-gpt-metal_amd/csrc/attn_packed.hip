@@ -44,7 +44,7 @@
 // accumulates dq; another owns 32 keys per wave and accumulates dk and dv over all
 // query heads of the key head's group, so no gradient is added to by two
 // workgroups: no atomics, the same bits every time. Four of 2048 (16 heads on 8 of 128, bf16): dq 156 us,
-// dk and dv 239 and 32 for the sums of two parts; the matrix unit is busy in half
+// dk and dv DKV; the matrix unit is busy in half
 // of dq's cycles and a third of the other's, whose pairs of waves wait for one another.
 #include <algorithm>
 #include <climits>
@@ -1265,18 +1265,25 @@ bool one_launch(const dgm_attn_cfg* c) {
                        2 * dgm::kCus;
 }
 
-// Workgroups that share a key tile's steps: enough for three to a CU, each with a step
-// or more at the sequences' average length (four blocks of 2048, 544 causal tiles: 336 us
-// whole, two parts 279 and 28 for the sums when this was taken. 15 of 1 to 1280, one fp32 head of 128, forward and
-// backward 375 us, with two steps or more each; 301 so). One launch for dq, dk and dv is worth more
-// than parts of a few steps: dq then runs beside them. fp32, 4 heads of 32 over four times
-// 256, 41 us in parts, 28 whole; bf16, 4 heads of 64 over 1024, 62 and 47; but 8 query heads
-// on 2 over 900 rows 40 and 50.
+// Workgroups that share a key tile's steps, each with a step or more at the sequences' average length (15
+// of 1 to 1280, one fp32 head of 128, forward and backward 375 us, with two steps or more each; 301 so):
+// as many as give
+//  * bf16 of more than 64 columns, whose tiles fill a CU's LDS with one workgroup: one to a CU. In the order of
+//    falling work, the longest beside the shortest, more only add sums to write and read
+//    (four blocks of 2048, 16 heads on 8 of 128: 410 us whole, 467 in two parts; six of 1024, 16 on 4: 229, 246);
+//  * fp32 of more than 32 columns, also one to a CU but with steps six times as long: two (seven of 1 to
+//    1024, 12 heads on 4 of 64: 252 us with one, 213 with two, 220 with three);
+//  * the others, of which a CU holds two or more: three (24 heads on 8 of 64, six of 283 on average: 80 us,
+//    87 with two, 84 with four).
+// One launch for dq, dk and dv is worth more than parts of a few steps: dq then runs beside them.
+// fp32, 4 heads of 32 over four times 256, 41 us in parts, 28 whole; bf16, 4 heads of 64 over 1024, 62 and
+// 47; but 8 query heads on 2 over 900 rows 40 and 50.
 int64_t dkv_parts(const dgm_attn_cfg* c) {
     const int64_t tiles = slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH;
     const int64_t steps = (c->rows / std::max<int64_t>(c->nseq, 1) + 63) / 64 * (c->H / c->KVH);
     if (steps <= (c->H == c->KVH ? 16 : 4) && one_launch(c)) return 1;
-    return std::max<int64_t>(1, std::min<int64_t>({16, (3 * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps}));
+    const int per_cu = c->type == DGM_TYPE_BF16 ? (c->D > 64 ? 1 : 3) : c->D > 32 ? 2 : 3;
+    return std::max<int64_t>(1, std::min<int64_t>({16, (per_cu * dgm::kCus + tiles - 1) / std::max<int64_t>(tiles, 1), steps}));
 }
 
 template <typename S>
