@@ -728,6 +728,11 @@ struct BwdArgs {
 
 // dq: a wave's 32 queries against tiles of 64 keys. dS^T = P^T (dP^T - delta)
 // with dP^T = V dout^T; dq^T += K^T dS^T. delta = dout . out on the way, kept for the next kernel.
+//
+// A bf16 out is off by half a step, and so is delta, which over a few keys is as large as dP: two tokens' dq and dk were up
+// to six times as far off as their rounding. Where a sequence lies in one tile, delta is the sum of P dP, which it
+// stands for, from a first pass over the tile (a pass of its own: in the loop it would cost registers, and four
+// of 2048 430 us -> 443); over more keys out is small beside v, and its rounding beside dP (from 65 on no more than 1.5 times).
 template <typename S>
 struct DqRoom {
     __align__(16) uint8_t room[S::template kRoom<S::DT * 16>];
@@ -777,10 +782,27 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<S>& sh, uint32_
             for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(x[j], y[j], delta);
         }
     delta += __shfl_xor(delta, 32, 64);
-    if (in && h == 0 && kg == 0) a.delta[int64_t(head) * a.rows + at] = delta;
     float lse = in ? a.lse[int64_t(head) * a.rows + at] : 0.0f;
     asm volatile("" : "+v"(lse), "+v"(delta));
     const int last = a.causal && in ? row : rw.len - 1;
+    if constexpr (sizeof(T) == 2)
+        if (rw.len <= TILE) {
+            copies_ready();
+            if (kg == 0 && q0 < rw.len) {
+                f32x16 s[KB], dp[KB];
+                mm_rows2<T, DP, ROWS>(s, dp, lds[0][0], lds[0][1], 0, qf, gf, lane);
+                float sum = 0.0f;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float p = exp2_hw(__builtin_fmaf(s[kb][e], a.c, -lse));
+                        sum += 32 * kb + 8 * (e / 4) + e % 4 + 4 * h <= last ? p * dp[kb][e] : 0.0f;
+                    }
+                delta = sum + __shfl_xor(sum, 32, 64);
+            }
+        }
+    if (in && h == 0 && kg == 0) a.delta[int64_t(head) * a.rows + at] = delta;
     f32x16 acc[DT];
 #pragma unroll
     for (int n = 0; n < DT; ++n) acc[n] = f32x16{};
@@ -883,10 +905,26 @@ struct DkvRoom {
     __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];                                  // q and dout
     bf16x8 hand[DkvShape<T, DP>::NW][kPieces<T> + kSlopePieces<T>][2][64];            // P and dS, by wave, piece, 16 rows
     __align__(16) float stat[2][2][64];                                               // lse and delta, of two tiles
+    float sums[2][64];                                                                // of P dP, by pair of waves
     Marks<DP, 1> marks[2];
 };
 
-// kOwnDelta: delta from out and dout here, not from the dq kernel.
+// A wave's sums of 16 rows over 32 lanes, halving the rows that a lane has at each exchange: lane 2i of
+// the 32 is left with row i's (16 exchanges, where one row after the other takes 80).
+__device__ __forceinline__ float sum_lanes(f32x16 x, int lane) {
+#pragma unroll
+    for (int n = 8; n >= 1; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const bool up = lane & (2 * n);
+            const float keep = up ? x[i + n] : x[i], give = up ? x[i] : x[i + n];
+            x[i] = keep + __shfl_xor(give, 2 * n, 64);
+        }
+    return x[0] + __shfl_xor(x[0], 1, 64);
+}
+
+// kOwnDelta: delta from out and dout here, not from the dq kernel; in a bf16 sequence of one tile
+// the sum of P dP, as there (2.5 us).
 template <typename T, int DP, int DC, bool kOwnDelta>
 __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, uint32_t index) {
     using L = Lds<T, DP, 64>;
@@ -990,6 +1028,25 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
         const bool hidden = a.causal && row0 < (rw.tile + 1) * BK;
         const bool active = k0 < rw.len && !(a.causal && row0 + TILE <= k0);
         const bool dirty = hidden && __syncthreads_or(cq.bad(qt) || cg.bad(gt));
+        if constexpr (kOwnDelta && sizeof(T) == 2)
+            if (rw.len <= TILE) {   // row0 and the keys' first are 0
+                static_assert(NW == 4 && BK == TILE, "two pairs of waves have all keys");
+                f32x16 p[1]{}, dp[1]{};
+                if (active) mm_rows2<T, DP, 64>(p, dp, qt, gt, half, kf, vf, lane);
+                const int r0 = 32 * half + 4 * h, lo = (a.causal ? row : 0) - r0, hi = rw.len - r0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int i = 8 * (e / 4) + e % 4;
+                    const float w = exp2_hw(__builtin_fmaf(p[0][e], a.c, -lse[i])) * dp[0][e];
+                    dp[0][e] = in && i >= lo && i < hi ? w : 0.0f;
+                }
+                const float sum = sum_lanes(dp[0], lane);
+                const int e = (lane & 31) >> 1;
+                if ((lane & 1) == 0) sh.sums[wave >> 1][32 * half + 8 * (e / 4) + e % 4 + 4 * h] = sum;
+                __syncthreads();
+                if (threadIdx.x < TILE) stat[t % 2][1][threadIdx.x] = sh.sums[0][threadIdx.x] + sh.sums[1][threadIdx.x];
+                __syncthreads();
+            }
         if (active) {
             f32x16 p1[1], ds1[1];
             mm_rows2<T, DP, 64>(p1, ds1, qt, gt, half, kf, vf, lane);

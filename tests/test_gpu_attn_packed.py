@@ -470,3 +470,37 @@ def test_masked_values_in_every_layout(gpu, dgm, type_, D, H, KVH, lens):
             assert torch.equal(getattr(c, name)[rows], getattr(clean, name)[rows]), (what, name)
         if what in "kv":
             assert c.out[at:].isnan().any(2).all()
+
+
+@pytest.mark.parametrize("lens", [[2], [1, 3, 7, 64], [33, 40, 17]])
+@pytest.mark.parametrize("KVH,D", [(8, 32), (2, 32), (8, 64), (2, 64), (8, 80), (2, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_keys_keep_the_precision_of_bf16(gpu, dgm, lens, KVH, D, causal):
+    """Over a tile of keys or less dq and dk are rounded where they are written, not where out was: delta is as exact as
+    the products, and dS is taken in two pieces, off by 2^-8 of what one is."""
+    c = Case(dgm, "bf16", 8, KVH, D, lens, causal)
+    gpu.begin()
+    c.forward(gpu)
+    c.backward(gpu)
+    gpu.end()
+    q, k, v, dout = (t.double() for t in (c.q, c.k, c.v, c.dout))
+    want, off = ([torch.zeros_like(q), torch.zeros_like(k)] for _ in range(2))
+    for a, b in zip(c.starts_list[:-1], c.starts_list[1:]):
+        n = b - a
+        seen = torch.ones(n, n, dtype=torch.bool, device="cuda")
+        seen = seen.tril() if causal else seen
+        for h in range(8):
+            g = h * KVH // 8
+            args = [t.contiguous() for t in (q[a:b, h], k[a:b, g], v[a:b, g])]
+            S, W, eW = attn_ref.scores(args[0], args[1], c.scale, seen)
+            lse = torch.logsumexp(S, 1, keepdim=True)
+            eP = 2 * eW + (n + 4) * attn_ref.U + 4 * attn_ref.U * lse.abs()
+            near = (W * (eP + (D + n + 4) * attn_ref.U)) @ args[2].abs()    # the sum of P dP, as an error of out
+            (dq, dk, _), e0 = attn_ref.backward(*args, c.scale, seen, near, dout[a:b, h].contiguous(), False)
+            _, e1 = attn_ref.backward(*args, c.scale, seen, near, dout[a:b, h].contiguous(), True)
+            for i, (x, at) in enumerate(((dq, h), (dk, g))):
+                want[i][a:b, at] += x
+                off[i][a:b, at] += e0[i] + 2.0 ** -8 * (e1[i] - e0[i]) + 4 * n * attn_ref.U * x.abs()
+    for i, name in enumerate(("dq", "dk")):
+        bound = off[i] + attn_ref.rounding(torch.bfloat16) * (want[i].abs() + off[i]) + 1e-30
+        attn_ref.assert_within(getattr(c, name), want[i], bound, name)
