@@ -247,15 +247,18 @@ struct Frags {
     }
 };
 
-// acc += A B over their pieces: for fp32 the six products that reach 2^-24 of the largest.
-template <int PA, int PB>
+// acc += A B over their pieces: for fp32 the six products that reach 2^-24 of the largest. kTurned: in the
+// order that the product with A and B exchanged takes, for the same bits as it.
+template <bool kTurned = false, int PA, int PB>
 __device__ __forceinline__ void mfma_pieces(f32x16& acc, const bf16x8 (&a)[PA], const bf16x8 (&b)[PB]) {
 #pragma unroll
     for (int s = PA + PB - 2; s >= 0; --s)   // the small ones first
 #pragma unroll
-        for (int i = 0; i < PA; ++i)
+        for (int n = 0; n < PA; ++n) {
+            const int i = kTurned ? PA - 1 - n : n;
             if (s < 3 && s - i >= 0 && s - i < PB)
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[s - i], acc, 0, 0, 0);
+        }
 }
 
 constexpr int kRead = 0x100, kMfma = 0x8;   // instruction classes of __builtin_amdgcn_sched_group_barrier
@@ -305,7 +308,8 @@ __device__ __forceinline__ void mm_rows(f32x16 (&out)[KB], const uint8_t* tile, 
     reads_ahead<P, DC / 16 * KB>();
 }
 
-// The same of two tiles and two sets of vectors, for KB blocks from kb0 on.
+// The same of two tiles and two sets of vectors, for KB blocks from kb0 on; the bits of mm_rows of
+// the columns as a tile and the tile as columns.
 template <typename T, int DP, int ROWS, int KB, int DC>
 __device__ __forceinline__ void mm_rows2(f32x16 (&out)[KB], f32x16 (&out2)[KB], const uint8_t* tile, const uint8_t* tile2,
                                          int kb0, const Frags<T, DC>& b, const Frags<T, DC>& b2, int lane) {
@@ -331,8 +335,8 @@ __device__ __forceinline__ void mm_rows2(f32x16 (&out)[KB], f32x16 (&out2)[KB], 
                 x[p] = *reinterpret_cast<const bf16x8*>(tile + p * L::PLANE + at);
                 x2[p] = *reinterpret_cast<const bf16x8*>(tile2 + p * L::PLANE + at);
             }
-            mfma_pieces(out[kb], x, y);
-            mfma_pieces(out2[kb], x2, y2);
+            mfma_pieces<true>(out[kb], x, y);
+            mfma_pieces<true>(out2[kb], x2, y2);
         }
     }
     reads_ahead<P, 2 * (DC / 16) * KB>();
@@ -729,10 +733,12 @@ struct BwdArgs {
 // dq: a wave's 32 queries against tiles of 64 keys. dS^T = P^T (dP^T - delta)
 // with dP^T = V dout^T; dq^T += K^T dS^T. delta = dout . out on the way, kept for the next kernel.
 //
-// A bf16 out is off by half a step, and so is delta, which over a few keys is as large as dP: two tokens' dq and dk were up
-// to six times as far off as their rounding. Where a sequence lies in one tile, delta is the sum of P dP, which it
-// stands for, from a first pass over the tile (a pass of its own: in the loop it would cost registers, and four
-// of 2048 430 us -> 443); over more keys out is small beside v, and its rounding beside dP (from 65 on no more than 1.5 times).
+// Over a few keys delta is as large as dP, and what rounded out, or the sums of either, is off by stays
+// in dS: two bf16 tokens' dq and dk were up to six times as far off as their rounding, fp32 ones' 1e-6. Where a sequence lies in
+// one tile (fp32: has 16 keys or less), delta comes from a first pass over it: what it stands for, the sum of P dP by that of P, as a
+// difference from dP of key 0, so that one key alone leaves exactly 0. (A pass of its own: in the loop it would
+// cost registers, and four of 2048 430 us -> 443.) Over more keys out is small beside v, and so is its rounding (from 65
+// on no more than 1.5 times the gradients' own).
 template <typename S>
 struct DqRoom {
     __align__(16) uint8_t room[S::template kRoom<S::DT * 16>];
@@ -785,23 +791,27 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<S>& sh, uint32_
     float lse = in ? a.lse[int64_t(head) * a.rows + at] : 0.0f;
     asm volatile("" : "+v"(lse), "+v"(delta));
     const int last = a.causal && in ? row : rw.len - 1;
-    if constexpr (sizeof(T) == 2)
-        if (rw.len <= TILE) {
-            copies_ready();
-            if (kg == 0 && q0 < rw.len) {
-                f32x16 s[KB], dp[KB];
-                mm_rows2<T, DP, ROWS>(s, dp, lds[0][0], lds[0][1], 0, qf, gf, lane);
-                float sum = 0.0f;
+    if (rw.len <= (sizeof(T) == 2 ? TILE : 16)) {
+        turn(ck, cv, lds[0], [] {});
+        if (kg == 0 && q0 < rw.len) {
+            f32x16 s[KB], dp[KB];
+            mm_rows<T, DP, ROWS>(s, lds[0][0], qf, lane);
+            mm_rows<T, DP, ROWS>(dp, lds[0][1], gf, lane);
+            const float ref = __shfl(dp[0][0], lane & 31, 64);
+            float sum = 0.0f, weights = 0.0f;
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p = exp2_hw(__builtin_fmaf(s[kb][e], a.c, -lse));
-                        sum += 32 * kb + 8 * (e / 4) + e % 4 + 4 * h <= last ? p * dp[kb][e] : 0.0f;
-                    }
-                delta = sum + __shfl_xor(sum, 32, 64);
-            }
+                for (int e = 0; e < 16; ++e) {
+                    const bool see = 32 * kb + 8 * (e / 4) + e % 4 + 4 * h <= last;
+                    const float p = see ? exp2_hw(__builtin_fmaf(s[kb][e], a.c, -lse)) : 0.0f;
+                    weights += p;
+                    sum += see ? p * (dp[kb][e] - ref) : 0.0f;
+                }
+            sum += __shfl_xor(sum, 32, 64);
+            delta = ref + sum / (weights + __shfl_xor(weights, 32, 64));
         }
+    }
     if (in && h == 0 && kg == 0) a.delta[int64_t(head) * a.rows + at] = delta;
     f32x16 acc[DT];
 #pragma unroll
@@ -905,26 +915,10 @@ struct DkvRoom {
     __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];                                  // q and dout
     bf16x8 hand[DkvShape<T, DP>::NW][kPieces<T> + kSlopePieces<T>][2][64];            // P and dS, by wave, piece, 16 rows
     __align__(16) float stat[2][2][64];                                               // lse and delta, of two tiles
-    float sums[2][64];                                                                // of P dP, by pair of waves
     Marks<DP, 1> marks[2];
 };
 
-// A wave's sums of 16 rows over 32 lanes, halving the rows that a lane has at each exchange: lane 2i of
-// the 32 is left with row i's (16 exchanges, where one row after the other takes 80).
-__device__ __forceinline__ float sum_lanes(f32x16 x, int lane) {
-#pragma unroll
-    for (int n = 8; n >= 1; n >>= 1)
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const bool up = lane & (2 * n);
-            const float keep = up ? x[i + n] : x[i], give = up ? x[i] : x[i + n];
-            x[i] = keep + __shfl_xor(give, 2 * n, 64);
-        }
-    return x[0] + __shfl_xor(x[0], 1, 64);
-}
-
-// kOwnDelta: delta from out and dout here, not from the dq kernel; in a bf16 sequence of one tile
-// the sum of P dP, as there (2.5 us).
+// kOwnDelta: delta from out and dout here, not from the dq kernel.
 template <typename T, int DP, int DC, bool kOwnDelta>
 __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, uint32_t index) {
     using L = Lds<T, DP, 64>;
@@ -1028,25 +1022,6 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
         const bool hidden = a.causal && row0 < (rw.tile + 1) * BK;
         const bool active = k0 < rw.len && !(a.causal && row0 + TILE <= k0);
         const bool dirty = hidden && __syncthreads_or(cq.bad(qt) || cg.bad(gt));
-        if constexpr (kOwnDelta && sizeof(T) == 2)
-            if (rw.len <= TILE) {   // row0 and the keys' first are 0
-                static_assert(NW == 4 && BK == TILE, "two pairs of waves have all keys");
-                f32x16 p[1]{}, dp[1]{};
-                if (active) mm_rows2<T, DP, 64>(p, dp, qt, gt, half, kf, vf, lane);
-                const int r0 = 32 * half + 4 * h, lo = (a.causal ? row : 0) - r0, hi = rw.len - r0;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int i = 8 * (e / 4) + e % 4;
-                    const float w = exp2_hw(__builtin_fmaf(p[0][e], a.c, -lse[i])) * dp[0][e];
-                    dp[0][e] = in && i >= lo && i < hi ? w : 0.0f;
-                }
-                const float sum = sum_lanes(dp[0], lane);
-                const int e = (lane & 31) >> 1;
-                if ((lane & 1) == 0) sh.sums[wave >> 1][32 * half + 8 * (e / 4) + e % 4 + 4 * h] = sum;
-                __syncthreads();
-                if (threadIdx.x < TILE) stat[t % 2][1][threadIdx.x] = sh.sums[0][threadIdx.x] + sh.sums[1][threadIdx.x];
-                __syncthreads();
-            }
         if (active) {
             f32x16 p1[1], ds1[1];
             mm_rows2<T, DP, 64>(p1, ds1, qt, gt, half, kf, vf, lane);
@@ -1312,13 +1287,12 @@ int dkv_keys(const dgm_attn_cfg* c) {
     return c->D <= 32 ? DkvShape<float, 32>::BK : c->D <= 64 ? DkvShape<float, 64>::BK : DkvShape<float, 128>::BK;
 }
 
-// dq and dk, dv can go in one launch: with as many threads to a workgroup, and no more
-// workgroups than two to a CU.
+// dq and dk, dv can go in one launch, each with its own delta from out and dout: with as many threads
+// to a workgroup, no more workgroups than two to a CU, an exact out (fp32) and more than a few keys to a sequence.
 template <typename T, int DP>
-constexpr bool kOneLaunch = DkvShape<T, DP>::NW == 4 && DP <= 64;
+constexpr bool kOneLaunch = sizeof(T) == 4 && DP == 32;
 bool one_launch(const dgm_attn_cfg* c) {
-    const bool fits = c->D <= 32 || (c->D <= 64 && c->type == DGM_TYPE_BF16);
-    return fits && slot_count(c->rows, c->nseq, 128) * c->H + slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH <=
+    return c->type == DGM_TYPE_F32 && c->D <= 32 && c->rows > 32 * c->nseq && slot_count(c->rows, c->nseq, 128) * c->H + slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH <=
                        2 * dgm::kCus;
 }
 
@@ -1333,8 +1307,7 @@ bool one_launch(const dgm_attn_cfg* c) {
 //  * the others, of which a CU holds two or more: three (24 heads on 8 of 64, six of 283 on average: 80 us,
 //    87 with two, 84 with four).
 // One launch for dq, dk and dv is worth more than parts of a few steps: dq then runs beside them.
-// fp32, 4 heads of 32 over four times 256, 41 us in parts, 28 whole; bf16, 4 heads of 64 over 1024, 62 and
-// 47; but 8 query heads on 2 over 900 rows 40 and 50.
+// fp32, 4 heads of 32 over four times 256, 41 us in parts, 28 whole; but 8 query heads on 2 over 900 rows 40 and 50.
 int64_t dkv_parts(const dgm_attn_cfg* c) {
     const int64_t tiles = slot_count(c->rows, c->nseq, dkv_keys(c)) * c->KVH;
     const int64_t steps = (c->rows / std::max<int64_t>(c->nseq, 1) + 63) / 64 * (c->H / c->KVH);

@@ -504,3 +504,16 @@ def test_few_keys_keep_the_precision_of_bf16(gpu, dgm, lens, KVH, D, causal):
     for i, name in enumerate(("dq", "dk")):
         bound = off[i] + attn_ref.rounding(torch.bfloat16) * (want[i].abs() + off[i]) + 1e-30
         attn_ref.assert_within(getattr(c, name), want[i], bound, name)
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("KVH,D", [(8, 32), (2, 64), (8, 96), (2, 128)])
+def test_one_key_has_no_slope(gpu, dgm, type_, KVH, D):
+    """A softmax over one key is 1 whatever the score: dq and dk are 0, not what rounding leaves."""
+    c = Case(dgm, type_, 8, KVH, D, [1, 1, 1])
+    gpu.begin()
+    c.forward(gpu)
+    c.backward(gpu)
+    gpu.end()
+    assert not c.dq.any() and not c.dk.any()
+    c.check(True)
