@@ -382,6 +382,8 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
             f32x4 sc[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) sc[b] = f32x4{0, 0, 0, 0};
+            // fp32: four sums, each a quarter as long (heads of 256 over 5000 keys were off by twice what the plain sums are).
+            f32x4 quarter[4] = {};
 #pragma unroll
             for (int kk = 0; kk < Q::KC; ++kk)
 #pragma unroll
@@ -395,11 +397,12 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) attn_pa
                         } else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                sc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][kk][i]),
-                                                                             __uint_as_float(y[i]), sc[b], 0, 0, 0);
+                                quarter[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(now.k[b][kk][i]),
+                                                                                  __uint_as_float(y[i]), quarter[i], 0, 0, 0);
                         }
                     }
                 }
+            if constexpr (sizeof(CT) == 4) sc[0] = (quarter[0] + quarter[1]) + (quarter[2] + quarter[3]);
             // The keys' registers are free for those of the next round.
             row = row_of(t + 1, id1);
             if (t + 1 < t1) now.load_k(a.c, kc, row);
