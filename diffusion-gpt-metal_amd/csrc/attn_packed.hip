@@ -36,15 +36,15 @@
 //    first, and the sums that they belong to spoilt afterwards.
 //
 // Long sequences are bound by the matrix unit: a prompt of 8192 (32 heads on 8 of 128,
-// bf16) takes 530 us, 1,037 TFLOP/s, where a library product reaches 1,158; four of 640 to 2048 in
-// fp32 (16 heads on 4 of 64) 108 us, 150 TFLOP/s, where a library product reaches 153. Short ones
+// bf16) takes 524 us, 1,050 TFLOP/s, where a library product reaches 1,158; four of 640 to 2048 in
+// fp32 (16 heads on 4 of 64) 106 us, 153 TFLOP/s, where a library product reaches 153. Short ones
 // are a chain of waits: starts, tiles, exponentials, rows out (16 of 64: 6 us).
 //
 // The backward recomputes P from lse. One kernel owns 32 queries per wave and
 // accumulates dq; another owns 32 keys per wave and accumulates dk and dv over all
 // query heads of the key head's group, so no gradient is added to by two
 // workgroups: no atomics, the same bits every time. Four of 2048 (16 heads on 8 of 128, bf16): dq 156 us,
-// dk and dv DKV; the matrix unit is busy in half
+// dk and dv 212; the matrix unit is busy in half
 // of dq's cycles and a third of the other's, whose pairs of waves wait for one another.
 #include <algorithm>
 #include <climits>

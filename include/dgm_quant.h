@@ -479,9 +479,8 @@ int dgm_biasGrad(dgm_gpu* g, const float* dy, float* db, int64_t M, int64_t N);
  * keys and values of past tokens can be kept in pages.
  *
  * Types: DGM_TYPE_F32 or DGM_TYPE_BF16. Scores, softmax statistics and sums
- * are fp32 for both; for bf16 the probabilities (and in the backward their
- * gradients) are rounded to bf16 between the two products. dgm_set_math does not
- * change these calls.
+ * are fp32 for both; for bf16 the probabilities are rounded to bf16 between the
+ * two products. dgm_set_math does not change these calls.
  *
  * Sequence starts, lengths and page tables are read on the device only, so that
  * captured graphs can be replayed with other ones. Where they are wrong (starts out of
