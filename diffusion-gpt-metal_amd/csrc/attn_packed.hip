@@ -130,7 +130,7 @@ struct Feed {
                 for (int i = 0; i < N; ++i) {
                     const uint32_t off =
                         uint32_t(row) * uint32_t(ldb) + uint32_t((slot ^ L::swizzle(row + i * STEP)) << 4);
-                    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(base + i * NT * 16),
+                    asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(base + i * NT * 16),
                                  "v"(off), "s"(first + i * STEP * ldb)
                                  : "memory", "m0");
                 }
@@ -151,7 +151,7 @@ struct Feed {
                 for (int i = 0; i < N; ++i) {
                     const int r = row + i * STEP, c = slot ^ L::swizzle(r);
                     if (r < rows && c * 8 < D)
-                        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base + i * NT * 16),
+                        asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, off" ::"s"(base + i * NT * 16),
                                      "v"(src + r * ldb + c * 16)
                                      : "memory", "m0");
                     else

@@ -278,6 +278,11 @@ inline unsigned ceil_div(int64_t a, int64_t b) { return unsigned((a + b - 1) / b
 
 }  // namespace dgm
 
+// The start of an asm string that copies from memory straight into LDS, at the address in operand 0
+// (global_load_lds_*): the instruction set asks for one wait state between a scalar write of m0 and the copy.
+// The compiler puts it before the copies of its own builtin, and not into an asm string.
+#define DGM_M0 "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+
 #define DGM_LAUNCH_CHECK(g, name)                         \
     do {                                                  \
         int _rc = ::dgm::check_launch((g), (name));       \

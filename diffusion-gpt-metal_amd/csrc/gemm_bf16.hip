@@ -181,7 +181,7 @@ __global__ __launch_bounds__(NTW) void gemm_bf16_kernel(Bf16Args a) {
             const uint32_t lds = lds0 + uint32_t(st * TILE_X + p * 128 * RS);
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + j * 8 * RS),
+                asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(lds + j * 8 * RS),
                              "v"(aoff[j] + uint32_t(ks * BK * 2)), "s"(a.Xb)
                              : "memory", "m0");
         };

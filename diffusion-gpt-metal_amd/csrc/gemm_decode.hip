@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * (DEC_KW * MW + 1), 1) void decode_kernel(DecAr
 #pragma clang diagnostic ignored "-Winline-asm"
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
+                    asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
                                  "v"(doff[i] + uint32_t(chunk) * 128u), "s"(a.W)
                                  : "memory", "m0");
 #pragma clang diagnostic pop
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(64 * (DEC_KW * MW + 1), 1) void decode_kernel(DecAr
 #pragma clang diagnostic ignored "-Winline-asm"
 #pragma unroll
                 for (int i = 0; i < SQ; ++i)
-                    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
+                    asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
                                  "v"(srow + 4u * uint32_t(min(first + 4 * i, a.groups - 4))), "s"(a.S)
                                  : "memory", "m0");
 #pragma clang diagnostic pop
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(64 * (DEC_KW * MW + 1), 1) void decode_kernel(DecAr
 #pragma clang diagnostic ignored "-Winline-asm"
             const int ng = ((2 * (ch0 + nch) - 1) >> a.gshift) - g0 + 1;
             for (int g = 0; g < ng; ++g)
-                asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + DEC_LDS + g * 256),
+                asm volatile(DGM_M0 "global_load_lds_dword %1, %2" ::"s"(lds0 + DEC_LDS + g * 256),
                              "v"(srow + 4u * uint32_t(g0 + g)), "s"(a.S)
                              : "memory", "m0");
 #pragma clang diagnostic pop
@@ -868,7 +868,7 @@ __global__ __launch_bounds__(DS_THREADS, 1) void decode_small_kernel(DecArgs a, 
                 const uint32_t lds = lds0 + DS_WOFF + uint32_t((t % DS_WS) * 4 + cw) * DS_WBLK;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
+                    asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
                                  "v"(woff[i]), "s"(src)
                                  : "memory", "m0");
             }
@@ -876,7 +876,7 @@ __global__ __launch_bounds__(DS_THREADS, 1) void decode_small_kernel(DecArgs a, 
         dma_interval(0);
         const uint32_t srow = uint32_t(min(n0 + lane, a.N - 1)) * uint32_t(a.groups) * 4u;
         for (int g = 0; g < a.groups; ++g)
-            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + DS_SOFF + g * 256),
+            asm volatile(DGM_M0 "global_load_lds_dword %1, %2" ::"s"(lds0 + DS_SOFF + g * 256),
                          "v"(srow + 4u * uint32_t(g)), "s"(a.S)
                          : "memory", "m0");
         if (T > 1) dma_interval(1);
@@ -914,7 +914,7 @@ __global__ __launch_bounds__(DS_THREADS, 1) void decode_small_kernel(DecArgs a, 
         const uint32_t lds = xlds + uint32_t(slot) * DS_XSLOT;
 #pragma unroll
         for (int j = 0; j < XI; ++j)
-            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + j * 1024), "v"(xsrc[j]),
+            asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(lds + j * 1024), "v"(xsrc[j]),
                          "s"(src)
                          : "memory", "m0");
     };

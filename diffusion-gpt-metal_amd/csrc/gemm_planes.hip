@@ -614,11 +614,11 @@ __global__ __launch_bounds__(64 * T::WAVES, 2) void plane_gemm_kernel(PlaneGroup
         const uint32_t lds = lds0 + uint32_t(slot) * T::STAGE + uint32_t(wave * T::UPW) * 1024u;
 #pragma unroll
         for (int i = 0; i < T::UPW; ++i)
-            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
+            asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2" ::"s"(lds + i * 1024),
                          "v"(at * (T::AU == T::BU ? T::AU * 1024u : step_bytes[i]) + uint32_t(lane) * 16u), "s"(src[i])
                          : "memory", "m0");
         if constexpr (CODE)   // waves past the tile's columns load them again
-            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(
+            asm volatile(DGM_M0 "global_load_lds_dword %1, %2" ::"s"(
                              lds0 + uint32_t(slot) * T::STAGE + T::UNITS * 1024u +
                              uint32_t(wave % (T::TN / 64)) * 256u),
                          "v"(at / uint32_t(a.gps) * uint32_t(a.scale_ld) * 4u + scol), "s"(a.scales)

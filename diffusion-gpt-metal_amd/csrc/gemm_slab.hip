@@ -76,9 +76,9 @@ struct SlabArgs {
     int M, N, K, groups, gshift, rowb;
 };
 
-#define SB_DMA16(lds, voff, base)                                                               \
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(voff), \
-                 "s"(base)                                                                      \
+#define SB_DMA16(lds, voff, base)                                                  \
+    asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(voff), \
+                 "s"(base)                                                         \
                  : "memory", "m0")
 
 template <int N>
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(64 * SB_WAVES, 1) void slab_kernel(SlabArgs a) {
     for (int t = 0; t < 2; ++t) {
         const int r = min(n0 + 16 * t + (lane >> 2), a.N - 1);
         const uint32_t g = uint32_t(sl * SB_NB + (lane & 3)) >> a.gshift;
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(
+        asm volatile(DGM_M0 "global_load_lds_dword %1, %2" ::"s"(
                          lds0 + uint32_t(SB_S_OFF + (w * SB_ROWS + 16 * t) * SB_NB * 4)),
                      "v"((uint32_t(r) * uint32_t(a.groups) + g) * 4u), "s"(a.S)
                      : "memory", "m0");

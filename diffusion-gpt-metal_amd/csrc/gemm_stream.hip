@@ -61,9 +61,9 @@ struct StreamArgs {
 // reserves M0 but uses it in this kernel for nothing else (no LDS-DMA
 // builtins, no indexed register access). Weights are read once per call:
 // non-temporal, so that they do not evict X and the scales from L2.
-#define ST_DMA(lds, voff, base)                                                                 \
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(voff), \
-                 "s"(base)                                                                      \
+#define ST_DMA(lds, voff, base)                                                    \
+    asm volatile(DGM_M0 "global_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(voff), \
+                 "s"(base)                                                         \
                  : "memory", "m0")
 
 template <int N>
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(64 * NW, 1) void stream_i8_kernel(StreamArgs a) {
         const uint32_t send = uint32_t(a.N) * uint32_t(a.groups) * 4u;
         for (int i = w; i < a.ns; i += NW, ++nsw) {
             const uint32_t src = sbase + uint32_t(i) * 256u + 4u * uint32_t(lane);
-            asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + a.s_off + uint32_t(i) * 256u),
+            asm volatile(DGM_M0 "global_load_lds_dword %1, %2" ::"s"(lds0 + a.s_off + uint32_t(i) * 256u),
                          "v"(src < send ? src : send - 4u), "s"(a.S)
                          : "memory", "m0");
         }
