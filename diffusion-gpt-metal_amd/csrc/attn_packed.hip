@@ -717,6 +717,34 @@ __global__ void __launch_bounds__(S::NT, S::DP <= (sizeof(typename S::T) == 2 ? 
 template <typename T>
 constexpr int kSlopePieces = sizeof(T) == 2 ? 2 : 3;
 
+// Delta of rows that see kFewKeys keys or less. Over few keys it is as large as dP, and what rounded out, or the sums of
+// either, is off by stays in dS. 400 sequences of 128 causal bf16 tokens, heads of 128, dq's error by that of rounding it once:
+// median 2.2 and at the worst 420 in the row of two keys, 1.0 and 30 of four, 0.2 and 3 from 65 on; fp32 rows of two keys were
+// 1e-6 off. So there it is what it stands for, the sum of P dP by that of P, as a difference from dP of key 0, and
+// one key alone leaves exactly 0. It goes by the keys that a row sees and by nothing else, so that neither the rest of the batch
+// nor the layout changes a row's delta.
+template <typename T>
+constexpr int kFewKeys = sizeof(T) == 2 ? 64 : 16;
+template <typename T>
+constexpr int kFewBlocks = (kFewKeys<T> + 31) / 32;   // of 32 keys
+
+struct FewKeys {
+    float ref = 0.0f, sum = 0.0f, weights = 0.0f;
+    // Of 32 keys, a query in each lane pair: s and dP as mm_rows leaves them, keys up to element lim are seen.
+    __device__ __forceinline__ void add(const f32x16& s, const f32x16& dp, int lim, float c, float lse) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const bool see = 8 * (e / 4) + e % 4 <= lim;
+            const float p = see ? exp2_hw(__builtin_fmaf(s[e], c, -lse)) : 0.0f;
+            weights += p;
+            sum += see ? p * (dp[e] - ref) : 0.0f;
+        }
+    }
+    __device__ __forceinline__ float delta() const {
+        return ref + (sum + __shfl_xor(sum, 32, 64)) / (weights + __shfl_xor(weights, 32, 64));
+    }
+};
+
 struct BwdArgs {
     const void *q, *k, *v, *out, *dout;
     void *dq, *dk, *dv;
@@ -731,14 +759,8 @@ struct BwdArgs {
 };
 
 // dq: a wave's 32 queries against tiles of 64 keys. dS^T = P^T (dP^T - delta)
-// with dP^T = V dout^T; dq^T += K^T dS^T. delta = dout . out on the way, kept for the next kernel.
-//
-// Over a few keys delta is as large as dP, and what rounded out, or the sums of either, is off by stays
-// in dS: two bf16 tokens' dq and dk were up to six times as far off as their rounding, fp32 ones' 1e-6. Where a sequence lies in
-// one tile (fp32: has 16 keys or less), delta comes from a first pass over it: what it stands for, the sum of P dP by that of P, as a
-// difference from dP of key 0, so that one key alone leaves exactly 0. (A pass of its own: in the loop it would
-// cost registers, and four of 2048 430 us -> 443.) Over more keys out is small beside v, and so is its rounding (from 65
-// on no more than 1.5 times the gradients' own).
+// with dP^T = V dout^T; dq^T += K^T dS^T. delta = dout . out on the way, kept for the next kernel; of rows that see few keys,
+// from a first pass over those. (A pass of its own: in the loop it would cost registers, and four of 2048 430 us -> 443.)
 template <typename S>
 struct DqRoom {
     __align__(16) uint8_t room[S::template kRoom<S::DT * 16>];
@@ -791,25 +813,21 @@ __device__ __forceinline__ void dq_body(const BwdArgs& a, DqRoom<S>& sh, uint32_
     float lse = in ? a.lse[int64_t(head) * a.rows + at] : 0.0f;
     asm volatile("" : "+v"(lse), "+v"(delta));
     const int last = a.causal && in ? row : rw.len - 1;
-    if (rw.len <= (sizeof(T) == 2 ? TILE : 16)) {
+    static_assert(ROWS >= kFewKeys<T> && ROWS >= 32 * kFewBlocks<T>, "the first tile holds the few keys");
+    if (a.causal ? rw.tile * BQ < kFewKeys<T> : rw.len <= kFewKeys<T>) {
         turn(ck, cv, lds[0], [] {});
-        if (kg == 0 && q0 < rw.len) {
-            f32x16 s[KB], dp[KB];
-            mm_rows<T, DP, ROWS>(s, lds[0][0], qf, lane);
-            mm_rows<T, DP, ROWS>(dp, lds[0][1], gf, lane);
-            const float ref = __shfl(dp[0][0], lane & 31, 64);
-            float sum = 0.0f, weights = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const bool see = 32 * kb + 8 * (e / 4) + e % 4 + 4 * h <= last;
-                    const float p = see ? exp2_hw(__builtin_fmaf(s[kb][e], a.c, -lse)) : 0.0f;
-                    weights += p;
-                    sum += see ? p * (dp[kb][e] - ref) : 0.0f;
-                }
-            sum += __shfl_xor(sum, 32, 64);
-            delta = ref + sum / (weights + __shfl_xor(weights, 32, 64));
+        if (q0 < rw.len && (!a.causal || q0 < kFewKeys<T>)) {   // each of a block's waves for itself
+            FewKeys few;
+#pragma unroll 1   // unrolled, four of 2048 take 4 us more: registers
+            for (int kb = 0; kb < kFewBlocks<T>; ++kb) {
+                f32x16 s[1], dp[1];
+                mm_rows<T, DP, ROWS>(s, lds[0][0] + kb * 32 * L::RB, qf, lane);
+                mm_rows<T, DP, ROWS>(dp, lds[0][1] + kb * 32 * L::RB, gf, lane);
+                if (kb == 0) few.ref = __shfl(dp[0][0], lane & 31, 64);
+                few.add(s[0], dp[0], last - 32 * kb - 4 * h, a.c, lse);
+            }
+            const float of_few = few.delta();
+            delta = last < kFewKeys<T> ? of_few : delta;
         }
     }
     if (in && h == 0 && kg == 0) a.delta[int64_t(head) * a.rows + at] = delta;
