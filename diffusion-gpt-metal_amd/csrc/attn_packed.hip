@@ -730,7 +730,8 @@ constexpr int kFewBlocks = (kFewKeys<T> + 31) / 32;   // of 32 keys
 
 struct FewKeys {
     float ref = 0.0f, sum = 0.0f, weights = 0.0f;
-    // Of 32 keys, a query in each lane pair: s and dP as mm_rows leaves them, keys up to element lim are seen.
+    // Of 32 keys, a query in each lane pair: s and dP as mm_rows leaves them, keys up to element lim are seen. The same
+    // order in every kernel, for the same bits.
     __device__ __forceinline__ void add(const f32x16& s, const f32x16& dp, int lim, float c, float lse) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -933,10 +934,11 @@ struct DkvRoom {
     __align__(16) uint8_t lds[L::NBUF][2][L::BYTES];                                  // q and dout
     bf16x8 hand[DkvShape<T, DP>::NW][kPieces<T> + kSlopePieces<T>][2][64];            // P and dS, by wave, piece, 16 rows
     __align__(16) float stat[2][2][64];                                               // lse and delta, of two tiles
+    __align__(16) float few[32];                                                      // delta of rows that see few keys
     Marks<DP, 1> marks[2];
 };
 
-// kOwnDelta: delta from out and dout here, not from the dq kernel.
+// kOwnDelta: delta from out and dout (or of few keys) here, not from the dq kernel.
 template <typename T, int DP, int DC, bool kOwnDelta>
 __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, uint32_t index) {
     using L = Lds<T, DP, 64>;
@@ -1040,6 +1042,38 @@ __device__ __forceinline__ void dkv_body(const BwdArgs& a, DkvRoom<T, DP>& sh, u
         const bool hidden = a.causal && row0 < (rw.tile + 1) * BK;
         const bool active = k0 < rw.len && !(a.causal && row0 + TILE <= k0);
         const bool dirty = hidden && __syncthreads_or(cq.bad(qt) || cg.bad(gt));
+        if constexpr (kOwnDelta) {
+            // Rows that see few keys are among the first 32, their keys among this wave's: no other one sees those. The
+            // dq kernel's products, keys as rows and queries as columns, with the same bits.
+            static_assert(kFewKeys<T> <= 32 && kFewBlocks<T> == 1, "one wave has them");
+            if (k0 == 0 && half == 0 && row0 == 0 && (a.causal || rw.len <= kFewKeys<T>)) {
+                f32x16 s{}, dp{};
+#pragma unroll
+                for (int kk = 0; kk < DC / 16; ++kk) {
+                    bf16x8 kx[PP], vx[PP], x[PP], y[PP];
+#pragma unroll
+                    for (int p = 0; p < PP; ++p) {
+                        const int at = p * L::PLANE + L::at(lane & 31, 2 * kk + h);
+                        kx[p] = kf.f[p][kk];
+                        vx[p] = vf.f[p][kk];
+                        x[p] = *reinterpret_cast<const bf16x8*>(qt + at);
+                        y[p] = *reinterpret_cast<const bf16x8*>(gt + at);
+                    }
+                    mfma_pieces(s, kx, x);
+                    mfma_pieces(dp, vx, y);
+                }
+                const int r = lane & 31, seen = a.causal && r < rw.len ? r : rw.len - 1;   // its last key
+                FewKeys few;
+                few.ref = __shfl(dp[0], r, 64);
+                few.add(s, dp, seen - 4 * h, a.c, stat[t % 2][0][r]);
+                const float of_few = few.delta();
+                if (h == 0) sh.few[r] = seen < kFewKeys<T> ? of_few : stat[t % 2][1][r];
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                delta = sh.few + 4 * h;
+            }
+        }
         if (active) {
             f32x16 p1[1], ds1[1];
             mm_rows2<T, DP, 64>(p1, ds1, qt, gt, half, kf, vf, lane);
@@ -1151,7 +1185,7 @@ __global__ void __launch_bounds__((64 * DkvShape<T, DP>::NW), (sizeof(T) == 4 &&
 }
 
 // Both in one launch, a workgroup one or the other, for grids that the chip holds at once:
-// forward and backward of 16 sequences of 64 (4 heads of 32, fp32) take 15 us so, 22 in three launches.
+// forward and backward of 16 sequences of 64 (4 heads of 32, fp32) take 16 us so, 22 in three launches.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, 2) attn_packed_grads_kernel(BwdArgs a, uint32_t first, int64_t dkv_slots) {
     __shared__ union Room {
@@ -1306,7 +1340,7 @@ int dkv_keys(const dgm_attn_cfg* c) {
 }
 
 // dq and dk, dv can go in one launch, each with its own delta from out and dout: with as many threads
-// to a workgroup, no more workgroups than two to a CU, an exact out (fp32) and more than a few keys to a sequence.
+// to a workgroup, no more workgroups than two to a CU, an exact out (fp32) and more than 32 rows to a sequence on average.
 template <typename T, int DP>
 constexpr bool kOneLaunch = sizeof(T) == 4 && DP == 32;
 bool one_launch(const dgm_attn_cfg* c) {
