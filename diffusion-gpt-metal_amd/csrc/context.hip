@@ -7,6 +7,7 @@
 
 #include "attn.hpp"
 #include "common.hpp"
+#include "reports.hpp"
 
 namespace {
 
@@ -16,33 +17,16 @@ namespace {
 __device__ __align__(256) uint8_t scratch[dgm::kScratchBytes];
 
 // What the attention and cache kernels find wrong in sequence starts, lengths and page
-// tables, which only the device reads: two words a context, in host memory, so that
-// dgm_end looks at them without a copy. Never freed: a captured graph may outlive its
-// context. Contexts beyond kReports at once share the last.
-constexpr int kReports = 512;
-std::mutex reports_mu;
-uint32_t* reports = nullptr;
-bool report_used[kReports] = {};
+// tables, which only the device reads; in host memory, so that dgm_end looks at it without a copy.
+dgm::ReportWords reports;
 
 uint32_t* take_report() {
-    std::lock_guard<std::mutex> lock(reports_mu);
-    if (!reports) {
+    return reports.take([](size_t bytes) -> void* {
         void* p = nullptr;
-        if (hipHostMalloc(&p, kReports * 2 * sizeof(uint32_t), hipHostMallocPortable | hipHostMallocMapped) != hipSuccess) {
-            (void)hipGetLastError();
-            return nullptr;
-        }
-        reports = static_cast<uint32_t*>(p);
-    }
-    int i = 0;
-    while (i < kReports - 1 && report_used[i]) ++i;
-    report_used[i] = true;
-    reports[2 * i] = reports[2 * i + 1] = 0;
-    return reports + 2 * i;
-}
-void return_report(uint32_t* words) {
-    std::lock_guard<std::mutex> lock(reports_mu);
-    if (words) report_used[(words - reports) / 2] = false;
+        const hipError_t e = hipHostMalloc(&p, bytes, hipHostMallocPortable | hipHostMallocMapped);
+        if (e != hipSuccess) (void)hipGetLastError();
+        return e == hipSuccess ? p : nullptr;
+    });
 }
 
 constexpr int kMaxDevices = 64;
@@ -284,7 +268,6 @@ void dgm_gpu_destroy(dgm_gpu* g) {
     for (int i = 0; i < g->n_planes_retired; ++i) (void)hipFree(g->planes_retired[i]);
     if (g->planes_event) (void)hipEventDestroy(g->planes_event);
     if (g->own_stream) (void)hipStreamDestroy(g->own_stream);
-    return_report(g->seq_report);
     delete g;
 }
 

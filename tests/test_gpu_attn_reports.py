@@ -1,0 +1,59 @@
+"""Reports of bad starts and pages: the region's end of the context that launched the kernels, and of no other."""
+from __future__ import annotations
+
+import pytest
+
+from test_gpu_attn_paged import cache_case
+
+pytestmark = pytest.mark.gpu
+
+
+class Step:
+    """A decode of two sequences, whose table is right until spoil()."""
+
+    def __init__(self, dgm, torch):
+        self.dgm = dgm
+        self.cfg, self.q, self.kc, self.vc, self.pages, self.n = cache_case(dgm, "f32", "f32", 4, 2, 32, 16, [40, 9])
+        self.out = torch.zeros_like(self.q)
+        self.ws = None
+
+    def __call__(self, gpu):
+        import torch
+        if self.ws is None:
+            self.ws = torch.empty(gpu.attnPagedDecode_ws_bytes(self.cfg, 2, 4), dtype=torch.uint8, device="cuda")
+        gpu.attnPagedDecode(self.cfg, self.dgm.DGM_TYPE_F32, self.q, self.kc, self.vc, self.pages, self.n, self.out,
+                            self.ws, self.ws.numel(), 2, 4)
+
+    def spoil(self):
+        self.pages[0, 1] = -1
+
+
+def test_a_graph_that_outlives_its_context_blames_no_other(dgm, torch_cuda):
+    torch = torch_cuda
+    stream = torch.cuda.Stream()
+    step = Step(dgm, torch)
+    g = dgm.GPU(stream=stream)
+    g.begin()
+    step(g)
+    g.end()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    g.begin()
+    with torch.cuda.graph(graph, stream=stream):
+        step(g)
+    g.end()
+    g.close()
+    others = [dgm.GPU(stream=stream) for _ in range(4)]
+    try:
+        step.spoil()
+        torch.cuda.synchronize()
+        for x in others:
+            x.begin()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        stream.synchronize()
+        for x in others:
+            x.end()
+    finally:
+        for x in others:
+            x.close()
