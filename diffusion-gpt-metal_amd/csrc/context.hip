@@ -23,8 +23,12 @@ dgm::ReportWords reports;
 uint32_t* take_report() {
     return reports.take([](size_t bytes) -> void* {
         void* p = nullptr;
+        // Another thread, or the caller, may be capturing a graph, which an allocation would end.
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        const bool set = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
         const hipError_t e = hipHostMalloc(&p, bytes, hipHostMallocPortable | hipHostMallocMapped);
         if (e != hipSuccess) (void)hipGetLastError();
+        if (set) (void)hipThreadExchangeStreamCaptureMode(&mode);
         return e == hipSuccess ? p : nullptr;
     });
 }

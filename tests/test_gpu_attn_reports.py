@@ -1,8 +1,12 @@
 """Reports of bad starts and pages: the region's end of the context that launched the kernels, and of no other."""
 from __future__ import annotations
 
+import subprocess
+import sys
+
 import pytest
 
+from conftest import PKG_DIR
 from test_gpu_attn_paged import cache_case
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +61,38 @@ def test_a_graph_that_outlives_its_context_blames_no_other(dgm, torch_cuda):
     finally:
         for x in others:
             x.close()
+
+
+CAPTURE = """
+import importlib.util, os, sys
+import torch
+PKG = sys.argv[1]
+spec = importlib.util.spec_from_file_location("dgm_amd", os.path.join(PKG, "__init__.py"), submodule_search_locations=[PKG])
+dgm = importlib.util.module_from_spec(spec)
+sys.modules["dgm_amd"] = dgm
+spec.loader.exec_module(dgm)
+dgm.load_library()
+x = torch.zeros(8, device="cuda")
+x.add_(1)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+    x.add_(1)
+    g = dgm.GPU()
+    x.add_(1)
+for want in (3, 5):
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (x == want).all(), x
+g.begin()
+g.zero(x, 8)
+g.end()
+assert (x == 0).all()
+print("ok")
+"""
+
+
+def test_a_first_context_may_be_created_during_a_capture(torch_cuda):
+    """The process's first context, whose words are allocated then, leaves the capture whole."""
+    done = subprocess.run([sys.executable, "-c", CAPTURE, PKG_DIR], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and done.stdout.strip() == "ok", done.stderr
