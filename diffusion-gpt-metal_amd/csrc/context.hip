@@ -208,7 +208,7 @@ uint8_t* planes_buffer(dgm_gpu* g, size_t bytes) {
     return static_cast<uint8_t*>(g->planes);
 }
 
-// After a synchronize: records an error if such a kernel reported one.
+// After a synchronize: records an error if such a kernel reported one, and clears the reports.
 void sequence_check(dgm_gpu* g) {
     const bool starts = __atomic_exchange_n(g->seq_report + dgm_attn::kBadStarts, 0u, __ATOMIC_ACQUIRE);
     const bool pages = __atomic_exchange_n(g->seq_report + dgm_attn::kBadPages, 0u, __ATOMIC_ACQUIRE);
@@ -316,10 +316,9 @@ int dgm_end(dgm_gpu* g) {
     if (e == hipSuccess) e = hipGetLastError();
     if (e != hipSuccess)
         dgm::fail(g, DGM_ERR_HIP, "HIP error after %s: %s", g->last_kernel, hipGetErrorString(e));
-    else {
-        if (g->spin_waits) dgm::decode_wait_check(g);
-        dgm::sequence_check(g);
-    }
+    else if (g->spin_waits)
+        dgm::decode_wait_check(g);
+    dgm::sequence_check(g);   // after an error, too: what this region found is not the next one's
     return g->first_err;
 }
 

@@ -1,6 +1,7 @@
 """Reports of bad starts and pages: the region's end of the context that launched the kernels, and of no other."""
 from __future__ import annotations
 
+import ctypes
 import subprocess
 import sys
 
@@ -96,3 +97,26 @@ def test_a_first_context_may_be_created_during_a_capture(torch_cuda):
     """The process's first context, whose words are allocated then, leaves the capture whole."""
     done = subprocess.run([sys.executable, "-c", CAPTURE, PKG_DIR], capture_output=True, text=True, timeout=100)
     assert done.returncode == 0 and done.stdout.strip() == "ok", done.stderr
+
+
+def test_a_failed_region_leaves_no_report_behind(dgm, torch_cuda):
+    """A HIP error at the region's end is what it returns; the next region begins without its reports."""
+    torch = torch_cuda
+    stream = torch.cuda.Stream()
+    step = Step(dgm, torch)
+    step.spoil()
+    g = dgm.GPU(stream=stream)
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    try:
+        torch.cuda.synchronize()
+        g.begin()
+        step(g)
+        stream.synchronize()
+        assert hip.hipSetDevice(-1) != 0        # an error that waits to be asked for
+        with pytest.raises(dgm.DgmError) as e:
+            g.end()
+        assert e.value.code == dgm.DGM_ERR_HIP
+        g.begin()
+        g.end()
+    finally:
+        g.close()
