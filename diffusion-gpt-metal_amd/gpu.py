@@ -12,9 +12,10 @@ where the reference calls fatalError / exit(1).
 from __future__ import annotations
 
 import ctypes
+import sys
 from typing import Any, Optional
 
-from .abi import (DGM_MATH_BF16, DGM_MATH_FP32, AdamP, AttnCfg, BiasP, CacheCfg, DgmError, DiTCfg,
+from .abi import (DGM_MATH_BF16, DGM_MATH_FP32, DGM_TYPE_BF16, DGM_TYPE_F32, AdamP, AttnCfg, BiasP, CacheCfg, DgmError, DiTCfg,
                   DiTGrads, DiTWeights, EmbBwdP, EmbP, GemmP, PosP, QuantP, ReduceP, ScaleP,
                   UnaryP, load_library)
 
@@ -31,6 +32,46 @@ def _ptr(t: Any) -> Optional[int]:
             raise ValueError("buffers must live in device memory")
         return t.data_ptr()
     raise TypeError(f"cannot take a device address of {type(t).__name__}")
+
+
+# Classes of the device tensors that the attention calls take: one look tells both type and place. Set where
+# torch is loaded (without it there are no tensors).
+_F32: Any = ()
+_I32: Any = ()
+_ELEMENTS: dict = {}       # by DGM_TYPE_*
+_DTYPES: dict = {(): None}
+
+
+def _elements(code: int) -> Any:
+    global _F32, _I32
+    if not _ELEMENTS and "torch" in sys.modules:
+        import torch
+        _F32, _I32 = torch.cuda.FloatTensor, torch.cuda.IntTensor
+        _ELEMENTS.update({DGM_TYPE_F32: _F32, DGM_TYPE_BF16: torch.cuda.BFloat16Tensor})
+        _DTYPES.update({_F32: torch.float32, _I32: torch.int32, torch.cuda.BFloat16Tensor: torch.bfloat16})
+    return _ELEMENTS.get(code, ())      # (): a code that the library refuses
+
+
+def _typed(t: Any, kind: Any, what: str) -> Optional[int]:
+    """_ptr of a tensor of that class: the attention calls read what the device
+    holds, and one of another type would be read as something else. Raw addresses
+    are taken as they are."""
+    if isinstance(t, kind):
+        return t.data_ptr()
+    p, dtype = _ptr(t), _DTYPES[kind]
+    if dtype is not None and getattr(t, "dtype", dtype) is not dtype:
+        raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+    return p
+
+
+def _ints(t: Any, what: str) -> Optional[int]:
+    """_ptr of starts, lengths or a page table: int32, rows back to back."""
+    if isinstance(t, _I32) and t.is_contiguous():
+        return t.data_ptr()
+    p = _typed(t, _I32, what)
+    if hasattr(t, "is_contiguous") and not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return p
 
 
 def Buf(count: int, device: str = "cuda"):
@@ -241,36 +282,46 @@ class GPU:
     # -- attention over packed sequences and over a paged cache ---------------
     def attnPackedFwd(self, cfg: AttnCfg, q, k, v, starts, out, lse=None) -> None:
         """Attention of sequences back to back, starts int32 [nseq + 1] on the
-        device; lse [H, rows] for a backward."""
-        self._check(self.lib.dgm_attnPackedFwd(self.h, ctypes.byref(cfg), _ptr(q), _ptr(k), _ptr(v), _ptr(starts),
-                                               _ptr(out), _ptr(lse)))
+        device; lse float32 [H, rows] for a backward. TypeError for tensors of
+        another type than cfg.type's, here and in the calls below."""
+        el = _elements(cfg.type)
+        self._check(self.lib.dgm_attnPackedFwd(
+            self.h, ctypes.byref(cfg), _typed(q, el, "q"), _typed(k, el, "k"), _typed(v, el, "v"), _ints(starts, "starts"),
+            _typed(out, el, "out"), _typed(lse, _F32, "lse")))
 
     def attnPackedBwd_ws_bytes(self, cfg: AttnCfg) -> int:
         return int(self.lib.dgm_attnPackedBwd_ws_bytes(ctypes.byref(cfg)))
 
     def attnPackedBwd(self, cfg: AttnCfg, q, k, v, starts, out, lse, dout, dq, dk, dv, ws, ws_bytes: int) -> None:
         """The gradients of attnPackedFwd from its out and lse (overwritten)."""
-        self._check(self.lib.dgm_attnPackedBwd(self.h, ctypes.byref(cfg), _ptr(q), _ptr(k), _ptr(v), _ptr(starts),
-                                               _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv),
-                                               _ptr(ws), ws_bytes))
+        el = _elements(cfg.type)
+        self._check(self.lib.dgm_attnPackedBwd(
+            self.h, ctypes.byref(cfg), _typed(q, el, "q"), _typed(k, el, "k"), _typed(v, el, "v"), _ints(starts, "starts"),
+            _typed(out, el, "out"), _typed(lse, _F32, "lse"), _typed(dout, el, "dout"), _typed(dq, el, "dq"),
+            _typed(dk, el, "dk"), _typed(dv, el, "dv"), _ptr(ws), ws_bytes))
 
     def cacheWrite(self, cfg: CacheCfg, type: int, k, v, starts, lens, pages, kcache, vcache, rows: int, nseq: int,
                    ldk: int = 0, ldv: int = 0) -> None:
         """Rows of k and v into the pages of a cache: row r of sequence s
-        becomes position lens[s] + r - starts[s]."""
-        self._check(self.lib.dgm_cacheWrite(self.h, ctypes.byref(cfg), type, _ptr(k), _ptr(v), _ptr(starts),
-                                            _ptr(lens), _ptr(pages), _ptr(kcache), _ptr(vcache), rows, nseq, ldk, ldv))
+        becomes position lens[s] + r - starts[s]. starts, lens, pages int32."""
+        el, held = _elements(type), _elements(cfg.type)
+        self._check(self.lib.dgm_cacheWrite(
+            self.h, ctypes.byref(cfg), type, _typed(k, el, "k"), _typed(v, el, "v"), _ints(starts, "starts"),
+            _ints(lens, "lens"), _ints(pages, "pages"), _typed(kcache, held, "kcache"), _typed(vcache, held, "vcache"),
+            rows, nseq, ldk, ldv))
 
     def attnPagedDecode_ws_bytes(self, cfg: CacheCfg, nseq: int, H: int) -> int:
         return int(self.lib.dgm_attnPagedDecode_ws_bytes(ctypes.byref(cfg), nseq, H))
 
     def attnPagedDecode(self, cfg: CacheCfg, type: int, q, kcache, vcache, pages, lens, out, ws, ws_bytes: int,
                         nseq: int, H: int, ldq: int = 0, ldo: int = 0, scale: Optional[float] = None) -> None:
-        """Attention of one new token per sequence over lens[s] cached positions;
-        scale defaults to 1 / sqrt(D)."""
-        self._check(self.lib.dgm_attnPagedDecode(self.h, ctypes.byref(cfg), type, _ptr(q), _ptr(kcache), _ptr(vcache),
-                                                 _ptr(pages), _ptr(lens), _ptr(out), _ptr(ws), ws_bytes, nseq, H, ldq,
-                                                 ldo, cfg.D ** -0.5 if scale is None else scale))
+        """Attention of one new token per sequence over lens[s] cached positions
+        (lens, pages int32); scale defaults to 1 / sqrt(D)."""
+        el, held = _elements(type), _elements(cfg.type)
+        self._check(self.lib.dgm_attnPagedDecode(
+            self.h, ctypes.byref(cfg), type, _typed(q, el, "q"), _typed(kcache, held, "kcache"),
+            _typed(vcache, held, "vcache"), _ints(pages, "pages"), _ints(lens, "lens"), _typed(out, el, "out"), _ptr(ws),
+            ws_bytes, nseq, H, ldq, ldo, cfg.D ** -0.5 if scale is None else scale))
 
     # -- training step (src/GPU.swift:200-210, 274-277, 324-350, 420-429) -----
     def adam(self, w, g, m, v, n: int, lr: float, b1: float, b2: float, eps: float, wd: float,
