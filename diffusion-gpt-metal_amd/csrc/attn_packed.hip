@@ -15,9 +15,10 @@
 //    one product, with P rounded to bf16 (half a step is 2^-9 of a weight's binade, and
 //    the roundings of a row's weights are independent, so a row's error stays about that of
 //    rounding its output once). fp32 tensors are split into three bf16 pieces of 8
-//    bits, exactly, and take the six products of pieces that reach 2^-24 of the
-//    largest: 192 cycles for 32x32x16, which v_mfma_f32_32x32x2_f32 does in 512.
-//    Scores, statistics and accumulators are fp32.
+//    bits, exactly, and take the six largest of their nine products: 192 cycles for
+//    32x32x16, which v_mfma_f32_32x32x2_f32 does in 512. The pieces are cut and not
+//    rounded, so that none overflows; the three products left out are then of the product's
+//    sign, up to 2^-21 of it and 2^-24.5 on average. Scores, statistics and accumulators are fp32.
 //  * Tiles of 64 (32) keys stay row-major in LDS: the A operand of the second product
 //    is read transposed (ds_read_b64_tr_b16), and 16-byte chunks are XOR-swizzled so
 //    that both reads are free of bank conflicts. bf16 tiles go from memory straight into
@@ -36,16 +37,18 @@
 //    first, and the sums that they belong to spoilt afterwards.
 //
 // Long sequences are bound by the matrix unit: a prompt of 8192 (32 heads on 8 of 128,
-// bf16) takes 524 us, 1,050 TFLOP/s, where a library product reaches 1,158; four of 640 to 2048 in
-// fp32 (16 heads on 4 of 64) 106 us, 153 TFLOP/s, where a library product reaches 153. Short ones
+// bf16) takes 530 us, 1,040 TFLOP/s, where a library product reaches 1,158; four of 640 to 2048 in
+// fp32 (16 heads on 4 of 64) 108 us, 151 TFLOP/s, where a library product reaches 153; fp32 heads of 128
+// run one wave to a SIMD (256 us, 127 TFLOP/s), and of 256 spill (63 to 70). Short ones
 // are a chain of waits: starts, tiles, exponentials, rows out (16 of 64: 6 us).
 //
 // The backward recomputes P from lse. One kernel owns 32 queries per wave and
 // accumulates dq; another owns 32 keys per wave and accumulates dk and dv over all
 // query heads of the key head's group, so no gradient is added to by two
-// workgroups: no atomics, the same bits every time. Four of 2048 (16 heads on 8 of 128, bf16): dq 156 us,
-// dk and dv 212; the matrix unit is busy in half
-// of dq's cycles and a third of the other's, whose pairs of waves wait for one another.
+// workgroups: no atomics, the same bits every time. Four of 2048 (16 heads on 8 of 128, bf16), back to back: forward 88 us, dq
+// 151, dk and dv 186; the matrix unit is busy in half of dq's cycles and in 42% of the other's, whose waves wait for one another
+// twice a tile. dq keeps 56 B a lane in scratch there (fp32 heads of 64 in pairs of waves 160, of 128 in narrow blocks 188): addresses
+// of copies and query pieces, and a reload waits for every copy asked for before it.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -60,6 +63,8 @@ using namespace dgm_attn;
 // An operand in bf16 pieces: one, or the three of an fp32 value.
 template <typename T>
 constexpr int kPieces = sizeof(T) == 2 ? 1 : 3;
+
+constexpr int64_t kMaxStride = int64_t(1) << 23;   // elements from row to row: see Feed::start
 
 // ---- tiles in LDS ----------------------------------------------------------------
 
@@ -125,6 +130,8 @@ struct Feed {
                 uint64_t(uniform(uint32_t(at >> 32))) << 32 | uniform(uint32_t(at)));
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+            static_assert(uint64_t(STEP - 1) * kMaxStride * sizeof(T) + L::RB <= UINT32_MAX,
+                          "a thread's first row and slot are a 32-bit offset from the tile's start");
             const auto whole = [&]() __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -247,7 +254,7 @@ struct Frags {
     }
 };
 
-// acc += A B over their pieces: for fp32 the six products that reach 2^-24 of the largest. kTurned: in the
+// acc += A B over their pieces: for fp32 the six largest products. kTurned: in the
 // order that the product with A and B exchanged takes, for the same bits as it.
 template <bool kTurned = false, int PA, int PB>
 __device__ __forceinline__ void mfma_pieces(f32x16& acc, const bf16x8 (&a)[PA], const bf16x8 (&b)[PB]) {
@@ -1235,8 +1242,6 @@ __global__ void __launch_bounds__(256) attn_packed_sum_kernel(BwdArgs a) {
 
 // ---- host ----------------------------------------------------------------------
 
-constexpr int64_t kMaxStride = int64_t(1) << 23;   // a tile's 64 rows within the copies' 32-bit offsets
-
 // Strides of 0 mean rows back to back.
 struct Strides {
     int64_t q, k, v, o;
@@ -1294,7 +1299,7 @@ int slots_of(dgm_gpu* g, const char* name, const dgm_attn_cfg* c, int per, int h
 //    not in its backward, short of registers (four of 1024: 370, 376).
 //  * Sequences of one tile have nothing to share (16 of 64: 6.6, 7.5); lengths differ, and the longest
 //    sets the time, so that an average of two is enough (18 of 1 to 745, bf16 of 80, forward and
-//    backward 98 -> 88; nine of 100, 8 heads of 128: bf16 63, 66, fp32 135 -> 128).
+//    backward 98 -> 88; the call's rows by its sequences, those of none among them; nine of 100, 8 heads of 128: bf16 63, 66, fp32 135 -> 128).
 template <typename T>
 Kind kind_of(const dgm_attn_cfg* c, bool forward) {
     const int64_t average = c->rows / c->nseq;
