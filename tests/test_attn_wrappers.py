@@ -92,7 +92,7 @@ def test_tables_are_contiguous(g, dgm, name):
 
 @pytest.mark.parametrize("name", NAMES)
 def test_addresses_and_absent_buffers_pass(g, dgm, name):
-    """Raw addresses carry no type; what is absent is the library's to judge; so is an unknown type code."""
+    """Raw addresses carry no type; the library refuses what is absent, and an unknown type code."""
     call, types = calls(dgm, F32, F32)[name]
     call(g, **{n: 4096 for n in types})
     call(g, **{n: None for n in types})
