@@ -10,10 +10,10 @@ from .abi import (DGM_ERR_ARG, DGM_ERR_BITS, DGM_ERR_HIP, DGM_ERR_NOT_BEGUN,
                   DGM_MATH_FP32, DGM_NOALLOC_SCRATCH_BYTES, DGM_OK, DGM_TYPE_BF16, DGM_TYPE_F32, HEADER, LIB_PATH, PROTOTYPES,
                   DIT_LINEARS, DIT_NORMS, DgmError, DiTCfg, DiTLinear,
                   DiTWeights, AttnCfg, CacheCfg, GemmP, QuantP, AdamP, EmbP, EmbBwdP, PosP, BiasP,
-                  ReduceP, ScaleP, UnaryP, DiTGrads, load_library)
-from .gpu import GPU, Buf, RawBuf
+                  ReduceP, ScaleP, UnaryP, DiTGrads, NormCfg, LossCfg, RowsCfg, AdamTensor, AdamPlan, load_library)
+from .gpu import GPU, Buf, RawBuf, adam_tensor
 from .dit import DiTBlock, DiTConfig, rope_tables
-from .train import Param, bias_corrections, grad_norm, optimizer_step, zero_grads
+from .train import AdamMany, Param, bias_corrections, grad_norm, optimizer_step, zero_grads
 from .ckpt import load_dit_block, load_gpt, read_tdit, read_tgmt, save_tdit, save_tgmt
 
 __all__ = [
@@ -25,4 +25,5 @@ __all__ = [
     "PosP", "BiasP", "ReduceP", "ScaleP", "UnaryP", "Param", "bias_corrections", "grad_norm",
     "optimizer_step", "zero_grads", "DiTGrads", "load_dit_block", "load_gpt", "read_tdit", "read_tgmt",
     "save_tdit", "save_tgmt", "AttnCfg", "CacheCfg", "DGM_TYPE_F32", "DGM_TYPE_BF16",
+    "NormCfg", "LossCfg", "RowsCfg", "AdamTensor", "AdamPlan", "adam_tensor", "AdamMany",
 ]

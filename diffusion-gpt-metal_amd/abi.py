@@ -84,6 +84,38 @@ class CacheCfg(ctypes.Structure):
 assert ctypes.sizeof(AttnCfg) == 72 and ctypes.sizeof(CacheCfg) == 32
 
 
+class NormCfg(ctypes.Structure):
+    """dgm_norm_cfg: layer norm of rows [rows, cols]."""
+    _fields_ = [("type", ctypes.c_int32), ("eps", ctypes.c_float), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
+
+
+class LossCfg(ctypes.Structure):
+    """dgm_loss_cfg: cross-entropy of logits [rows, V] (row stride 0: V)."""
+    _fields_ = [("type", ctypes.c_int32), ("scale", ctypes.c_float)] + [(n, ctypes.c_int64) for n in ("rows", "V", "ld")]
+
+
+class RowsCfg(ctypes.Structure):
+    """dgm_rows_cfg: embeddings [rows, C] of a table [V, C]."""
+    _fields_ = ([("type", ctypes.c_int32), ("tableType", ctypes.c_int32), ("scale", ctypes.c_float), ("pad", ctypes.c_int32)]
+                + [(n, ctypes.c_int64) for n in ("rows", "C", "V")])
+
+
+class AdamTensor(ctypes.Structure):
+    """dgm_adam_tensor: one parameter of dgm_adamMany (see adam_tensor in gpu.py)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("w", "grad", "m", "v", "mscale", "vscale", "q", "scale")]
+                + [("n", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("decay", "bits", "qGroup", "pad")])
+
+
+class AdamPlan(ctypes.Structure):
+    """dgm_adam_plan: tensors laid out for dgm_adamMany."""
+    _fields_ = ([("table", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("tensors", "chunks", "elements")]
+                + [("stateBits", ctypes.c_int32), ("pad", ctypes.c_int32)])
+
+
+assert ctypes.sizeof(NormCfg) == 24 and ctypes.sizeof(LossCfg) == 32 and ctypes.sizeof(RowsCfg) == 40
+assert ctypes.sizeof(AdamTensor) == 88 and ctypes.sizeof(AdamPlan) == 40
+
+
 class TgmtHeader(ctypes.Structure):
     """dgm_tgmt_header: GPT.save's header fields (src/GPT.swift:265-281)."""
     _fields_ = [(n, ctypes.c_uint32) for n in ("version", "bits", "vocab", "block", "layers", "heads", "embd",
@@ -227,6 +259,18 @@ PROTOTYPES = {
     "dgm_cacheWrite": (_I, [_P, ctypes.POINTER(CacheCfg), _I64] + [_P] * 7 + [_I64] * 4),
     "dgm_attnPagedDecode_ws_bytes": (_I64, [ctypes.POINTER(CacheCfg), _I64, _I64]),
     "dgm_attnPagedDecode": (_I, [_P, ctypes.POINTER(CacheCfg), _I64] + [_P] * 7 + [_I64] * 5 + [_F]),
+    "dgm_layerNormFwd": (_I, [_P, ctypes.POINTER(NormCfg)] + [_P] * 8),
+    "dgm_layerNormBwd_ws_bytes": (_I64, [ctypes.POINTER(NormCfg)]),
+    "dgm_layerNormBwd": (_I, [_P, ctypes.POINTER(NormCfg)] + [_P] * 10 + [_I64]),
+    "dgm_crossEntropy": (_I, [_P, ctypes.POINTER(LossCfg)] + [_P] * 6),
+    "dgm_embedRows": (_I, [_P, ctypes.POINTER(RowsCfg), _P, _P, _P]),
+    "dgm_embedRowsBwd_ws_bytes": (_I64, [ctypes.POINTER(RowsCfg)]),
+    "dgm_embedRowsBwd": (_I, [_P, ctypes.POINTER(RowsCfg), _P, _P, _P, _I, _P, _I64]),
+    "dgm_adamMany_plan_bytes": (_I64, [ctypes.POINTER(AdamTensor), _I64, _I64]),
+    "dgm_adamMany_plan": (_I, [_P, ctypes.POINTER(AdamTensor), _I64, _I64, _P, _I64, ctypes.POINTER(AdamPlan)]),
+    "dgm_adamMany_norm": (_I, [_P, ctypes.POINTER(AdamPlan), _F, _P]),
+    "dgm_adamMany": (_I, [_P, ctypes.POINTER(AdamPlan), _P] + [_F] * 7),
+    "dgm_adamMany_states": (_I, [_P, ctypes.POINTER(AdamPlan), _P, _P]),
     "dgm_adamw": (_I, [_P, _P, _P, _P, _P, ctypes.POINTER(AdamP)]),
     "dgm_adam": (_I, [_P, _P, _P, _P, _P, _I64] + [_F] * 7),
     "dgm_adam_quantize": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64] + [_F] * 7),

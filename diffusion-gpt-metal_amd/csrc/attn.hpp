@@ -17,7 +17,7 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 // Words of the context's report (dgm_gpu::seq_report), which dgm_end reads.
-constexpr int kBadStarts = 0, kBadPages = 1;
+constexpr int kBadStarts = 0, kBadPages = 1, kBadTokens = 2;
 
 __device__ __forceinline__ void report(uint32_t* words, int which) {
     __hip_atomic_store(words + which, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);

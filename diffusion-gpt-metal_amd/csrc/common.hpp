@@ -62,8 +62,8 @@ struct dgm_gpu {
     bool lending = false;
     uint8_t* lent = nullptr;
     size_t lent_bytes = 0;
-    // Two words of host memory that the attention and cache kernels set where they find
-    // bad sequence starts and pages; read and cleared by dgm_end.
+    // Words of host memory that kernels set where they find bad sequence starts, pages,
+    // tokens or targets (dgm::ReportWords); read and cleared by dgm_end.
     uint32_t* seq_report = nullptr;
 };
 

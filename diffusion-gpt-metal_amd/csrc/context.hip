@@ -16,8 +16,8 @@ namespace {
 // only the per-device address from hipGetSymbolAddress, never this name.
 __device__ __align__(256) uint8_t scratch[dgm::kScratchBytes];
 
-// What the attention and cache kernels find wrong in sequence starts, lengths and page
-// tables, which only the device reads; in host memory, so that dgm_end looks at it without a copy.
+// What kernels find wrong in sequence starts, lengths, page tables, tokens and
+// targets, which only the device reads; in host memory, so that dgm_end looks at it without a copy.
 dgm::ReportWords reports;
 
 uint32_t* take_report() {
@@ -212,11 +212,14 @@ uint8_t* planes_buffer(dgm_gpu* g, size_t bytes) {
 void sequence_check(dgm_gpu* g) {
     const bool starts = __atomic_exchange_n(g->seq_report + dgm_attn::kBadStarts, 0u, __ATOMIC_ACQUIRE);
     const bool pages = __atomic_exchange_n(g->seq_report + dgm_attn::kBadPages, 0u, __ATOMIC_ACQUIRE);
+    const bool tokens = __atomic_exchange_n(g->seq_report + dgm_attn::kBadTokens, 0u, __ATOMIC_ACQUIRE);
     if (starts)
         fail(g, DGM_ERR_SHAPE, "sequence starts are out of order or beyond the rows: results are not valid");
     else if (pages)
         fail(g, DGM_ERR_SHAPE, "a sequence is longer than its page table, or names a page that the cache does not have: "
                                "those rows were left out");
+    else if (tokens)
+        fail(g, DGM_ERR_SHAPE, "a token or target is beyond the vocabulary: its row was left out");
 }
 
 int ws_error(dgm_gpu* g) { return g->first_err != DGM_OK ? g->first_err : DGM_ERR_HIP; }

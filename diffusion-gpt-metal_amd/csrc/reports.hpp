@@ -6,12 +6,12 @@
 
 namespace dgm {
 
-// Two words a context, from blocks of host memory that the device writes. None is handed out
+// Four words a context, from blocks of host memory that the device writes. None is handed out
 // twice, nor freed: a captured graph may outlive the context that it reports to, and then
-// writes where nobody reads. That is 8 bytes for each context of a process.
+// writes where nobody reads. That is 16 bytes for each context of a process.
 class ReportWords {
 public:
-    static constexpr int kWords = 2, kContexts = 512;   // of a context; contexts of a block
+    static constexpr int kWords = 4, kContexts = 512;   // of a context; contexts of a block
     // alloc(bytes): such memory, or nullptr, which is then the result.
     template <typename Alloc>
     uint32_t* take(const Alloc& alloc) {

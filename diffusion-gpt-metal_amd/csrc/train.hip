@@ -28,6 +28,7 @@
 //   per-lane sums, 16 or 32 rows per batch with all loads issued first. dx is
 //   read once in total and each sum keeps the reference's order, so results
 //   are bitwise the reference's.
+#include "adam_math.hpp"
 #include "common.hpp"
 #include "quant_math.hpp"
 
@@ -37,19 +38,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
-struct AdamArgs {
-    float lr, b1, b2, eps, wd, invBC1, invBC2;
-};
-
-// One element of adamw (metal/kernels.metal:795-801), literally.
-__device__ __forceinline__ void adam_elem(float& w, float g, float& m, float& v, const AdamArgs& a) {
-    const float mi = a.b1 * m + (1.0f - a.b1) * g;
-    const float vi = a.b2 * v + (1.0f - a.b2) * g * g;
-    m = mi;
-    v = vi;
-    const float upd = (mi * a.invBC1) / (sqrtf(vi * a.invBC2) + a.eps);
-    w -= a.lr * (upd + a.wd * w);
-}
+using dgm::AdamArgs;
+using dgm::adam_elem;
 
 // 8 elements per lane; n8 = n / 8 lanes do vector work, the tail (n % 8) is
 // done element-wise by the first lanes of the last block.

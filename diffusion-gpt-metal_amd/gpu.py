@@ -13,11 +13,11 @@ from __future__ import annotations
 
 import ctypes
 import sys
-from typing import Any, Optional
+from typing import Any, List, Optional
 
-from .abi import (DGM_MATH_BF16, DGM_MATH_FP32, DGM_TYPE_BF16, DGM_TYPE_F32, AdamP, AttnCfg, BiasP, CacheCfg, DgmError, DiTCfg,
-                  DiTGrads, DiTWeights, EmbBwdP, EmbP, GemmP, PosP, QuantP, ReduceP, ScaleP,
-                  UnaryP, load_library)
+from .abi import (DGM_MATH_BF16, DGM_MATH_FP32, DGM_TYPE_BF16, DGM_TYPE_F32, AdamP, AdamPlan, AdamTensor, AttnCfg, BiasP,
+                  CacheCfg, DgmError, DiTCfg, DiTGrads, DiTWeights, EmbBwdP, EmbP, GemmP, LossCfg, NormCfg, PosP, QuantP,
+                  ReduceP, RowsCfg, ScaleP, UnaryP, load_library)
 
 
 def _ptr(t: Any) -> Optional[int]:
@@ -72,6 +72,68 @@ def _ints(t: Any, what: str) -> Optional[int]:
     if hasattr(t, "is_contiguous") and not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
     return p
+
+
+def _rows(t: Any, dtype: str, count: int, what: str) -> Optional[int]:
+    """_ptr of at least `count` elements of the torch dtype of that name, back to back. Raw
+    addresses are taken as they are; None is an absent buffer."""
+    p = _ptr(t)
+    if hasattr(t, "dtype"):
+        if str(t.dtype) != dtype:
+            raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous")
+        if t.numel() < count:
+            raise ValueError(f"{what} holds {t.numel()} elements, {count} needed")
+    return p
+
+
+_TORCH_F32, _TORCH_I32 = "torch.float32", "torch.int32"
+_TORCH_TYPES = {DGM_TYPE_F32: _TORCH_F32, DGM_TYPE_BF16: "torch.bfloat16"}
+
+
+def _dtype(code: int) -> str:
+    return _TORCH_TYPES.get(code, _TORCH_F32)      # a code that the library refuses
+
+
+def _bytes(ws: Any, nbytes: int) -> Optional[int]:
+    """_ptr of a workspace that is said to have nbytes."""
+    p = _ptr(ws)
+    if hasattr(ws, "element_size") and ws.numel() * ws.element_size() < nbytes:
+        raise ValueError(f"the workspace holds {ws.numel() * ws.element_size()} bytes, not {nbytes}")
+    return p
+
+
+class _AdamTensor(AdamTensor):
+    """With its buffers, which a plan keeps."""
+    held: tuple = ()
+
+
+def adam_tensor(w, grad, m, v, mscale=None, vscale=None, *, decay: bool, q=None, scale=None, bits: int = 0,
+                qGroup: int = 0) -> AdamTensor:
+    """One parameter of GPU.adamMany_plan, from device tensors: fp32 w and grad; m and v fp32, or int8 and uint8 codes
+    with mscale and vscale, one float for each 256 elements; with bits, the codes and scales that
+    its linear reads."""
+    n = w.numel()
+    blocks = -(-n // 256)
+    codes = mscale is not None
+    first, second = ("torch.int8", "torch.uint8") if codes else (_TORCH_F32, _TORCH_F32)
+    t = _AdamTensor(
+        w=_rows(w, _TORCH_F32, n, "w"), grad=_rows(grad, _TORCH_F32, n, "grad"), m=_rows(m, first, n, "m"),
+        v=_rows(v, second, n, "v"), mscale=_rows(mscale, _TORCH_F32, blocks, "mscale"),
+        vscale=_rows(vscale, _TORCH_F32, blocks, "vscale"), n=n, decay=int(bool(decay)), bits=bits, qGroup=qGroup)
+    if bits and qGroup > 0:
+        t.scale = _rows(scale, _TORCH_F32, n // qGroup, "scale")
+        if hasattr(q, "element_size") and q.numel() * q.element_size() * 8 < n * bits:
+            raise ValueError(f"q holds {q.numel() * q.element_size()} bytes, {n * bits // 8} needed")
+        t.q = _ptr(q)
+    t.held = (w, grad, m, v, mscale, vscale, q, scale)
+    return t
+
+
+class _AdamPlan(AdamPlan):
+    """With its table and the tensors that it names."""
+    held: tuple = ()
 
 
 def Buf(count: int, device: str = "cuda"):
@@ -323,6 +385,80 @@ class GPU:
             _typed(vcache, held, "vcache"), _ints(pages, "pages"), _ints(lens, "lens"), _typed(out, el, "out"), _ptr(ws),
             ws_bytes, nseq, H, ldq, ldo, cfg.D ** -0.5 if scale is None else scale))
 
+    # -- a training step around its linears ------------------------------------
+    # Tensors of another dtype than the call reads are a TypeError, those that are too small or not
+    # contiguous a ValueError; raw addresses pass.
+    def layerNormFwd(self, cfg: NormCfg, x, res, weight, bias, sum, y, mean=None, rstd=None) -> None:
+        """y = layer norm of sum = x + res (both None: of x)."""
+        el, n = _dtype(cfg.type), cfg.rows * cfg.cols
+        self._check(self.lib.dgm_layerNormFwd(
+            self.h, ctypes.byref(cfg), _rows(x, el, n, "x"), _rows(res, el, n, "res"), _rows(weight, _TORCH_F32, cfg.cols, "weight"),
+            _rows(bias, _TORCH_F32, cfg.cols, "bias"), _rows(sum, el, n, "sum"), _rows(y, el, n, "y"),
+            _rows(mean, _TORCH_F32, cfg.rows, "mean"), _rows(rstd, _TORCH_F32, cfg.rows, "rstd")))
+
+    def layerNormBwd_ws_bytes(self, cfg: NormCfg) -> int:
+        return int(self.lib.dgm_layerNormBwd_ws_bytes(ctypes.byref(cfg)))
+
+    def layerNormBwd(self, cfg: NormCfg, x, mean, rstd, weight, dy, dsum, dx, dweight, dbias, ws, ws_bytes: int) -> None:
+        """dx = dsum + the gradient through the norm; dweight and dbias are added to."""
+        el, n = _dtype(cfg.type), cfg.rows * cfg.cols
+        self._check(self.lib.dgm_layerNormBwd(
+            self.h, ctypes.byref(cfg), _rows(x, el, n, "x"), _rows(mean, _TORCH_F32, cfg.rows, "mean"),
+            _rows(rstd, _TORCH_F32, cfg.rows, "rstd"), _rows(weight, _TORCH_F32, cfg.cols, "weight"), _rows(dy, el, n, "dy"),
+            _rows(dsum, el, n, "dsum"), _rows(dx, el, n, "dx"), _rows(dweight, _TORCH_F32, cfg.cols, "dweight"),
+            _rows(dbias, _TORCH_F32, cfg.cols, "dbias"), _bytes(ws, ws_bytes), ws_bytes))
+
+    def crossEntropy(self, cfg: LossCfg, logits, targets, loss, rowScale=None, lse=None, dlogits=None) -> None:
+        """Cross-entropy of logits [rows, V] with int32 targets (negative: the row does not count), and its gradient."""
+        el, rows = _dtype(cfg.type), cfg.rows
+        n = (rows - 1) * (cfg.ld or cfg.V) + cfg.V if rows > 0 else 0
+        self._check(self.lib.dgm_crossEntropy(
+            self.h, ctypes.byref(cfg), _rows(logits, el, n, "logits"), _rows(targets, _TORCH_I32, rows, "targets"),
+            _rows(rowScale, _TORCH_F32, rows, "rowScale"), _rows(loss, _TORCH_F32, rows, "loss"),
+            _rows(lse, _TORCH_F32, rows, "lse"), _rows(dlogits, el, n, "dlogits")))
+
+    def embedRows(self, cfg: RowsCfg, tokens, table, y) -> None:
+        """y[r] = scale * table[tokens[r]]; tokens int32, -1 for none."""
+        self._check(self.lib.dgm_embedRows(
+            self.h, ctypes.byref(cfg), _rows(tokens, _TORCH_I32, cfg.rows, "tokens"),
+            _rows(table, _dtype(cfg.tableType), cfg.V * cfg.C, "table"), _rows(y, _dtype(cfg.type), cfg.rows * cfg.C, "y")))
+
+    def embedRowsBwd_ws_bytes(self, cfg: RowsCfg) -> int:
+        return int(self.lib.dgm_embedRowsBwd_ws_bytes(ctypes.byref(cfg)))
+
+    def embedRowsBwd(self, cfg: RowsCfg, tokens, dy, dtable, ws, ws_bytes: int, accumulate: bool = False) -> None:
+        """The gradient of embedRows in the fp32 dtable [V, C], overwritten or added to."""
+        self._check(self.lib.dgm_embedRowsBwd(
+            self.h, ctypes.byref(cfg), _rows(tokens, _TORCH_I32, cfg.rows, "tokens"),
+            _rows(dy, _dtype(cfg.type), cfg.rows * cfg.C, "dy"), _rows(dtable, _TORCH_F32, cfg.V * cfg.C, "dtable"),
+            1 if accumulate else 0, _bytes(ws, ws_bytes), ws_bytes))
+
+    def adamMany_plan(self, tensors: List[AdamTensor], stateBits: int = 32) -> AdamPlan:
+        """Lays tensors (of adam_tensor) out for adamMany, and keeps them. Waits for the stream; not during a capture."""
+        import torch
+        listed = (AdamTensor * len(tensors))(*tensors)
+        size = int(self.lib.dgm_adamMany_plan_bytes(listed, len(tensors), stateBits))
+        plan = _AdamPlan()
+        table = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda") if size >= 0 else None
+        self._check(self.lib.dgm_adamMany_plan(self.h, listed, len(tensors), stateBits, _ptr(table), size, ctypes.byref(plan)))
+        plan.held = (table, tuple(tensors))
+        return plan
+
+    def adamMany_norm(self, plan: AdamPlan, clip: float, out) -> None:
+        """out[0] = the norm of all gradients, out[1] = the factor that clips it."""
+        self._check(self.lib.dgm_adamMany_norm(self.h, ctypes.byref(plan), clip, _rows(out, _TORCH_F32, 2, "out")))
+
+    def adamMany(self, plan: AdamPlan, lr: float, b1: float, b2: float, eps: float, wd: float, invBC1: float,
+                 invBC2: float, factor=None) -> None:
+        """adam (with codes: adamQuantize) of every tensor of the plan; the gradients times factor[0]."""
+        self._check(self.lib.dgm_adamMany(self.h, ctypes.byref(plan), _rows(factor, _TORCH_F32, 1, "factor"), lr, b1, b2, eps,
+                                          wd, invBC1, invBC2))
+
+    def adamMany_states(self, plan: AdamPlan, m, v) -> None:
+        """The values of 8-bit moments, tensor behind tensor, each from the next multiple of 256."""
+        self._check(self.lib.dgm_adamMany_states(self.h, ctypes.byref(plan), _rows(m, _TORCH_F32, plan.elements, "m"),
+                                                 _rows(v, _TORCH_F32, plan.elements, "v")))
+
     # -- training step (src/GPU.swift:200-210, 274-277, 324-350, 420-429) -----
     def adam(self, w, g, m, v, n: int, lr: float, b1: float, b2: float, eps: float, wd: float,
              invBC1: float, invBC2: float) -> None:
@@ -424,4 +560,4 @@ class GPU:
         self._check(self.lib.dgm_bias_grad(self.h, _ptr(dY), _ptr(db), ctypes.byref(p)))
 
 
-__all__ = ["GPU", "Buf", "RawBuf", "DGM_MATH_FP32", "DGM_MATH_BF16"]
+__all__ = ["GPU", "Buf", "RawBuf", "adam_tensor", "DGM_MATH_FP32", "DGM_MATH_BF16"]

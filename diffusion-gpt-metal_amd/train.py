@@ -14,7 +14,7 @@ from __future__ import annotations
 import math
 from typing import Iterable, List, Optional
 
-from .gpu import GPU, Buf, RawBuf
+from .gpu import GPU, Buf, RawBuf, adam_tensor
 
 
 class Param:
@@ -99,4 +99,65 @@ def optimizer_step(gpu: GPU, params: List[Param], lr: float, wd: float, clip: fl
     return norm
 
 
-__all__ = ["Param", "bias_corrections", "zero_grads", "grad_norm", "optimizer_step"]
+class AdamMany:
+    """AdamW over all parameters in one launch (GPU.adamMany), the re-quantization of the
+    quantized ones in it, the norm of all gradients and the clip's factor on the device: a
+    step never waits for the host. No counterpart in the reference, which dispatches
+    once a parameter; with 32-bit moments and without a clip the buffers end up the same bits as optimizer_step's.
+
+    state_bits 8 keeps the moments as codes in self.codes, about a quarter of the memory; they start at
+    zero, and the parameters' own m and v are given up (None). Make it again if a
+    parameter's buffers are replaced."""
+
+    def __init__(self, gpu: GPU, params: Iterable[Param], state_bits: int = 32):
+        import torch
+        self.gpu, self.params, self.state_bits = gpu, list(params), state_bits
+        self.codes, self.rest, tensors = {}, [], []
+        for p in self.params:
+            n, moments = p.count, (p.m, p.v)
+            if state_bits == 8:
+                def buf(count, dtype):
+                    return torch.zeros(max(count, 1), dtype=dtype, device=p.w.device)
+                moments = (buf(n, torch.int8), buf(n, torch.uint8), *(buf(-(-n // 256), torch.float32) for _ in range(2)))
+                self.codes[p.name] = moments
+                moments = tuple(t[:n] for t in moments[:2]) + moments[2:]
+                p.m = p.v = None
+            codes = {}
+            if p.quantized and p.bits != 32:
+                G = p.qGroup
+                if p.cols % G == 0 and 8 <= G <= 512 and G & (G - 1) == 0:
+                    codes = {"q": p.q, "scale": p.scale, "bits": p.bits, "qGroup": G}
+                else:
+                    self.rest.append(p)
+            tensors.append(adam_tensor(p.w[:n], p.g[:n], moments[0][:n], moments[1][:n], *moments[2:], decay=p.decay, **codes))
+        self.plan = gpu.adamMany_plan(tensors, state_bits)
+        self.norm = Buf(2)
+
+    def step(self, lr: float, wd: float, clip: float, step_index: int, b1: float = 0.9, b2: float = 0.95,
+             eps: float = 1e-8):
+        """One update (inside an open begin()/end() region). With clip > 0 returns the device
+        tensor [norm, factor] that the next step overwrites; the gradients are scaled on the way, not in memory."""
+        inv1, inv2 = bias_corrections(b1, b2, step_index)
+        factor = None
+        if clip > 0:
+            self.gpu.adamMany_norm(self.plan, clip, self.norm)
+            factor = self.norm[1:]
+        self.gpu.adamMany(self.plan, lr, b1, b2, eps, wd, inv1, inv2, factor=factor)
+        for p in self.rest:
+            self.gpu.quantize(p.w, p.q, p.scale, p.rows, p.cols, p.bits, p.qGroup)
+        return self.norm if clip > 0 else None
+
+    def moments(self):
+        """{name: (m, v)} as fp32 tensors, for a checkpoint (inside an open region; with 8 bits what the codes stand for)."""
+        if self.state_bits == 32:
+            return {p.name: (p.m, p.v) for p in self.params}
+        m, v = Buf(self.plan.elements), Buf(self.plan.elements)
+        self.gpu.adamMany_states(self.plan, m, v)
+        out, at = {}, 0
+        for p in self.params:
+            out[p.name] = (m[at:at + p.count], v[at:at + p.count])
+            at += -(-p.count // 256) * 256
+        return out
+
+
+__all__ = ["Param", "AdamMany", "bias_corrections", "zero_grads", "grad_norm", "optimizer_step"]
