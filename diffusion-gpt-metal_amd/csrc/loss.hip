@@ -48,22 +48,30 @@ __device__ __forceinline__ Target target_of(const LossArgs& a, int64_t row, bool
     return r;
 }
 
-template <int V, typename T>
-__device__ __forceinline__ void store_slope(T* row, int c, int cols, const float (&z)[V], float m, float inv, const Target& t) {
-    float d[V];
-    const float k = t.k * inv;
+// Piece c of a row's gradient from its e^(z - m): k / sum times those, `hot` at the target.
+template <typename T, int V>
+__device__ __forceinline__ void store_slopes(T* dz, int c, float (&e)[V], float k, const Target& t, float hot) {
+    piece_t<T, V> d;
 #pragma unroll
-    for (int j = 0; j < V; ++j) d[j] = exp_of(z[j], m) * k;
-    if (t.at >= c && t.at < c + V) {
+    for (int j = 0; j < V; ++j) e[j] *= k;
+    if (uint32_t(t.at - c * V) < uint32_t(V)) {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (c + j == t.at) d[j] = (exp_of(z[j], m) * inv - 1.0f) * t.k;
+        for (int j = 0; j < V; ++j) e[j] = c * V + j == t.at ? hot : e[j];
     }
-    if (t.at < 0) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = 0.0f;
-    }
-    store_piece<V>(row, c, cols, d);
+    for (int j = 0; j < V; ++j) d[j] = T(e[j]);
+    reinterpret_cast<piece_t<T, V>*>(dz)[c] = d;
+}
+
+// The gradient of a row that counts for nothing, whatever it holds.
+template <typename T, int V>
+__device__ __forceinline__ void store_zeros(T* dz, int cols, int lane, int lanes) {
+    const int whole = cols / V;
+    piece_t<T, V> d;
+#pragma unroll
+    for (int j = 0; j < V; ++j) d[j] = T(0.0f);
+    for (int c = lane; c < whole; c += lanes) reinterpret_cast<piece_t<T, V>*>(dz)[c] = d;
+    if (whole * V + lane < cols) dz[whole * V + lane] = T(0.0f);
 }
 
 template <typename T>
@@ -73,38 +81,65 @@ __device__ __forceinline__ void store_row(const LossArgs& a, int64_t row, const 
     if (a.loss) a.loss[row] = t.at < 0 ? 0.0f : lse - t.z;
 }
 
-// TEAM lanes hold a row, CH pieces of 16 bytes each: one read, one write.
-template <typename T, int TEAM, int CH>
-__global__ __launch_bounds__(threads_of(TEAM)) void loss_kernel(LossArgs a) {
+// TEAM lanes hold a row in registers as it came, CH pieces of 16 bytes each and one element behind the last
+// whole piece: one read, one write.
+template <typename T, int TEAM, int CH, int WAVES>
+__global__ __launch_bounds__(threads_of(TEAM), WAVES) void loss_kernel(LossArgs a) {
     constexpr int V = kVec<T>, TEAMS = threads_of(TEAM) / TEAM;
     __shared__ float slots[2][16];
-    const int lane = threadIdx.x % TEAM;
+    const int lane = threadIdx.x % TEAM, whole = a.V / V, rest = a.V - whole * V;
     for (int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / TEAM; row < a.rows; row += int64_t(gridDim.x) * TEAMS) {
         const T* z = static_cast<const T*>(a.z) + row * a.ld;
-        float x[CH][V];
+        piece_t<T, V> x[CH];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) load_piece<V>(z, (i * TEAM + lane) * V, a.V, x[i], kNegInf);
+        for (int i = 0; i < CH; ++i) {
+            if (i * TEAM + lane < whole) {
+                x[i] = reinterpret_cast<const piece_t<T, V>*>(z)[i * TEAM + lane];
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[i][j] = T(kNegInf);
+            }
+        }
+        float last = lane < rest ? float(z[whole * V + lane]) : kNegInf;
         const Target t = target_of<T>(a, row, lane == 0);
-        float m = kNegInf;
+        float m = last;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
+            if (i * TEAM < whole)
 #pragma unroll
-            for (int j = 0; j < V; ++j) m = fmaxf(m, x[i][j]);
+                for (int j = 0; j < V; ++j) m = fmaxf(m, float(x[i][j]));
         m = team_max<TEAM>(m, slots[0]);
         m = m == kNegInf ? 0.0f : m;   // a row of nothing else: a sum of 0, lse -inf
-        float s = 0.0f;
+        last = exp_of(last, m);
+        float s = last;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
+            if (i * TEAM < whole)
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += exp_of(x[i][j], m);
+                for (int j = 0; j < V; ++j) {
+                    const float e = exp_of(float(x[i][j]), m);
+                    s += e;
+                    if constexpr (sizeof(T) == 4) x[i][j] = e;
+                }
         s = team_sum<TEAM>(s, slots[1]);
         if (lane == 0) store_row<T>(a, row, t, m, s);
-        if (a.dz) {
-            T* dz = static_cast<T*>(a.dz) + row * a.ld;
-            const float inv = 1.0f / s;
-#pragma unroll
-            for (int i = 0; i < CH; ++i) store_slope<V>(dz, (i * TEAM + lane) * V, a.V, x[i], m, inv, t);
+        if (!a.dz) continue;
+        T* dz = static_cast<T*>(a.dz) + row * a.ld;
+        if (t.at < 0) {
+            store_zeros<T, V>(dz, a.V, lane, TEAM);
+            continue;
         }
+        const float inv = 1.0f / s, k = t.k * inv, hot = (exp_of(t.z, m) * inv - 1.0f) * t.k;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            if (i * TEAM + lane < whole) {
+                float e[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) e[j] = sizeof(T) == 4 ? float(x[i][j]) : exp_of(float(x[i][j]), m);
+                store_slopes<T, V>(dz, i * TEAM + lane, e, k, t, hot);
+            }
+        }
+        if (lane < rest) dz[whole * V + lane] = T(whole * V + lane == t.at ? hot : last * k);
     }
 }
 
@@ -135,15 +170,23 @@ __global__ __launch_bounds__(1024) void loss_long_kernel(LossArgs a) {
         const float all = team_max<1024>(m, slots[0]);
         s = team_sum<1024>(m == kNegInf ? s : s * exp_of(m, all), slots[1]);
         if (threadIdx.x == 0) store_row<T>(a, row, t, all, s);
-        if (a.dz) {
-            T* dz = static_cast<T*>(a.dz) + row * a.ld;
-            const float inv = 1.0f / s;
-            for (int c = threadIdx.x * V; c < a.V; c += 1024 * V) {
-                float x[V];
-                load_piece<V>(z, c, a.V, x, kNegInf);
-                store_slope<V>(dz, c, a.V, x, all, inv, t);
-            }
+        if (!a.dz) continue;
+        T* dz = static_cast<T*>(a.dz) + row * a.ld;
+        if (t.at < 0) {
+            store_zeros<T, V>(dz, a.V, threadIdx.x, 1024);
+            continue;
         }
+        const float inv = 1.0f / s, k = t.k * inv, hot = (exp_of(t.z, all) * inv - 1.0f) * t.k;
+        const int whole = a.V / V, at = whole * V + threadIdx.x;
+        const float last = at < a.V ? float(z[at]) : 0.0f;
+        for (int c = threadIdx.x; c < whole; c += 1024) {
+            float e[V];
+            load_piece<V>(z, c * V, a.V, e);
+#pragma unroll
+            for (int j = 0; j < V; ++j) e[j] = exp_of(e[j], all);
+            store_slopes<T, V>(dz, c, e, k, t, hot);
+        }
+        if (at < a.V) dz[at] = T(at == t.at ? hot : exp_of(last, all) * k);
     }
 }
 
@@ -151,16 +194,24 @@ template <typename T>
 void launch(dgm_gpu* g, const LossArgs& a) {
     constexpr int V = kVec<T>;
     const auto blocks = [&](int teams) { return dim3(unsigned(std::min<int64_t>((a.rows + teams - 1) / teams, 1 << 20))); };
-    const int n = (a.V + V - 1) / V;   // pieces
-    if (n <= 16) loss_kernel<T, 16, 1><<<blocks(16), dim3(256), 0, g->stream>>>(a);
-    else if (n <= 32) loss_kernel<T, 16, 2><<<blocks(16), dim3(256), 0, g->stream>>>(a);
-    else if (n <= 128) loss_kernel<T, 64, 2><<<blocks(4), dim3(256), 0, g->stream>>>(a);
-    else if (n <= 256) loss_kernel<T, 64, 4><<<blocks(4), dim3(256), 0, g->stream>>>(a);
-    else if (n <= 1024) loss_kernel<T, 256, 4><<<blocks(1), dim3(256), 0, g->stream>>>(a);
-    else if (n <= 2048) loss_kernel<T, 256, 8><<<blocks(1), dim3(256), 0, g->stream>>>(a);
-    else if (n <= 4096) loss_kernel<T, 1024, 4><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
-    else if (n <= 8192) loss_kernel<T, 1024, 8><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
-    else loss_long_kernel<T><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
+    const int n = a.V / V;   // whole pieces
+    // Lanes to a row. Several rows have to be on a CU at once, some of them being loaded while others are summed and
+    // stored, so registers bound the choice (us, gradients): 4096 fp32 rows of 8000 pieces 192 with 1024 lanes (one
+    // workgroup), 212 with 512 (two); 8192 bf16 rows of 6282, whose elements are unpacked and raised twice, 356 with
+    // 512 and 455 with 1024; 16384 fp32 rows of 2000 192 (512 lanes, 207 with 256), of 250 28 (a wave, 29 with 256); 16384
+    // bf16 rows of 937 90 (256 lanes, 102 with 512). Losses alone need no row held: 517 fp32 rows of
+    // 8000 15 in the loop below, 18 in registers. bf16 rows of 16032 228 in registers, 258 in the loop.
+    if (n <= 16) loss_kernel<T, 16, 1, 8><<<blocks(16), dim3(256), 0, g->stream>>>(a);
+    else if (n <= 32) loss_kernel<T, 16, 2, 8><<<blocks(16), dim3(256), 0, g->stream>>>(a);
+    else if (n <= 128) loss_kernel<T, 64, 2, 8><<<blocks(4), dim3(256), 0, g->stream>>>(a);
+    else if (n <= 256) loss_kernel<T, 64, 4, 8><<<blocks(4), dim3(256), 0, g->stream>>>(a);
+    else if (n <= 1024) loss_kernel<T, 256, 4, 8><<<blocks(1), dim3(256), 0, g->stream>>>(a);
+    else if (!a.dz || n > 16384) loss_long_kernel<T><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
+    else if (n <= 2048) loss_kernel<T, 256, 8, 6><<<blocks(1), dim3(256), 0, g->stream>>>(a);
+    else if (n <= 4096) loss_kernel<T, 512, 8, 6><<<blocks(1), dim3(512), 0, g->stream>>>(a);
+    else if (n <= 8192 && sizeof(T) == 4) loss_kernel<T, 1024, 8, 4><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
+    else if (n <= 8192) loss_kernel<T, 512, 16, 4><<<blocks(1), dim3(512), 0, g->stream>>>(a);
+    else loss_kernel<T, 1024, 16, 4><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
 }
 
 }  // namespace
