@@ -5,9 +5,10 @@
 //   y[r] = scale table[tok[r]];  dtable[v] = (dtable[v] +) scale sum of dy[r] over the rows r with tok[r] = v
 //
 // The gradient sorts the tokens (stable, by digits of up to 9 bits), so that a token's rows lie together
-// and each is read once. A unit, one wave, adds up to kSeg sorted rows of 64 pieces of columns; runs within its
+// and each is read once. A unit, one wave, adds up a segment of the sorted rows in 256 columns; runs within its
 // segment it writes, what crosses a segment's end it leaves in the workspace, and a last launch joins those in
-// the order of the rows. Nothing is added to by two waves: no atomics on results, the same bits every time.
+// the order of the rows. Few tokens of a small vocabulary are not sorted: a workgroup for each vocabulary row looks
+// for its rows itself. Nothing is added to by two workgroups: no atomics on results, the same bits every time.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -57,8 +58,9 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(LookupArgs a) {
 // ---- the tokens in order ----------------------------------------------------------
 
 constexpr int kSortThreads = 1024, kTile = 4096, kPerWave = kTile / 16, kBatches = kPerWave / 64;
+constexpr int kRun = 2048, kRunWave = kRun / 16, kRunBatches = kRunWave / 64;   // of the sort over several workgroups
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
-constexpr int kMaxBlocks = 256;   // sorting workgroups, each with a run of tiles
+constexpr int kMaxBlocks = 256;   // workgroups of that sort, each with a run of kRun elements or several
 
 struct SortArgs {
     const uint32_t* tokens;               // of the first pass, which makes keys of them: V for rows without one
@@ -69,7 +71,7 @@ struct SortArgs {
     int64_t n;
     int64_t per;                          // elements of a workgroup's run
     uint32_t V;
-    int shift, bits, blocks;
+    int passes, shift, bits, blocks;
     float* zero;                          // memory to clear beside the sort's first launch (may be null)
     int64_t zero_n;
 };
@@ -89,6 +91,100 @@ __device__ void clear(float* p, int64_t n, int64_t thread, int64_t threads) {
         for (int64_t i = (n & ~int64_t(3)) + thread; i < n; i += threads) p[i] = 0.0f;
     } else {
         for (int64_t i = thread; i < n; i += threads) p[i] = 0.0f;
+    }
+}
+
+// Up to kTile rows in one workgroup, by the digits, the lowest first, elements of a digit in their order: behind the smaller
+// digits, the same digit of the waves before, of the wave's batches before, and of the lanes before.
+__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(SortArgs a) {
+    __shared__ uint32_t held[kTile];
+    __shared__ uint16_t from[kTile];
+    __shared__ uint16_t count[16][kMaxBins];
+    __shared__ uint32_t base[kMaxBins], sums[16];
+    if (blockIdx.x > 0) {   // the others clear
+        clear(a.zero, a.zero_n, int64_t(blockIdx.x - 1) * kSortThreads + threadIdx.x, int64_t(gridDim.x - 1) * kSortThreads);
+        return;
+    }
+    const int bins = 1 << a.bits, t = threadIdx.x, lane = t & 63, wave = t >> 6, at0 = wave * kPerWave + lane;
+    const int n = int(a.n);
+    uint32_t key[kBatches];
+    uint16_t row[kBatches];
+#pragma unroll
+    for (int u = 0; u < kBatches; ++u) {
+        const int i = at0 + u * 64;
+        key[u] = i < n ? key_of<true>(a, i) : 0;
+        row[u] = uint16_t(i);
+    }
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const int shift = pass * a.bits;
+        for (int d = t; d < 16 * bins; d += kSortThreads) count[d >> a.bits][d & (bins - 1)] = 0;
+        __syncthreads();
+        uint32_t rank[kBatches];
+#pragma unroll
+        for (int u = 0; u < kBatches; ++u) {
+            const bool in = at0 + u * 64 < n;
+            const uint32_t digit = (key[u] >> shift) & (bins - 1);
+            uint64_t same = __ballot(in);
+            for (int b = 0; b < a.bits; ++b) {
+                const bool one = (digit >> b) & 1;
+                const uint64_t ones = __ballot(one);
+                same &= one ? ones : ~ones;
+            }
+            const uint32_t under = __builtin_amdgcn_mbcnt_hi(uint32_t(same >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same), 0));
+            const uint32_t had = count[wave][digit];
+            // A wave's LDS accesses complete in the order of issue; the fences keep the compiler's.
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (in && under == 0) count[wave][digit] = uint16_t(had + __popcll(same));
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            rank[u] = had + under;
+        }
+        __syncthreads();
+        // Of each digit: what the waves before have, and all; then a scan over the digits.
+        uint32_t total = 0;
+        if (t < bins) {
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                const uint32_t c = count[w][t];
+                count[w][t] = uint16_t(total);
+                total += c;
+            }
+        }
+        uint32_t scan = total;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t o = __shfl_up(scan, off, 64);
+            scan += lane >= off ? o : 0;
+        }
+        if (lane == 63) sums[wave] = scan;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) scan += sums[w];
+        if (t < bins) base[t] = scan - total;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kBatches; ++u) {
+            if (at0 + u * 64 >= n) continue;
+            const uint32_t digit = (key[u] >> shift) & (bins - 1);
+            const uint32_t to = base[digit] + count[wave][digit] + rank[u];
+            held[to] = key[u];
+            from[to] = row[u];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kBatches; ++u) {
+            if (at0 + u * 64 >= n) continue;
+            key[u] = held[at0 + u * 64];
+            row[u] = from[at0 + u * 64];
+        }
+        // The next pass writes counts, which no one reads any more, and these behind two more barriers.
+    }
+#pragma unroll
+    for (int u = 0; u < kBatches; ++u) {
+        const int i = at0 + u * 64;
+        if (i >= n) continue;
+        a.keys_out[i] = key[u];
+        a.rows_out[i] = row[u];
     }
 }
 
@@ -140,19 +236,19 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
     for (int w = 0; w < wave; ++w) scan += sums[w];
     if (t < bins) base[t] = scan - total + before;
     const int64_t from = int64_t(blockIdx.x) * a.per, to = std::min<int64_t>(a.n, from + a.per);
-    for (int64_t tile = from; tile < to; tile += kTile) {
+    for (int64_t tile = from; tile < to; tile += kRun) {
         for (int d = t; d < 16 * bins; d += kSortThreads) count[d / bins][d & (bins - 1)] = 0;
         __syncthreads();
-        uint32_t key[kBatches], row[kBatches], rank[kBatches];
+        uint32_t key[kRunBatches], row[kRunBatches], rank[kRunBatches];
 #pragma unroll
-        for (int u = 0; u < kBatches; ++u) {
-            const int64_t i = tile + wave * kPerWave + u * 64 + lane;
+        for (int u = 0; u < kRunBatches; ++u) {
+            const int64_t i = tile + wave * kRunWave + u * 64 + lane;
             key[u] = i < to ? key_of<FIRST>(a, i) : 0;
             row[u] = FIRST ? uint32_t(i) : i < to ? a.rows[i] : 0;
         }
 #pragma unroll
-        for (int u = 0; u < kBatches; ++u) {
-            const bool in = tile + wave * kPerWave + u * 64 + lane < to;
+        for (int u = 0; u < kRunBatches; ++u) {
+            const bool in = tile + wave * kRunWave + u * 64 + lane < to;
             const uint32_t digit = (key[u] >> a.shift) & (bins - 1);
             uint64_t same = __ballot(in);
             for (int b = 0; b < a.bits; ++b) {
@@ -182,8 +278,8 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
         }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kBatches; ++u) {
-            if (tile + wave * kPerWave + u * 64 + lane >= to) continue;
+        for (int u = 0; u < kRunBatches; ++u) {
+            if (tile + wave * kRunWave + u * 64 + lane >= to) continue;
             const uint32_t digit = (key[u] >> a.shift) & (bins - 1);
             const uint32_t at = base[digit] + count[wave][digit] + rank[u];
             a.keys_out[at] = key[u];
@@ -196,8 +292,24 @@ __global__ __launch_bounds__(kSortThreads) void embed_place_kernel(SortArgs a) {
 
 // ---- sums ---------------------------------------------------------------------------
 
-constexpr int kSeg = 64;     // sorted rows of a unit
-constexpr int kAhead = 8;    // of them asked for together
+constexpr int kMaxSeg = 64, kMinSeg = 8;   // sorted rows of a unit
+constexpr int kAhead = 8;                  // of them asked for together
+
+// Columns of a lane: 4 where rows are whole pieces of 4, else 1. Lanes behind a row's end load its last ones and store nothing.
+inline int cols_of(int64_t C) { return C % 4 == 0 ? 4 : 1; }
+template <int N, typename T>
+__device__ __forceinline__ void load_cols(const T* p, float (&x)[N]) {
+    const piece_t<T, N> v = *reinterpret_cast<const piece_t<T, N>*>(p);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = float(v[j]);
+}
+template <int N>
+__device__ __forceinline__ void store_cols(float* p, bool live, const float (&x)[N]) {
+    piece_t<float, N> v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = x[j];
+    if (live) *reinterpret_cast<piece_t<float, N>*>(p) = v;
+}
 
 struct SumArgs {
     const void* dy;
@@ -206,48 +318,46 @@ struct SumArgs {
     float *head, *tail;   // [segments][C]: of a run from the segment before, of one into the next
     int64_t n;
     uint32_t V;
-    int C, slabs, add;
+    int C, slabs, add, seg;
     int64_t segs;
     float scale;
 };
 
+// A vocabulary row's sum into the gradient; `old` is what it held (0 where it is overwritten).
 template <int N>
-__device__ __forceinline__ void finish(const SumArgs& a, uint32_t v, int c, float (&acc)[N]) {
-    float* row = a.out + int64_t(v) * a.C;
-    float old[N];
+__device__ __forceinline__ void finish(const SumArgs& a, uint32_t v, int c, bool live, float (&acc)[N], const float (&old)[N]) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) old[j] = 0.0f;
-    if (a.add && c < a.C) load_piece<N>(row, c, a.C, old);
-#pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = a.add ? old[j] + a.scale * acc[j] : a.scale * acc[j];
-    store_piece<N>(row, c, a.C, acc);
+    for (int j = 0; j < N; ++j) acc[j] = old[j] + a.scale * acc[j];
+    store_cols<N>(a.out + int64_t(v) * a.C + c, live, acc);
 }
 
-template <typename T>
+template <typename T, int N>
 __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
-    constexpr int N = kVec<T>;
     const int lane = threadIdx.x & 63;
-    const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t unit = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (unit >= a.segs * a.slabs) return;
-    const int64_t seg = unit / a.slabs, p0 = seg * kSeg;
-    const int c = (int(unit - seg * a.slabs) * 64 + lane) * N;
-    const int64_t p = p0 + lane;
-    const uint32_t key = p < a.n ? a.keys[p] : a.V, row = p < a.n ? a.rows[p] : 0;
-    const uint32_t prev = p0 > 0 ? a.keys[p0 - 1] : kNone, next = p0 + kSeg < a.n ? a.keys[p0 + kSeg] : kNone;
+    const int64_t seg = unit / a.slabs, p0 = seg * a.seg, p = p0 + lane;
+    const int col = (int(unit - seg * a.slabs) * 64 + lane) * N, c = std::min(col, a.C - N);
+    const bool live = col < a.C;
+    const bool in = lane < a.seg && p < a.n;
+    const uint32_t key = in ? a.keys[p] : a.V, row = in ? a.rows[p] : 0;
+    const uint32_t prev = p0 > 0 ? a.keys[p0 - 1] : kNone, next = p0 + a.seg < a.n ? a.keys[p0 + a.seg] : kNone;
     const int n = __popcll(__ballot(key < a.V));   // sorted: rows without a token come last
     if (n == 0) return;
-    const uint32_t left = __shfl_up(key, 1, 64);
+    const uint32_t left = __shfl_up(key, 1, 64), right = __shfl_down(key, 1, 64);
     const uint64_t heads = __ballot(key != (lane ? left : prev));   // a run begins
-    float acc[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+    const uint64_t tails = __ballot(key != (lane + 1 == a.seg ? next : right));   // and ends
+    float acc[N] = {};
     for (int i0 = 0; i0 < n; i0 += kAhead) {
-        float x[kAhead][N];
+        // The rows, and what the runs that end among them are added to, all on their way together.
+        float x[kAhead][N], old[kAhead][N] = {};
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int i = i0 + u < n ? i0 + u : n - 1;
             const uint32_t r = __builtin_amdgcn_readlane(row, i);
-            load_piece<N>(static_cast<const T*>(a.dy) + int64_t(r) * a.C, c, a.C, x[u]);
+            load_cols<N>(static_cast<const T*>(a.dy) + int64_t(r) * a.C + c, x[u]);
+            if (a.add && (tails >> i & 1))
+                load_cols<N>(a.out + int64_t(uint32_t(__builtin_amdgcn_readlane(key, i))) * a.C + c, old[u]);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
@@ -255,47 +365,132 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs a) {
             if (i >= n) break;
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] += x[u][j];
-            const uint32_t v = __builtin_amdgcn_readlane(key, i);
-            const bool last = i + 1 == n ? !(n == kSeg && next == v) : (heads >> (i + 1)) & 1;
+            const bool last = tails >> i & 1;
             if (!last && i + 1 < n) continue;
             const bool begun = heads & (~uint64_t(0) >> (63 - i));   // in this segment
-            if (begun && last) finish<N>(a, v, c, acc);
-            else store_piece<N>((begun ? a.tail : a.head) + seg * a.C, c, a.C, acc);
+            if (begun && last) finish<N>(a, __builtin_amdgcn_readlane(key, i), c, live, acc, old[u]);
+            else store_cols<N>((begun ? a.tail : a.head) + seg * a.C + c, live, acc);
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] = 0.0f;
         }
     }
 }
 
-// A run that begins in segment `seg` and goes on: its tail there, then the heads of the segments behind it.
+// A run that begins in segment `seg` and goes on: its tail there, then the heads of the segments behind it, in four
+// shares of the workgroup's waves.
+template <int N>
 __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
-    constexpr int N = 4;
-    const int lane = threadIdx.x & 63;
-    const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (unit >= a.segs * a.slabs) return;
-    const int64_t seg = unit / a.slabs, p0 = seg * kSeg, end = p0 + kSeg;
+    __shared__ float sums[4][64 * N];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t seg = blockIdx.x / a.slabs, p0 = seg * a.seg, end = p0 + a.seg;
     if (end >= a.n) return;
-    const uint32_t v = a.keys[end - 1];
-    if (v >= a.V || a.keys[end] != v) return;
-    if (p0 > 0 && a.keys[p0 - 1] == v) return;   // it began before
-    const int c = (int(unit - seg * a.slabs) * 64 + lane) * N;
-    float acc[N];
-    load_piece<N>(a.tail + seg * a.C, c, a.C, acc);
-    for (int64_t s = seg + 1;; s += 64) {
-        // Segments s .. s + 63 that this run reaches: it holds their first row.
-        const int64_t first = (s + lane) * kSeg;
-        const uint64_t in = __ballot(first < a.n && a.keys[first < a.n ? first : 0] == v);
-        const int count = in == ~uint64_t(0) ? 64 : __builtin_ctzll(~in);
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
-            float x[N];
-            load_piece<N>(a.head + (s + i) * a.C, c, a.C, x);
-#pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] += x[j];
+    const uint32_t v = a.keys[end - 1], next = a.keys[end], prev = p0 > 0 ? a.keys[p0 - 1] : kNone, first = a.keys[p0];
+    if (v >= a.V || next != v) return;
+    if (first == v && prev == v) return;   // it began before
+    // Segments behind this one that the run reaches: it holds their first row.
+    int64_t count = 0;
+    for (;; count += 64) {
+        const int64_t at = (seg + 1 + count + lane) * a.seg;
+        const uint64_t in = __ballot(at < a.n && a.keys[at < a.n ? at : 0] == v);
+        if (in != ~uint64_t(0)) {
+            count += __builtin_ctzll(~in);
+            break;
         }
-        if (count < 64) break;
     }
-    finish<N>(a, v, c, acc);
+    const int col = (int(blockIdx.x - seg * a.slabs) * 64 + lane) * N, c = std::min(col, a.C - N);
+    const bool live = col < a.C;
+    float acc[N] = {}, old[N] = {};
+    if (wave == 0) load_cols<N>(a.tail + seg * a.C + c, acc);
+    if (wave == 0 && a.add) load_cols<N>(a.out + int64_t(v) * a.C + c, old);
+    const int64_t from = seg + 1 + count * wave / 4, to = seg + 1 + count * (wave + 1) / 4;
+#pragma unroll 8
+    for (int64_t s = from; s < to; ++s) {
+        float x[N];
+        load_cols<N>(a.head + s * a.C + c, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += x[j];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) sums[wave][lane * N + j] = acc[j];
+    __syncthreads();
+    if (wave) return;
+    for (int w = 1; w < 4; ++w)
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += sums[w][lane * N + j];
+    finish<N>(a, v, c, live, acc, old);
+}
+
+// ---- without a sort ---------------------------------------------------------------------
+
+constexpr int kDirectWaves = 16, kDirectRows = 4096;
+
+// One vocabulary row in 64 N columns. The waves look through a share of the tokens each and list the rows that they
+// find in their order; then each adds up a share of the list.
+template <typename T, int N>
+__global__ __launch_bounds__(64 * kDirectWaves) void embed_direct_kernel(SumArgs a, const uint32_t* __restrict__ tokens, uint32_t* words) {
+    __shared__ uint16_t list[kDirectRows];
+    __shared__ int found[kDirectWaves];
+    __shared__ float sums[kDirectWaves][64 * N];
+    constexpr int kTokens = kDirectRows / (64 * kDirectWaves);   // of a lane
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t v = blockIdx.x / a.slabs;
+    const int col = (int(blockIdx.x - v * a.slabs) * 64 + lane) * N, c = std::min(col, a.C - N);
+    const bool live = col < a.C;
+    const int each = (int(a.n) + 64 * kDirectWaves - 1) / (64 * kDirectWaves);   // batches of 64 tokens of a wave
+    uint64_t hits[kTokens];
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+        const int i = (wave * each + u) * 64 + lane;
+        const uint32_t t = u < each && i < a.n ? tokens[i] : kNone;
+        if (blockIdx.x == 0 && t >= a.V && t != kNone) report(words, kBadTokens);
+        hits[u] = __ballot(t == v);
+        n += __popcll(hits[u]);
+    }
+    if (lane == 0) found[wave] = n;
+    float old[N] = {};
+    if (a.add && wave == 0) load_cols<N>(a.out + int64_t(v) * a.C + c, old);
+    __syncthreads();
+    int all = 0, at = 0;
+#pragma unroll
+    for (int w = 0; w < kDirectWaves; ++w) {
+        at = w == wave ? all : at;
+        all += found[w];
+    }
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+        if (hits[u] >> lane & 1)
+            list[at + __builtin_amdgcn_mbcnt_hi(uint32_t(hits[u] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(hits[u]), 0))] =
+                uint16_t((wave * each + u) * 64 + lane);
+        at += __popcll(hits[u]);
+    }
+    if (all == 0 && a.add) return;
+    __syncthreads();
+    float acc[N] = {};
+    const int to = all * (wave + 1) / kDirectWaves;
+    for (int i0 = all * wave / kDirectWaves; i0 < to; i0 += kAhead) {
+        float x[kAhead][N];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int r = __builtin_amdgcn_readfirstlane(list[i0 + u < to ? i0 + u : to - 1]);
+            load_cols<N>(static_cast<const T*>(a.dy) + int64_t(r) * a.C + c, x[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (i0 + u < to)
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[j] += x[u][j];
+    }
+    const int waves = all < kDirectWaves ? all : kDirectWaves;   // with all < 16 some shares in between are empty: zeros
+#pragma unroll
+    for (int j = 0; j < N; ++j) sums[wave][lane * N + j] = acc[j];
+    __syncthreads();
+    if (wave) return;
+    if (waves)
+        for (int w = 1; w < kDirectWaves; ++w)
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[j] += sums[w][lane * N + j];
+    finish<N>(a, v, c, live, acc, old);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -312,28 +507,54 @@ int check(dgm_gpu* g, const char* name, const dgm_rows_cfg* c) {
     return DGM_OK;
 }
 
+// Workgroups of vocabulary row x columns up to which they look for their rows themselves: each costs about 4.5 ns
+// whether it finds any or not (1024 rows of 65 x 128: 12 us with the lookup, 21 sorted; 4096 rows of 1000 x 256 14.5 and 27; 2000
+// workgroups still even: 4096 rows of 256 x 2048 31.6 and 29.5).
+constexpr int64_t kDirectGroups = 2048;
+
 // What the gradient's launches need of a configuration.
 struct Plan {
     int passes, bits, blocks;
     int64_t per, segs;
+    int slabs, seg;
+    bool direct;
     int64_t lists, hist, parts;   // bytes of the workspace's areas
     int64_t bytes() const { return lists + hist + parts; }
 };
 int64_t round16(int64_t n) { return (n + 15) & ~int64_t(15); }
 Plan plan_of(const dgm_rows_cfg* c) {
     Plan p;
+    const int64_t wide = 64 * cols_of(c->C);
+    p.slabs = int((c->C + wide - 1) / wide);
+    p.direct = c->rows > 0 && c->rows <= kDirectRows && c->V <= kDirectGroups && c->V * p.slabs <= kDirectGroups;
+    if (p.direct) {
+        p.lists = p.hist = p.parts = 0;
+        return p;
+    }
     int width = 1;
     while ((int64_t(1) << width) <= c->V) ++width;   // keys 0 .. V
     p.passes = (width + kMaxBits - 1) / kMaxBits;
     p.bits = (width + p.passes - 1) / p.passes;
-    const int64_t tiles = (c->rows + kTile - 1) / kTile, each = (tiles + kMaxBlocks - 1) / kMaxBlocks;
-    p.per = each * kTile;
-    p.blocks = int(each ? (tiles + each - 1) / each : 0);
-    p.segs = (c->rows + kSeg - 1) / kSeg;
-    p.lists = 4 * round16(c->rows * 4);
+    const int64_t runs = (c->rows + kRun - 1) / kRun, each = (runs + kMaxBlocks - 1) / kMaxBlocks;
+    p.per = each * kRun;
+    p.blocks = c->rows <= kTile ? 0 : int((runs + each - 1) / each);
     p.hist = round16(int64_t(p.blocks) * (4 << p.bits));
+    // Shorter segments where there is little work: 8 waves to a CU, if so many can be.
+    p.seg = kMaxSeg;
+    while (p.seg > kMinSeg && (c->rows + p.seg - 1) / p.seg * p.slabs < 8 * dgm::kCus) p.seg /= 2;
+    p.segs = (c->rows + p.seg - 1) / p.seg;
+    p.lists = 4 * round16(c->rows * 4);
     p.parts = 2 * round16(p.segs * c->C * 4);
     return p;
+}
+
+// f(type of dy, columns of a lane).
+template <typename F>
+void by_shape(const dgm_rows_cfg* c, const F& f) {
+    using four = std::integral_constant<int, 4>;
+    using one = std::integral_constant<int, 1>;
+    if (c->type == DGM_TYPE_F32) cols_of(c->C) == 4 ? f(float{}, four{}) : f(float{}, one{});
+    else cols_of(c->C) == 4 ? f(__bf16{}, four{}) : f(__bf16{}, one{});
 }
 
 // Waves of `count` units of work fit one launch's bound on threads.
@@ -383,54 +604,75 @@ int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens
     if (rc) return rc;
     rc = check(g, "embedRowsBwd", cfg);
     if (rc) return rc;
-    if (!dtable || (cfg->rows > 0 && (!tokens || !dy || !ws))) return dgm::fail(g, DGM_ERR_ARG, "embedRowsBwd: null buffer");
     const Plan p = plan_of(cfg);
+    if (!dtable || (cfg->rows > 0 && (!tokens || !dy)) || (p.bytes() > 0 && !ws))
+        return dgm::fail(g, DGM_ERR_ARG, "embedRowsBwd: null buffer");
     if (ws_bytes < p.bytes())
         return dgm::fail(g, DGM_ERR_ARG, "embedRowsBwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)p.bytes());
     if (!dgm::aligned(tokens, 4) || !dgm::aligned(dy, size_t(type_bytes(cfg->type))) || !dgm::aligned(dtable, 4) || !dgm::aligned(ws, 16))
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "embedRowsBwd: a buffer is not aligned to its elements, or the workspace to 16 bytes");
-    const int n = 16 / type_bytes(cfg->type);
-    const int64_t slabs = (cfg->C + 64 * n - 1) / (64 * n), join = (cfg->C + 255) / 256;
-    if (!fits(p.segs * slabs) || !fits(p.segs * join))
+    if (!p.direct && !fits(p.segs * p.slabs * 4))
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "embedRowsBwd: %lld rows of %lld exceed one launch", (long long)cfg->rows, (long long)cfg->C);
     OnDevice on(g->device);
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "embedRowsBwd: %s", hipGetErrorString(on.err));
+    SumArgs a{dy, nullptr, nullptr, dtable, nullptr, nullptr, cfg->rows, uint32_t(cfg->V), int(cfg->C), p.slabs, accumulate ? 1 : 0,
+              0, 0, cfg->scale};
+    if (p.direct) {
+        const dim3 grid(unsigned(cfg->V) * unsigned(p.slabs)), block(64 * kDirectWaves);
+        by_shape(cfg, [&](auto t, auto n) {
+            embed_direct_kernel<decltype(t), decltype(n)::value><<<grid, block, 0, g->stream>>>(a, tokens, g->seq_report);
+        });
+        DGM_LAUNCH_CHECK(g, "embed_direct");
+        return DGM_OK;
+    }
     uint8_t* at = static_cast<uint8_t*>(ws);
     uint32_t* lists[4];
     for (auto& l : lists) {
         l = reinterpret_cast<uint32_t*>(at);
         at += p.lists / 4;
     }
-    SortArgs s{tokens, nullptr, nullptr, nullptr, nullptr, reinterpret_cast<uint32_t*>(at), g->seq_report, cfg->rows, p.per,
-               uint32_t(cfg->V), 0, p.bits, p.blocks, accumulate ? nullptr : dtable, accumulate ? 0 : cfg->V * cfg->C};
+    const int64_t zero_n = accumulate ? 0 : cfg->V * cfg->C;
+    const unsigned clearing = unsigned(std::min<int64_t>((zero_n + 16 * kSortThreads - 1) / (16 * kSortThreads), 2048));
+    SortArgs s{tokens, nullptr, nullptr, lists[0], lists[1], reinterpret_cast<uint32_t*>(at), g->seq_report, cfg->rows, p.per,
+               uint32_t(cfg->V), p.passes, 0, p.bits, p.blocks, dtable, zero_n};
     at += p.hist;
-    const unsigned clearing = unsigned(std::min<int64_t>((s.zero_n + 16 * kSortThreads - 1) / (16 * kSortThreads), 2048));
-    if (p.blocks + clearing == 0) return DGM_OK;
-    embed_hist_kernel<true><<<dim3(unsigned(p.blocks) + clearing), dim3(kSortThreads), 0, g->stream>>>(s);
-    DGM_LAUNCH_CHECK(g, "embed_hist");
-    if (p.blocks == 0) return DGM_OK;
-    for (int i = 0; i < p.passes; ++i) {
-        s.shift = i * p.bits;
-        s.keys_out = lists[2 * (i & 1)];
-        s.rows_out = lists[2 * (i & 1) + 1];
-        const dim3 grid{unsigned(p.blocks)}, block{kSortThreads};
-        if (i) embed_hist_kernel<false><<<grid, block, 0, g->stream>>>(s);
-        if (i) embed_place_kernel<false><<<grid, block, 0, g->stream>>>(s);
-        else embed_place_kernel<true><<<grid, block, 0, g->stream>>>(s);
+    const dim3 block{kSortThreads};
+    if (p.blocks == 0) {
+        if (cfg->rows + zero_n == 0) return DGM_OK;
+        embed_sort_kernel<<<dim3(1 + clearing), block, 0, g->stream>>>(s);
+        DGM_LAUNCH_CHECK(g, "embed_sort");
+        if (cfg->rows == 0) return DGM_OK;
+        s.keys = lists[0];
+        s.rows = lists[1];
+    } else {
+        const dim3 grid{unsigned(p.blocks)};
+        embed_hist_kernel<true><<<dim3(unsigned(p.blocks) + clearing), block, 0, g->stream>>>(s);
+        embed_place_kernel<true><<<grid, block, 0, g->stream>>>(s);
+        for (int i = 1; i < p.passes; ++i) {
+            s.shift = i * p.bits;
+            s.keys = s.keys_out;
+            s.rows = s.rows_out;
+            s.keys_out = lists[2 * (i & 1)];
+            s.rows_out = lists[2 * (i & 1) + 1];
+            embed_hist_kernel<false><<<grid, block, 0, g->stream>>>(s);
+            embed_place_kernel<false><<<grid, block, 0, g->stream>>>(s);
+        }
         DGM_LAUNCH_CHECK(g, "embed_place");
         s.keys = s.keys_out;
         s.rows = s.rows_out;
     }
-    float* parts = reinterpret_cast<float*>(at);
-    SumArgs a{dy, s.keys, s.rows, dtable, parts, parts + p.parts / 8, cfg->rows, uint32_t(cfg->V), int(cfg->C), int(slabs),
-              accumulate ? 1 : 0, p.segs, cfg->scale};
-    const dim3 grid(dgm::ceil_div(p.segs * slabs, 4));
-    if (cfg->type == DGM_TYPE_F32) embed_sum_kernel<float><<<grid, dim3(256), 0, g->stream>>>(a);
-    else embed_sum_kernel<__bf16><<<grid, dim3(256), 0, g->stream>>>(a);
+    a.keys = s.keys;
+    a.rows = s.rows;
+    a.head = reinterpret_cast<float*>(at);
+    a.tail = a.head + p.parts / 8;
+    a.seg = p.seg;
+    a.segs = p.segs;
+    const dim3 grid(dgm::ceil_div(p.segs * p.slabs, 4));
+    by_shape(cfg, [&](auto t, auto n) { embed_sum_kernel<decltype(t), decltype(n)::value><<<grid, dim3(256), 0, g->stream>>>(a); });
     DGM_LAUNCH_CHECK(g, "embed_sum");
     if (p.segs > 1) {
-        a.slabs = int(join);
-        embed_join_kernel<<<dim3(dgm::ceil_div(p.segs * join, 4)), dim3(256), 0, g->stream>>>(a);
+        const dim3 join{unsigned(p.segs * p.slabs)};
+        by_shape(cfg, [&](auto, auto n) { embed_join_kernel<decltype(n)::value><<<join, dim3(256), 0, g->stream>>>(a); });
         DGM_LAUNCH_CHECK(g, "embed_join");
     }
     return DGM_OK;

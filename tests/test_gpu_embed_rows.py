@@ -241,9 +241,10 @@ def test_refusals(dgm, gpu, torch_cuda):
     for k in ("tokens", "table", "y"):
         refused(dgm.DGM_ERR_ARG, which="lookup", **{k: None})
         refused(dgm.DGM_ERR_UNSUPPORTED, which="lookup", **{k: addr[k] + 2})
+    large = dict(V=1 << 22)         # too many vocabulary rows for each to look for its tokens: those are sorted, in a workspace
     for k in ("tokens", "dy", "dtable", "ws"):
-        refused(dgm.DGM_ERR_ARG, which="gradient", **{k: None})
-        refused(dgm.DGM_ERR_UNSUPPORTED, which="gradient", **{k: addr[k] + 2})
-    c = dgm.RowsCfg(type=0, tableType=0, scale=1.0, rows=4, C=8, V=16)
-    refused(dgm.DGM_ERR_ARG, which="gradient", ws_bytes=gpu.embedRowsBwd_ws_bytes(c) - 1)
+        refused(dgm.DGM_ERR_ARG, large, which="gradient", **{k: None})
+        refused(dgm.DGM_ERR_UNSUPPORTED, large, which="gradient", **{k: addr[k] + 2})
+    c = dgm.RowsCfg(type=0, tableType=0, scale=1.0, rows=4, C=8, V=1 << 22)
+    refused(dgm.DGM_ERR_ARG, large, which="gradient", ws_bytes=gpu.embedRowsBwd_ws_bytes(c) - 1)
     refused(dgm.DGM_ERR_UNSUPPORTED, dict(rows=1 << 30, C=1 << 24), which="gradient", ws_bytes=1 << 62)
