@@ -574,7 +574,7 @@ int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, cons
 typedef struct dgm_norm_cfg {
     int32_t type;                  /* DGM_TYPE_* of the rows                    */
     float eps;                     /* >= 0                                      */
-    int64_t rows, cols;            /* rows up to 2^31 - 1, cols up to 32768     */
+    int64_t rows, cols;            /* rows up to 2^31 - 1, cols up to 16384     */
 } dgm_norm_cfg;
 
 /* sum = x + res (rounded to the rows' type; res and sum may both be NULL: x itself),

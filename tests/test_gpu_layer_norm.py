@@ -53,7 +53,8 @@ def backward(gpu, cfg, s, x, dsum, dx=None, dw=True, db=True):
 # Around every border between kernels, and odd rows that start anywhere.
 SIZES = [(1, 1), (3, 2), (5, 7), (17, 64), (33, 127), (1, 128), (40, 129), (7, 300), (9, 512), (6, 513), (5, 1000), (4, 1024),
          (4, 1025), (3, 2047), (3, 2048), (5, 2049), (2, 4096), (3, 4097), (2, 8191), (2, 8192), (2, 8193), (1, 16384),
-         (2, 16385), (1, 32768), (2, 32767), (700, 96), (1500, 130), (1030, 2056), (2100, 40)]
+         (2, 16383), (300, 12000), (700, 96), (1500, 130), (1030, 2056), (2100, 40),
+         (2100, 500), (2101, 1000), (600, 2000), (300, 4096), (130, 8192)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -271,19 +272,21 @@ def test_refusals(dgm, gpu, torch_cuda):
     refused(dgm.DGM_ERR_ARG, cfg(cols=0))
     refused(dgm.DGM_ERR_ARG, cfg(eps=-1.0))
     refused(dgm.DGM_ERR_ARG, cfg(eps=float("nan")))
-    refused(dgm.DGM_ERR_UNSUPPORTED, cfg(cols=32769))
+    refused(dgm.DGM_ERR_UNSUPPORTED, cfg(cols=16385))
     refused(dgm.DGM_ERR_UNSUPPORTED, cfg(rows=1 << 31))
     for k in ("x", "w", "y", "sum", "res"):
         refused(dgm.DGM_ERR_ARG, cfg(), fwd={k: None}, bwd=None)
-    for k in ("x", "w", "dy", "dx", "mean", "rstd", "ws"):
+    for k in ("x", "w", "dy", "dx", "mean", "rstd"):
         refused(dgm.DGM_ERR_ARG, cfg(), fwd=None, bwd={k: None})
+    large = cfg(rows=3000)          # whose sums go through the workspace
+    refused(dgm.DGM_ERR_ARG, large, fwd=None, bwd={"ws": None})
+    refused(dgm.DGM_ERR_ARG, large, fwd=None, ws=gpu.layerNormBwd_ws_bytes(large) - 1)
     for k in ("x", "w", "y", "sum", "res", "mean", "b"):
         refused(dgm.DGM_ERR_UNSUPPORTED, cfg(), fwd={k: addr[k] + 2}, bwd=None)
     for k in ("x", "dy", "dx", "dsum", "dw", "db", "mean", "rstd"):
         refused(dgm.DGM_ERR_UNSUPPORTED, cfg(), fwd=None, bwd={k: addr[k] + 2})
     for k in ("x", "dy"):
         refused(dgm.DGM_ERR_ARG, cfg(), fwd=None, bwd={"dx": addr[k]})
-    refused(dgm.DGM_ERR_ARG, cfg(), fwd=None, ws=gpu.layerNormBwd_ws_bytes(cfg()) - 1)
     with pytest.raises(dgm.DgmError) as e:      # no open region
         gpu.layerNormFwd(cfg(), s["x"], None, s["w"], None, None, s["y"])
     assert e.value.code == dgm.DGM_ERR_NOT_BEGUN
