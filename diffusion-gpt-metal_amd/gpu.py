@@ -12,6 +12,7 @@ where the reference calls fatalError / exit(1).
 from __future__ import annotations
 
 import ctypes
+import struct
 import sys
 from typing import Any, List, Optional
 
@@ -34,21 +35,25 @@ def _ptr(t: Any) -> Optional[int]:
     raise TypeError(f"cannot take a device address of {type(t).__name__}")
 
 
-# Classes of the device tensors that the attention calls take: one look tells both type and place. Set where
+# Classes of the device tensors that the calls without a counterpart in the reference take: one look tells both type and place. Set where
 # torch is loaded (without it there are no tensors).
 _F32: Any = ()
 _I32: Any = ()
+_I8: Any = ()
+_U8: Any = ()
 _ELEMENTS: dict = {}       # by DGM_TYPE_*
 _DTYPES: dict = {(): None}
 
 
 def _elements(code: int) -> Any:
-    global _F32, _I32
+    global _F32, _I32, _I8, _U8
     if not _ELEMENTS and "torch" in sys.modules:
         import torch
         _F32, _I32 = torch.cuda.FloatTensor, torch.cuda.IntTensor
+        _I8, _U8 = torch.cuda.CharTensor, torch.cuda.ByteTensor
         _ELEMENTS.update({DGM_TYPE_F32: _F32, DGM_TYPE_BF16: torch.cuda.BFloat16Tensor})
-        _DTYPES.update({_F32: torch.float32, _I32: torch.int32, torch.cuda.BFloat16Tensor: torch.bfloat16})
+        _DTYPES.update({_F32: torch.float32, _I32: torch.int32, _I8: torch.int8, _U8: torch.uint8,
+                        torch.cuda.BFloat16Tensor: torch.bfloat16})
     return _ELEMENTS.get(code, ())      # (): a code that the library refuses
 
 
@@ -74,26 +79,20 @@ def _ints(t: Any, what: str) -> Optional[int]:
     return p
 
 
-def _rows(t: Any, dtype: str, count: int, what: str) -> Optional[int]:
-    """_ptr of at least `count` elements of the torch dtype of that name, back to back. Raw
-    addresses are taken as they are; None is an absent buffer."""
-    p = _ptr(t)
-    if hasattr(t, "dtype"):
-        if str(t.dtype) != dtype:
-            raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+def _rows(t: Any, kind: Any, count: int, what: str) -> Optional[int]:
+    """_ptr of a tensor of that class with at least `count` elements, back to back. Raw addresses are
+    taken as they are; None is an absent buffer."""
+    if isinstance(t, kind) and t.is_contiguous() and t.numel() >= count:   # what most calls pass
+        return t.data_ptr()
+    if t is None:
+        return None
+    p = _typed(t, kind, what)
+    if hasattr(t, "is_contiguous"):
         if not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous")
         if t.numel() < count:
             raise ValueError(f"{what} holds {t.numel()} elements, {count} needed")
     return p
-
-
-_TORCH_F32, _TORCH_I32 = "torch.float32", "torch.int32"
-_TORCH_TYPES = {DGM_TYPE_F32: _TORCH_F32, DGM_TYPE_BF16: "torch.bfloat16"}
-
-
-def _dtype(code: int) -> str:
-    return _TORCH_TYPES.get(code, _TORCH_F32)      # a code that the library refuses
 
 
 def _bytes(ws: Any, nbytes: int) -> Optional[int]:
@@ -109,24 +108,28 @@ class _AdamTensor(AdamTensor):
     held: tuple = ()
 
 
+_pack_adam_tensor = struct.Struct("9q4i").pack      # the fields of dgm_adam_tensor; a Structure's constructor takes 3 us
+
+
 def adam_tensor(w, grad, m, v, mscale=None, vscale=None, *, decay: bool, q=None, scale=None, bits: int = 0,
                 qGroup: int = 0) -> AdamTensor:
     """One parameter of GPU.adamMany_plan, from device tensors: fp32 w and grad; m and v fp32, or int8 and uint8 codes
     with mscale and vscale, one float for each 256 elements; with bits, the codes and scales that
     its linear reads."""
+    f32 = _elements(DGM_TYPE_F32) and _F32
     n = w.numel()
     blocks = -(-n // 256)
-    codes = mscale is not None
-    first, second = ("torch.int8", "torch.uint8") if codes else (_TORCH_F32, _TORCH_F32)
-    t = _AdamTensor(
-        w=_rows(w, _TORCH_F32, n, "w"), grad=_rows(grad, _TORCH_F32, n, "grad"), m=_rows(m, first, n, "m"),
-        v=_rows(v, second, n, "v"), mscale=_rows(mscale, _TORCH_F32, blocks, "mscale"),
-        vscale=_rows(vscale, _TORCH_F32, blocks, "vscale"), n=n, decay=int(bool(decay)), bits=bits, qGroup=qGroup)
+    first, second = (f32, f32) if mscale is None else (_I8, _U8)
+    codes = scales = None
     if bits and qGroup > 0:
-        t.scale = _rows(scale, _TORCH_F32, n // qGroup, "scale")
+        scales = _rows(scale, f32, n // qGroup, "scale")
         if hasattr(q, "element_size") and q.numel() * q.element_size() * 8 < n * bits:
             raise ValueError(f"q holds {q.numel() * q.element_size()} bytes, {n * bits // 8} needed")
-        t.q = _ptr(q)
+        codes = _ptr(q)
+    t = _AdamTensor.from_buffer_copy(_pack_adam_tensor(
+        _rows(w, f32, n, "w") or 0, _rows(grad, f32, n, "grad") or 0, _rows(m, first, n, "m") or 0, _rows(v, second, n, "v") or 0,
+        _rows(mscale, f32, blocks, "mscale") or 0, _rows(vscale, f32, blocks, "vscale") or 0, codes or 0, scales or 0, n,
+        1 if decay else 0, bits, qGroup, 0))
     t.held = (w, grad, m, v, mscale, vscale, q, scale)
     return t
 
@@ -390,47 +393,49 @@ class GPU:
     # contiguous a ValueError; raw addresses pass.
     def layerNormFwd(self, cfg: NormCfg, x, res, weight, bias, sum, y, mean=None, rstd=None) -> None:
         """y = layer norm of sum = x + res (both None: of x)."""
-        el, n = _dtype(cfg.type), cfg.rows * cfg.cols
+        el, n = _elements(cfg.type), cfg.rows * cfg.cols
         self._check(self.lib.dgm_layerNormFwd(
-            self.h, ctypes.byref(cfg), _rows(x, el, n, "x"), _rows(res, el, n, "res"), _rows(weight, _TORCH_F32, cfg.cols, "weight"),
-            _rows(bias, _TORCH_F32, cfg.cols, "bias"), _rows(sum, el, n, "sum"), _rows(y, el, n, "y"),
-            _rows(mean, _TORCH_F32, cfg.rows, "mean"), _rows(rstd, _TORCH_F32, cfg.rows, "rstd")))
+            self.h, ctypes.byref(cfg), _rows(x, el, n, "x"), _rows(res, el, n, "res"), _rows(weight, _F32, cfg.cols, "weight"),
+            _rows(bias, _F32, cfg.cols, "bias"), _rows(sum, el, n, "sum"), _rows(y, el, n, "y"),
+            _rows(mean, _F32, cfg.rows, "mean"), _rows(rstd, _F32, cfg.rows, "rstd")))
 
     def layerNormBwd_ws_bytes(self, cfg: NormCfg) -> int:
         return int(self.lib.dgm_layerNormBwd_ws_bytes(ctypes.byref(cfg)))
 
     def layerNormBwd(self, cfg: NormCfg, x, mean, rstd, weight, dy, dsum, dx, dweight, dbias, ws, ws_bytes: int) -> None:
         """dx = dsum + the gradient through the norm; dweight and dbias are added to."""
-        el, n = _dtype(cfg.type), cfg.rows * cfg.cols
+        el, n = _elements(cfg.type), cfg.rows * cfg.cols
         self._check(self.lib.dgm_layerNormBwd(
-            self.h, ctypes.byref(cfg), _rows(x, el, n, "x"), _rows(mean, _TORCH_F32, cfg.rows, "mean"),
-            _rows(rstd, _TORCH_F32, cfg.rows, "rstd"), _rows(weight, _TORCH_F32, cfg.cols, "weight"), _rows(dy, el, n, "dy"),
-            _rows(dsum, el, n, "dsum"), _rows(dx, el, n, "dx"), _rows(dweight, _TORCH_F32, cfg.cols, "dweight"),
-            _rows(dbias, _TORCH_F32, cfg.cols, "dbias"), _bytes(ws, ws_bytes), ws_bytes))
+            self.h, ctypes.byref(cfg), _rows(x, el, n, "x"), _rows(mean, _F32, cfg.rows, "mean"),
+            _rows(rstd, _F32, cfg.rows, "rstd"), _rows(weight, _F32, cfg.cols, "weight"), _rows(dy, el, n, "dy"),
+            _rows(dsum, el, n, "dsum"), _rows(dx, el, n, "dx"), _rows(dweight, _F32, cfg.cols, "dweight"),
+            _rows(dbias, _F32, cfg.cols, "dbias"), _bytes(ws, ws_bytes), ws_bytes))
 
     def crossEntropy(self, cfg: LossCfg, logits, targets, loss, rowScale=None, lse=None, dlogits=None) -> None:
         """Cross-entropy of logits [rows, V] with int32 targets (negative: the row does not count), and its gradient."""
-        el, rows = _dtype(cfg.type), cfg.rows
+        el, rows = _elements(cfg.type), cfg.rows
         n = (rows - 1) * (cfg.ld or cfg.V) + cfg.V if rows > 0 else 0
         self._check(self.lib.dgm_crossEntropy(
-            self.h, ctypes.byref(cfg), _rows(logits, el, n, "logits"), _rows(targets, _TORCH_I32, rows, "targets"),
-            _rows(rowScale, _TORCH_F32, rows, "rowScale"), _rows(loss, _TORCH_F32, rows, "loss"),
-            _rows(lse, _TORCH_F32, rows, "lse"), _rows(dlogits, el, n, "dlogits")))
+            self.h, ctypes.byref(cfg), _rows(logits, el, n, "logits"), _rows(targets, _I32, rows, "targets"),
+            _rows(rowScale, _F32, rows, "rowScale"), _rows(loss, _F32, rows, "loss"),
+            _rows(lse, _F32, rows, "lse"), _rows(dlogits, el, n, "dlogits")))
 
     def embedRows(self, cfg: RowsCfg, tokens, table, y) -> None:
         """y[r] = scale * table[tokens[r]]; tokens int32, -1 for none."""
+        el, held = _elements(cfg.type), _elements(cfg.tableType)
         self._check(self.lib.dgm_embedRows(
-            self.h, ctypes.byref(cfg), _rows(tokens, _TORCH_I32, cfg.rows, "tokens"),
-            _rows(table, _dtype(cfg.tableType), cfg.V * cfg.C, "table"), _rows(y, _dtype(cfg.type), cfg.rows * cfg.C, "y")))
+            self.h, ctypes.byref(cfg), _rows(tokens, _I32, cfg.rows, "tokens"), _rows(table, held, cfg.V * cfg.C, "table"),
+            _rows(y, el, cfg.rows * cfg.C, "y")))
 
     def embedRowsBwd_ws_bytes(self, cfg: RowsCfg) -> int:
         return int(self.lib.dgm_embedRowsBwd_ws_bytes(ctypes.byref(cfg)))
 
     def embedRowsBwd(self, cfg: RowsCfg, tokens, dy, dtable, ws, ws_bytes: int, accumulate: bool = False) -> None:
         """The gradient of embedRows in the fp32 dtable [V, C], overwritten or added to."""
+        el = _elements(cfg.type)
         self._check(self.lib.dgm_embedRowsBwd(
-            self.h, ctypes.byref(cfg), _rows(tokens, _TORCH_I32, cfg.rows, "tokens"),
-            _rows(dy, _dtype(cfg.type), cfg.rows * cfg.C, "dy"), _rows(dtable, _TORCH_F32, cfg.V * cfg.C, "dtable"),
+            self.h, ctypes.byref(cfg), _rows(tokens, _I32, cfg.rows, "tokens"),
+            _rows(dy, el, cfg.rows * cfg.C, "dy"), _rows(dtable, _F32, cfg.V * cfg.C, "dtable"),
             1 if accumulate else 0, _bytes(ws, ws_bytes), ws_bytes))
 
     def adamMany_plan(self, tensors: List[AdamTensor], stateBits: int = 32) -> AdamPlan:
@@ -446,18 +451,21 @@ class GPU:
 
     def adamMany_norm(self, plan: AdamPlan, clip: float, out) -> None:
         """out[0] = the norm of all gradients, out[1] = the factor that clips it."""
-        self._check(self.lib.dgm_adamMany_norm(self.h, ctypes.byref(plan), clip, _rows(out, _TORCH_F32, 2, "out")))
+        _elements(DGM_TYPE_F32)
+        self._check(self.lib.dgm_adamMany_norm(self.h, ctypes.byref(plan), clip, _rows(out, _F32, 2, "out")))
 
     def adamMany(self, plan: AdamPlan, lr: float, b1: float, b2: float, eps: float, wd: float, invBC1: float,
                  invBC2: float, factor=None) -> None:
         """adam (with codes: adamQuantize) of every tensor of the plan; the gradients times factor[0]."""
-        self._check(self.lib.dgm_adamMany(self.h, ctypes.byref(plan), _rows(factor, _TORCH_F32, 1, "factor"), lr, b1, b2, eps,
+        _elements(DGM_TYPE_F32)
+        self._check(self.lib.dgm_adamMany(self.h, ctypes.byref(plan), _rows(factor, _F32, 1, "factor"), lr, b1, b2, eps,
                                           wd, invBC1, invBC2))
 
     def adamMany_states(self, plan: AdamPlan, m, v) -> None:
         """The values of 8-bit moments, tensor behind tensor, each from the next multiple of 256."""
-        self._check(self.lib.dgm_adamMany_states(self.h, ctypes.byref(plan), _rows(m, _TORCH_F32, plan.elements, "m"),
-                                                 _rows(v, _TORCH_F32, plan.elements, "v")))
+        _elements(DGM_TYPE_F32)
+        self._check(self.lib.dgm_adamMany_states(self.h, ctypes.byref(plan), _rows(m, _F32, plan.elements, "m"),
+                                                 _rows(v, _F32, plan.elements, "v")))
 
     # -- training step (src/GPU.swift:200-210, 274-277, 324-350, 420-429) -----
     def adam(self, w, g, m, v, n: int, lr: float, b1: float, b2: float, eps: float, wd: float,

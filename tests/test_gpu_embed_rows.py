@@ -53,10 +53,12 @@ def backward(dgm, gpu, cfg, t, dy, dtable, add):
     assert (ws[size:] == 0x7F).all()
 
 
-# Segments of 64 sorted rows, tiles of 4096, digits of up to 9 bits (V of 511, 512: one pass or two), several workgroups.
+# With and without a sort (up to 4096 rows, vocabulary x columns / 256 up to 2048), by one workgroup (4096 rows) or several;
+# digits of up to 9 bits (V of 511, 512: one pass or two); segments of 8 to 64 sorted rows.
 SIZES = [(1, 1, 1), (2, 5, 1), (63, 7, 3), (64, 8, 3), (65, 33, 4), (130, 260, 1), (1000, 20, 65), (4096, 12, 511), (4097, 12, 512),
          (5000, 130, 40), (9000, 9, 50257), (20000, 4, 2), (3000, 515, 200), (300, 2050, 31), (70000, 3, 262143), (70001, 3, 262144),
-         (33, 64, 2 ** 27)]
+         (33, 64, 2 ** 27), (1, 9, 5000), (1025, 5, 3000), (2500, 260, 5000), (4096, 12, 70000), (3500, 8, 2 ** 24), (4100, 4096, 2000),
+         (30000, 1028, 300)]
 
 
 @pytest.mark.parametrize("add", [False, True])

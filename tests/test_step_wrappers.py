@@ -152,3 +152,35 @@ def test_8_bit_codes_by_both_ways():
         assert (np.abs(np.abs(c.reshape(-1, 256)) - root) <= 0.5 + 1e-9).mean() > 0.999     # all but 0s that v raises to 1
         again = (ref.decode_v if second else ref.decode_m)(c, s)
         assert np.array_equal(ref.encode(again, second)[0], c)
+
+
+FIRST = r"""
+import sys, torch
+sys.path.insert(0, "tests")
+from conftest import load_package
+from test_step_wrappers import Dev, calls
+from test_attn_wrappers import Lib
+dgm = load_package()
+g = dgm.GPU.__new__(dgm.GPU)
+g.lib, g.h = Lib(), 0
+call, args = calls(dgm, torch.float32)[sys.argv[1]]
+for k in args:
+    try:
+        call(g, **{n: Dev(torch.zeros(c, dtype=torch.int64 if n == k else d)) for n, (d, c) in args.items()})
+    except TypeError as e:
+        assert str(e).startswith(k), e
+    else:
+        raise SystemExit(k + " passed")
+    break
+g.h = None
+"""
+
+
+@pytest.mark.parametrize("name", ["layerNormFwd", "crossEntropy", "embedRows", "embedRowsBwd", "adamMany", "adamMany_states"])
+def test_the_first_call_of_a_process_looks_at_types(name):
+    import subprocess
+    import sys
+
+    from conftest import REPO
+    done = subprocess.run([sys.executable, "-c", FIRST, name], cwd=REPO, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
