@@ -15,31 +15,31 @@ namespace {
 
 using namespace dgm_step;
 
-// A lane's share of a row: CH whole pieces of 16 bytes as they came, and one of the elements behind the last whole
-// piece of the row. What the row does not have is zeros.
+// A lane's share of a row: CH whole pieces of 16 bytes as they came, and one of the elements around those. What the
+// row does not have is zeros.
 template <typename T, int TEAM, int CH>
 struct Share {
     static constexpr int V = kVec<T>;
     piece_t<T, V> piece[CH];
     float last;
 
-    __device__ __forceinline__ void load(const T* row, int whole, int rest, int lane) {
+    __device__ __forceinline__ void load(const T* row, const Span& w, int lane) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            if (i * TEAM + lane < whole) {
-                piece[i] = reinterpret_cast<const piece_t<T, V>*>(row)[i * TEAM + lane];
+            if (i * TEAM + lane < w.whole) {
+                piece[i] = *reinterpret_cast<const piece_t<T, V>*>(row + w.head + (i * TEAM + lane) * V);
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) piece[i][j] = T(0.0f);
             }
         }
-        last = lane < rest ? float(row[whole * V + lane]) : 0.0f;
+        last = w.last >= 0 ? float(row[w.last]) : 0.0f;
     }
-    __device__ __forceinline__ void store(T* row, int whole, int rest, int lane) const {
+    __device__ __forceinline__ void store(T* row, const Span& w, int lane) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (i * TEAM + lane < whole) reinterpret_cast<piece_t<T, V>*>(row)[i * TEAM + lane] = piece[i];
-        if (lane < rest) row[whole * V + lane] = T(last);
+            if (i * TEAM + lane < w.whole) *reinterpret_cast<piece_t<T, V>*>(row + w.head + (i * TEAM + lane) * V) = piece[i];
+        if (w.last >= 0) row[w.last] = T(last);
     }
 };
 
@@ -55,30 +55,30 @@ struct Floats {
             for (int j = 0; j < V; ++j) piece[i][j] = x;
         last = x;
     }
-    __device__ __forceinline__ void load(const float* row, int whole, int rest, int lane) {
+    __device__ __forceinline__ void load(const float* row, const Span& w, int lane) {
         fill(0.0f);
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (i * TEAM + lane < whole) {
+            if (i * TEAM + lane < w.whole) {
 #pragma unroll
                 for (int j = 0; j < V; j += 4) {
-                    const piece_t<float, 4> v = *reinterpret_cast<const piece_t<float, 4>*>(row + (i * TEAM + lane) * V + j);
+                    const piece_t<float, 4> v = *reinterpret_cast<const piece_t<float, 4>*>(row + w.head + (i * TEAM + lane) * V + j);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) piece[i][j + k] = v[k];
                 }
             }
-        if (lane < rest) last = row[whole * V + lane];
+        if (w.last >= 0) last = row[w.last];
     }
-    __device__ __forceinline__ void store(float* row, int whole, int rest, int lane) const {
+    __device__ __forceinline__ void store(float* row, const Span& w, int lane) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (i * TEAM + lane < whole) {
+            if (i * TEAM + lane < w.whole) {
 #pragma unroll
                 for (int j = 0; j < V; j += 4)
-                    *reinterpret_cast<piece_t<float, 4>*>(row + (i * TEAM + lane) * V + j) =
+                    *reinterpret_cast<piece_t<float, 4>*>(row + w.head + (i * TEAM + lane) * V + j) =
                         piece_t<float, 4>{piece[i][j], piece[i][j + 1], piece[i][j + 2], piece[i][j + 3]};
             }
-        if (lane < rest) row[whole * V + lane] = last;
+        if (w.last >= 0) row[w.last] = last;
     }
 };
 
@@ -97,21 +97,22 @@ template <typename T, int TEAM, int CH>
 __global__ __launch_bounds__(threads_of(TEAM)) void norm_fwd_kernel(FwdArgs a) {
     constexpr int V = kVec<T>, TEAMS = threads_of(TEAM) / TEAM;
     __shared__ float slots[2][16];
-    const int lane = threadIdx.x % TEAM, whole = a.cols / V, rest = a.cols - whole * V;
+    const int lane = threadIdx.x % TEAM;
     const float n = float(a.cols);
     for (int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / TEAM; row < a.rows; row += int64_t(gridDim.x) * TEAMS) {
         const int64_t at = row * a.cols;
+        const Span p = span_of(static_cast<const T*>(a.x) + at, a.cols, lane);
         Share<T, TEAM, CH> x;
-        x.load(static_cast<const T*>(a.x) + at, whole, rest, lane);
+        x.load(static_cast<const T*>(a.x) + at, p, lane);
         if (a.res) {
             Share<T, TEAM, CH> r;
-            r.load(static_cast<const T*>(a.res) + at, whole, rest, lane);
+            r.load(static_cast<const T*>(a.res) + at, p, lane);
 #pragma unroll
             for (int i = 0; i < CH; ++i)
 #pragma unroll
                 for (int j = 0; j < V; ++j) x.piece[i][j] = T(float(x.piece[i][j]) + float(r.piece[i][j]));
             x.last = float(T(x.last + r.last));
-            x.store(static_cast<T*>(a.sum) + at, whole, rest, lane);
+            x.store(static_cast<T*>(a.sum) + at, p, lane);
         }
         float s = x.last;
 #pragma unroll
@@ -119,11 +120,11 @@ __global__ __launch_bounds__(threads_of(TEAM)) void norm_fwd_kernel(FwdArgs a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) s += float(x.piece[i][j]);
         const float mean = team_sum<TEAM>(s, slots[0]) / n;
-        const float d = lane < rest ? x.last - mean : 0.0f;
+        const float d = p.last >= 0 ? x.last - mean : 0.0f;
         float ss = d * d;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (i * TEAM + lane < whole)
+            if (i * TEAM + lane < p.whole)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float e = float(x.piece[i][j]) - mean;
@@ -135,8 +136,8 @@ __global__ __launch_bounds__(threads_of(TEAM)) void norm_fwd_kernel(FwdArgs a) {
             if (a.rstd) a.rstd[row] = rstd;
         }
         Floats<V, TEAM, CH> w, b;
-        w.load(a.w, whole, rest, lane);
-        if (a.b) b.load(a.b, whole, rest, lane);
+        w.load(a.w, p, lane);
+        if (a.b) b.load(a.b, p, lane);
         else b.fill(0.0f);
 #pragma unroll
         for (int i = 0; i < CH; ++i)
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(threads_of(TEAM)) void norm_fwd_kernel(FwdArgs a) {
             for (int j = 0; j < V; ++j)
                 x.piece[i][j] = T(__builtin_fmaf((float(x.piece[i][j]) - mean) * rstd, w.piece[i][j], b.piece[i][j]));
         x.last = __builtin_fmaf(d * rstd, w.last, b.last);
-        x.store(static_cast<T*>(a.y) + at, whole, rest, lane);
+        x.store(static_cast<T*>(a.y) + at, p, lane);
     }
 }
 
@@ -199,12 +200,17 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
     }
     __shared__ float slots[2][TEAMS][2][TEAM > 64 ? TEAM / 64 : 1];
     __shared__ float held[TEAMS > 1 && !APART ? TEAMS : 1][TEAMS > 1 && !APART ? TEAM * CH * V : 1];
-    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, whole = a.cols / V, rest = a.cols - whole * V;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     const float n = float(a.cols);
     const T *x0 = static_cast<const T*>(a.x), *y0 = static_cast<const T*>(a.dy), *s0 = static_cast<const T*>(a.dsum);
     const int64_t step = int64_t(a.groups) * TEAMS;
+    const int64_t first = int64_t(blockIdx.x) * TEAMS;
+    // A lane's columns stay the same over its rows: where rows of odd lengths follow at odd distances, all have their pieces
+    // from the first element on.
+    const bool even = (step & 1) == 0 || (a.cols & 1) == 0;
+    const Span p = span_of(even ? x0 + (first + team) * a.cols : x0, a.cols, lane);
     Floats<V, TEAM, CH> w, dw, db;
-    w.load(a.w, whole, rest, lane);
+    w.load(a.w, p, lane);
     dw.fill(0.0f);
     db.fill(0.0f);
     Share<T, TEAM, CH> x, y, s;
@@ -212,14 +218,13 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
     const auto load = [&](int64_t row) {
         if (row < a.rows) {
             const int64_t at = row * a.cols;
-            x.load(x0 + at, whole, rest, lane);
-            y.load(y0 + at, whole, rest, lane);
-            if (a.dsum) s.load(s0 + at, whole, rest, lane);
+            x.load(x0 + at, p, lane);
+            y.load(y0 + at, p, lane);
+            if (a.dsum) s.load(s0 + at, p, lane);
             mean = a.mean[row];
             rstd = a.rstd[row];
         }
     };
-    const int64_t first = int64_t(blockIdx.x) * TEAMS;
     if (AHEAD) load(first + team);
     int turn = 0;
     for (int64_t base = first; base < a.rows; base += step, turn ^= 1) {
@@ -240,11 +245,11 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
         if (in) {
 #pragma unroll
             for (int i = 0; i < CH; ++i)
-                if (i * TEAM + lane < whole)
+                if (i * TEAM + lane < p.whole)
 #pragma unroll
                     for (int j = 0; j < V; ++j)
                         term(float(cx.piece[i][j]), float(cy.piece[i][j]), w.piece[i][j], dw.piece[i][j], db.piece[i][j]);
-            if (lane < rest) term(cx.last, cy.last, w.last, dw.last, db.last);
+            if (p.last >= 0) term(cx.last, cy.last, w.last, dw.last, db.last);
         }
         if constexpr (TEAM == 16) {
             s1 = dgm_rows::row16_sum(s1);
@@ -282,7 +287,7 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
             for (int j = 0; j < V; ++j)
                 cx.piece[i][j] = T(slope(float(cx.piece[i][j]), float(cy.piece[i][j]), w.piece[i][j], a.dsum ? float(cs.piece[i][j]) : 0.0f));
         cx.last = slope(cx.last, cy.last, w.last, a.dsum ? cs.last : 0.0f);
-        cx.store(static_cast<T*>(a.dx) + row * a.cols, whole, rest, lane);
+        cx.store(static_cast<T*>(a.dx) + row * a.cols, p, lane);
     }
     if constexpr (APART) return;
     float* part = a.part + int64_t(blockIdx.x) * 2 * a.cols;
@@ -290,10 +295,10 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
     for (int k = 0; k < 2; ++k) {
         const Floats<V, TEAM, CH>& own = k ? db : dw;
         if constexpr (TEAMS == 1) {
-            own.store(part + k * a.cols, whole, rest, lane);
+            own.store(part + k * a.cols, p, lane);
         } else {
             __syncthreads();
-            own.store(held[team], whole, rest, lane);
+            own.store(held[team], p, lane);
             __syncthreads();
             for (int c = threadIdx.x; c < a.cols; c += TEAM * TEAMS) {
                 float sum = held[0][c];

@@ -48,30 +48,30 @@ __device__ __forceinline__ Target target_of(const LossArgs& a, int64_t row, bool
     return r;
 }
 
-// Piece c of a row's gradient from its e^(z - m): k / sum times those, `hot` at the target.
+// A piece of a row's gradient, from column c on, of its e^(z - m): k / sum times those, `hot` at the target.
 template <typename T, int V>
 __device__ __forceinline__ void store_slopes(T* dz, int c, float (&e)[V], float k, const Target& t, float hot) {
     piece_t<T, V> d;
 #pragma unroll
     for (int j = 0; j < V; ++j) e[j] *= k;
-    if (uint32_t(t.at - c * V) < uint32_t(V)) {
+    if (uint32_t(t.at - c) < uint32_t(V)) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) e[j] = c * V + j == t.at ? hot : e[j];
+        for (int j = 0; j < V; ++j) e[j] = c + j == t.at ? hot : e[j];
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = T(e[j]);
-    reinterpret_cast<piece_t<T, V>*>(dz)[c] = d;
+    *reinterpret_cast<piece_t<T, V>*>(dz + c) = d;
 }
 
 // The gradient of a row that counts for nothing, whatever it holds.
 template <typename T, int V>
 __device__ __forceinline__ void store_zeros(T* dz, int cols, int lane, int lanes) {
-    const int whole = cols / V;
+    const Span w = span_of(dz, cols, lane);
     piece_t<T, V> d;
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = T(0.0f);
-    for (int c = lane; c < whole; c += lanes) reinterpret_cast<piece_t<T, V>*>(dz)[c] = d;
-    if (whole * V + lane < cols) dz[whole * V + lane] = T(0.0f);
+    for (int c = lane; c < w.whole; c += lanes) *reinterpret_cast<piece_t<T, V>*>(dz + w.head + c * V) = d;
+    if (w.last >= 0) dz[w.last] = T(0.0f);
 }
 
 template <typename T>
@@ -87,25 +87,26 @@ template <typename T, int TEAM, int CH, int WAVES>
 __global__ __launch_bounds__(threads_of(TEAM), WAVES) void loss_kernel(LossArgs a) {
     constexpr int V = kVec<T>, TEAMS = threads_of(TEAM) / TEAM;
     __shared__ float slots[2][16];
-    const int lane = threadIdx.x % TEAM, whole = a.V / V, rest = a.V - whole * V;
+    const int lane = threadIdx.x % TEAM;
     for (int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / TEAM; row < a.rows; row += int64_t(gridDim.x) * TEAMS) {
         const T* z = static_cast<const T*>(a.z) + row * a.ld;
+        const Span w = span_of(z, a.V, lane);
         piece_t<T, V> x[CH];
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            if (i * TEAM + lane < whole) {
-                x[i] = reinterpret_cast<const piece_t<T, V>*>(z)[i * TEAM + lane];
+            if (i * TEAM + lane < w.whole) {
+                x[i] = *reinterpret_cast<const piece_t<T, V>*>(z + w.head + (i * TEAM + lane) * V);
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) x[i][j] = T(kNegInf);
             }
         }
-        float last = lane < rest ? float(z[whole * V + lane]) : kNegInf;
+        float last = w.last >= 0 ? float(z[w.last]) : kNegInf;
         const Target t = target_of<T>(a, row, lane == 0);
         float m = last;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (i * TEAM < whole)
+            if (i * TEAM < w.whole)
 #pragma unroll
                 for (int j = 0; j < V; ++j) m = fmaxf(m, float(x[i][j]));
         m = team_max<TEAM>(m, slots[0]);
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(threads_of(TEAM), WAVES) void loss_kernel(LossArgs 
         float s = last;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
-            if (i * TEAM < whole)
+            if (i * TEAM < w.whole)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float e = exp_of(float(x[i][j]), m);
@@ -132,14 +133,14 @@ __global__ __launch_bounds__(threads_of(TEAM), WAVES) void loss_kernel(LossArgs 
         const float inv = 1.0f / s, k = t.k * inv, hot = (exp_of(t.z, m) * inv - 1.0f) * t.k;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            if (i * TEAM + lane < whole) {
+            if (i * TEAM + lane < w.whole) {
                 float e[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) e[j] = sizeof(T) == 4 ? float(x[i][j]) : exp_of(float(x[i][j]), m);
-                store_slopes<T, V>(dz, i * TEAM + lane, e, k, t, hot);
+                store_slopes<T, V>(dz, w.head + (i * TEAM + lane) * V, e, k, t, hot);
             }
         }
-        if (lane < rest) dz[whole * V + lane] = T(whole * V + lane == t.at ? hot : last * k);
+        if (w.last >= 0) dz[w.last] = T(w.last == t.at ? hot : last * k);
     }
 }
 
@@ -152,20 +153,21 @@ __global__ __launch_bounds__(1024) void loss_long_kernel(LossArgs a) {
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* z = static_cast<const T*>(a.z) + row * a.ld;
         const Target t = target_of<T>(a, row, threadIdx.x == 0);
-        float m = kNegInf, s = 0.0f;
-        for (int c = threadIdx.x * V; c < a.V; c += 1024 * V) {
-            float x[V];
-            load_piece<V>(z, c, a.V, x, kNegInf);
-            float top = x[0];
+        const Span w = span_of(z, a.V, threadIdx.x);
+        const float last = w.last >= 0 ? float(z[w.last]) : kNegInf;
+        float m = last, s = last == kNegInf ? 0.0f : exp_of(last, m);
+        for (int c = threadIdx.x; c < w.whole; c += 1024) {
+            const piece_t<T, V> x = *reinterpret_cast<const piece_t<T, V>*>(z + w.head + c * V);
+            float top = float(x[0]);
 #pragma unroll
-            for (int j = 1; j < V; ++j) top = fmaxf(top, x[j]);
+            for (int j = 1; j < V; ++j) top = fmaxf(top, float(x[j]));
             if (top > m) {
                 s *= exp_of(m, top);
                 m = top;
             }
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (c + j < a.V && x[j] != kNegInf) s += exp_of(x[j], m);
+                if (float(x[j]) != kNegInf) s += exp_of(float(x[j]), m);
         }
         const float all = team_max<1024>(m, slots[0]);
         s = team_sum<1024>(m == kNegInf ? s : s * exp_of(m, all), slots[1]);
@@ -177,16 +179,14 @@ __global__ __launch_bounds__(1024) void loss_long_kernel(LossArgs a) {
             continue;
         }
         const float inv = 1.0f / s, k = t.k * inv, hot = (exp_of(t.z, all) * inv - 1.0f) * t.k;
-        const int whole = a.V / V, at = whole * V + threadIdx.x;
-        const float last = at < a.V ? float(z[at]) : 0.0f;
-        for (int c = threadIdx.x; c < whole; c += 1024) {
+        for (int c = threadIdx.x; c < w.whole; c += 1024) {
+            const piece_t<T, V> x = *reinterpret_cast<const piece_t<T, V>*>(z + w.head + c * V);
             float e[V];
-            load_piece<V>(z, c * V, a.V, e);
 #pragma unroll
-            for (int j = 0; j < V; ++j) e[j] = exp_of(e[j], all);
-            store_slopes<T, V>(dz, c, e, k, t, hot);
+            for (int j = 0; j < V; ++j) e[j] = exp_of(float(x[j]), all);
+            store_slopes<T, V>(dz, w.head + c * V, e, k, t, hot);
         }
-        if (at < a.V) dz[at] = T(at == t.at ? hot : exp_of(last, all) * k);
+        if (w.last >= 0) dz[w.last] = T(w.last == t.at ? hot : exp_of(last, all) * k);
     }
 }
 
