@@ -196,6 +196,7 @@ PROTOTYPES = {
     "dgm_gpu_destroy": (None, [_P]),
     "dgm_gpu_set_stream": (_I, [_P, _P]),
     "dgm_gpu_stream": (_P, [_P]),
+    "dgm_gpu_device": (_I, [_P]),
     "dgm_set_math": (_I, [_P, _I]),
     "dgm_get_math": (_I, [_P]),
     "dgm_begin": (_I, [_P]),

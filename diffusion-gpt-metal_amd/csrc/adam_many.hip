@@ -342,17 +342,24 @@ int check(dgm_gpu* g, const dgm_adam_tensor* list, int64_t count, int64_t stateB
     return DGM_OK;
 }
 
-// Whether two of the buffers that a step writes overlap (a tensor named twice among them).
-bool overlap(std::vector<std::pair<uintptr_t, uintptr_t>>& spans) {
-    std::sort(spans.begin(), spans.end());
-    for (size_t i = 1; i < spans.size(); ++i)
-        if (spans[i].first < spans[i - 1].second) return true;
+typedef std::vector<std::pair<uintptr_t, uintptr_t>> Spans;
+
+// Whether two of the buffers that a step writes overlap (a tensor named twice among them), or one of them a gradient.
+bool overlap(Spans& written, const Spans& read) {
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].first < written[i - 1].second) return true;
+    for (const auto& r : read) {
+        // Those written lie apart: the last one that begins before r's end is the only one that can reach into r.
+        const auto after = std::lower_bound(written.begin(), written.end(), std::make_pair(r.second, uintptr_t(0)));
+        if (after != written.begin() && std::prev(after)->second > r.first) return true;
+    }
     return false;
 }
 
 int fill_plan(dgm_gpu* g, const dgm_adam_tensor* list, int64_t count, int64_t stateBits, const Sizes& s, void* table) {
     std::vector<uint8_t> host(size_t(s.partials_at()));
-    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    Spans spans, grads;
     Tensor* tensors = reinterpret_cast<Tensor*>(host.data());
     Chunk* chunks = reinterpret_cast<Chunk*>(host.data() + s.tensors * int64_t(sizeof(Tensor)));
     int64_t flat = 0;
@@ -369,6 +376,7 @@ int fill_plan(dgm_gpu* g, const dgm_adam_tensor* list, int64_t count, int64_t st
             spans.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + uintptr_t(bytes));
         };
         span(t.w, 4 * t.n);
+        grads.emplace_back(reinterpret_cast<uintptr_t>(t.grad), reinterpret_cast<uintptr_t>(t.grad) + uintptr_t(4 * t.n));
         span(t.m, eight ? t.n : 4 * t.n);
         span(t.v, eight ? t.n : 4 * t.n);
         if (eight) {
@@ -383,7 +391,7 @@ int fill_plan(dgm_gpu* g, const dgm_adam_tensor* list, int64_t count, int64_t st
         flat += round_up(t.n, kBlock);
         ++at;
     }
-    if (overlap(spans)) return dgm::fail(g, DGM_ERR_ARG, "adamMany: two of the buffers that a step writes overlap");
+    if (overlap(spans, grads)) return dgm::fail(g, DGM_ERR_ARG, "adamMany: two of the buffers that a step writes overlap, or one and a gradient");
     hipError_t err = hipMemcpyAsync(table, host.data(), host.size(), hipMemcpyHostToDevice, g->stream);
     if (err == hipSuccess) err = hipStreamSynchronize(g->stream);
     if (err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "adamMany_plan: %s", hipGetErrorString(err));
@@ -481,7 +489,7 @@ int dgm_adamMany_states(dgm_gpu* g, const dgm_adam_plan* plan, float* m, float* 
     if (rc) return rc;
     if (plan->stateBits != 8) return dgm::fail(g, DGM_ERR_BITS, "adamMany_states: the plan's moments are not in 8 bits");
     if (plan->chunks == 0) return DGM_OK;
-    if (!m || !v) return dgm::fail(g, DGM_ERR_ARG, "adamMany_states: null buffer");
+    if (!m || !v || m == v) return dgm::fail(g, DGM_ERR_ARG, "adamMany_states: null buffer, or one for both");
     if (!dgm::aligned(m, 16) || !dgm::aligned(v, 16)) return dgm::fail(g, DGM_ERR_UNSUPPORTED, "adamMany_states: a buffer is not 16-byte aligned");
     OnDevice on(g->device);
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "adamMany_states: %s", hipGetErrorString(on.err));

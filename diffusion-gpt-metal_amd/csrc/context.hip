@@ -293,6 +293,8 @@ int dgm_gpu_set_stream(dgm_gpu* g, void* hip_stream) {
     return DGM_OK;
 }
 
+int dgm_gpu_device(const dgm_gpu* g) { return g ? g->device : -1; }
+
 void* dgm_gpu_stream(const dgm_gpu* g) { return g ? static_cast<void*>(g->stream) : nullptr; }
 
 int dgm_set_math(dgm_gpu* g, int mode) {

@@ -568,8 +568,8 @@ void by_shape(const dgm_rows_cfg* c, const F& f) {
     else cols_of(c->C) == 4 ? f(__bf16{}, four{}) : f(__bf16{}, one{});
 }
 
-// Waves of `count` units of work fit one launch's bound on threads.
-bool fits(int64_t units) { return units <= int64_t(UINT32_MAX) / 64 - 4; }
+// Whether a workgroup of 256 for each segment and slab is within a launch's bound on threads.
+bool one_launch(const Plan& p) { return p.direct || p.segs * p.slabs <= int64_t(UINT32_MAX) / 256; }
 
 }  // namespace
 
@@ -606,7 +606,8 @@ int dgm_embedRows(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens, c
 
 int64_t dgm_embedRowsBwd_ws_bytes(const dgm_rows_cfg* cfg) {
     if (check(nullptr, "", cfg) != DGM_OK) return -1;
-    return plan_of(cfg).bytes();
+    const Plan p = plan_of(cfg);
+    return one_launch(p) ? p.bytes() : -1;
 }
 
 int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens, const void* dy, float* dtable,
@@ -622,7 +623,7 @@ int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens
         return dgm::fail(g, DGM_ERR_ARG, "embedRowsBwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)p.bytes());
     if (!dgm::aligned(tokens, 4) || !dgm::aligned(dy, size_t(type_bytes(cfg->type))) || !dgm::aligned(dtable, 4) || !dgm::aligned(ws, 16))
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "embedRowsBwd: a buffer is not aligned to its elements, or the workspace to 16 bytes");
-    if (!p.direct && !fits(p.segs * p.slabs * 4))
+    if (!one_launch(p))
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "embedRowsBwd: %lld rows of %lld exceed one launch", (long long)cfg->rows, (long long)cfg->C);
     OnDevice on(g->device);
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "embedRowsBwd: %s", hipGetErrorString(on.err));

@@ -424,6 +424,7 @@ int dgm_layerNormFwd(dgm_gpu* g, const dgm_norm_cfg* cfg, const void* x, const v
     if (cfg->rows == 0) return DGM_OK;
     if (!x || !weight || !y) return dgm::fail(g, DGM_ERR_ARG, "layerNormFwd: null buffer");
     if (!res != !sum) return dgm::fail(g, DGM_ERR_ARG, "layerNormFwd: a residual and its sum go together");
+    if (sum == y || (mean && mean == rstd)) return dgm::fail(g, DGM_ERR_ARG, "layerNormFwd: two results share memory");
     const size_t e = size_t(type_bytes(cfg->type));
     if (!dgm::aligned(x, e) || !dgm::aligned(res, e) || !dgm::aligned(sum, e) || !dgm::aligned(y, e) ||
         !dgm::aligned(weight, 4) || !dgm::aligned(bias, 4) || !dgm::aligned(mean, 4) || !dgm::aligned(rstd, 4))
@@ -456,6 +457,7 @@ int dgm_layerNormBwd(dgm_gpu* g, const dgm_norm_cfg* cfg, const void* x, const f
     if (cfg->rows == 0) return DGM_OK;
     if (!x || !mean || !rstd || !weight || !dy || !dx || (!ws && dgm_layerNormBwd_ws_bytes(cfg) > 0))
         return dgm::fail(g, DGM_ERR_ARG, "layerNormBwd: null buffer");
+    if (dweight && dweight == dbias) return dgm::fail(g, DGM_ERR_ARG, "layerNormBwd: dweight and dbias share memory");
     if (dx == x || dx == dy) return dgm::fail(g, DGM_ERR_ARG, "layerNormBwd: dx may share memory with dsum alone");
     if (ws_bytes < dgm_layerNormBwd_ws_bytes(cfg))
         return dgm::fail(g, DGM_ERR_ARG, "layerNormBwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,

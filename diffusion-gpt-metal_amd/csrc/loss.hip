@@ -229,6 +229,7 @@ extern "C" int dgm_crossEntropy(dgm_gpu* g, const dgm_loss_cfg* cfg, const void*
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "crossEntropy: rows beyond 2^31 - 1 or a row stride beyond 2^30");
     if (cfg->rows == 0 || (!loss && !lse && !dlogits)) return DGM_OK;
     if (!logits || !targets) return dgm::fail(g, DGM_ERR_ARG, "crossEntropy: null buffer");
+    if (loss && loss == lse) return dgm::fail(g, DGM_ERR_ARG, "crossEntropy: loss and lse share memory");
     const size_t e = size_t(type_bytes(cfg->type));
     if (!dgm::aligned(logits, e) || !dgm::aligned(dlogits, e) || !dgm::aligned(targets, 4) || !dgm::aligned(rowScale, 4) ||
         !dgm::aligned(loss, 4) || !dgm::aligned(lse, 4))

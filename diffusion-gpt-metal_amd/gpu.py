@@ -185,6 +185,12 @@ class GPU:
     def stream(self) -> int:
         return self.lib.dgm_gpu_stream(self.h) or 0
 
+    def torch_stream(self):
+        """With it torch works on the context's device and stream: what is allocated and filled there is there for the
+        calls that follow, and memory given back is not handed out again before they are done."""
+        import torch
+        return torch.cuda.stream(torch.cuda.ExternalStream(self.stream, device=self.lib.dgm_gpu_device(self.h)))
+
     def set_math(self, mode: int) -> None:
         self._check(self.lib.dgm_set_math(self.h, mode))
 
@@ -444,7 +450,8 @@ class GPU:
         listed = (AdamTensor * len(tensors))(*tensors)
         size = int(self.lib.dgm_adamMany_plan_bytes(listed, len(tensors), stateBits))
         plan = _AdamPlan()
-        table = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda") if size >= 0 else None
+        with self.torch_stream():
+            table = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda") if size >= 0 else None
         self._check(self.lib.dgm_adamMany_plan(self.h, listed, len(tensors), stateBits, _ptr(table), size, ctypes.byref(plan)))
         plan.held = (table, tuple(tensors))
         return plan

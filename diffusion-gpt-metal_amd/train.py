@@ -106,32 +106,35 @@ class AdamMany:
     once a parameter; with 32-bit moments and without a clip the buffers end up the same bits as optimizer_step's.
 
     state_bits 8 keeps the moments as codes in self.codes, about a quarter of the memory; they start at
-    zero, and the parameters' own m and v are given up (None). Make it again if a
-    parameter's buffers are replaced."""
+    zero, and the parameters' own m and v are given up (None). Its own buffers are made on the
+    context's stream. Make it again if a parameter's buffers are replaced."""
 
     def __init__(self, gpu: GPU, params: Iterable[Param], state_bits: int = 32):
         import torch
         self.gpu, self.params, self.state_bits = gpu, list(params), state_bits
         self.codes, self.rest, tensors = {}, [], []
-        for p in self.params:
-            n, moments = p.count, (p.m, p.v)
-            if state_bits == 8:
-                def buf(count, dtype):
-                    return torch.zeros(max(count, 1), dtype=dtype, device=p.w.device)
-                moments = (buf(n, torch.int8), buf(n, torch.uint8), *(buf(-(-n // 256), torch.float32) for _ in range(2)))
-                self.codes[p.name] = moments
-                moments = tuple(t[:n] for t in moments[:2]) + moments[2:]
-                p.m = p.v = None
-            codes = {}
-            if p.quantized and p.bits != 32:
-                G = p.qGroup
-                if p.cols % G == 0 and 8 <= G <= 512 and G & (G - 1) == 0:
-                    codes = {"q": p.q, "scale": p.scale, "bits": p.bits, "qGroup": G}
-                else:
-                    self.rest.append(p)
-            tensors.append(adam_tensor(p.w[:n], p.g[:n], moments[0][:n], moments[1][:n], *moments[2:], decay=p.decay, **codes))
+        if len({p.name for p in self.params}) < len(self.params):
+            raise ValueError("two parameters have one name")
+        with gpu.torch_stream():
+            self.norm = Buf(2)
+            for p in self.params:
+                n, moments = p.count, (p.m, p.v)
+                if state_bits == 8:
+                    blocks = -(-n // 256)
+                    moments = self.codes[p.name] = [
+                        torch.zeros(max(count, 1), dtype=dtype, device=p.w.device)
+                        for count, dtype in ((n, torch.int8), (n, torch.uint8), (blocks, torch.float32), (blocks, torch.float32))]
+                codes, G = {}, p.qGroup
+                if p.quantized and p.bits != 32:
+                    if p.cols % G == 0 and 8 <= G <= 512 and G & (G - 1) == 0:
+                        codes = {"q": p.q, "scale": p.scale, "bits": p.bits, "qGroup": G}
+                    else:
+                        self.rest.append(p)
+                tensors.append(adam_tensor(p.w[:n], p.g[:n], moments[0][:n], moments[1][:n], *moments[2:], decay=p.decay, **codes))
         self.plan = gpu.adamMany_plan(tensors, state_bits)
-        self.norm = Buf(2)
+        if state_bits == 8:
+            for p in self.params:
+                p.m = p.v = None
 
     def step(self, lr: float, wd: float, clip: float, step_index: int, b1: float = 0.9, b2: float = 0.95,
              eps: float = 1e-8):
@@ -151,7 +154,8 @@ class AdamMany:
         """{name: (m, v)} as fp32 tensors, for a checkpoint (inside an open region; with 8 bits what the codes stand for)."""
         if self.state_bits == 32:
             return {p.name: (p.m, p.v) for p in self.params}
-        m, v = Buf(self.plan.elements), Buf(self.plan.elements)
+        with self.gpu.torch_stream():
+            m, v = Buf(self.plan.elements), Buf(self.plan.elements)
         self.gpu.adamMany_states(self.plan, m, v)
         out, at = {}, 0
         for p in self.params:

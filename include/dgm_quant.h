@@ -94,6 +94,8 @@ void dgm_gpu_destroy(dgm_gpu* g);
  * context's own; NULL restores the context's stream. */
 int dgm_gpu_set_stream(dgm_gpu* g, void* hip_stream);
 void* dgm_gpu_stream(const dgm_gpu* g);
+/* The context's device, -1 without one. */
+int dgm_gpu_device(const dgm_gpu* g);
 int dgm_set_math(dgm_gpu* g, int mode);
 int dgm_get_math(const dgm_gpu* g);
 
@@ -569,7 +571,8 @@ int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, cons
  * out, and the context's next dgm_end returns DGM_ERR_SHAPE. Outputs must not overlap
  * inputs or one another unless said so. Nothing is allocated, every call but
  * dgm_adamMany_plan can be captured, and results are the same bits every time. Calls that
- * overlap in time need a workspace each. DGM_ERR_UNSUPPORTED for sizes beyond those named. */
+ * overlap in time need a workspace each. DGM_ERR_UNSUPPORTED for sizes beyond those named, and
+ * where one launch cannot hold the work. */
 
 typedef struct dgm_norm_cfg {
     int32_t type;                  /* DGM_TYPE_* of the rows                    */
@@ -631,7 +634,8 @@ int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens
  * [ceil(n / 256)]), and where its linear reads codes, those and their scales
  * (bits 8 or 4 as in dgm_quantize of rows of whole groups; qGroup a power of two from 8 to 512; bits 0:
  * none). A moment in 8 bits is c |c| mscale (c = -127 .. 127) or (c^2 vscale)^2
- * (c = 0 .. 255), and all zeros stand for zeros. */
+ * (c = 0 .. 255), and all zeros stand for zeros; an infinity or NaN among 256 makes their
+ * scale, and so all their moments from then on, NaN. */
 typedef struct dgm_adam_tensor {
     float* w;
     const float* grad;
@@ -653,7 +657,7 @@ typedef struct dgm_adam_plan {     /* filled in by dgm_adamMany_plan            
  * calls below, in `table`: device memory of at least dgm_adamMany_plan_bytes bytes
  * (-1 for a list that is refused), kept as long as the plan is used. stateBits: 32 or 8. Waits for
  * the context's stream; not during a graph capture (DGM_ERR_UNSUPPORTED). DGM_ERR_ARG where
- * buffers that a step writes overlap (a tensor named twice). Needs no open region. */
+ * buffers that a step writes overlap (a tensor named twice), or one and a gradient. Needs no open region. */
 int64_t dgm_adamMany_plan_bytes(const dgm_adam_tensor* tensors, int64_t count, int64_t stateBits);
 int dgm_adamMany_plan(dgm_gpu* g, const dgm_adam_tensor* tensors, int64_t count, int64_t stateBits, void* table,
                       int64_t bytes, dgm_adam_plan* plan);

@@ -297,6 +297,28 @@ def test_many_tensors(dgm, gpu, torch_cuda):
 
 
 @pytest.mark.parametrize("state", [32, 8])
+def test_offsets_beyond_32_bits(dgm, gpu, torch_cuda, state):
+    """The last elements of a tensor of more than 2^31 are those of a small one."""
+    n, few = (1 << 31) + 2048 + 77, 2048 + 77
+    small = Tensors(dgm, [few], [0], state=state)
+    t = small.list[0]
+    big = {k: torch.zeros(n if t[k].numel() == few else -(-n // 256), dtype=t[k].dtype, device="cuda") for k in t if isinstance(t[k], torch.Tensor)}
+    for k, x in big.items():
+        x[-t[k].numel():] = t[k]
+    plan = gpu.adamMany_plan([dgm.adam_tensor(big["w"], big["g"], big["m"], big["v"], big.get("ms"), big.get("vs"), decay=True)], state)
+    one = gpu.adamMany_plan(small.tensors(), state)
+    out = torch.zeros(2, 2, device="cuda")
+    gpu.begin()
+    for i, p in enumerate((plan, one)):
+        gpu.adamMany_norm(p, 0.25, out[i])
+        gpu.adamMany(p, **HYPER, factor=out[i, 1:])
+    gpu.end()
+    assert torch.equal(out[0], out[1])
+    assert all(torch.equal(x[-t[k].numel():], t[k]) for k, x in big.items())
+    assert not big["w"][:1000].any()
+
+
+@pytest.mark.parametrize("state", [32, 8])
 def test_graphs(dgm, gpu, torch_cuda, state):
     s, other = (Tensors(dgm, SIZES, [0, 1], state=state) for _ in range(2))
     side = torch.cuda.Stream()
@@ -368,7 +390,10 @@ def test_refusals(dgm, gpu, torch_cuda):
     refused(dgm.DGM_ERR_ARG, [tensor(), tensor()])                      # named twice
     refused(dgm.DGM_ERR_ARG, [tensor(m=at + 2044)])                     # m begins inside w
     refused(dgm.DGM_ERR_ARG, [tensor(bits=8, qGroup=8, q=at + 12288 + 2040)])
+    refused(dgm.DGM_ERR_ARG, [tensor(grad=at + 2044)])                  # a gradient that a step would write to
+    refused(dgm.DGM_ERR_ARG, [tensor(), tensor(w=at + 32768, grad=at + 8192 - 4, m=at + 36864, v=at + 40960)])
     gpu.adamMany_plan([tensor(m=at + 2048)])                            # next to it
+    gpu.adamMany_plan([tensor(), tensor(w=at + 32768, m=at + 36864, v=at + 40960)])     # one gradient for two
     with pytest.raises(dgm.DgmError):
         gpu.end()
     plan = gpu.adamMany_plan([tensor()])
@@ -379,6 +404,13 @@ def test_refusals(dgm, gpu, torch_cuda):
             call()
         with pytest.raises(dgm.DgmError):
             gpu.end()
+    gpu.begin()
+    with pytest.raises(dgm.DgmError):
+        gpu.adamMany_states(gpu.adamMany_plan([eight()], 8), base, base)
+    with pytest.raises(dgm.DgmError):
+        gpu.end()
+    with pytest.raises(ValueError, match="one name"):
+        dgm.AdamMany(gpu, [dgm.Param("a", 2, 8, False, True, 4, 8) for _ in range(2)])
     with pytest.raises(TypeError, match="m must be torch.float32"):
         dgm.adam_tensor(base, base, base.to(torch.int8), base, decay=True)
     with pytest.raises(ValueError, match="v holds"):

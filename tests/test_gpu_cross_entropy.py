@@ -189,6 +189,28 @@ def test_gradient_against_differences(dgm, gpu, torch_cuda, V):
     assert abs(diff - slope) <= abs(wide - diff) + (eu + ed) / (2 * h) + 4 * ref.U * (s["dz"].double() * d.double()).abs().sum().item()
 
 
+@pytest.mark.parametrize("rows,V", [(70000, 32003), (15000, 150001), (20000000, 130)])
+def test_offsets_beyond_32_bits(dgm, gpu, torch_cuda, rows, V):
+    """The last rows of more than 2^31 logits are those of a call on them alone."""
+    s = make(5, V, BF16, 8)
+    z = torch.zeros(rows, V, dtype=BF16, device="cuda")
+    z[-5:] = s["z"]
+    t = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    t[-5:] = s["targets"]
+    dz, loss, lse = torch.ones_like(z), torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    cfg, few = (dgm.LossCfg(type=dgm.DGM_TYPE_BF16, scale=0.5, rows=n, V=V) for n in (rows, 5))
+    gpu.begin()
+    gpu.crossEntropy(few, s["z"], s["targets"], s["loss"], None, s["lse"], s["dz"])
+    gpu.crossEntropy(cfg, z, t, loss, None, lse, dz)
+    gpu.end()
+    # Rows that lie at odd elements go into pieces elsewhere, and sums of them another way.
+    _, _, want, eloss, else_, edz = ref.cross_entropy(s["z"], s["targets"], 0.5)
+    within(loss[-5:], s["loss"][:5], 2 * eloss)
+    within(lse[-5:], s["lse"][:5], 2 * else_)
+    within(dz[-5:], want, edz, BF16)
+    assert not dz[:100].any() and not dz[-105:-5].any()
+
+
 def test_repeats_streams_and_graphs(dgm, gpu, torch_cuda):
     rows, V = 300, 5003
     s = make(rows, V, BF16, 4)
@@ -245,6 +267,7 @@ def test_refusals(dgm, gpu, torch_cuda):
     refused(dgm.DGM_ERR_UNSUPPORTED, dict(ld=(1 << 30) + 1))
     for k in ("z", "targets"):
         refused(dgm.DGM_ERR_ARG, **{k: None})
+    refused(dgm.DGM_ERR_ARG, lse=addr["loss"])
     for k in addr:
         refused(dgm.DGM_ERR_UNSUPPORTED, **{k: addr[k] + 2})
     gpu.begin()

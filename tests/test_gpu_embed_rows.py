@@ -180,6 +180,40 @@ def test_lookup_and_gradient_are_adjoint(dgm, gpu, torch_cuda):
     assert abs(a.sum() - b.sum()) <= (ref.U * a.abs()).sum() + (err * w.double().abs()).sum()
 
 
+def test_offsets_beyond_32_bits(dgm, gpu, torch_cuda):
+    """Rows of a table and of a batch of more than 2^31 elements."""
+    V, C = 524300, 4100
+    table = torch.zeros(V, C, dtype=BF16, device="cuda")
+    dtable = torch.ones(V, C, device="cuda")
+    t = torch.tensor([V - 1, 3, V - 2, V - 1], dtype=torch.int32, device="cuda")
+    table[t.long()] = torch.randn(4, C, device="cuda").bfloat16()
+    table[V - 1] = 2.5
+    dy, y = torch.randint(-9, 9, (4, C), device="cuda").float(), torch.zeros(4, C, device="cuda")
+    cfg = rows_cfg(dgm, F32, 4, C, V, 2.0, BF16)
+    gpu.begin()
+    gpu.embedRows(cfg, t, table, y)
+    backward(dgm, gpu, cfg, t, dy, dtable, False)
+    assert torch.equal(y, 2 * table[t.long()].float())
+    assert torch.equal(dtable[V - 1], 2 * (dy[0] + dy[3])) and torch.equal(dtable[V - 2], 2 * dy[2]) and torch.equal(dtable[3], 2 * dy[1])
+    assert not dtable[V - 1000:V - 2].any() and not dtable[:3].any()
+    gpu.end()
+    del dtable, table
+    rows, C = 2100000, 1030
+    t = torch.full((rows,), 5, dtype=torch.int32, device="cuda")
+    t[-7:] = torch.arange(7, device="cuda")
+    dy = torch.zeros(rows, C, dtype=BF16, device="cuda")
+    dy[-7:] = torch.randint(-9, 9, (7, C), device="cuda").bfloat16()
+    dy[17] = 64
+    dtable = torch.zeros(3000, C, device="cuda")
+    cfg = rows_cfg(dgm, BF16, rows, C, 3000, 1.0)
+    gpu.begin()
+    backward(dgm, gpu, cfg, t, dy, dtable, False)
+    gpu.embedRows(cfg, t, dtable, dy)
+    gpu.end()
+    assert torch.equal(dy[-7:].float(), dtable[:7]) and torch.equal(dy[1].float(), dtable[5]) and not dtable[7:].any()
+    assert (dtable[5] >= 64 - 9).all() and (dtable[5] <= 64 + 9).all()
+
+
 def test_repeats_streams_and_graphs(dgm, gpu, torch_cuda):
     rows, C, V = 6000, 65, 1000
     side = torch.cuda.Stream()

@@ -197,6 +197,34 @@ def test_gradient_against_differences(dgm, gpu, torch_cuda, cols):
     assert abs(diff - slope) <= abs(wide - diff) + (eu + ed) / (2 * h)
 
 
+@pytest.mark.parametrize("cols,rows", [(16384, 131080), (200, 10737500)])
+def test_offsets_beyond_32_bits(dgm, gpu, torch_cuda, cols, rows):
+    """The last rows of more than 2^31 elements are those of a call on them alone, and the sums of all rows count them."""
+    s = make(4, cols, BF16, 2)
+    x, dy = (torch.zeros(rows, cols, dtype=BF16, device="cuda") for _ in range(2))
+    x[-4:], dy[-4:] = s["x"], s["dy"]
+    y, dx = torch.zeros_like(x), torch.zeros_like(x)
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    cfg, few = (dgm.NormCfg(type=dgm.DGM_TYPE_BF16, eps=EPS, rows=n, cols=cols) for n in (rows, 4))
+    s["dw"].zero_()
+    s["db"].zero_()
+    gpu.begin()
+    gpu.layerNormFwd(few, s["x"], None, s["w"], s["b"], None, s["y"], s["mean"], s["rstd"])
+    gpu.layerNormFwd(cfg, x, None, s["w"], s["b"], None, y, mean, rstd)
+    backward(gpu, few, s, s["x"], None)
+    dw, db = s["dw"].clone(), s["db"].clone()
+    assert torch.equal(y[-4:], s["y"]) and torch.equal(mean[-4:], s["mean"]) and torch.equal(rstd[-4:], s["rstd"])
+    whole = {**s, "mean": mean, "rstd": rstd, "dy": dy, "dx": dx}
+    s["dw"].zero_()
+    s["db"].zero_()
+    backward(gpu, cfg, whole, x, None)
+    gpu.end()
+    assert torch.equal(dx[-4:], s["dx"]) and not dx[:100].any()
+    _, edw, edb = ref.layer_norm_bwd(s["x"], s["mean"], s["rstd"], s["w"], s["dy"], None, 300)[3:]
+    within(s["dw"], dw, 2 * edw)
+    within(s["db"], db, 2 * edb)
+
+
 def test_repeats_streams_and_graphs(dgm, gpu, torch_cuda):
     """The same bits on a stream of its own, and from every replay of a graph with other rows between."""
     rows, cols = 900, 768
@@ -287,6 +315,9 @@ def test_refusals(dgm, gpu, torch_cuda):
         refused(dgm.DGM_ERR_UNSUPPORTED, cfg(), fwd=None, bwd={k: addr[k] + 2})
     for k in ("x", "dy"):
         refused(dgm.DGM_ERR_ARG, cfg(), fwd=None, bwd={"dx": addr[k]})
+    refused(dgm.DGM_ERR_ARG, cfg(), fwd=None, bwd={"dw": addr["db"]})
+    refused(dgm.DGM_ERR_ARG, cfg(), fwd={"sum": addr["y"]}, bwd=None)
+    refused(dgm.DGM_ERR_ARG, cfg(), fwd={"mean": addr["rstd"]}, bwd=None)
     with pytest.raises(dgm.DgmError) as e:      # no open region
         gpu.layerNormFwd(cfg(), s["x"], None, s["w"], None, None, s["y"])
     assert e.value.code == dgm.DGM_ERR_NOT_BEGUN

@@ -116,7 +116,8 @@ def test_sizes_that_are_refused(dgm):
     assert emb(rows=5000) > 0 and emb() == 0                        # few tokens of a small vocabulary: no sort
     assert all(emb(**o) == -1 for o in (dict(type=2), dict(tableType=-1), dict(rows=-1), dict(C=0), dict(V=0), dict(V=1 << 31),
                                         dict(rows=(1 << 30) + 1), dict(C=(1 << 24) + 1), dict(scale=float("inf"))))
-    assert emb(rows=1 << 30, C=1 << 24) > 1 << 50        # no overflow on the way
+    assert emb(rows=1 << 30, C=1 << 24) == -1 and emb(rows=(1 << 30) - 64, C=4) > 1 << 33       # more than one launch; no overflow on the way
+    assert lib.dgm_gpu_device(None) == -1
     one = dgm.AdamTensor(w=4096, grad=8192, m=12288, v=16384, n=2048, decay=1)
     plan = lambda bits, t=one, n=1: lib.dgm_adamMany_plan_bytes(by(t), n, bits)
     assert plan(32) > 0 and plan(8) == -1 and plan(16) == -1 and plan(32, n=-1) == -1
