@@ -55,7 +55,7 @@ __device__ __forceinline__ void store_piece(T* row, int c, int cols, const float
 }
 
 // A row of `cols` elements as whole pieces, from its first element at a multiple of 4 bytes on (pieces at
-// odd multiples of 2 take more cycles: 8192 bf16 rows of 50257 logits 357 us that way, 320 this), and the up to 8 elements
+// odd multiples of 2 take more cycles: 8192 bf16 rows of 50257 logits 356 us that way, 304 this), and the up to 8 elements
 // before and behind those, one to a lane.
 struct Span {
     int head, whole, last;   // elements before the pieces; pieces; this lane's single element, -1 for none

@@ -623,7 +623,7 @@ typedef struct dgm_rows_cfg {
 int dgm_embedRows(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens, const void* table, void* y);
 /* dtable[v, :] = scale * the sum of dy[r, :] over the rows of token v, zeros for a token without rows;
  * accumulate != 0: added to dtable, whose other rows are not touched. The sums are
- * fp32, over a token's rows in their order, 64 of the sorted rows at a time. ws: at least dgm_embedRowsBwd_ws_bytes(cfg)
+ * fp32, over a token's rows in a fixed order. ws: at least dgm_embedRowsBwd_ws_bytes(cfg)
  * bytes (-1 for sizes that are refused). */
 int64_t dgm_embedRowsBwd_ws_bytes(const dgm_rows_cfg* cfg);
 int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens, const void* dy, float* dtable,
