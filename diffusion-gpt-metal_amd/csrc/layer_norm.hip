@@ -11,6 +11,10 @@
 
 #include "step.hpp"
 
+// Products are fused into sums where it is written: g, which is added up and then less its mean, has to be the same number both
+// times (the gradient of a row of one element is 0).
+#pragma clang fp contract(off)
+
 namespace {
 
 using namespace dgm_step;
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
         s2 /= n;
         const auto slope = [&](float xv, float yv, float wv, float sv) {
             const float xh = (xv - cmean) * crstd;
-            return sv + crstd * (yv * wv - s1 - xh * s2);
+            return __builtin_fmaf(crstd, __builtin_fmaf(-xh, s2, yv * wv - s1), sv);
         };
 #pragma unroll
         for (int i = 0; i < CH; ++i)

@@ -95,6 +95,13 @@ def _rows(t: Any, kind: Any, count: int, what: str) -> Optional[int]:
     return p
 
 
+def _strided(t: Any, kind: Any, rows: int, cols: int, ld: int, what: str) -> Optional[int]:
+    """_rows of `rows` rows of `cols` elements, `ld` apart; or a view of such rows, [rows, cols] with that stride."""
+    if (isinstance(t, kind) and t.dim() == 2 and t.stride() == (ld, 1) and t.shape[0] >= rows and t.shape[1] >= cols):
+        return t.data_ptr()
+    return _rows(t, kind, (rows - 1) * ld + cols if rows > 0 else 0, what)
+
+
 def _bytes(ws: Any, nbytes: int) -> Optional[int]:
     """_ptr of a workspace that is said to have nbytes."""
     p = _ptr(ws)
@@ -418,13 +425,13 @@ class GPU:
             _rows(dbias, _F32, cfg.cols, "dbias"), _bytes(ws, ws_bytes), ws_bytes))
 
     def crossEntropy(self, cfg: LossCfg, logits, targets, loss, rowScale=None, lse=None, dlogits=None) -> None:
-        """Cross-entropy of logits [rows, V] with int32 targets (negative: the row does not count), and its gradient."""
-        el, rows = _elements(cfg.type), cfg.rows
-        n = (rows - 1) * (cfg.ld or cfg.V) + cfg.V if rows > 0 else 0
+        """Cross-entropy of logits [rows, V] (row stride cfg.ld) with int32 targets (negative: the row does not count), and its
+        gradient."""
+        el, rows, V, ld = _elements(cfg.type), cfg.rows, cfg.V, cfg.ld or cfg.V
         self._check(self.lib.dgm_crossEntropy(
-            self.h, ctypes.byref(cfg), _rows(logits, el, n, "logits"), _rows(targets, _I32, rows, "targets"),
+            self.h, ctypes.byref(cfg), _strided(logits, el, rows, V, ld, "logits"), _rows(targets, _I32, rows, "targets"),
             _rows(rowScale, _F32, rows, "rowScale"), _rows(loss, _F32, rows, "loss"),
-            _rows(lse, _F32, rows, "lse"), _rows(dlogits, el, n, "dlogits")))
+            _rows(lse, _F32, rows, "lse"), _strided(dlogits, el, rows, V, ld, "dlogits")))
 
     def embedRows(self, cfg: RowsCfg, tokens, table, y) -> None:
         """y[r] = scale * table[tokens[r]]; tokens int32, -1 for none."""

@@ -155,6 +155,18 @@ def test_equal_elements_and_large_means(dgm, gpu, torch_cuda):
     within(s["y"][2:], y[2:], err[2:])
 
 
+@pytest.mark.parametrize("rows", [1, 77, 5000])
+def test_rows_of_one_element(dgm, gpu, torch_cuda, rows):
+    """The norm of one element is the bias, its gradient exactly 0 however the products round."""
+    s = make(rows, 1, F32, rows)
+    cfg = dgm.NormCfg(type=dgm.DGM_TYPE_F32, eps=EPS, rows=rows, cols=1)
+    gpu.begin()
+    gpu.layerNormFwd(cfg, s["x"], None, s["w"], s["b"], None, s["y"], s["mean"], s["rstd"])
+    backward(gpu, cfg, s, s["x"], None)
+    gpu.end()
+    assert (s["y"] == s["b"]).all() and (s["dx"] == 0).all()
+
+
 def test_no_rows(dgm, gpu, torch_cuda):
     s = make(2, 64, F32)
     cfg = dgm.NormCfg(type=dgm.DGM_TYPE_F32, eps=EPS, rows=0, cols=64)

@@ -185,3 +185,34 @@ def test_the_first_call_of_a_process_looks_at_types(name):
     from conftest import REPO
     done = subprocess.run([sys.executable, "-c", FIRST, name], cwd=REPO, capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stderr
+
+
+def test_views_of_logits(g, dgm, monkeypatch):
+    """Rows of a padded vocabulary may be passed as a view; one with another stride, or too small, is refused."""
+    from dgm_amd import gpu as module
+    z = torch.zeros(3, 10)
+    monkeypatch.setattr(module, "_elements", lambda code: torch.Tensor)
+    monkeypatch.setattr(module, "_typed", lambda t, kind, what: t if t is None or isinstance(t, int) else t.data_ptr())
+    cfg = dgm.LossCfg(type=dgm.DGM_TYPE_F32, scale=1.0, rows=3, V=7, ld=10)
+    g.crossEntropy(cfg, z[:, :7], 4096, 8192, dlogits=z)
+    assert g.lib.calls[0][1][2] == z.data_ptr()
+    for bad in (z[:, :6], z[:2, :7], torch.zeros(3, 11)[:, :7], torch.zeros(10, 3).t()):
+        with pytest.raises(ValueError, match="^logits"):
+            g.crossEntropy(cfg, bad, 4096, 8192)
+    assert len(g.lib.calls) == 1
+
+
+def test_structures_are_the_header_s(dgm, tmp_path):
+    import ctypes
+    import os
+    import subprocess
+
+    from conftest import REPO
+    lines = ["#include <stddef.h>", '#include "dgm_quant.h"']
+    for name, cls in (("dgm_norm_cfg", dgm.NormCfg), ("dgm_loss_cfg", dgm.LossCfg), ("dgm_rows_cfg", dgm.RowsCfg),
+                      ("dgm_adam_tensor", dgm.AdamTensor), ("dgm_adam_plan", dgm.AdamPlan)):
+        lines.append(f'_Static_assert(sizeof({name}) == {ctypes.sizeof(cls)}, "{name}");')
+        lines += [f'_Static_assert(offsetof({name}, {f}) == {getattr(cls, f).offset}, "{name}.{f}");' for f, _ in cls._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ["int main(void) { return 0; }"]))
+    subprocess.run(["gcc", "-std=c11", "-fsyntax-only", "-I", os.path.join(REPO, "include"), str(src)], check=True)
