@@ -7,7 +7,7 @@
 // The gradient sorts the tokens (stable, by digits of up to 9 bits), so that a token's rows lie together
 // and each is read once. A unit, one wave, adds up a segment of the sorted rows in 256 columns; runs within its
 // segment it writes, what crosses a segment's end it leaves in the workspace, and a last launch joins those in
-// the order of the rows. Few tokens of a small vocabulary are not sorted: a workgroup for each vocabulary row looks
+// the order of the rows. Few tokens, or a few more of a small vocabulary, are not sorted: a workgroup for each looks
 // for its rows itself. Nothing is added to by two workgroups: no atomics on results, the same bits every time.
 #include <algorithm>
 #include <cmath>
@@ -99,6 +99,10 @@ __device__ void clear(float* p, int64_t n, int64_t thread, int64_t threads) {
     } else {
         for (int64_t i = thread; i < n; i += threads) p[i] = 0.0f;
     }
+}
+
+__global__ __launch_bounds__(256) void embed_clear_kernel(float* p, int64_t n) {
+    clear(p, n, int64_t(blockIdx.x) * 256 + threadIdx.x, int64_t(gridDim.x) * 256);
 }
 
 // Up to kTile rows in one workgroup, by the digits, the lowest first, elements of a digit in their order: behind the
@@ -437,28 +441,37 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a) {
 
 // ---- without a sort ---------------------------------------------------------------------
 
-constexpr int kDirectWaves = 16, kDirectRows = 4096;
+constexpr int kDirectRows = 4096;
 
-// One vocabulary row in 64 N columns. The waves look through a share of the tokens each and list the rows that they
-// find in their order; then each adds up a share of the list. A chain of two loads: 1024 rows of 65 x 128 5.3 us.
-template <typename T, int N>
+// One token in 64 N columns: the token of each vocabulary row, or (BYROW) that of each row that has it first. The waves
+// look through a share of the tokens each and list the rows that they find in their order; then each adds up a share of the
+// list. A chain of two loads: 1024 rows of 65 x 128 5.3 us.
+template <typename T, int N, int kDirectWaves, bool BYROW>
 __global__ __launch_bounds__(64 * kDirectWaves) void embed_direct_kernel(SumArgs a, const uint32_t* __restrict__ tokens, uint32_t* words) {
     __shared__ uint16_t list[kDirectRows];
     __shared__ int found[kDirectWaves];
     __shared__ float sums[kDirectWaves][64 * N];
     constexpr int kTokens = kDirectRows / (64 * kDirectWaves);   // of a lane
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t v = blockIdx.x / a.slabs;
-    const int col = (int(blockIdx.x - v * a.slabs) * 64 + lane) * N, c = std::min(col, a.C - N);
+    const uint32_t which = blockIdx.x / a.slabs, v = BYROW ? tokens[which] : which;
+    const int col = (int(blockIdx.x - which * a.slabs) * 64 + lane) * N, c = std::min(col, a.C - N);
     const bool live = col < a.C;
     const int each = (int(a.n) + 64 * kDirectWaves - 1) / (64 * kDirectWaves);   // batches of 64 tokens of a wave
     uint64_t hits[kTokens];
+    if (BYROW && v >= a.V) {
+        if (v != kNone && threadIdx.x == 0) report(words, kBadTokens);
+        return;
+    }
     int n = 0;
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
+        if (u >= each) {
+            hits[u] = 0;
+            continue;
+        }
         const int i = (wave * each + u) * 64 + lane;
-        const uint32_t t = u < each && i < a.n ? tokens[i] : kNone;
-        if (blockIdx.x == 0 && t >= a.V && t != kNone) report(words, kBadTokens);
+        const uint32_t t = i < a.n ? tokens[i] : kNone;
+        if (!BYROW && blockIdx.x == 0 && t >= a.V && t != kNone) report(words, kBadTokens);
         hits[u] = __ballot(t == v);
         n += __popcll(hits[u]);
     }
@@ -481,6 +494,7 @@ __global__ __launch_bounds__(64 * kDirectWaves) void embed_direct_kernel(SumArgs
     }
     if (all == 0 && a.add) return;
     __syncthreads();
+    if (BYROW && list[0] != which) return;   // a row before has it
     float acc[N] = {};
     const int to = all * (wave + 1) / kDirectWaves;
     for (int i0 = all * wave / kDirectWaves; i0 < to; i0 += kAhead) {
@@ -522,17 +536,17 @@ int check(dgm_gpu* g, const char* name, const dgm_rows_cfg* c) {
     return DGM_OK;
 }
 
-// Workgroups of vocabulary row x columns up to which they look for their rows themselves: each costs about 4.5 ns
-// whether it finds any or not (1024 rows of 65 x 128: 12 us with the lookup, 21 sorted; 4096 rows of 1000 x 256 14.5 and 27; 2000
-// workgroups still even: 4096 rows of 256 x 2048 31.6 and 29.5).
-constexpr int64_t kDirectGroups = 2048;
+// Workgroups of token x columns up to which tokens are not sorted, each workgroup looking for its own (us with the lookup,
+// added): 1000 rows of 50257 x 512, 2000 workgroups, 11 (sorted 17); 4000 rows of 50257 x 512, 8000, 30 (sorted 26). Up to
+// kWideGroups of them have 16 waves: 4000 rows of 200 x 512 18 (22 with four); 2000 workgroups 15 with sixteen.
+constexpr int64_t kDirectGroups = 2048, kWideGroups = 512;
 
 // What the gradient's launches need of a configuration.
 struct Plan {
     int passes, bits, blocks;
     int64_t per, segs;
     int slabs, seg;
-    bool direct;
+    bool direct, byrow;
     int64_t lists, hist, parts;   // bytes of the workspace's areas
     int64_t bytes() const { return lists + hist + parts; }
 };
@@ -541,7 +555,9 @@ Plan plan_of(const dgm_rows_cfg* c) {
     Plan p;
     const int64_t wide = 64 * cols_of(c->C);
     p.slabs = int((c->C + wide - 1) / wide);
-    p.direct = c->rows > 0 && c->rows <= kDirectRows && c->V <= kDirectGroups && c->V * p.slabs <= kDirectGroups;
+    const int64_t keys = std::min(c->V, c->rows);
+    p.byrow = c->rows < c->V;
+    p.direct = c->rows > 0 && c->rows <= kDirectRows && keys * p.slabs <= kDirectGroups;
     if (p.direct) {
         p.lists = p.hist = p.parts = 0;
         return p;
@@ -634,9 +650,22 @@ int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens
     SumArgs a{dy, nullptr, nullptr, dtable, nullptr, nullptr, cfg->rows, uint32_t(cfg->V), int(cfg->C), p.slabs, accumulate ? 1 : 0,
               0, 0, cfg->scale};
     if (p.direct) {
-        const dim3 grid(unsigned(cfg->V) * unsigned(p.slabs)), block(64 * kDirectWaves);
+        const dim3 grid(unsigned(p.byrow ? cfg->rows : cfg->V) * unsigned(p.slabs));
+        if (p.byrow && !accumulate) {
+            const int64_t n = cfg->V * cfg->C;
+            embed_clear_kernel<<<dim3(unsigned(std::min<int64_t>((n + 4095) / 4096, 2048))), dim3(256), 0, g->stream>>>(dtable, n);
+            DGM_LAUNCH_CHECK(g, "embed_clear");
+        }
         by_shape(cfg, [&](auto t, auto n) {
-            embed_direct_kernel<decltype(t), decltype(n)::value><<<grid, block, 0, g->stream>>>(a, tokens, g->seq_report);
+            constexpr int N = decltype(n)::value;
+            using T = decltype(t);
+            if (grid.x <= kWideGroups) {
+                if (p.byrow) embed_direct_kernel<T, N, 16, true><<<grid, dim3(1024), 0, g->stream>>>(a, tokens, g->seq_report);
+                else embed_direct_kernel<T, N, 16, false><<<grid, dim3(1024), 0, g->stream>>>(a, tokens, g->seq_report);
+            } else {
+                if (p.byrow) embed_direct_kernel<T, N, 4, true><<<grid, dim3(256), 0, g->stream>>>(a, tokens, g->seq_report);
+                else embed_direct_kernel<T, N, 4, false><<<grid, dim3(256), 0, g->stream>>>(a, tokens, g->seq_report);
+            }
         });
         DGM_LAUNCH_CHECK(g, "embed_direct");
         return DGM_OK;

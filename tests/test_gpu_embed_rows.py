@@ -53,12 +53,13 @@ def backward(dgm, gpu, cfg, t, dy, dtable, add):
     assert (ws[size:] == 0x7F).all()
 
 
-# With and without a sort (up to 4096 rows, vocabulary x columns / 256 up to 2048), by one workgroup (4096 rows) or several;
+# Without a sort by the vocabulary's rows or by the batch's (up to 4096 rows, the fewer of them x columns / 256 up to 2048; 512 with
+# wide workgroups), sorted by one workgroup (4096 rows) or several;
 # digits of up to 9 bits (V of 511, 512: one pass or two); segments of 8 to 64 sorted rows.
 SIZES = [(1, 1, 1), (2, 5, 1), (63, 7, 3), (64, 8, 3), (65, 33, 4), (130, 260, 1), (1000, 20, 65), (4096, 12, 511), (4097, 12, 512),
          (5000, 130, 40), (9000, 9, 50257), (20000, 4, 2), (3000, 515, 200), (300, 2050, 31), (70000, 3, 262143), (70001, 3, 262144),
          (33, 64, 2 ** 27), (1, 9, 5000), (1025, 5, 3000), (2500, 260, 5000), (4096, 12, 70000), (3500, 8, 2 ** 24), (4100, 4096, 2000),
-         (30000, 1028, 300)]
+         (30000, 1028, 300), (511, 9, 700), (2047, 8, 5000), (2048, 33, 2049), (700, 700, 800), (1500, 300, 1000), (4096, 12, 2049)]
 
 
 @pytest.mark.parametrize("add", [False, True])
@@ -124,7 +125,7 @@ def test_order_of_a_token_s_rows(dgm, gpu, torch_cuda):
     assert dtable[4, 0] == 2.0 ** 24 + 2 and dtable[9, 0] == 5
 
 
-@pytest.mark.parametrize("rows,V", [(100, 65), (5000, 300), (5000, 70000)])
+@pytest.mark.parametrize("rows,V", [(100, 65), (100, 70000), (3000, 70000), (5000, 300), (5000, 70000)])
 def test_tokens_beyond_the_vocabulary(dgm, gpu, torch_cuda, rows, V):
     C = 24
     t = text(rows, V, 5)
@@ -277,10 +278,10 @@ def test_refusals(dgm, gpu, torch_cuda):
     for k in ("tokens", "table", "y"):
         refused(dgm.DGM_ERR_ARG, which="lookup", **{k: None})
         refused(dgm.DGM_ERR_UNSUPPORTED, which="lookup", **{k: addr[k] + 2})
-    large = dict(V=1 << 22)         # too many vocabulary rows for each to look for its tokens: those are sorted, in a workspace
+    large = dict(rows=5000, V=1 << 22)         # too many for each to look for its own: they are sorted, in a workspace
     for k in ("tokens", "dy", "dtable", "ws"):
-        refused(dgm.DGM_ERR_ARG, large, which="gradient", **{k: None})
-        refused(dgm.DGM_ERR_UNSUPPORTED, large, which="gradient", **{k: addr[k] + 2})
-    c = dgm.RowsCfg(type=0, tableType=0, scale=1.0, rows=4, C=8, V=1 << 22)
+        refused(dgm.DGM_ERR_ARG, large, which="gradient", ws_bytes=1 << 20, **{k: None})
+        refused(dgm.DGM_ERR_UNSUPPORTED, large, which="gradient", ws_bytes=1 << 20, **{k: addr[k] + 2})
+    c = dgm.RowsCfg(type=0, tableType=0, scale=1.0, rows=5000, C=8, V=1 << 22)
     refused(dgm.DGM_ERR_ARG, large, which="gradient", ws_bytes=gpu.embedRowsBwd_ws_bytes(c) - 1)
     refused(dgm.DGM_ERR_UNSUPPORTED, dict(rows=1 << 30, C=1 << 24), which="gradient", ws_bytes=1 << 62)
