@@ -146,14 +146,15 @@ __global__ __launch_bounds__(threads_of(TEAM), WAVES) void loss_kernel(LossArgs 
 }
 
 // Rows beyond what a workgroup's registers hold: the maximum and the sum that
-// belongs to it in one pass, the gradient in a second, from the cache where the row is still there.
+// belongs to it in one pass, the gradient in a second, from the cache where the row is still there. Workgroups of one
+// row (grid's y) share the second.
 template <typename T>
-__global__ __launch_bounds__(1024) void loss_long_kernel(LossArgs a) {
+__global__ __launch_bounds__(1024, 8) void loss_long_kernel(LossArgs a) {
     constexpr int V = kVec<T>;
     __shared__ float slots[2][16];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* z = static_cast<const T*>(a.z) + row * a.ld;
-        const Target t = target_of<T>(a, row, threadIdx.x == 0);
+        const Target t = target_of<T>(a, row, blockIdx.y == 0 && threadIdx.x == 0);
         const Span w = span_of(z, a.V, threadIdx.x);
         const float last = w.last >= 0 ? float(z[w.last]) : kNegInf;
         float m = last, s = last == kNegInf ? 0.0f : exp_of(last, m);
@@ -166,28 +167,29 @@ __global__ __launch_bounds__(1024) void loss_long_kernel(LossArgs a) {
                 s *= exp_of(m, top);
                 m = top;
             }
+            const float base = m == kNegInf ? 0.0f : m;   // -inf is e^-inf from any base but itself
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (float(x[j]) != kNegInf) s += exp_of(float(x[j]), m);
+            for (int j = 0; j < V; ++j) s += exp_of(float(x[j]), base);
         }
         const float all = team_max<1024>(m, slots[0]);
         s = team_sum<1024>(m == kNegInf ? s : s * exp_of(m, all), slots[1]);
-        if (threadIdx.x == 0) store_row<T>(a, row, t, all, s);
+        if (blockIdx.y == 0 && threadIdx.x == 0) store_row<T>(a, row, t, all, s);
         if (!a.dz) continue;
         T* dz = static_cast<T*>(a.dz) + row * a.ld;
         if (t.at < 0) {
-            store_zeros<T, V>(dz, a.V, threadIdx.x, 1024);
+            if (blockIdx.y == 0) store_zeros<T, V>(dz, a.V, threadIdx.x, 1024);
             continue;
         }
         const float inv = 1.0f / s, k = t.k * inv, hot = (exp_of(t.z, all) * inv - 1.0f) * t.k;
-        for (int c = threadIdx.x; c < w.whole; c += 1024) {
+        const int part = int(int64_t(w.whole) * blockIdx.y / gridDim.y), end = int(int64_t(w.whole) * (blockIdx.y + 1) / gridDim.y);
+        for (int c = part + threadIdx.x; c < end; c += 1024) {
             const piece_t<T, V> x = *reinterpret_cast<const piece_t<T, V>*>(z + w.head + c * V);
             float e[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) e[j] = exp_of(float(x[j]), all);
             store_slopes<T, V>(dz, w.head + c * V, e, k, t, hot);
         }
-        if (w.last >= 0) dz[w.last] = T(w.last == t.at ? hot : exp_of(last, all) * k);
+        if (blockIdx.y == 0 && w.last >= 0) dz[w.last] = T(w.last == t.at ? hot : exp_of(last, all) * k);
     }
 }
 
@@ -201,13 +203,21 @@ void launch(dgm_gpu* g, const LossArgs& a) {
     // workgroup), 212 with 512 (two); 8192 bf16 rows of 6282, whose elements are unpacked and raised twice, 356 with
     // 512 and 455 with 1024; 16384 fp32 rows of 2000 192 (512 lanes, 207 with 256), of 250 28 (a wave, 29 with 256); 16384
     // bf16 rows of 937 90 (256 lanes, 102 with 512). Losses alone need no row held: 517 fp32 rows of
-    // 8000 15 in the loop below, 18 in registers. bf16 rows of 16032 228 in registers, 258 in the loop.
+    // 8000 15 in the loop below, 18 in registers; 16384 of 1250 111 and 56. bf16 rows of 16032 228 in registers, 258 in the loop.
+    // Few long rows: workgroups share a row's gradient, each after the whole row's sum (that of one workgroup is bound by its exponentials,
+    // 200,000 fp32 logits 28 us in one, 16 shared; 32 rows of 100,000 20 and 17, 128 of 50,000 12.6 and 13.8). Not where
+    // the gradient replaces the logits, which the others still read.
+    if (a.dz && a.dz != a.z && n > 4096 && a.rows <= 32) {
+        const unsigned parts = unsigned(std::min<int64_t>(dgm::kCus / a.rows, (n + 1023) / 1024));
+        loss_long_kernel<T><<<dim3(unsigned(a.rows), parts), dim3(1024), 0, g->stream>>>(a);
+        return;
+    }
     if (n <= 16) loss_kernel<T, 16, 1, 8><<<blocks(16), dim3(256), 0, g->stream>>>(a);
     else if (n <= 32) loss_kernel<T, 16, 2, 8><<<blocks(16), dim3(256), 0, g->stream>>>(a);
     else if (n <= 128) loss_kernel<T, 64, 2, 8><<<blocks(4), dim3(256), 0, g->stream>>>(a);
     else if (n <= 256) loss_kernel<T, 64, 4, 8><<<blocks(4), dim3(256), 0, g->stream>>>(a);
     else if (n <= 1024) loss_kernel<T, 256, 4, 8><<<blocks(1), dim3(256), 0, g->stream>>>(a);
-    else if (!a.dz || n > 16384) loss_long_kernel<T><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
+    else if ((!a.dz && n > 4096) || n > 16384) loss_long_kernel<T><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
     else if (n <= 2048) loss_kernel<T, 256, 8, 6><<<blocks(1), dim3(256), 0, g->stream>>>(a);
     else if (n <= 4096) loss_kernel<T, 512, 8, 6><<<blocks(1), dim3(512), 0, g->stream>>>(a);
     else if (n <= 8192 && sizeof(T) == 4) loss_kernel<T, 1024, 8, 4><<<blocks(1), dim3(1024), 0, g->stream>>>(a);
