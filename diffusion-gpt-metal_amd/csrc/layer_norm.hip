@@ -12,12 +12,19 @@
 #include "step.hpp"
 
 // Products are fused into sums where it is written: g, which is added up and then less its mean, has to be the same number both
-// times (the gradient of a row of one element is 0).
+// times (the gradient of a row of one element is 0), and in short rows, where dx is what is left of terms that cancel (all but
+// eps / variance of it in rows of two), each operation is rounded on its own. Wide rows: 202 us fused, 213 not (16384 of 4096, bf16).
 #pragma clang fp contract(off)
 
 namespace {
 
 using namespace dgm_step;
+
+// a b + c, fused for rows that a wave or more lanes share.
+template <int TEAM>
+__device__ __forceinline__ float mul_add(float a, float b, float c) {
+    return TEAM > 16 ? __builtin_fmaf(a, b, c) : a * b + c;
+}
 
 // A lane's share of a row: CH whole pieces of 16 bytes as they came, and one of the elements around those. What the
 // row does not have is zeros.
@@ -133,7 +140,7 @@ __global__ __launch_bounds__(threads_of(TEAM)) void norm_fwd_kernel(FwdArgs a) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float e = float(x.piece[i][j]) - mean;
-                    ss = __builtin_fmaf(e, e, ss);
+                    ss = mul_add<TEAM>(e, e, ss);
                 }
         const float rstd = 1.0f / sqrtf(team_sum<TEAM>(ss, slots[1]) / n + a.eps);
         if (lane == 0) {
@@ -148,8 +155,8 @@ __global__ __launch_bounds__(threads_of(TEAM)) void norm_fwd_kernel(FwdArgs a) {
         for (int i = 0; i < CH; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                x.piece[i][j] = T(__builtin_fmaf((float(x.piece[i][j]) - mean) * rstd, w.piece[i][j], b.piece[i][j]));
-        x.last = __builtin_fmaf(d * rstd, w.last, b.last);
+                x.piece[i][j] = T(mul_add<TEAM>((float(x.piece[i][j]) - mean) * rstd, w.piece[i][j], b.piece[i][j]));
+        x.last = mul_add<TEAM>(d * rstd, w.last, b.last);
         x.store(static_cast<T*>(a.y) + at, p, lane);
     }
 }
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
             dwv = __builtin_fmaf(yv, xh, dwv);
             dbv += yv;
             s1 += g;
-            s2 = __builtin_fmaf(g, xh, s2);
+            s2 = mul_add<TEAM>(g, xh, s2);
         };
         if (in) {
 #pragma unroll
@@ -285,7 +292,7 @@ __global__ __launch_bounds__(TEAM* TEAMS, WAVES) void norm_bwd_kernel(BwdArgs a)
         s2 /= n;
         const auto slope = [&](float xv, float yv, float wv, float sv) {
             const float xh = (xv - cmean) * crstd;
-            return __builtin_fmaf(crstd, __builtin_fmaf(-xh, s2, yv * wv - s1), sv);
+            return mul_add<TEAM>(crstd, mul_add<TEAM>(-xh, s2, yv * wv - s1), sv);
         };
 #pragma unroll
         for (int i = 0; i < CH; ++i)
