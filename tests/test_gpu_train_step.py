@@ -167,3 +167,69 @@ def test_steps_as_a_graph(dgm, torch_cuda, state):
     own.end()
     own.close()
     assert losses[2] != losses[0]
+
+
+def test_two_steps_at_once(dgm, torch_cuda):
+    """Two models on two contexts and streams, their steps in flight together: each the bits that it has alone."""
+    def run(together):
+        sides = [torch.cuda.Stream() for _ in range(2)]
+        owns = [dgm.GPU(stream=s) for s in sides]
+        models = [Model(dgm, g, 10 + i) for i, g in enumerate(owns)]
+        opts = [dgm.AdamMany(g, m.params, 8 if i else 32) for i, (g, m) in enumerate(zip(owns, models))]
+        torch.cuda.synchronize()
+        for g, m in zip(owns, models):
+            g.begin()
+            m.quantize()
+        for _ in range(4):
+            for g, m, o in zip(owns, models, opts):
+                m.forward()
+                m.backward()
+                o.step(1e-2, 0.1, 0.5, 1)
+                if not together:
+                    g.end()
+                    g.begin()
+        for g in owns:
+            g.end()
+        out = [[t.clone() for p in m.params for t in (p.w, p.g)] + [m.loss.clone(), m.dx.clone()] for m in models]
+        torch.cuda.synchronize()
+        for g in owns:
+            g.close()
+        return out
+    alone, both = run(False), run(True)
+    assert all(torch.equal(a, b) for x, y in zip(alone, both) for a, b in zip(x, y))
+
+
+def test_replays_report_tokens_and_targets(dgm, torch_cuda):
+    """A captured step that meets a token or target beyond the vocabulary tells the next end() of its context, and once."""
+    side = torch.cuda.Stream()
+    own = dgm.GPU(stream=side)
+    m = Model(dgm, own, 5)
+    torch.cuda.synchronize()
+    own.begin()
+    m.quantize()
+    m.forward()
+    own.end()
+    own.begin()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        own.embedRows(m.rows, m.tokens, m.p["wte"].w, m.x)
+        own.crossEntropy(m.loss_cfg, m.logits, m.targets, m.loss)
+    tokens, targets = m.tokens.clone(), m.targets.clone()
+    for where, what in ((None, None), (m.tokens, V), (None, None), (m.targets, V + 7), (m.tokens, -2), (None, None)):
+        m.tokens.copy_(tokens)
+        m.targets.copy_(targets)
+        if where is not None:
+            where[3] = what
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        if where is None:
+            own.end()
+        else:
+            with pytest.raises(dgm.DgmError, match="beyond the vocabulary") as e:
+                own.end()
+            assert e.value.code == dgm.DGM_ERR_SHAPE
+            assert (m.x[3] == 0).all() if where is m.tokens else m.loss[3] == 0
+        own.begin()
+    own.end()
+    own.close()
