@@ -15,6 +15,16 @@
 // v 255^4 = max v (c + 1/2)^4 (to 2^-53). A hardware root says which border to ask. A v that is not 0 keeps a
 // code of 1 at least, so that no step divides by eps alone. A largest below 2^-120 counts as 0; an infinity or NaN
 // makes its block's scale NaN.
+//
+// Nearest codes alone would hold what moves by less than half a code a step, and for good: with b1 = 0.9 an m of c <= 9
+// without gradients, whose weight then moves on without end, and a v far below its gradients' squares, whose weight's
+// steps stay several times too large. Two codes that stay are therefore moved by one:
+//   m toward 0 where |m| shrank and sm did not, nor grew by over an eighth (that moves the codes' places, so that one
+//     that stays says nothing), c (1 - b1) < 1 (larger codes follow a decay) and v's code times (1 - b2) is below 4. It is
+//     some steps after the last gradient (v decays by rounding to 2 / (1 - b2)), and always where b2 > 0.984. Weights with
+//     gradients keep their nearest codes, which a push at every shrinking would draw toward 0.
+//   v away from 0 where it grew to over 9 - 8 b2 of itself, as by g^2 > 9 v, and rv did not: a step is then soon at most 3 times AdamW's. Nearer ones
+//     keep the nearest code: pushed at every growth, v would end at its largest g^2.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -113,6 +123,28 @@ __device__ __forceinline__ float v_value(int c, float rv) {
     return root * root;
 }
 
+// The bytes of w that are below n (up to 256), as their high bits.
+__device__ __forceinline__ u32x2 bytes_below(u32x2 w, uint32_t n) {
+    constexpr uint32_t kHigh = 0x80808080u;
+    if (n > 128) return (~w | ~((w | kHigh) - (n - 128) * 0x01010101u)) & kHigh;
+    return ~(w | ((w | kHigh) - n * 0x01010101u)) & kHigh;
+}
+
+// Codes from which on none are held: v's (where (c + 1/2)^4 is c^4 times that growth, and two more for roundings; 255 has no
+// next one), v's of moments that are, and those moments' (1 at least).
+struct Held {
+    uint32_t grown, quiet, small;
+    float growth;   // of a v with g^2 = 9 v
+};
+Held held_of(const AdamArgs& a) {
+    Held l{0, 0, 1, std::max(9.0f - 8.0f * a.b2, 1.0f)};
+    const double q = l.growth, n = q > 1.0 ? 0.5 / (std::sqrt(std::sqrt(q)) - 1.0) + 2.0 : 255.0;
+    l.grown = n < 255.0 ? uint32_t(n) : 255;
+    while (l.quiet < 256 && float(l.quiet) * (1.0f - a.b2) < 4.0f) ++l.quiet;
+    while (l.small < 128 && float(l.small) * (1.0f - a.b1) < 1.0f) ++l.small;
+    return l;
+}
+
 // The largest of a block of 32 lanes, as bits: an infinity or NaN is larger than what is finite.
 __device__ __forceinline__ uint32_t block_max(uint32_t x) {
 #pragma unroll
@@ -120,7 +152,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t x) {
     return x;
 }
 
-// Codes of 8 moments of a block whose largest is `top`, and the block's scale.
+// The nearest codes of 8 moments of a block whose largest is `top`, and the block's scale.
 template <bool SECOND>
 __device__ __forceinline__ u32x2 encode(const float (&x)[8], float top, float& scale) {
     constexpr float kMost = SECOND ? 255.0f : 127.0f;
@@ -153,7 +185,7 @@ __device__ __forceinline__ u32x2 encode(const float (&x)[8], float top, float& s
 // Nontemporal accesses were slower by up to 14% (8 bits) or no faster.
 template <int STATE>
 __global__ __launch_bounds__(kThreads) void adam_many_kernel(const Tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
-                                                             const float* __restrict__ factor, AdamArgs a) {
+                                                             const float* __restrict__ factor, AdamArgs a, Held l) {
     const Chunk ch = chunks[blockIdx.x];
     const Tensor t = tensors[ch.tensor];
     const float f = factor ? *factor : 1.0f;
@@ -165,16 +197,20 @@ __global__ __launch_bounds__(kThreads) void adam_many_kernel(const Tensor* __res
     get8(t.w, at, left, vec, w);
     get8(t.g, at, left, vec, g);
     const int64_t block = at / kBlock;
+    u32x2 cm0, cv0;   // what the moments were
+    float sm0, rv0;
     if constexpr (STATE == 32) {
         get8(static_cast<const float*>(t.m), at, left, vec, m);
         get8(static_cast<const float*>(t.v), at, left, vec, v);
     } else {
-        const u32x2 cm = get_codes(t.m, at, left, vec), cv = get_codes(t.v, at, left, vec);
-        const float sm = left > 0 ? ((const gfloat*)t.ms)[block] : 0.0f, rv = left > 0 ? ((const gfloat*)t.vs)[block] : 0.0f;
+        cm0 = get_codes(t.m, at, left, vec);
+        cv0 = get_codes(t.v, at, left, vec);
+        sm0 = left > 0 ? ((const gfloat*)t.ms)[block] : 0.0f;
+        rv0 = left > 0 ? ((const gfloat*)t.vs)[block] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            m[j] = m_value(code_of(cm, j, true), sm);
-            v[j] = v_value(code_of(cv, j, false), rv);
+            m[j] = m_value(code_of(cm0, j, true), sm0);
+            v[j] = v_value(code_of(cv0, j, false), rv0);
         }
     }
     if (factor) {
@@ -199,7 +235,27 @@ __global__ __launch_bounds__(kThreads) void adam_many_kernel(const Tensor* __res
         mm = block_max(mm);
         mv = block_max(mv);
         float sm, rv;
-        const u32x2 cm = encode<false>(m, __uint_as_float(mm), sm), cv = encode<true>(v, __uint_as_float(mv), rv);
+        u32x2 cm = encode<false>(m, __uint_as_float(mm), sm), cv = encode<true>(v, __uint_as_float(mv), rv);
+        // Codes that can be held, of 8 at once; then each of a lane that has some.
+        u32x2 v_held = rv > 0.0f && rv <= rv0 ? bytes_below(cv ^ cv0, 1) & bytes_below(cv, l.grown) : u32x2{0, 0};
+        if (v_held[0] | v_held[1]) {
+            u32x2 up = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) up[j / 4] |= v[j] > l.growth * v_value(code_of(cv, j, false), rv0) ? 1u << (8 * (j & 3)) : 0u;
+            cv += up & (v_held >> 7);
+        }
+        u32x2 m_held = sm >= sm0 && sm <= 1.125f * sm0 ? bytes_below(cm ^ cm0, 1) & bytes_below(cv, l.quiet) : u32x2{0, 0};
+        if (m_held[0] | m_held[1]) {
+            m_held &= bytes_below(cm, l.small) | bytes_below(~cm, l.small - 1);   // c >= 0; |c| - 1 of c < 0
+            u32x2 down = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) down[j / 4] |= fabsf(m[j]) < fabsf(m_value(code_of(cm, j, true), sm0)) ? 1u << (8 * (j & 3)) : 0u;
+            down &= m_held >> 7;
+            // A byte above 0 less 1, one below 0 and 1 (-1: 0, without a carry into the next).
+            const u32x2 below0 = cm >> 7 & 0x01010101u;
+            cm -= down & ~below0;
+            cm = ((cm & 0x7F7F7F7Fu) + (down & below0)) ^ (cm & 0x80808080u);
+        }
         put_codes(t.m, at, left, vec, cm);
         put_codes(t.v, at, left, vec, cv);
         if (left > 0 && at % kBlock == 0) {
@@ -481,9 +537,10 @@ int dgm_adamMany(dgm_gpu* g, const dgm_adam_plan* plan, const float* factor, flo
     OnDevice on(g->device);
     if (on.err != hipSuccess) return dgm::fail(g, DGM_ERR_HIP, "adamMany: %s", hipGetErrorString(on.err));
     const AdamArgs a{lr, b1, b2, eps, wd, invBC1, invBC2};
+    const Held held = plan->stateBits == 8 ? held_of(a) : Held{};
     const dim3 grid{unsigned(plan->chunks)}, block{kThreads};
-    if (plan->stateBits == 32) adam_many_kernel<32><<<grid, block, 0, g->stream>>>(tensors_of(plan), chunks_of(plan), factor, a);
-    else adam_many_kernel<8><<<grid, block, 0, g->stream>>>(tensors_of(plan), chunks_of(plan), factor, a);
+    if (plan->stateBits == 32) adam_many_kernel<32><<<grid, block, 0, g->stream>>>(tensors_of(plan), chunks_of(plan), factor, a, held);
+    else adam_many_kernel<8><<<grid, block, 0, g->stream>>>(tensors_of(plan), chunks_of(plan), factor, a, held);
     DGM_LAUNCH_CHECK(g, "adam_many");
     return DGM_OK;
 }

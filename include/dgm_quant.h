@@ -635,7 +635,14 @@ int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens
  * (bits 8 or 4 as in dgm_quantize of rows of whole groups; qGroup a power of two from 8 to 512; bits 0:
  * none). A moment in 8 bits is c |c| mscale (c = -127 .. 127) or (c^2 vscale)^2
  * (c = 0 .. 255), and all zeros stand for zeros; an infinity or NaN among 256 makes their
- * scale, and so all their moments from then on, NaN. */
+ * scale, and so all their moments from then on, NaN. The code is the nearest one (of the
+ * roots), but for moments that rounding would hold: an m that shrank while its code stays and
+ * the scale does not shrink, nor grow by over an eighth, goes one code down where c (1 - b1) < 1
+ * and v's code times (1 - b2) is below 4; a v whose code stays while the scale does not grow goes
+ * one up where it grew to over 9 - 8 b2 of itself (a gradient's square of over 9 times it). So weights without gradients come to rest as with 32-bit
+ * moments. Moments far below the largest of their 256 are coarse: of steady gradients below
+ * 1.5e-4 of the largest m stays 0, and a v that decays by less than half a code a step (c < 2 /
+ * (1 - b2)) keeps its code, so that such weights' steps are smaller than AdamW's. */
 typedef struct dgm_adam_tensor {
     float* w;
     const float* grad;
