@@ -13,8 +13,8 @@
 // The code is that of the nearest root (ties up), decided exactly: c and c + 1 meet where
 // |m| 127^2 = max|m| (c + 1/2)^2, whose sides are exact in 64 bits (24 + 14 and 24 + 16 bits), and where
 // v 255^4 = max v (c + 1/2)^4 (to 2^-53). A hardware root says which border to ask. A v that is not 0 keeps a
-// code of 1 at least, so that no step divides by eps alone. A largest below 2^-120 counts as 0; an infinity or NaN
-// makes its block's scale NaN.
+// code of 1 at least, and that a value above 0, so that its steps do not divide by eps alone; but a block whose largest is
+// below 2^-120 counts as zeros. An infinity or NaN makes its block's scale NaN.
 //
 // Nearest codes alone would hold what moves by less than half a code a step, and for good: with b1 = 0.9 an m of c <= 9
 // without gradients, whose weight then moves on without end, and a v far below its gradients' squares, whose weight's
@@ -118,9 +118,23 @@ __device__ __forceinline__ int code_of(u32x2 c, int j, bool sign) {
 }
 
 __device__ __forceinline__ float m_value(int c, float sm) { return float(c * abs(c)) * sm; }
+// At least the smallest number of all where there is a code: squares of roots below 2^-74.5 would be 0. As bits, so that a NaN stays.
 __device__ __forceinline__ float v_value(int c, float rv) {
     const float root = float(c * c) * rv;
-    return root * root;
+    return __uint_as_float(max(__float_as_uint(root * root), min(__float_as_uint(root), 1u)));
+}
+// 8 of them: only scales below 2^-74 need to be looked at.
+__device__ __forceinline__ void v_values(u32x2 codes, float rv, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int c = code_of(codes, j, false);
+        const float root = float(c * c) * rv;
+        v[j] = root * root;
+    }
+    if (rv < 0x1p-74f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v_value(code_of(codes, j, false), rv);
+    }
 }
 
 // The bytes of w that are below n (up to 256), as their high bits.
@@ -208,10 +222,8 @@ __global__ __launch_bounds__(kThreads) void adam_many_kernel(const Tensor* __res
         sm0 = left > 0 ? ((const gfloat*)t.ms)[block] : 0.0f;
         rv0 = left > 0 ? ((const gfloat*)t.vs)[block] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            m[j] = m_value(code_of(cm0, j, true), sm0);
-            v[j] = v_value(code_of(cv0, j, false), rv0);
-        }
+        for (int j = 0; j < 8; ++j) m[j] = m_value(code_of(cm0, j, true), sm0);
+        v_values(cv0, rv0, v);
     }
     if (factor) {
 #pragma unroll
@@ -349,10 +361,8 @@ __global__ __launch_bounds__(kThreads) void adam_states_kernel(const Tensor* __r
     const float sm = ((const gfloat*)t.ms)[at / kBlock], rv = ((const gfloat*)t.vs)[at / kBlock];
     float x[8], y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = m_value(code_of(cm, j, true), sm);
-        y[j] = v_value(code_of(cv, j, false), rv);
-    }
+    for (int j = 0; j < 8; ++j) x[j] = m_value(code_of(cm, j, true), sm);
+    v_values(cv, rv, y);
     put8(m, t.flat + at, left, true, x);
     put8(v, t.flat + at, left, true, y);
 }

@@ -634,7 +634,8 @@ int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens
  * [ceil(n / 256)]), and where its linear reads codes, those and their scales
  * (bits 8 or 4 as in dgm_quantize of rows of whole groups; qGroup a power of two from 8 to 512; bits 0:
  * none). A moment in 8 bits is c |c| mscale (c = -127 .. 127) or (c^2 vscale)^2
- * (c = 0 .. 255), and all zeros stand for zeros; an infinity or NaN among 256 makes their
+ * (c = 0 .. 255; 2^-149 at least where c > 0), and all zeros stand for zeros. Moments of
+ * 256 whose largest is below 2^-120 count as 0; an infinity or NaN among them makes their
  * scale, and so all their moments from then on, NaN. The code is the nearest one (of the
  * roots), but for moments that rounding would hold: an m that shrank while its code stays and
  * the scale does not shrink, nor grow by over an eighth, goes one code down where c (1 - b1) < 1

@@ -15,8 +15,10 @@ def zeros(blocks):
 
 
 def values(state):
+    """What the codes stand for; a v of a code above 0 is above 0."""
     cm, sm, cv, rv = state
-    return ref.decode_m(cm, sm), ref.decode_v(cv, rv)
+    v = ref.decode_v(cv, rv)
+    return ref.decode_m(cm, sm), np.where((v == 0) & (cv > 0) & np.repeat(rv > 0, 256), F(2.0 ** -149), v).astype(F)
 
 
 def follow(state, m, v, b1, b2):

@@ -77,3 +77,32 @@ def test_weights_without_gradients_come_to_rest(dgm, gpu, torch_cuda, b2):
     x = torch.corrcoef(torch.stack([eight[~half], full[~half]]))[0, 1]
     assert x >= (0.999 if b2 == 0.95 else 0.99)
     assert 0.8 <= eight[~half].norm() / full[~half].norm() <= 1.1
+
+
+def test_second_moments_of_the_smallest_blocks(dgm, gpu, torch_cuda):
+    """Blocks whose largest v is 2^-120 and a little more: code 1 stands for 2^-32 of that, less than half the smallest fp32 number. It is above 0
+    all the same, so that a step with an eps of 0 is finite."""
+    n = 256 * 8
+    g = torch.full((8, 256), 2.0 ** -74.5, device="cuda")       # v 2^-149
+    g[:, 1::3] = 2.0 ** -70
+    g[:, 0] = torch.tensor([2.0 ** (-60 + k / 8) for k in range(8)], device="cuda")
+    g = g.view(-1)
+    s = Moments(dgm, gpu, n, g)
+    w, state = s.w.cpu().numpy(), a8.zeros(8)
+    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    hyper = dict(lr=1e-3, b1=0.0, b2=0.0, eps=0.0, wd=0.0)
+    for t in range(3):
+        if t:      # what the codes stand for, nothing new
+            hyper.update(b1=0.5, b2=0.96875)
+            g.zero_()
+        w, state, _ = a8.step(w, g.cpu().numpy(), state, **hyper, inv1=1.0, inv2=1.0)
+        gpu.begin()
+        gpu.adamMany(s.plan, **hyper, invBC1=1.0, invBC2=1.0)
+        gpu.adamMany_states(s.plan, m, v)
+        gpu.end()
+        want = a8.values(state)
+        assert np.array_equal(m.cpu().numpy(), want[0]) and np.array_equal(v.cpu().numpy(), want[1])
+        assert np.array_equal(s.w.cpu().numpy(), w, equal_nan=True)
+        if t == 0:
+            assert (s.v > 0).all() and (v > 0).all() and (s.v == 1).any()
+    assert torch.isfinite(s.w.view(8, 256)[1:]).all()      # the first one's largest fell below 2^-120, where all are zeros
