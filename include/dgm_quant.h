@@ -607,7 +607,8 @@ typedef struct dgm_loss_cfg {
  * zeros, whatever its logits. rowScale (float [rows]) may be NULL for ones, and each of loss, lse and
  * dlogits; dlogits may be logits itself. Elements behind V of a row are neither
  * read nor written. A logit of -inf has probability 0; a row of nothing else
- * has lse -inf and a loss and gradient that are not numbers, as has one with a NaN or +inf. */
+ * has lse -inf and a loss and gradient that are not numbers, as has one with a NaN or +inf. The
+ * loss is not taken from the rounded lse: what is added to all logits of a row does not change it. */
 int dgm_crossEntropy(dgm_gpu* g, const dgm_loss_cfg* cfg, const void* logits, const int32_t* targets,
                      const float* rowScale, float* loss, float* lse, void* dlogits);
 
