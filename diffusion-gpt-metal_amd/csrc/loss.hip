@@ -237,7 +237,7 @@ extern "C" int dgm_crossEntropy(dgm_gpu* g, const dgm_loss_cfg* cfg, const void*
     const int64_t ld = cfg->ld ? cfg->ld : cfg->V;
     if (cfg->rows < 0 || cfg->V < 1 || !std::isfinite(cfg->scale)) return dgm::fail(g, DGM_ERR_ARG, "crossEntropy: bad sizes or scale");
     if (ld < cfg->V) return dgm::fail(g, DGM_ERR_SHAPE, "crossEntropy: a row stride is shorter than the vocabulary");
-    if (cfg->rows > dgm::kMaxIndex || ld > dgm::kMaxIndex / 2)
+    if (cfg->rows > dgm::kMaxIndex || ld > (int64_t(1) << 30))
         return dgm::fail(g, DGM_ERR_UNSUPPORTED, "crossEntropy: rows beyond 2^31 - 1 or a row stride beyond 2^30");
     if (cfg->rows == 0 || (!loss && !lse && !dlogits)) return DGM_OK;
     if (!logits || !targets) return dgm::fail(g, DGM_ERR_ARG, "crossEntropy: null buffer");
