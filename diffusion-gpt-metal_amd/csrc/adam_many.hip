@@ -23,8 +23,8 @@
 //     that stays says nothing), c (1 - b1) < 1 (larger codes follow a decay) and v's code times (1 - b2) is below 4. It is
 //     some steps after the last gradient (v decays by rounding to 2 / (1 - b2)), and always where b2 > 0.984. Weights with
 //     gradients keep their nearest codes, which a push at every shrinking would draw toward 0.
-//   v away from 0 where it grew to over 9 - 8 b2 of itself, as by g^2 > 9 v, and rv did not: a step is then soon at most 3 times AdamW's. Nearer ones
-//     keep the nearest code: pushed at every growth, v would end at its largest g^2.
+//   v away from 0 where it grew to over 9 - 8 b2 of itself, as by g^2 > 9 v, and rv did not: a step is then soon at most
+//     3 times AdamW's. Nearer ones keep the nearest code: pushed at every growth, v would end at its largest g^2.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -194,9 +194,11 @@ __device__ __forceinline__ u32x2 encode(const float (&x)[8], float top, float& s
 }
 
 // Bound by memory: 28 bytes an element with moments of 32 bits, 16 with 8. 353 M elements in 388 tensors 1825 us (5.4
-// TB/s) and 1069 (5.3); the character GPT's 0.8 M in 68, 6 us. A workgroup finds its work by two scalar loads, whatever the
-// sizes; the 8-bit codes' roots and 64-bit borders stay below the memory's time (without a branch; IEEE roots would not).
-// Nontemporal accesses were slower by up to 14% (8 bits) or no faster.
+// TB/s) and 1132 (5.0); the character GPT's 0.8 M in 68, 6 us. A workgroup finds its work by two scalar loads, whatever the
+// sizes; the 8-bit codes' roots and 64-bit borders stay below the memory's time (without a branch; IEEE roots would not), the
+// search for codes that are held adds 5% (b2 0.999, where more may be: 10%). Nontemporal accesses were slower by up to 14% (8 bits)
+// or no faster. With the linears' codes, 303 M elements of those: int8 1952 us in groups of 64, 1960 of 8, 1953 of 512 (5.3 TB/s),
+// int4 1913; codes that do not lie at multiples of `bits` bytes take all of a tensor's accesses apart, 4360 us.
 template <int STATE>
 __global__ __launch_bounds__(kThreads) void adam_many_kernel(const Tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
                                                              const float* __restrict__ factor, AdamArgs a, Held l) {
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(1024) void adam_factor_kernel(const double* __restr
     out[1] = clip > 0.0f && norm > clip ? clip / (norm + 1e-6f) : 1.0f;
 }
 
-// The values that 8-bit moments stand for, tensor behind tensor, each rounded up to a block. 353 M elements 699 us (5.0 TB/s).
+// The values that 8-bit moments stand for, tensor behind tensor, each rounded up to a block. 353 M elements 607 us (5.8 TB/s).
 __global__ __launch_bounds__(kThreads) void adam_states_kernel(const Tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
                                                                float* __restrict__ m, float* __restrict__ v) {
     const Chunk ch = chunks[blockIdx.x];

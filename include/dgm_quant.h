@@ -563,16 +563,17 @@ int dgm_attnPagedDecode(dgm_gpu* g, const dgm_cache_cfg* cfg, int64_t type, cons
                         int64_t ws_bytes, int64_t nseq, int64_t H, int64_t ldq, int64_t ldo, float scale);
 
 /* ---- a training step around its linears ---------------------------------------
- * No counterpart among the reference's wrappers: what a language model's step needs
- * between its linears and attention. Rows lie back to back and may have any length;
- * buffers are aligned to their elements (workspaces and plans: 16 bytes). Types:
- * DGM_TYPE_F32 or DGM_TYPE_BF16; sums, statistics and parameters are fp32. Tokens,
- * targets and plans are read on the device only; a token or target beyond the vocabulary is left
- * out, and the context's next dgm_end returns DGM_ERR_SHAPE. Outputs must not overlap
- * inputs or one another unless said so. Nothing is allocated, every call but
- * dgm_adamMany_plan can be captured, and results are the same bits every time. Calls that
- * overlap in time need a workspace each. DGM_ERR_UNSUPPORTED for sizes beyond those named, and
- * where one launch cannot hold the work. */
+ * No counterpart among the reference's wrappers: what a language model's step
+ * needs between its linears and attention. Rows lie back to back and may have any
+ * length; buffers are aligned to their elements (workspaces and plans: 16 bytes).
+ * Types: DGM_TYPE_F32 or DGM_TYPE_BF16; sums, statistics and parameters are fp32.
+ * Tokens, targets and plans are read on the device only; a token or target beyond
+ * the vocabulary is left out, and the context's next dgm_end returns
+ * DGM_ERR_SHAPE. Outputs must not overlap inputs or one another unless said so.
+ * Nothing is allocated, every call but dgm_adamMany_plan can be captured, and
+ * results are the same bits every time. Calls that overlap in time need a
+ * workspace each. DGM_ERR_UNSUPPORTED for sizes beyond those named, and where one
+ * launch cannot hold the work. */
 
 typedef struct dgm_norm_cfg {
     int32_t type;                  /* DGM_TYPE_* of the rows                    */
@@ -580,16 +581,17 @@ typedef struct dgm_norm_cfg {
     int64_t rows, cols;            /* rows up to 2^31 - 1, cols up to 16384     */
 } dgm_norm_cfg;
 
-/* sum = x + res (rounded to the rows' type; res and sum may both be NULL: x itself),
- * y = (sum - mean) * rstd * weight + bias with each row's mean and rstd = 1 /
- * sqrt(variance + eps). bias, mean and rstd (float [rows], for a backward) may be NULL.
- * sum may be x or res itself, and y what is read no more. */
+/* sum = x + res (rounded to the rows' type; res and sum may both be NULL: x
+ * itself), y = (sum - mean) * rstd * weight + bias with each row's mean and rstd
+ * = 1 / sqrt(variance + eps). bias, mean and rstd (float [rows], for a backward)
+ * may be NULL. sum may be x or res itself, and y what is read no more. */
 int dgm_layerNormFwd(dgm_gpu* g, const dgm_norm_cfg* cfg, const void* x, const void* res, const float* weight,
                      const float* bias, void* sum, void* y, float* mean, float* rstd);
-/* From the rows that were normalised (x, or sum) and their mean and rstd: dx = dsum
- * + the gradient through the norm (dsum: what reaches the sum by another way, may be NULL,
- * may be dx itself), dweight += and dbias += (either may be NULL). ws: at least
- * dgm_layerNormBwd_ws_bytes(cfg) bytes (-1 for sizes that are refused). */
+/* From the rows that were normalised (x, or sum) and their mean and rstd: dx =
+ * dsum + the gradient through the norm (dsum: what reaches the sum by another
+ * way, may be NULL, may be dx itself), dweight += and dbias += (either may be
+ * NULL). ws: at least dgm_layerNormBwd_ws_bytes(cfg) bytes (-1 for sizes that are
+ * refused). */
 int64_t dgm_layerNormBwd_ws_bytes(const dgm_norm_cfg* cfg);
 int dgm_layerNormBwd(dgm_gpu* g, const dgm_norm_cfg* cfg, const void* x, const float* mean, const float* rstd,
                      const float* weight, const void* dy, const void* dsum, void* dx, float* dweight, float* dbias,
@@ -601,14 +603,16 @@ typedef struct dgm_loss_cfg {
     int64_t rows, V, ld;           /* row stride in elements, 0 for V; up to 2^30 */
 } dgm_loss_cfg;
 
-/* Softmax cross-entropy: loss[r] = lse[r] - logits[r, targets[r]], lse the natural logarithm
- * of the row's sum of e^logit, and dlogits[r, v] = scale * rowScale[r] * (softmax - [v =
- * target]). Targets are int32; a row with a negative one has a loss of 0 and a gradient of
- * zeros, whatever its logits. rowScale (float [rows]) may be NULL for ones, and each of loss, lse and
+/* Softmax cross-entropy: loss[r] = lse[r] - logits[r, targets[r]], lse the
+ * natural logarithm of the row's sum of e^logit, and dlogits[r, v] = scale *
+ * rowScale[r] * (softmax - [v = target]). Targets are int32; a row with a
+ * negative one has a loss of 0 and a gradient of zeros, whatever its logits.
+ * rowScale (float [rows]) may be NULL for ones, and each of loss, lse and
  * dlogits; dlogits may be logits itself. Elements behind V of a row are neither
- * read nor written. A logit of -inf has probability 0; a row of nothing else
- * has lse -inf and a loss and gradient that are not numbers, as has one with a NaN or +inf. The
- * loss is not taken from the rounded lse: what is added to all logits of a row does not change it. */
+ * read nor written. A logit of -inf has probability 0; a row of nothing else has
+ * lse -inf and a loss and gradient that are not numbers, as has one with a NaN or
+ * +inf. The loss is not taken from the rounded lse: what is added to all logits
+ * of a row does not change it. */
 int dgm_crossEntropy(dgm_gpu* g, const dgm_loss_cfg* cfg, const void* logits, const int32_t* targets,
                      const float* rowScale, float* loss, float* lse, void* dlogits);
 
@@ -622,29 +626,32 @@ typedef struct dgm_rows_cfg {
 /* y[r, :] = scale * table[tokens[r], :], rounded once. Token 0xFFFFFFFF (-1) is
  * none: a row of zeros, without a report. */
 int dgm_embedRows(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens, const void* table, void* y);
-/* dtable[v, :] = scale * the sum of dy[r, :] over the rows of token v, zeros for a token without rows;
- * accumulate != 0: added to dtable, whose other rows are not touched. The sums are
- * fp32, over a token's rows in a fixed order. ws: at least dgm_embedRowsBwd_ws_bytes(cfg)
- * bytes (-1 for sizes that are refused). */
+/* dtable[v, :] = scale * the sum of dy[r, :] over the rows of token v, zeros for
+ * a token without rows; accumulate != 0: added to dtable, whose other rows are
+ * not touched. The sums are fp32, over a token's rows in a fixed order. ws: at
+ * least dgm_embedRowsBwd_ws_bytes(cfg) bytes (-1 for sizes that are refused). */
 int64_t dgm_embedRowsBwd_ws_bytes(const dgm_rows_cfg* cfg);
 int dgm_embedRowsBwd(dgm_gpu* g, const dgm_rows_cfg* cfg, const uint32_t* tokens, const void* dy, float* dtable,
                      int accumulate, void* ws, int64_t ws_bytes);
 
-/* One parameter tensor of n elements: master w, gradient, moments m and v (float [n];
- * in 8 bits: int8 and uint8 codes [n], with a scale for each 256 elements, float
- * [ceil(n / 256)]), and where its linear reads codes, those and their scales
- * (bits 8 or 4 as in dgm_quantize of rows of whole groups; qGroup a power of two from 8 to 512; bits 0:
- * none). A moment in 8 bits is c |c| mscale (c = -127 .. 127) or (c^2 vscale)^2
- * (c = 0 .. 255; 2^-149 at least where c > 0), and all zeros stand for zeros. Moments of
- * 256 whose largest is below 2^-120 count as 0; an infinity or NaN among them makes their
- * scale, and so all their moments from then on, NaN. The code is the nearest one (of the
- * roots), but for moments that rounding would hold: an m that shrank while its code stays and
- * the scale does not shrink, nor grow by over an eighth, goes one code down where c (1 - b1) < 1
- * and v's code times (1 - b2) is below 4; a v whose code stays while the scale does not grow goes
- * one up where it grew to over 9 - 8 b2 of itself (a gradient's square of over 9 times it). So weights without gradients come to rest as with 32-bit
- * moments. Moments far below the largest of their 256 are coarse: of steady gradients below
- * 1.5e-4 of the largest m stays 0, and a v that decays by less than half a code a step (c < 2 /
- * (1 - b2)) keeps its code, so that such weights' steps are smaller than AdamW's. */
+/* One parameter tensor of n elements: master w, gradient, moments m and v (float
+ * [n]; in 8 bits: int8 and uint8 codes [n], with a scale for each 256 elements,
+ * float [ceil(n / 256)]), and where its linear reads codes, those and their
+ * scales (bits 8 or 4 as in dgm_quantize of rows of whole groups; qGroup a power
+ * of two from 8 to 512; bits 0: none). A moment in 8 bits is c |c| mscale (c =
+ * -127 .. 127) or (c^2 vscale)^2 (c = 0 .. 255; 2^-149 at least where c > 0), and
+ * all zeros stand for zeros. Moments of 256 whose largest is below 2^-120 count
+ * as 0; an infinity or NaN among them makes their scale, and so all their moments
+ * from then on, NaN. The code is the nearest one (of the roots), but for moments
+ * that rounding would hold: an m that shrank while its code stays and the scale
+ * does not shrink, nor grow by over an eighth, goes one code down where c (1 -
+ * b1) < 1 and v's code times (1 - b2) is below 4; a v whose code stays while the
+ * scale does not grow goes one up where it grew to over 9 - 8 b2 of itself (a
+ * gradient's square of over 9 times it). So weights without gradients come to
+ * rest as with 32-bit moments. Moments far below the largest of their 256 are
+ * coarse: of steady gradients below 1.5e-4 of the largest m stays 0, and a v that
+ * decays by less than half a code a step (c < 2 / (1 - b2)) keeps its code, so
+ * that such weights' steps are smaller than AdamW's. */
 typedef struct dgm_adam_tensor {
     float* w;
     const float* grad;
@@ -662,26 +669,35 @@ typedef struct dgm_adam_plan {     /* filled in by dgm_adamMany_plan            
     int32_t stateBits, pad;
 } dgm_adam_plan;
 
-/* Lays a list of tensors (host memory; those of 0 elements are left out) out for the
- * calls below, in `table`: device memory of at least dgm_adamMany_plan_bytes bytes
- * (-1 for a list that is refused), kept as long as the plan is used. stateBits: 32 or 8. Waits for
- * the context's stream; not during a graph capture (DGM_ERR_UNSUPPORTED). DGM_ERR_ARG where
- * buffers that a step writes overlap (a tensor named twice), or one and a gradient. Needs no open region. */
+/* Lays a list of tensors (host memory; those of 0 elements are left out) out for
+ * the calls below, in `table`: device memory of at least dgm_adamMany_plan_bytes
+ * bytes (-1 for a list that is refused), kept as long as the plan is used.
+ * stateBits: 32 or 8. Waits for the context's stream; not during a graph capture
+ * (DGM_ERR_UNSUPPORTED). DGM_ERR_ARG where buffers that a step writes overlap (a
+ * tensor named twice), or one and a gradient. Needs no open region. A plan holds
+ * addresses and sizes, nothing else of the tensors: it is made once, and again
+ * where a buffer moves (68 tensors 0.5 ms on the host, 388 2.5 ms with the Python
+ * wrappers), so gradients should keep their buffers from step to step. */
 int64_t dgm_adamMany_plan_bytes(const dgm_adam_tensor* tensors, int64_t count, int64_t stateBits);
 int dgm_adamMany_plan(dgm_gpu* g, const dgm_adam_tensor* tensors, int64_t count, int64_t stateBits, void* table,
                       int64_t bytes, dgm_adam_plan* plan);
-/* out[0] = the norm of all gradients, out[1] = the factor that brings it down to clip:
- * clip / (norm + 1e-6) where clip > 0 and norm > clip, else 1 (device memory). The squares are summed
- * in 64 bits. Calls on one plan must not overlap in time. */
+/* out[0] = the norm of all gradients, out[1] = the factor that brings it down to
+ * clip: clip / (norm + 1e-6) where clip > 0 and norm > clip, else 1 (device
+ * memory). The squares are summed in 64 bits. Calls on one plan must not overlap
+ * in time. */
 int dgm_adamMany_norm(dgm_gpu* g, const dgm_adam_plan* plan, float clip, float* out);
 /* dgm_adam of every tensor, wd 0 for those without decay, in one launch; with
- * bits, dgm_adam_quantize. factor (device memory, may be NULL): one float that the gradients
- * are multiplied by on the way (they are not written). With 32-bit moments
- * the results are those calls' bits. */
+ * bits, dgm_adam_quantize. factor (device memory, may be NULL): one float that
+ * the gradients are multiplied by on the way (they are not written). With 32-bit
+ * moments the results are those calls' bits. lr, the corrections and the others
+ * are taken by value: a captured graph repeats those of its capture. Where they
+ * change from step to step, capture what comes before and make this call between
+ * the replays. */
 int dgm_adamMany(dgm_gpu* g, const dgm_adam_plan* plan, const float* factor, float lr, float b1, float b2, float eps,
                  float wd, float invBC1, float invBC2);
-/* The values of a plan's 8-bit moments (for a checkpoint): m and v [elements], 16-byte aligned, tensor behind tensor,
- * each from the next multiple of 256; what lies between is not written. */
+/* The values of a plan's 8-bit moments (for a checkpoint): m and v [elements],
+ * 16-byte aligned, tensor behind tensor, each from the next multiple of 256; what
+ * lies between is not written. */
 int dgm_adamMany_states(dgm_gpu* g, const dgm_adam_plan* plan, float* m, float* v);
 
 /* ---- checkpoints (host code, no context) ----------------------------------
