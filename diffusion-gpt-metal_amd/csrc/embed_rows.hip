@@ -34,8 +34,8 @@ struct LookupArgs {
     float scale;
     int team;   // lanes to a row, a power of two up to 256
 };
-// Pieces begin at a row's first element, whatever its address: rows of 4097 bf16 20.7 us, of 4096 19.5, of 1001 8.1 and of 1000 7.6 (8192
-// of them): the table's rows and those of y begin at different ones, so that both cannot have them at multiples of 4 bytes.
+// Pieces begin at a row's first element, whatever its address: the table's row and y's begin at different ones, so that not both can have
+// them at multiples of 4 bytes (8192 bf16 rows of 4097 20.7 us, of 4096 19.5; of 1001 8.1, of 1000 7.6).
 // 16-byte pieces that a lane asks for together (8192 rows of 4096, fp32: 41.4 us, with one 42.4, with four from half the lanes
 // 41.2; 32768 bf16 rows of 512 9.6, 10.0, 10.4).
 constexpr int kPieces = 2;
@@ -314,9 +314,9 @@ constexpr int kAhead = 8;                  // of them asked for together
 
 // Everything that is added up is read once, and said so to the caches: 32768 bf16 rows of 50257 x 2048 with the lookup 143 us,
 // 151 with ordinary loads; 16384 of 300 x 4096 74 and 87.
-// Columns of a lane: 4 where rows are whole pieces of 4, else 1 (4 behind a row's end would need its last lane's apart; 8192 rows of
-// 50257 x 4096, added, 76.6 us, of 4097 95; bf16 66 and 85; of 1000 40 and of 1001 52). Lanes behind a row's end load its last ones and
-// store nothing.
+// Columns of a lane: 4 where rows are whole pieces of 4, else 1, so that no lane's columns are cut by a row's end (8192 rows of
+// 50257 x 4096, added, 77 us, of 4097 95; bf16 66 and 85; of 1000 40, of 1001 52). Lanes behind a row's end load its last
+// ones and store nothing.
 inline int cols_of(int64_t C) { return C % 4 == 0 ? 4 : 1; }
 template <int N, typename T>
 __device__ __forceinline__ void load_cols(const T* p, float (&x)[N]) {

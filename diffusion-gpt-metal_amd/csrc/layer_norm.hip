@@ -172,7 +172,8 @@ struct BwdArgs {
     float *dw, *db;        // of the columns' workgroups
 };
 
-// The sums of 32 columns over all rows, a share of the rows to each 32 threads.
+// The sums of 32 columns over all rows, a share of the rows to each 32 threads. Eight rows are added up by themselves first: they
+// are on their way together, and a share of up to 128 rows is 24 additions long at most, not 128.
 template <typename T, int THREADS>
 __device__ __forceinline__ void norm_columns(const BwdArgs& a, int block) {
     constexpr int SHARES = THREADS / 32;
@@ -180,13 +181,24 @@ __device__ __forceinline__ void norm_columns(const BwdArgs& a, int block) {
     const int t = threadIdx.x & 31, share = threadIdx.x >> 5, c = block * 32 + t;
     float dw = 0.0f, db = 0.0f;
     if (c < a.cols) {
-#pragma unroll 8
-        for (int r = share; r < int(a.rows); r += SHARES) {
+        const auto add = [&](int r, float& w, float& b) {
             const float x = float(static_cast<const T*>(a.x)[int64_t(r) * a.cols + c]);
             const float y = float(static_cast<const T*>(a.dy)[int64_t(r) * a.cols + c]);
-            dw = __builtin_fmaf(y, (x - a.mean[r]) * a.rstd[r], dw);
-            db += y;
+            w = __builtin_fmaf(y, (x - a.mean[r]) * a.rstd[r], w);
+            b += y;
+        };
+        int r = share;
+        for (; r + 7 * SHARES < int(a.rows); r += 8 * SHARES) {
+            float w = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) add(r + u * SHARES, w, b);
+            dw += w;
+            db += b;
         }
+        float w = 0.0f, b = 0.0f;
+        for (; r < int(a.rows); r += SHARES) add(r, w, b);
+        dw += w;
+        db += b;
     }
     sums[0][share][t] = dw;
     sums[1][share][t] = db;

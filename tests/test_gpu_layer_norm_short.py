@@ -49,3 +49,23 @@ def test_rows_of_two(dgm, gpu, torch_cuda, dtype, residual):
     s2 = (gx[:, :1] + gx[:, 1:]) / F(2)
     inner = -xh * s2 + (g - s1)
     assert same(dx, r * inner + of(dsum) if residual else r * inner)
+
+
+@pytest.mark.parametrize("rows,cols", [(1024, 128), (1023, 33), (2048, 512), (77, 1000), (5, 7), (1, 3)])
+def test_sums_over_rows_of_unlike_sizes(dgm, gpu, torch_cuda, rows, cols):
+    """A row of 2^24 first and rows of 1 behind it, which a running sum that holds the first would lose one by one. The rows are in 16 shares, which
+    add eights of rows, then those, and at last the shares and what was there: u of the sum of magnitudes for each addition in a row."""
+    dy = torch.ones(rows, cols, device="cuda")
+    dy[0] = 2.0 ** 24
+    x = torch.randn(rows, cols, device="cuda")
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    w, dx, dw, db = torch.ones(cols, device="cuda"), torch.zeros_like(x), torch.zeros(cols, device="cuda"), torch.zeros(cols, device="cuda")
+    cfg = dgm.NormCfg(type=dgm.DGM_TYPE_F32, eps=1e-5, rows=rows, cols=cols)
+    assert gpu.layerNormBwd_ws_bytes(cfg) == 0
+    gpu.begin()
+    gpu.layerNormBwd(cfg, x, mean, rstd, w, dy, None, dx, dw, db, None, 0)
+    gpu.end()
+    u = 2.0 ** -24
+    for got, terms in ((db, dy.double()), (dw, dy.double() * x.double())):
+        adds = 8 + -(-rows // 128) + 16 + 1
+        assert ((got.double() - terms.sum(0)).abs() <= adds * u * terms.abs().sum(0)).all()
