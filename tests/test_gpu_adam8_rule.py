@@ -50,6 +50,34 @@ def test_codes_are_numpy_s(dgm, gpu, torch_cuda, b1, b2):
     assert moved[1] > 0 and (moved[0] > 0) == (b1 > 0.0)
 
 
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_codes_of_tensors_at_any_element(dgm, gpu, torch_cuda, offset):
+    """The same where buffers begin between 16-byte boundaries, and end inside a lane's 8 elements."""
+    n, pad = N - 77, lambda x: np.concatenate([x, np.zeros(-len(x) % 256, x.dtype)])
+    rng = np.random.default_rng(offset)
+    part = lambda dtype, count: torch.full((count + offset + 8,), 3, dtype=dtype, device="cuda")[offset:offset + count].zero_()
+    w8, g, m, v, ms, vs = (part(t, k) for t, k in ((torch.float32, n), (torch.float32, n), (torch.int8, n), (torch.uint8, n),
+                                                   (torch.float32, BLOCKS), (torch.float32, BLOCKS)))
+    plan = gpu.adamMany_plan([dgm.adam_tensor(w8, g, m, v, ms, vs, decay=False)], 8)
+    w, state, moved = np.zeros(N, a8.F), a8.zeros(BLOCKS), 0
+    for t in range(40):
+        x = rng.standard_normal(n).astype(a8.F)
+        x[rng.permutation(n) % 3 == 0] *= a8.F(1e-3)
+        if t > 5:
+            x[np.arange(n) % 5 == 0] = 0
+        g.copy_(torch.from_numpy(x))
+        hyper, inv = dict(lr=1e-3, b1=0.9, b2=0.95, eps=1e-8, wd=0.0), (1 / (1 - 0.9 ** (t + 1)), 1 / (1 - 0.95 ** (t + 1)))
+        w, state, where = a8.step(w, pad(x), state, **hyper, inv1=inv[0], inv2=inv[1])
+        moved += where[0].sum()
+        gpu.begin()
+        gpu.adamMany(plan, **hyper, invBC1=inv[0], invBC2=inv[1])
+        gpu.end()
+        assert np.array_equal(w8.cpu().numpy(), w[:n])
+        for got, want, k in zip((m, ms, v, vs), state, (n, BLOCKS, n, BLOCKS)):
+            assert np.array_equal(got.cpu().numpy(), want[:k]), t
+    assert moved > 0
+
+
 @pytest.mark.parametrize("b2", [0.95, 0.999])
 def test_weights_without_gradients_come_to_rest(dgm, gpu, torch_cuda, b2):
     """From step 100 on the first half of each block has no gradients: over 1000 steps its weights move within a factor of 2 of
